@@ -1,0 +1,458 @@
+// Embedding rows and the gradient of their table.
+//
+//   out[i][:]    = scale * table[id_i][:]
+//   dtable[v][:] = scale * sum over i with id_i = v, in ascending i, of dy[i][:]
+//
+// The gradient groups the positions by id with a stable sort instead of adding with atomics, so every row of the table is
+// written once, by one wave, in an order that depends on the ids alone: the same call returns the same bits.  Sums are fp32,
+// rounded once if the table is bf16.  An id outside [0, rows) reads as a NaN row and contributes to no gradient (ids live on
+// the device; nothing here waits for the host).
+#include "common.h"
+
+namespace {
+
+constexpr int SORT1 = 8192;          // ids that one workgroup sorts in LDS
+constexpr int TILE = 2048;           // ids per workgroup of a radix pass: four waves with 512 consecutive ids each
+constexpr int MAXBINS = 256;
+constexpr int CHUNK = 64;            // sorted positions of one id that are summed ahead when they fill an aligned chunk ...
+constexpr int SUPER = 64;            // ... and aligned runs of so many such chunks
+
+template <typename T> __device__ __forceinline__ float ldf(const T* p) { return (float)*p; }
+template <typename T> struct Vec4;
+template <> struct Vec4<float> { typedef f32x4 t; };
+template <> struct Vec4<bf16_t> { typedef bf16x4 t; };
+template <typename T> __device__ __forceinline__ f32x4 ld4(const T* p) {
+    const typename Vec4<T>::t v = *(const typename Vec4<T>::t*)p;
+    return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+template <typename T> __device__ __forceinline__ void st4(T* p, f32x4 v) {
+    typename Vec4<T>::t o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
+    *(typename Vec4<T>::t*)p = o;
+}
+
+__device__ __forceinline__ long long load_id(const void* ids, int ids64, size_t i) {
+    return ids64 ? ((const long long*)ids)[i] : (long long)((const int*)ids)[i];
+}
+
+// ---- rows -------------------------------------------------------------------------------------------------------
+// One thread per 4 (or, for odd widths and unaligned tensors, 1) elements of the output; bound by the bytes of the rows.
+template <typename TI, typename TO, int VEC>
+__global__ __launch_bounds__(256) void embed_rows_kernel(const void* __restrict__ ids, int ids64, const TI* __restrict__ table,
+                                                         TO* __restrict__ out, unsigned total, unsigned per_row, long long rows,
+                                                         int width, float scale) {
+    const unsigned idx = blockIdx.x * 256u + threadIdx.x;
+    if (idx >= total) return;
+    const unsigned row = idx / per_row, c = (idx - row * per_row) * VEC;
+    const long long id = load_id(ids, ids64, row);
+    const bool ok = id >= 0 && id < rows;
+    const TI* src = table + (size_t)(ok ? id : 0) * width + c;
+    TO* dst = out + (size_t)row * width + c;
+    if constexpr (VEC == 4) {
+        f32x4 v = {NAN, NAN, NAN, NAN};
+        if (ok) v = ld4(src) * scale;
+        st4(dst, v);
+    } else {
+        *dst = ok ? (TO)(ldf(src) * scale) : (TO)NAN;
+    }
+}
+
+// ---- sort: up to SORT1 ids by one workgroup -----------------------------------------------------------------------
+// Bitonic network over id * 2^posbits + position: unique keys, so the order is that of a stable sort.
+template <typename KEY>
+__global__ __launch_bounds__(1024) void sort_small_kernel(const void* __restrict__ ids, int ids64, int n, int n2, int posbits,
+                                                          unsigned rows, unsigned* __restrict__ keys, unsigned* __restrict__ pos) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    KEY* s = (KEY*)smem;
+    for (int i = threadIdx.x; i < n2; i += blockDim.x) {
+        KEY k = ~(KEY)0;
+        if (i < n) {
+            const long long id = load_id(ids, ids64, i);
+            k = ((KEY)(id >= 0 && id < (long long)rows ? (unsigned)id : rows) << posbits) | (KEY)i;
+        }
+        s[i] = k;
+    }
+    __syncthreads();
+    for (int size = 2; size <= n2; size <<= 1)
+        for (int step = size >> 1; step > 0; step >>= 1) {
+            for (int t = threadIdx.x; t < n2 / 2; t += blockDim.x) {
+                const int i = ((t & ~(step - 1)) << 1) | (t & (step - 1)), j = i + step;
+                const KEY a = s[i], b = s[j];
+                if ((a > b) == ((i & size) == 0)) { s[i] = b; s[j] = a; }
+            }
+            __syncthreads();
+        }
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        keys[i] = (unsigned)(s[i] >> posbits);
+        pos[i] = (unsigned)(s[i] & (((KEY)1 << posbits) - 1));
+    }
+}
+
+// ---- sort: any number of ids, least significant digit first ---------------------------------------------------------
+// FIRST: the input is the id list itself (position = index); else (keys, pos) of the previous pass.
+template <bool FIRST>
+__device__ __forceinline__ unsigned pass_key(const void* ids, int ids64, const unsigned* keys, size_t i, unsigned rows) {
+    if (!FIRST) return keys[i];
+    const long long id = load_id(ids, ids64, i);
+    return id >= 0 && id < (long long)rows ? (unsigned)id : rows;
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(256) void radix_count_kernel(const void* __restrict__ ids, int ids64, const unsigned* __restrict__ keys,
+                                                          int n, unsigned rows, int shift, unsigned mask, int tiles,
+                                                          unsigned* __restrict__ counts) {
+    __shared__ unsigned hist[MAXBINS];
+    hist[threadIdx.x] = 0;
+    __syncthreads();
+    const int base = blockIdx.x * TILE;
+#pragma unroll
+    for (int u = 0; u < TILE / 256; ++u) {
+        const int i = base + u * 256 + threadIdx.x;
+        if (i < n) atomicAdd(&hist[(pass_key<FIRST>(ids, ids64, keys, i, rows) >> shift) & mask], 1u);
+    }
+    __syncthreads();
+    if (threadIdx.x <= mask) counts[(size_t)threadIdx.x * tiles + blockIdx.x] = hist[threadIdx.x];
+}
+
+// In place: counts -> exclusive prefix sums, one workgroup, 4096 consecutive entries per round.
+__global__ __launch_bounds__(1024) void scan_kernel(unsigned* __restrict__ counts, int total) {
+    __shared__ unsigned wsum[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    unsigned carry = 0;
+    for (int base = 0; base < total; base += 4096) {
+        const int i = base + threadIdx.x * 4;
+        unsigned v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = i + e < total ? counts[i + e] : 0u;
+        const unsigned mine = v[0] + v[1] + v[2] + v[3];
+        unsigned inc = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned t = __shfl_up(inc, o, 64);
+            if (lane >= o) inc += t;
+        }
+        if (lane == 63) wsum[wave] = inc;
+        __syncthreads();
+        unsigned before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) { if (w < wave) before += wsum[w]; all += wsum[w]; }
+        unsigned run = carry + before + inc - mine;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { if (i + e < total) counts[i + e] = run; run += v[e]; }
+        carry += all;
+        __syncthreads();
+    }
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(256) void radix_scatter_kernel(const void* __restrict__ ids, int ids64, const unsigned* __restrict__ keys,
+                                                            const unsigned* __restrict__ pos, int n, unsigned rows, int shift, int bits,
+                                                            int tiles, const unsigned* __restrict__ starts,
+                                                            unsigned* __restrict__ keys_out, unsigned* __restrict__ pos_out) {
+    constexpr int ROUNDS = TILE / 256;
+    __shared__ unsigned cnt[4][MAXBINS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned mask = (1u << bits) - 1;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) cnt[w][threadIdx.x] = 0;
+    __syncthreads();
+    const int base = blockIdx.x * TILE + wave * (TILE / 4);
+    unsigned key[ROUNDS], rank[ROUNDS];
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u) {
+        const int i = base + u * 64 + lane;
+        const bool in = i < n;
+        key[u] = in ? pass_key<FIRST>(ids, ids64, keys, i, rows) : 0u;
+        const unsigned d = (key[u] >> shift) & mask;
+        unsigned long long same = __ballot(in);              // lanes of this round that hold the same digit
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long has = __ballot((d >> b) & 1);
+            same &= (d >> b) & 1 ? has : ~has;
+        }
+        const unsigned long long below = same & ((1ull << lane) - 1);
+        const unsigned old = in ? cnt[wave][d] : 0u;
+        rank[u] = old + __popcll(below);
+        __builtin_amdgcn_wave_barrier();
+        if (in && below == 0) cnt[wave][d] = old + __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    {   // counts of the four waves -> where each wave's first entry of a digit goes
+        const unsigned d = threadIdx.x;
+        unsigned at = d <= mask ? starts[(size_t)d * tiles + blockIdx.x] : 0u;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { const unsigned c = cnt[w][d]; cnt[w][d] = at; at += c; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u) {
+        const int i = base + u * 64 + lane;
+        if (i < n) {
+            const unsigned at = cnt[wave][(key[u] >> shift) & mask] + rank[u];
+            keys_out[at] = key[u];
+            pos_out[at] = FIRST ? (unsigned)i : pos[i];
+        }
+    }
+}
+
+// ---- sums -----------------------------------------------------------------------------------------------------------
+// Adds `count` rows src[idx(j)][col0 ..] to acc: a wave, four columns per lane and sweep, four rows in flight.
+constexpr int SWEEPS = 4;            // 256 columns each
+template <int VEC, typename T, typename IDX>
+__device__ __forceinline__ void add_rows(f32x4 (&acc)[SWEEPS], const T* __restrict__ src, int width, int col0, int count, IDX idx) {
+    const int lane = threadIdx.x & 63;
+    int j = 0;
+    for (; j + 4 <= count; j += 4) {
+        const T* r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = src + (size_t)idx(j + e) * width;
+#pragma unroll
+        for (int s = 0; s < SWEEPS; ++s) {
+            const int c = col0 + s * 64 * VEC + lane * VEC;
+            if (c < width) {
+                if constexpr (VEC == 4) {
+                    const f32x4 a = ld4(r[0] + c), b = ld4(r[1] + c), d = ld4(r[2] + c), e = ld4(r[3] + c);
+                    acc[s] = acc[s] + a; acc[s] = acc[s] + b; acc[s] = acc[s] + d; acc[s] = acc[s] + e;
+                } else {
+                    const float a = ldf(r[0] + c), b = ldf(r[1] + c), d = ldf(r[2] + c), e = ldf(r[3] + c);
+                    acc[s][0] += a; acc[s][0] += b; acc[s][0] += d; acc[s][0] += e;
+                }
+            }
+        }
+    }
+    for (; j < count; ++j) {
+        const T* r = src + (size_t)idx(j) * width;
+#pragma unroll
+        for (int s = 0; s < SWEEPS; ++s) {
+            const int c = col0 + s * 64 * VEC + lane * VEC;
+            if (c < width) {
+                if constexpr (VEC == 4) acc[s] = acc[s] + ld4(r + c);
+                else acc[s][0] += ldf(r + c);
+            }
+        }
+    }
+}
+template <int VEC, typename T>
+__device__ __forceinline__ void put_row(T* __restrict__ dst, const f32x4 (&acc)[SWEEPS], int width, int col0, float scale) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int s = 0; s < SWEEPS; ++s) {
+        const int c = col0 + s * 64 * VEC + lane * VEC;
+        if (c < width) {
+            if constexpr (VEC == 4) st4(dst + c, acc[s] * scale);
+            else dst[c] = (T)(acc[s][0] * scale);
+        }
+    }
+}
+
+// Aligned chunks whose CHUNK positions all belong to one id: a wave sums each (blockIdx.y: 256 * VEC columns).
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void chunk_sum_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ pos, int n,
+                                                        unsigned rows, const T* __restrict__ dy, int width, float* __restrict__ part) {
+    const int c = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lo = c * CHUNK;
+    if (lo + CHUNK > n) return;
+    const unsigned k = keys[lo];
+    if (k >= rows || keys[lo + CHUNK - 1] != k) return;
+    const int col0 = blockIdx.y * SWEEPS * 64 * VEC;
+    f32x4 acc[SWEEPS] = {};
+    add_rows<VEC>(acc, dy, width, col0, CHUNK, [&](int j) { return pos[lo + j]; });
+    put_row<VEC>(part + (size_t)c * width, acc, width, col0, 1.f);
+}
+// ... and aligned runs of SUPER such chunks.
+template <int VEC>
+__global__ __launch_bounds__(64) void super_sum_kernel(const unsigned* __restrict__ keys, int n, unsigned rows, int width,
+                                                       const float* __restrict__ part, float* __restrict__ part2) {
+    const int lo = blockIdx.x * (CHUNK * SUPER);
+    if (lo + CHUNK * SUPER > n) return;
+    const unsigned k = keys[lo];
+    if (k >= rows || keys[lo + CHUNK * SUPER - 1] != k) return;
+    const int col0 = blockIdx.y * SWEEPS * 64 * VEC, c0 = blockIdx.x * SUPER;
+    f32x4 acc[SWEEPS] = {};
+    add_rows<VEC>(acc, part, width, col0, SUPER, [&](int j) { return (unsigned)(c0 + j); });
+    put_row<VEC>(part2 + (size_t)blockIdx.x * width, acc, width, col0, 1.f);
+}
+
+// Every row of the table, written once: a wave takes the sorted positions of its id (found by binary search) in order, whole
+// aligned chunks and runs of chunks from their sums; an id without positions gets zeros.
+constexpr int ROWS_PER_WG = 8;
+template <typename T, typename TO, int VEC>
+__global__ __launch_bounds__(256) void table_grad_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ pos, int n,
+                                                         unsigned rows, const T* __restrict__ dy, int width, float scale,
+                                                         const float* __restrict__ part, const float* __restrict__ part2,
+                                                         TO* __restrict__ dtable) {
+    __shared__ int start[ROWS_PER_WG + 1];
+    const unsigned v0 = blockIdx.x * ROWS_PER_WG;
+    if (threadIdx.x <= ROWS_PER_WG) {
+        const unsigned v = v0 + threadIdx.x;
+        int lo = 0, hi = n;                                   // first index with keys[index] >= v
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (keys[mid] < v) lo = mid + 1; else hi = mid;
+        }
+        start[threadIdx.x] = lo;
+    }
+    __syncthreads();
+    for (int r = threadIdx.x >> 6; r < ROWS_PER_WG; r += 4) {
+        const unsigned v = v0 + r;
+        if (v >= rows) break;
+        const int s = __builtin_amdgcn_readfirstlane(start[r]), e = __builtin_amdgcn_readfirstlane(start[r + 1]);
+        for (int col0 = 0; col0 < width; col0 += SWEEPS * 64 * VEC) {
+            f32x4 acc[SWEEPS] = {};
+            for (int i = s; i < e;) {
+                if (part2 && i % (CHUNK * SUPER) == 0 && i + CHUNK * SUPER <= e) {
+                    const int count = (e - i) / (CHUNK * SUPER), c0 = i / (CHUNK * SUPER);
+                    add_rows<VEC>(acc, part2, width, col0, count, [&](int j) { return (unsigned)(c0 + j); });
+                    i += count * CHUNK * SUPER;
+                } else if (part && i % CHUNK == 0 && i + CHUNK <= e) {
+                    int stop = e / CHUNK * CHUNK;             // as far as whole chunks go, or to the next run of chunks
+                    const int next = (i / (CHUNK * SUPER) + 1) * (CHUNK * SUPER);
+                    if (part2 && next < stop) stop = next;
+                    const int c0 = i / CHUNK;
+                    add_rows<VEC>(acc, part, width, col0, (stop - i) / CHUNK, [&](int j) { return (unsigned)(c0 + j); });
+                    i = stop;
+                } else {
+                    int stop = e;
+                    const int next = (i / CHUNK + 1) * CHUNK;
+                    if (part && next < stop) stop = next;
+                    const int i0 = i;
+                    add_rows<VEC>(acc, dy, width, col0, stop - i, [&](int j) { return pos[i0 + j]; });
+                    i = stop;
+                }
+            }
+            put_row<VEC>(dtable + (size_t)v * width, acc, width, col0, scale);
+        }
+    }
+}
+
+struct GradPlan {
+    int n, tiles, passes, bits, keybits;
+    size_t keys, pos, keys2, pos2, counts, part, part2, bytes;   // byte offsets into the workspace
+};
+static GradPlan grad_plan(long long n, long long rows, int width) {
+    GradPlan g = {};
+    g.n = (int)n;
+    g.keybits = 1;
+    while ((1ll << g.keybits) <= rows) ++g.keybits;               // `rows` itself is the key of an id out of range
+    g.passes = (g.keybits + 7) / 8;
+    g.bits = (g.keybits + g.passes - 1) / g.passes;
+    g.tiles = (int)((n + TILE - 1) / TILE);
+    size_t at = 0;
+    auto take = [&](size_t b) { const size_t o = at; at += (b + 255) / 256 * 256; return o; };
+    g.keys = take((size_t)n * 4);
+    g.pos = take((size_t)n * 4);
+    if (n > SORT1) {
+        g.keys2 = take((size_t)n * 4);
+        g.pos2 = take((size_t)n * 4);
+        g.counts = take((size_t)g.tiles * MAXBINS * 4);
+    }
+    g.part = take((size_t)(n / CHUNK) * width * 4);
+    g.part2 = take((size_t)(n / (CHUNK * SUPER)) * width * 4);
+    g.bytes = at;
+    return g;
+}
+
+static const char* bad_shape(long long n, long long rows, long long width) {
+    if (n < 0 || rows < 1 || width < 1) return "negative count or empty table";
+    if (n > (1ll << 30) || rows > (1ll << 30) || width > (1 << 20)) return "more than 2^30 ids or rows, or 2^20 columns";
+    if (n * width >= (1ll << 32)) return "more than 2^32 elements";
+    return nullptr;
+}
+
+template <typename T, typename TO, int VEC>
+static void launch_grad(const GradPlan& g, char* ws, const unsigned* keys, const unsigned* pos, unsigned rows, const void* dy, int width,
+                        float scale, void* dtable, hipStream_t st) {
+    const int cols = (width + SWEEPS * 64 * VEC - 1) / (SWEEPS * 64 * VEC);
+    const int chunks = g.n / CHUNK, supers = g.n / (CHUNK * SUPER);
+    float *part = (float*)(ws + g.part), *part2 = (float*)(ws + g.part2);
+    if (chunks) hipLaunchKernelGGL((chunk_sum_kernel<T, VEC>), dim3((chunks + 3) / 4, cols), dim3(256), 0, st, keys, pos, g.n, rows,
+                                   (const T*)dy, width, part);
+    if (supers) hipLaunchKernelGGL((super_sum_kernel<VEC>), dim3(supers, cols), dim3(64), 0, st, keys, g.n, rows, width, part, part2);
+    hipLaunchKernelGGL((table_grad_kernel<T, TO, VEC>), dim3((rows + ROWS_PER_WG - 1) / ROWS_PER_WG), dim3(256), 0, st, keys, pos, g.n,
+                       rows, (const T*)dy, width, scale, chunks ? part : nullptr, supers ? part2 : nullptr, (TO*)dtable);
+}
+
+template <typename TI, typename TO>
+static void launch_rows(const void* ids, int ids64, long long n, const void* table, long long rows, int width, float scale, void* out,
+                        bool vec, hipStream_t st) {
+    const unsigned per_row = vec ? width / 4 : width, total = (unsigned)(n * per_row);
+    const dim3 grid((unsigned)(((size_t)total + 255) / 256)), blk(256);
+    if (vec) hipLaunchKernelGGL((embed_rows_kernel<TI, TO, 4>), grid, blk, 0, st, ids, ids64, (const TI*)table, (TO*)out, total, per_row, rows, width, scale);
+    else hipLaunchKernelGGL((embed_rows_kernel<TI, TO, 1>), grid, blk, 0, st, ids, ids64, (const TI*)table, (TO*)out, total, per_row, rows, width, scale);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mi355_embedding_fwd(const void* ids, int ids64, long long n, const void* table, int table_bf16, long long rows, int width, float scale,
+                        void* out, int out_bf16, void* stream) {
+    if (const char* why = bad_shape(n, rows, width)) return mi355_fail(MI355_ERR_ARG, "embedding: %s", why);
+    if (n == 0) return MI355_OK;
+    if (!ids || !table || !out) return mi355_fail(MI355_ERR_ARG, "embedding: null pointer");
+    const hipStream_t st = (hipStream_t)stream;
+    const bool vec = width % 4 == 0 && (uintptr_t)table % (table_bf16 ? 8 : 16) == 0 && (uintptr_t)out % (out_bf16 ? 8 : 16) == 0;
+    ProfScope prof(FAM_ELEM, st, (double)n * width * ((table_bf16 ? 2 : 4) + (out_bf16 ? 2 : 4)));
+    if (table_bf16) {
+        if (out_bf16) launch_rows<bf16_t, bf16_t>(ids, ids64, n, table, rows, width, scale, out, vec, st);
+        else launch_rows<bf16_t, float>(ids, ids64, n, table, rows, width, scale, out, vec, st);
+    } else {
+        if (out_bf16) launch_rows<float, bf16_t>(ids, ids64, n, table, rows, width, scale, out, vec, st);
+        else launch_rows<float, float>(ids, ids64, n, table, rows, width, scale, out, vec, st);
+    }
+    return mi355_check_launch("embedding_fwd");
+}
+
+size_t mi355_embedding_bwd_workspace_bytes(long long n, long long rows, int width) {
+    if (bad_shape(n, rows, width)) return 0;
+    return grad_plan(n, rows, width).bytes;
+}
+
+int mi355_embedding_bwd(const void* ids, int ids64, long long n, const void* dy, int dy_bf16, long long rows, int width, float scale,
+                        void* dtable, int out_bf16, void* ws, size_t ws_bytes, void* stream) {
+    if (const char* why = bad_shape(n, rows, width)) return mi355_fail(MI355_ERR_ARG, "embedding_bwd: %s", why);
+    if (!dtable || (n > 0 && (!ids || !dy || !ws))) return mi355_fail(MI355_ERR_ARG, "embedding_bwd: null pointer");
+    const GradPlan g = grad_plan(n, rows, width);
+    if (ws_bytes < g.bytes) return mi355_fail(MI355_ERR_ARG, "embedding_bwd: workspace of %zu bytes, %zu needed", ws_bytes, g.bytes);
+    if ((uintptr_t)ws % 16) return mi355_fail(MI355_ERR_ARG, "embedding_bwd: workspace not 16-byte aligned");
+    const hipStream_t st = (hipStream_t)stream;
+    ProfScope prof(FAM_ELEM, st, (double)n * width * (dy_bf16 ? 2 : 4) + (double)rows * width * (out_bf16 ? 2 : 4));
+    char* w = (char*)ws;
+    unsigned *keys = (unsigned*)(w + g.keys), *pos = (unsigned*)(w + g.pos);
+    const unsigned R = (unsigned)rows;
+    if (n > 0 && n <= SORT1) {
+        int n2 = 2, posbits = 1;
+        while (n2 < n) { n2 <<= 1; ++posbits; }
+        const int threads = n2 / 2 < 64 ? 64 : n2 / 2 > 1024 ? 1024 : n2 / 2;
+        if (g.keybits + posbits <= 31)      // all ones stays free for the padding
+            hipLaunchKernelGGL((sort_small_kernel<unsigned>), dim3(1), dim3(threads), n2 * 4, st, ids, ids64, (int)n, n2, posbits, R, keys, pos);
+        else
+            hipLaunchKernelGGL((sort_small_kernel<unsigned long long>), dim3(1), dim3(threads), n2 * 8, st, ids, ids64, (int)n, n2, posbits, R, keys, pos);
+    } else if (n > 0) {
+        unsigned* counts = (unsigned*)(w + g.counts);
+        unsigned *k2 = (unsigned*)(w + g.keys2), *p2 = (unsigned*)(w + g.pos2);
+        const unsigned mask = (1u << g.bits) - 1;
+        const int total = (int)(mask + 1) * g.tiles;
+        for (int p = 0; p < g.passes; ++p) {
+            const bool into2 = ((g.passes - p) & 1) == 0;        // the last pass ends in (keys, pos)
+            const unsigned *ki = into2 ? keys : k2, *pi = into2 ? pos : p2;
+            unsigned *ko = into2 ? k2 : keys, *po = into2 ? p2 : pos;
+            const int shift = p * g.bits;
+            if (p == 0) hipLaunchKernelGGL((radix_count_kernel<true>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, g.n, R, shift, mask, g.tiles, counts);
+            else hipLaunchKernelGGL((radix_count_kernel<false>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, g.n, R, shift, mask, g.tiles, counts);
+            hipLaunchKernelGGL(scan_kernel, dim3(1), dim3(1024), 0, st, counts, total);
+            if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<true>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, pi, g.n, R, shift, g.bits, g.tiles, counts, ko, po);
+            else hipLaunchKernelGGL((radix_scatter_kernel<false>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, pi, g.n, R, shift, g.bits, g.tiles, counts, ko, po);
+        }
+    }
+    const bool vec = width % 4 == 0 && (uintptr_t)dy % (dy_bf16 ? 8 : 16) == 0 && (uintptr_t)dtable % (out_bf16 ? 8 : 16) == 0;
+#define GRAD(T, TO) (vec ? launch_grad<T, TO, 4>(g, w, keys, pos, R, dy, width, scale, dtable, st) \
+                         : launch_grad<T, TO, 1>(g, w, keys, pos, R, dy, width, scale, dtable, st))
+    if (dy_bf16) { if (out_bf16) GRAD(bf16_t, bf16_t); else GRAD(bf16_t, float); }
+    else { if (out_bf16) GRAD(float, bf16_t); else GRAD(float, float); }
+#undef GRAD
+    return mi355_check_launch("embedding_bwd");
+}
+
+}  // extern "C"

@@ -1,0 +1,321 @@
+// AdamW over many tensors in one launch, states in 32 or 8 bits, behind one launch for the global gradient norm.
+//
+//   g = c grad,  c = min(1, max_norm / (|grad| + 1e-6));   m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - lr / bc1 * m / (sqrt(v) / sqrt(bc2) + eps)
+//
+// A tensor's elements are dealt out in blocks of 256.  States of 8 bits hold one fp32 scale s per block (the largest magnitude
+// in it) and a code per element: m = s sgn(q) (q / 127)^2 and sqrt(v) = s (q / 255)^2.  The square gives small moments a finer
+// step than large ones (the smallest non-zero one is 6e-5 and 1.5e-5 of the largest), and holding the ROOT of v halves the
+// range that its code has to span; a root above zero keeps a code of at least 1, so no denominator falls to eps because its
+// code did.  The largest magnitude of a block is held exactly, as its scale; the
+// others move with it.
+//
+// The arithmetic between reading and writing 8-bit codes is fp64.  Vector fp64 runs at the rate of vector fp32 on this chip, one
+// Newton step on the hardware's reciprocal root is cheaper than a correctly rounded fp32 root, and a code then does not depend
+// on the order in which a compiler rounds the steps before it.  States of 32 bits are stepped in fp32, by the expressions of
+// the flat-buffer update, whose bits they reproduce.
+#include "common.h"
+
+namespace {
+
+constexpr int BLK = 256;             // elements that share a scale; one wave
+constexpr int WG_BLOCKS = 8;         // blocks per workgroup of four waves
+constexpr int PARTS = 256;           // partial sums of the norm
+
+// A code is the nearest whole number, the lower one of a tie: bf16 gradients from zero states do meet ties (a quarter of the
+// largest magnitude, at 127 / 2), and the margin keeps the fp64 steps' own rounding from deciding them.
+constexpr double HALF = 0.5 - 0x1p-30;
+
+// record of a tensor: parameter, bf16 copy (or 0), elements, first block in the flat moment arrays
+struct Rec { long long p, p16, n, block0; };
+// hyper: lr, beta1, beta2, eps, weight decay, bc1, bc2, max norm, 1 - lr wd, lr / bc1, 1 / sqrt(bc2), 1 - beta1, 1 - beta2
+enum { H_LR, H_B1, H_B2, H_EPS, H_WD, H_BC1, H_BC2, H_MAX, H_DECAY, H_STEP, H_RBC2, H_OMB1, H_OMB2 };
+
+// four gradients from element i of a tensor: fp32, or bf16 where the lowest bit of the address is set
+__device__ __forceinline__ f32x4 load_grad(long long g, size_t i, size_t n) {
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+    if (g & 1) {
+        const bf16_t* s = (const bf16_t*)(g & ~1ll) + i;
+        if (i + 4 <= n && ((uintptr_t)s & 7) == 0) {
+            const bf16x4 t = __builtin_nontemporal_load((const bf16x4*)s);
+            r = f32x4{(float)t[0], (float)t[1], (float)t[2], (float)t[3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (i + e < n) r[e] = (float)s[e];
+        }
+    } else {
+        const float* s = (const float*)g + i;
+        if (i + 4 <= n && ((uintptr_t)s & 15) == 0) r = *(const f32x4*)s;
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (i + e < n) r[e] = s[e];
+        }
+    }
+    return r;
+}
+
+// ---- norm: partial[b] = sum of the squares of a fixed share of the gradients, fp64, in a fixed order --------------------
+__global__ __launch_bounds__(1024) void multi_sumsq_kernel(const Rec* __restrict__ recs, const long long* __restrict__ grads,
+                                                           const int2* __restrict__ map, int n_wg, double* __restrict__ partial) {
+    __shared__ double red[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double acc = 0.0;
+    for (int e = blockIdx.x * 16 + wave; e < n_wg; e += PARTS * 16) {
+        const int2 at = map[e];
+        const long long g = grads[at.x];
+        if (g == 0) continue;
+        const size_t n = (size_t)recs[at.x].n, i0 = (size_t)at.y * BLK + lane * 4;
+        f32x4 v[WG_BLOCKS];
+#pragma unroll
+        for (int u = 0; u < WG_BLOCKS; ++u) {
+            const size_t i = i0 + u * BLK;
+            v[u] = i < n ? load_grad(g, i, n) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int u = 0; u < WG_BLOCKS; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc = fma((double)v[u][k], (double)v[u][k], acc);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o, 64);
+    if (lane == 0) red[wave] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int w = 0; w < 16; ++w) t += red[w];
+        partial[blockIdx.x] = t;
+    }
+}
+
+// every wave sums the partials in the same order
+__device__ __forceinline__ double total_sumsq(const double* __restrict__ partial) {
+    const int lane = threadIdx.x & 63;
+    double t = 0.0;
+#pragma unroll
+    for (int k = 0; k < PARTS / 64; ++k) t += partial[k * 64 + lane];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    return t;
+}
+
+// sqrt(x) to about 2^-45, x >= 0
+__device__ __forceinline__ double root(double x) {
+    const double y = __builtin_amdgcn_rsq(x), h = x * y;
+    const double r = fma(fma(-h, h, x), 0.5 * y, h);
+    return x > 0.0 ? r : 0.0;
+}
+// 1 / s to about 2^-45; 0 for a scale of 0
+__device__ __forceinline__ double inverse(float s) {
+    const double d = (double)s, y = __builtin_amdgcn_rcp(d);
+    return s > 0.f ? fma(fma(-d, y, 1.0), y, y) : 0.0;
+}
+
+__device__ __forceinline__ void store_param(const Rec& t, size_t i, f32x4 p) {
+    float* d = (float*)t.p + i;
+    bf16_t* d16 = (bf16_t*)t.p16 + i;
+    if (i + 4 <= (size_t)t.n && ((uintptr_t)d & 15) == 0) *(f32x4*)d = p;
+    else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (i + e < (size_t)t.n) d[e] = p[e];
+    }
+    if (t.p16) {
+        if (i + 4 <= (size_t)t.n && ((uintptr_t)d16 & 7) == 0)
+            *(bf16x4*)d16 = bf16x4{(bf16_t)p[0], (bf16_t)p[1], (bf16_t)p[2], (bf16_t)p[3]};
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (i + e < (size_t)t.n) d16[e] = (bf16_t)p[e];
+        }
+    }
+}
+__device__ __forceinline__ f32x4 load_param(const Rec& t, size_t i) {
+    const float* s = (const float*)t.p + i;
+    if (i + 4 <= (size_t)t.n && ((uintptr_t)s & 15) == 0) return *(const f32x4*)s;
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (i + e < (size_t)t.n) r[e] = s[e];
+    return r;
+}
+
+// The norm, what it says about the step: false = skip it (state[1] counts).
+__device__ __forceinline__ bool norm_of(const double* __restrict__ partial, float* __restrict__ state, double& norm) {
+    const double sq = total_sumsq(partial);
+    const bool fine = sq <= 3.4028234663852886e38;            // false for NaN; beyond fp32 is where the flat-buffer update skips
+    norm = sqrt(sq);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        state[0] = (float)norm;
+        if (!fine) state[1] += 1.f;
+    }
+    return fine;
+}
+
+#pragma clang fp contract(off)
+__global__ __launch_bounds__(256) void multi_adamw32_kernel(const Rec* __restrict__ recs, const long long* __restrict__ grads,
+                                                            const int2* __restrict__ map, float* __restrict__ m, float* __restrict__ v,
+                                                            const double* __restrict__ partial, const double* __restrict__ hyper,
+                                                            float* __restrict__ state) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double norm;
+    if (!norm_of(partial, state, norm)) return;
+    const int2 at = map[blockIdx.x];
+    const long long g = grads[at.x];
+    if (g == 0) return;
+    const Rec t = recs[at.x];
+    const float lr = (float)hyper[H_LR], b1 = (float)hyper[H_B1], b2 = (float)hyper[H_B2], eps = (float)hyper[H_EPS];
+    const float wd = (float)hyper[H_WD], bc1 = (float)hyper[H_BC1], bc2 = (float)hyper[H_BC2];
+    float scale = 1.f;
+    if (hyper[H_MAX] > 0.0) { const double c = hyper[H_MAX] / (norm + 1e-6); if (c < 1.0) scale = (float)c; }
+    const float decay = fmaf(-lr, wd, 1.f), rbc2 = 1.f / sqrtf(bc2), step = lr / bc1, omb1 = 1.f - b1, omb2 = 1.f - b2;
+#pragma unroll
+    for (int u = 0; u < WG_BLOCKS / 4; ++u) {
+        const size_t i = (size_t)(at.y + u * 4 + wave) * BLK + lane * 4;
+        if (i >= (size_t)t.n) return;
+        float* mp = m + (size_t)t.block0 * BLK + i;
+        float* vp = v + (size_t)t.block0 * BLK + i;
+        f32x4 pv = load_param(t, i), mv = *(const f32x4*)mp, vv = *(const f32x4*)vp;
+        const f32x4 gv = load_grad(g, i, (size_t)t.n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            // the roundings of the flat-buffer update, spelled out: which products fuse is otherwise the compiler's choice per kernel
+            const float gg = gv[e] * scale;
+            const float me = fmaf(omb1, gg, __fmul_rn(b1, mv[e]));
+            const float ve = __fadd_rn(__fmul_rn(b2, vv[e]), __fmul_rn(__fmul_rn(omb2, gg), gg));
+            const float denom = fmaf(sqrtf(ve), rbc2, eps);
+            const float pe = fmaf(decay, pv[e], -__fmul_rn(step, me / denom));
+            pv[e] = pe; mv[e] = me; vv[e] = ve;
+        }
+        *(f32x4*)mp = mv;
+        *(f32x4*)vp = vv;
+        store_param(t, i, pv);
+    }
+}
+
+#pragma clang fp contract(fast)
+__device__ __forceinline__ int sbyte(unsigned w, int e) { return (int)(w << (24 - 8 * e)) >> 24; }
+__device__ __forceinline__ int ubyte(unsigned w, int e) { return (int)((w >> (8 * e)) & 255u); }
+
+__global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict__ recs, const long long* __restrict__ grads,
+                                                           const int2* __restrict__ map, unsigned* __restrict__ m_codes,
+                                                           float* __restrict__ m_scales, unsigned* __restrict__ u_codes,
+                                                           float* __restrict__ u_scales, const double* __restrict__ partial,
+                                                           const double* __restrict__ hyper, float* __restrict__ state) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double norm;
+    if (!norm_of(partial, state, norm)) return;
+    const int2 at = map[blockIdx.x];
+    const long long g = grads[at.x];
+    if (g == 0) return;
+    const Rec t = recs[at.x];
+    const double b1 = hyper[H_B1], b2 = hyper[H_B2], omb1 = hyper[H_OMB1], omb2 = hyper[H_OMB2];
+    const float eps = (float)hyper[H_EPS], decay = (float)hyper[H_DECAY], step = (float)hyper[H_STEP], rbc2 = (float)hyper[H_RBC2];
+    double c = 1.0;
+    if (hyper[H_MAX] > 0.0) { c = hyper[H_MAX] / (norm + 1e-6); if (c > 1.0) c = 1.0; }
+    for (int u = 0; u < WG_BLOCKS / 4; ++u) {
+        const size_t tb = (size_t)(at.y + u * 4 + wave);             // block within the tensor
+        if (tb * BLK >= (size_t)t.n) return;
+        const size_t i = tb * BLK + lane * 4, blk = (size_t)t.block0 + tb, w = blk * (BLK / 4) + lane;
+        const bool in = i < (size_t)t.n;
+        f32x4 pv = {0.f, 0.f, 0.f, 0.f}, gv = pv;
+        if (in) { pv = load_param(t, i); gv = load_grad(g, i, (size_t)t.n); }
+        const unsigned mc = m_codes[w], uc = u_codes[w];
+        const double md = (double)m_scales[blk] * (1.0 / 16129.0), ud = (double)u_scales[blk] * (1.0 / 65025.0);
+        double me[4], ue[4];
+        float mmax = 0.f, umax = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double gg = (double)gv[e] * c;
+            const int qm = sbyte(mc, e), qu = ubyte(uc, e);
+            const double u0 = (double)(qu * qu) * ud;
+            me[e] = b1 * ((double)(qm * abs(qm)) * md) + omb1 * gg;
+            ue[e] = root(b2 * (u0 * u0) + omb2 * (gg * gg));
+            const float mf = (float)me[e], uf = (float)ue[e];
+            mmax = fmaxf(mmax, fabsf(mf));
+            umax = fmaxf(umax, uf);
+            pv[e] = pv[e] * decay - step * (mf / (uf * rbc2 + eps));
+        }
+        if (in) store_param(t, i, pv);
+        mmax = wave_max(mmax);
+        umax = wave_max(umax);
+        // a scale below the normal range is held as 0, with its codes: nothing of that size moves a parameter
+        mmax = mmax >= 0x1p-126f ? mmax : 0.f;
+        umax = umax >= 0x1p-126f ? umax : 0.f;
+        const double rm = inverse(mmax), ru = inverse(umax);
+        unsigned mo = 0, uo = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            int qm = (int)fma(127.0, root(fabs(me[e]) * rm), HALF);
+            int qu = (int)fma(255.0, root(ue[e] * ru), HALF);
+            qm = min(qm, 127);
+            qu = min(qu, 255);
+            if (ue[e] > 0.0 && umax > 0.f) qu = max(qu, 1);
+            if (me[e] < 0.0) qm = -qm;
+            mo |= (unsigned)(qm & 255) << (8 * e);
+            uo |= (unsigned)qu << (8 * e);
+        }
+        m_codes[w] = mo;
+        u_codes[w] = uo;
+        if (lane == 0) { m_scales[blk] = mmax; u_scales[blk] = umax; }
+    }
+}
+
+// the values that 8-bit states stand for, fp32, laid out like the codes
+__global__ __launch_bounds__(256) void moments_kernel(const unsigned* __restrict__ m_codes, const float* __restrict__ m_scales,
+                                                      const unsigned* __restrict__ u_codes, const float* __restrict__ u_scales,
+                                                      size_t words, float* __restrict__ m, float* __restrict__ v) {
+    const size_t w = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (w >= words) return;
+    const unsigned mc = m_codes[w], uc = u_codes[w];
+    const double md = (double)m_scales[w / (BLK / 4)] * (1.0 / 16129.0), ud = (double)u_scales[w / (BLK / 4)] * (1.0 / 65025.0);
+    f32x4 mo, vo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int qm = sbyte(mc, e), qu = ubyte(uc, e);
+        const double u = (double)(qu * qu) * ud;
+        mo[e] = (float)((double)(qm * abs(qm)) * md);
+        vo[e] = (float)(u * u);
+    }
+    *(f32x4*)(m + w * 4) = mo;
+    *(f32x4*)(v + w * 4) = vo;
+}
+
+static bool off16(const void* a) { return ((uintptr_t)a & 15) != 0; }
+
+}  // namespace
+
+extern "C" {
+
+int mi355_multi_adamw_parts(void) { return PARTS; }
+
+int mi355_multi_adamw_step(const long long* recs, const long long* grads, const int* map, int n_wg, int bits, void* m, float* m_scales,
+                           void* v, float* u_scales, double* partial, const double* hyper, float* state, double elements, void* stream) {
+    if (bits != 8 && bits != 32) return mi355_fail(MI355_ERR_ARG, "multi_adamw: states of 8 or 32 bits, not %d", bits);
+    if (n_wg < 0) return mi355_fail(MI355_ERR_ARG, "multi_adamw: negative workgroup count");
+    if (!partial || !hyper || !state || (n_wg > 0 && (!recs || !grads || !map || !m || !v || (bits == 8 && (!m_scales || !u_scales)))))
+        return mi355_fail(MI355_ERR_ARG, "multi_adamw: null pointer");
+    if (off16(m) || off16(v)) return mi355_fail(MI355_ERR_ARG, "multi_adamw: moments not 16-byte aligned");
+    if (n_wg == 0) return MI355_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    ProfScope prof(FAM_ELEM, st, elements * (bits == 8 ? 22.0 : 34.0));
+    hipLaunchKernelGGL(multi_sumsq_kernel, dim3(PARTS), dim3(1024), 0, st, (const Rec*)recs, grads, (const int2*)map, n_wg, partial);
+    if (bits == 32)
+        hipLaunchKernelGGL(multi_adamw32_kernel, dim3(n_wg), dim3(256), 0, st, (const Rec*)recs, grads, (const int2*)map, (float*)m,
+                           (float*)v, partial, hyper, state);
+    else
+        hipLaunchKernelGGL(multi_adamw8_kernel, dim3(n_wg), dim3(256), 0, st, (const Rec*)recs, grads, (const int2*)map, (unsigned*)m,
+                           m_scales, (unsigned*)v, u_scales, partial, hyper, state);
+    return mi355_check_launch("multi_adamw");
+}
+
+int mi355_adamw_moments(const void* m_codes, const float* m_scales, const void* u_codes, const float* u_scales, long long blocks, float* m,
+                        float* v, void* stream) {
+    if (blocks < 0) return mi355_fail(MI355_ERR_ARG, "adamw_moments: negative block count");
+    if (blocks == 0) return MI355_OK;
+    if (!m_codes || !m_scales || !u_codes || !u_scales || !m || !v) return mi355_fail(MI355_ERR_ARG, "adamw_moments: null pointer");
+    if (off16(m) || off16(v)) return mi355_fail(MI355_ERR_ARG, "adamw_moments: outputs not 16-byte aligned");
+    if (blocks > (1ll << 31)) return mi355_fail(MI355_ERR_ARG, "adamw_moments: more than 2^31 blocks");
+    const size_t words = (size_t)blocks * (BLK / 4);
+    hipLaunchKernelGGL(moments_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, (hipStream_t)stream, (const unsigned*)m_codes,
+                       m_scales, (const unsigned*)u_codes, u_scales, words, m, v);
+    return mi355_check_launch("adamw_moments");
+}
+
+}  // extern "C"

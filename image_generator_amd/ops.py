@@ -611,6 +611,57 @@ def attention_bwd(q, k, v, o, do, lse, heads, dq, dk, dv):
                                   _stream()), "attention_bwd")
 
 
+def _here(*tensors):
+    """Operands of one launch: all on the current device (a launch goes to its stream)."""
+    dev = torch.cuda.current_device() if tensors[0].is_cuda else None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("HIP device tensors required (no CPU path)")
+        if t.device.index != dev:
+            raise RuntimeError(f"a tensor on {t.device}, the current device is {dev}")
+
+
+def _ids(ids):
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"embedding: ids must be int32 or int64, got {ids.dtype}")
+    return ids.contiguous()
+
+
+def embedding_fwd(ids, table, scale=1.0, out_dtype=BF16):
+    """scale * table[ids]: ids int32 / int64 of any shape, table [rows, width] fp32 or bf16; out bf16 or fp32.  An id outside
+    the table reads as a NaN row (ids are on the device, nothing waits for them)."""
+    _here(table, ids)
+    if table.dim() != 2 or table.dtype not in (F32, BF16) or not table.is_contiguous():
+        raise RuntimeError("embedding: the table must be a contiguous fp32 or bf16 matrix")
+    if out_dtype not in (F32, BF16):
+        raise RuntimeError(f"embedding: outputs are fp32 or bf16, not {out_dtype}")
+    ids = _ids(ids)
+    out = torch.empty((*ids.shape, table.shape[1]), dtype=out_dtype, device=table.device)
+    check(lib.mi355_embedding_fwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(), table.data_ptr(), table.dtype == BF16,
+                                  table.shape[0], table.shape[1], scale, out.data_ptr(), out_dtype == BF16, _stream()),
+          "embedding_fwd")
+    return out
+
+
+def embedding_bwd(ids, dy, rows, scale=1.0, out_dtype=F32):
+    """Gradient [rows, width] of the table of `embedding_fwd`: scale times the sum of the dy rows of each id, in the order of
+    the positions (same call, same bits)."""
+    _here(dy, ids)
+    if dy.dtype not in (F32, BF16) or out_dtype not in (F32, BF16):
+        raise RuntimeError("embedding_bwd: gradients are fp32 or bf16")
+    if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape:
+        raise RuntimeError(f"embedding_bwd: gradient {tuple(dy.shape)} of ids {tuple(ids.shape)}")
+    ids, dy = _ids(ids), dy.contiguous()
+    width = dy.shape[-1]
+    ws = torch.empty(int(lib.mi355_embedding_bwd_workspace_bytes(ids.numel(), rows, width)), dtype=torch.uint8, device=dy.device)
+    out = torch.empty((rows, width), dtype=out_dtype, device=dy.device)
+    check(lib.mi355_embedding_bwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(), dy.data_ptr(), dy.dtype == BF16, rows, width,
+                                  scale, out.data_ptr(), out_dtype == BF16, ws.data_ptr(), ws.numel(), _stream()), "embedding_bwd")
+    return out
+
+
 def gelu_bf16(x):
     y = torch.empty_like(x)
     check(lib.mi355_gelu_bf16(x.data_ptr(), y.data_ptr(), x.numel(), _stream()), "gelu")
@@ -1217,6 +1268,26 @@ class AttentionFn(torch.autograd.Function):
         dq, dk, dv = AttentionFn._split(da, db, dc)
         attention_bwd(q, k, v, o, do, lse, ctx.heads, dq, dk, dv)
         return da, db, dc, None
+
+
+class EmbeddingFn(torch.autograd.Function):
+    """scale * table[ids], the gradient as one dense table (encoder/text_encoder.py:27)."""
+
+    @staticmethod
+    def forward(ctx, ids, table, scale, out_dtype):
+        ctx.save_for_backward(ids)
+        ctx.meta = (table.shape[0], scale, table.dtype)
+        return embedding_fwd(ids, table, scale, out_dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        rows, scale, dtype = ctx.meta
+        return None, embedding_bwd(ids, dy, rows, scale, dtype), None, None
+
+
+def embedding(ids, table, scale=1.0, out_dtype=BF16):
+    return EmbeddingFn.apply(ids, table, scale, out_dtype)
 
 
 class GegluFn(torch.autograd.Function):

@@ -420,6 +420,40 @@ int mi355_lora_pack(const long long* table, int n, void* stream);
 /* n records {src, dst, rows, cols, src_ld, dst_ld} (int64, device memory): dst[r][c] = src[r][c], fp32. */
 int mi355_copy2d_f32_batched(const long long* table, int n, void* stream);
 
+/* ---- embedding rows (nn.Embedding of encoder/text_encoder.py:14,27) and the gradient of their table -----------------------
+ * fwd: out[i][:] = scale * table[ids[i]][:], i < n; table [rows][width] and out [n][width] fp32 or bf16.
+ * bwd: dtable[v][:] = scale * sum of dy[i][:] over ids[i] = v in ascending i (fp32 sums, rounded once); every row of dtable is
+ * written, zeros where no id names it.  The order depends on the ids alone: equal calls return equal bits.
+ * ids: int32, or int64 (ids64 != 0).  An id outside [0, rows) reads as a NaN row and adds to no gradient.  ws: a device
+ * buffer of mi355_embedding_bwd_workspace_bytes(n, rows, width), 16-byte aligned, for this call alone.
+ * Limits: n, rows <= 2^30, width <= 2^20, n * width < 2^32. */
+int mi355_embedding_fwd(const void* ids, int ids64, long long n, const void* table, int table_bf16, long long rows, int width,
+                        float scale, void* out, int out_bf16, void* stream);
+size_t mi355_embedding_bwd_workspace_bytes(long long n, long long rows, int width);
+int mi355_embedding_bwd(const void* ids, int ids64, long long n, const void* dy, int dy_bf16, long long rows, int width, float scale,
+                        void* dtable, int out_bf16, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- AdamW over many tensors (train_encoder.py:42-49,109 `optimizer.step()`) ------------------------------------------------
+ * One launch for the norm of all gradients (fp64, fixed order), one for the update of all tensors, with the clip factor
+ * min(1, max_norm / (norm + 1e-6)) and the bf16 operand copies.  A step whose gradients' sum of squares is not a finite fp32
+ * number changes nothing but the skip count.
+ * recs: per tensor {parameter (fp32), bf16 copy or 0, elements, first block} (int64, device memory), a block being 256
+ * elements and a tensor's blocks following each other in the moment arrays (the last one padded).
+ * grads: per tensor the gradient's address, fp32, or bf16 with the lowest bit set; 0 leaves the tensor alone.
+ * map: per workgroup {tensor, first block within it} (int32), eight blocks each, n_wg of them covering every tensor.
+ * bits 32: m, v fp32 arrays.  bits 8: m int8 codes, v uint8 codes of its root, fp32 scales per block (csrc/multi_adamw.hip
+ * states what a code stands for).  partial: mi355_multi_adamw_parts() doubles of scratch.
+ * hyper (doubles): lr, beta1, beta2, eps, weight decay, 1 - beta1^t, 1 - beta2^t, max norm (<= 0: no clipping), 1 - lr wd,
+ * lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - beta1, 1 - beta2.  state (floats): [0] = norm, [1] += 1 when skipped.
+ * `elements`: how many in all, for the launch timing only. */
+int mi355_multi_adamw_parts(void);
+int mi355_multi_adamw_step(const long long* recs, const long long* grads, const int* map, int n_wg, int bits, void* m,
+                           float* m_scales, void* v, float* u_scales, double* partial, const double* hyper, float* state,
+                           double elements, void* stream);
+/* What 8-bit states stand for: m and v as fp32 arrays of 256 * blocks elements. */
+int mi355_adamw_moments(const void* m_codes, const float* m_scales, const void* u_codes, const float* u_scales, long long blocks,
+                        float* m, float* v, void* stream);
+
 /* ---- data plane: read-only LMDB (dataset.py:173-183,213-216; the file format make_lmdb.py:39-75 writes) ------------
  * Host code, no GPU.  liblmdb is not a dependency: the environment's data.mdb is mapped and its B+tree walked in place.
  * open: `path` is the environment directory (with data.mdb) or the data file; NULL + mi355_last_error() on failure.
