@@ -623,6 +623,74 @@ def _here(*tensors):
             raise RuntimeError(f"a tensor on {t.device}, the current device is {dev}")
 
 
+def _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed):
+    """Checks shared by the two directions of the document attention; (leading arguments, trailing arguments, sizes)."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    k_offsets = q_offsets if k_offsets is None else k_offsets
+    _here(q, k, v, q_offsets, k_offsets, prefix, slopes)
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"doc_attention: {heads} query heads on {kv_heads} key heads")
+    for name, t, h in (("q", q, heads), ("k", k, kv_heads), ("v", v, kv_heads)):
+        if t.dim() != 2 or t.dtype != BF16 or t.stride(1) != 1 and t.shape[1] > 1:
+            raise RuntimeError(f"doc_attention: {name} must be a bf16 matrix [tokens, heads * width] with adjacent columns")
+        if t.shape[1] % h or t.shape[1] // h != q.shape[1] // heads:
+            raise ValueError(f"doc_attention: {name} {tuple(t.shape)} for {h} heads of width {q.shape[1] // heads}")
+    if k.shape[0] != v.shape[0]:
+        raise ValueError(f"doc_attention: {k.shape[0]} keys, {v.shape[0]} values")
+    docs = q_offsets.numel() - 1
+    for name, t, n, dt in (("q_offsets", q_offsets, docs + 1, torch.int32), ("k_offsets", k_offsets, docs + 1, torch.int32),
+                           ("prefix", prefix, docs, torch.int32), ("slopes", slopes, heads, F32)):
+        if t is not None and (t.dtype != dt or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"doc_attention: {name} must be {n} contiguous {dt} values, got {t.numel()} {t.dtype}")
+    if docs < 1:
+        raise ValueError("doc_attention: offsets hold at least two entries")
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("doc_attention: no gradient reaches the slopes (detach them)")
+    if align not in ("end", "start"):
+        raise ValueError(f"doc_attention: align {align!r} is neither 'end' nor 'start'")
+    D = q.shape[1] // heads
+    head = (q_offsets.data_ptr(), k_offsets.data_ptr(), docs, _ptr(prefix), _ptr(slopes), cap or 0.0, causal, align == "start")
+    return head, (1.0 / math.sqrt(D) if scale is None else scale, drop_p, seed), (q.shape[0], k.shape[0], heads, kv_heads, D)
+
+
+def doc_attention_fwd(q, k, v, heads, q_offsets, k_offsets=None, kv_heads=None, causal=False, prefix=None, slopes=None, cap=0.0,
+                      scale=None, align="end", drop_p=0.0, seed=0):
+    """Attention over packed documents: q [Tq, heads * d], k / v [Tk, kv_heads * d] bf16 (row stride any multiple of 8); document
+    n owns the rows q_offsets[n]:q_offsets[n + 1] and the keys k_offsets[n]:k_offsets[n + 1] (int32 on the device; one list
+    if `k_offsets` is None).  Query i sits over key c, counted from the documents' ends (`align="end"`: appended queries) or
+    their starts, and sees its document's keys; with `causal` those up to c and the document's first `prefix[n]`.  `cap`:
+    scores become cap tanh(s / cap); `slopes` [heads]: minus slope times |c - j|.  Returns (out [Tq, heads * d],
+    lse [heads, Tq]); a query that sees nothing gets zeros and -inf."""
+    head, tail, sizes = _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed)
+    out = torch.empty(q.shape, dtype=BF16, device=q.device)
+    lse = torch.empty((heads, q.shape[0]), dtype=F32, device=q.device)
+    ws = torch.empty(int(lib.mi355_doc_attention_fwd_workspace_bytes(*sizes)), dtype=torch.uint8, device=q.device)
+    check(lib.mi355_doc_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *head, *sizes,
+                                      q.stride(0), k.stride(0), v.stride(0), out.stride(0), *tail, ws.data_ptr(), ws.numel(), _stream()),
+          "doc_attention_fwd")
+    return out, lse
+
+
+def doc_attention_bwd(do, q, k, v, o, lse, heads, q_offsets, k_offsets=None, kv_heads=None, causal=False, prefix=None, slopes=None,
+                      cap=0.0, scale=None, align="end", drop_p=0.0, seed=0, dq=None, dk=None, dv=None):
+    """(dq, dk, dv) of `doc_attention_fwd` for the gradient `do` of its output; `o`, `lse` are what it returned.  dq / dk / dv:
+    bf16 matrices to write (slices of one buffer, say); new ones by default."""
+    head, tail, sizes = _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed)
+    _here(do, o, lse, dq, dk, dv)
+    dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=q.device) if d is None else d for t, d in ((q, dq), (k, dk), (v, dv)))
+    for name, t, like in (("do", do, q), ("o", o, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if t.shape != like.shape or t.dtype != BF16 or t.stride(1) != 1 and t.shape[1] > 1:
+            raise RuntimeError(f"doc_attention_bwd: {name} must be a bf16 matrix {tuple(like.shape)} with adjacent columns")
+    if lse.shape != (heads, q.shape[0]) or lse.dtype != F32 or not lse.is_contiguous():
+        raise RuntimeError("doc_attention_bwd: lse is not the forward pass's")
+    ws = torch.empty(int(lib.mi355_doc_attention_bwd_workspace_bytes(q.shape[0], heads)), dtype=torch.uint8, device=q.device)
+    check(lib.mi355_doc_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+                                      dk.data_ptr(), dv.data_ptr(), *head, *sizes, q.stride(0), k.stride(0), v.stride(0), o.stride(0),
+                                      do.stride(0), dq.stride(0), dk.stride(0), dv.stride(0), *tail, ws.data_ptr(), ws.numel(), _stream()),
+          "doc_attention_bwd")
+    return dq, dk, dv
+
+
 def _ids(ids):
     if ids.dtype not in (torch.int32, torch.int64):
         raise RuntimeError(f"embedding: ids must be int32 or int64, got {ids.dtype}")
@@ -1268,6 +1336,48 @@ class AttentionFn(torch.autograd.Function):
         dq, dk, dv = AttentionFn._split(da, db, dc)
         attention_bwd(q, k, v, o, do, lse, ctx.heads, dq, dk, dv)
         return da, db, dc, None
+
+
+class DocAttentionFn(torch.autograd.Function):
+    """Attention over packed documents.  The operand layouts of `AttentionFn`, as matrices: a = [q | k | v] (b = c = None),
+    a = q and b = [k | v] (c = None), or three tensors; gradients come back in the same layout."""
+
+    @staticmethod
+    def _split(a, b, c, heads, kv_heads):
+        if b is None:
+            d = a.shape[1] // (heads + 2 * kv_heads)
+            return a[:, :heads * d], a[:, heads * d:(heads + kv_heads) * d], a[:, (heads + kv_heads) * d:]
+        if c is None:
+            half = b.shape[1] // 2
+            return a, b[:, :half], b[:, half:]
+        return a, b, c
+
+    @staticmethod
+    def forward(ctx, a, b, c, heads, kv_heads, how, q_offsets, k_offsets, prefix, slopes):
+        q, k, v = DocAttentionFn._split(a, b, c, heads, kv_heads)
+        o, lse = doc_attention_fwd(q, k, v, heads, q_offsets, k_offsets, kv_heads, prefix=prefix, slopes=slopes, **how)
+        ctx.save_for_backward(a, b, c, o, lse, q_offsets, k_offsets, prefix, slopes)
+        ctx.meta = (heads, kv_heads, how)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        a, b, c, o, lse, q_offsets, k_offsets, prefix, slopes = ctx.saved_tensors
+        heads, kv_heads, how = ctx.meta
+        da, db, dc = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (a, b, c))
+        q, k, v = DocAttentionFn._split(a, b, c, heads, kv_heads)
+        dq, dk, dv = DocAttentionFn._split(da, db, dc, heads, kv_heads)
+        doc_attention_bwd(do.contiguous(), q, k, v, o, lse, heads, q_offsets, k_offsets, kv_heads, prefix=prefix, slopes=slopes, dq=dq, dk=dk,
+                          dv=dv, **how)
+        return da, db, dc, None, None, None, None, None, None, None
+
+
+def doc_attention(a, b=None, c=None, *, heads, q_offsets, k_offsets=None, kv_heads=None, prefix=None, slopes=None, **how):
+    """Differentiable `doc_attention_fwd` (out only).  Operands: [q | k | v], or q and [k | v], or q, k and v."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("doc_attention: no gradient reaches the slopes (detach them)")
+    return DocAttentionFn.apply(a, b, c, heads, kv_heads, how, q_offsets, k_offsets, prefix, slopes)
 
 
 class EmbeddingFn(torch.autograd.Function):

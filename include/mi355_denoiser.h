@@ -420,6 +420,33 @@ int mi355_lora_pack(const long long* table, int n, void* stream);
 /* n records {src, dst, rows, cols, src_ld, dst_ld} (int64, device memory): dst[r][c] = src[r][c], fp32. */
 int mi355_copy2d_f32_batched(const long long* table, int n, void* stream);
 
+/* ---- attention over packed documents ---------------------------------------------------------------------------------------
+ * The text encoder's attention (encoder/text_encoder.py:16-23,31-34) without padding rows: tokens of many documents one behind
+ * another, q [Tq][Hq*D], k / v [Tk][Hkv*D] bf16 (row strides ld*, multiples of 8; all bases 16-byte aligned).  Document n holds
+ * the queries q_off[n] .. q_off[n+1]-1 and the keys k_off[n] .. k_off[n+1]-1 (int32, docs + 1 entries, ascending, on the device).
+ * Query i sits at key position c = i - q_end + k_end (align_start: i - q_begin + k_begin) and sees the keys j of its document,
+ * with `causal` those with j <= c or j < k_begin + prefix[n] (prefix: int32 [docs] or NULL):
+ *   t = scale q.k;  t = cap tanh(t / cap) if cap > 0;  score = t - slopes[head] |c - j|;  out = softmax(score) v
+ * slopes: fp32 [Hq] or NULL.  Hq is a multiple of Hkv; query head h reads key head h / (Hq / Hkv).  D: a multiple of 8, <= 128.
+ * A query that sees no key, or belongs to no document, gets a row of zeros and lse = -infinity; keys of no document get zero
+ * gradients.  What a query does not see never reaches its result, infinities and NaN included.  lse [Hq][Tq] in log2 units.
+ * drop_p, seed: dropout on the probabilities, the same in both directions for the same seed.
+ * Everything is summed in an order that depends on the sizes alone: equal calls return equal bits.  ws: a device buffer of the
+ * queried size, 16-byte aligned, for this call alone. */
+size_t mi355_doc_attention_fwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D);
+int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int* q_off, const int* k_off,
+                            int docs, const int* prefix, const float* slopes, float cap, int causal, int align_start, int Tq,
+                            int Tk, int Hq, int Hkv, int D, long long ldq, long long ldk, long long ldv, long long ldo,
+                            float scale, float drop_p, unsigned seed, void* ws, size_t ws_bytes, void* stream);
+/* o, lse: the forward pass's; dout like o with its own row stride lddo.  dq, dk, dv are written whole. */
+size_t mi355_doc_attention_bwd_workspace_bytes(int Tq, int Hq);
+int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq,
+                            void* dk, void* dv, const int* q_off, const int* k_off, int docs, const int* prefix,
+                            const float* slopes, float cap, int causal, int align_start, int Tq, int Tk, int Hq, int Hkv, int D,
+                            long long ldq, long long ldk, long long ldv, long long ldo, long long lddo, long long lddq,
+                            long long lddk, long long lddv, float scale, float drop_p, unsigned seed, void* ws,
+                            size_t ws_bytes, void* stream);
+
 /* ---- embedding rows (nn.Embedding of encoder/text_encoder.py:14,27) and the gradient of their table -----------------------
  * fwd: out[i][:] = scale * table[ids[i]][:], i < n; table [rows][width] and out [n][width] fp32 or bf16.
  * bwd: dtable[v][:] = scale * sum of dy[i][:] over ids[i] = v in ascending i (fp32 sums, rounded once); every row of dtable is

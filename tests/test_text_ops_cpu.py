@@ -38,3 +38,35 @@ def test_optimizer_refusals():
     assert step(32, 0, 16, None) == 0
     assert lib.mi355_adamw_moments(16, 16, 16, 16, -1, 16, 16, None) == -1
     assert lib.mi355_adamw_moments(16, 16, 16, 16, 4, 8, 16, None) == -1 and lib.mi355_adamw_moments(None, 16, 16, 16, 4, 16, 16, None) == -1
+
+
+def test_doc_attention_refusals():
+    from image_generator_amd import ops
+    from image_generator_amd._lib import lib
+    q, off = torch.zeros(4, 64, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.doc_attention_fwd(q, q, q, heads=2, q_offsets=off)
+    with pytest.raises(RuntimeError, match="slopes"):
+        ops.doc_attention(q, q, q, heads=2, q_offsets=off, slopes=torch.ones(2, requires_grad=True))
+    err = lambda: lib.mi355_last_error().decode()  # noqa: E731
+
+    def fwd(docs=1, prefix=None, cap=0.0, causal=0, Tq=4, Tk=4, Hq=2, Hkv=2, D=32, ld=64, ldo=64, drop=0.0, ptr=16, ws=16, ws_bytes=1 << 30, off=16):
+        return lib.mi355_doc_attention_fwd(ptr, ptr, ptr, ptr, 16, off, off, docs, prefix, None, cap, causal, 0, Tq, Tk, Hq, Hkv, D, ld, ld, ld, ldo,
+                                           1.0, drop, 0, ws, ws_bytes, None)
+
+    for kw, why in ((dict(docs=0), "document"), (dict(Tq=-1), "document"), (dict(Hq=3), "multiple"), (dict(D=36), "multiple of 8"),
+                    (dict(D=136), "128"), (dict(prefix=16), "prefix"), (dict(cap=-1.0), "cap"), (dict(cap=float("nan")), "cap"),
+                    (dict(drop=1.0), "dropout"), (dict(ld=60), "strides"), (dict(ldo=32), "strides"), (dict(ptr=8), "aligned"),
+                    (dict(ptr=None), "null"), (dict(off=None), "null"), (dict(ws=None), "workspace"), (dict(ws_bytes=0), "workspace"),
+                    (dict(Tq=1 << 30), "2^31"), (dict(ld=-64), "strides")):
+        assert fwd(**kw) == -1 and why in err(), (kw, err())
+    assert fwd(Tq=0) == 0
+
+    def bwd(ld=64, ldd=64, ptr=16, ws=16, ws_bytes=1 << 30, prefix=None):
+        return lib.mi355_doc_attention_bwd(ptr, ptr, ptr, ptr, ptr, 16, ptr, ptr, ptr, 16, 16, 1, prefix, None, 0.0, 0, 0, 4, 4, 2, 2, 32, ld, ld,
+                                           ld, ld, ld, ldd, ldd, ldd, 1.0, 0.0, 0, ws, ws_bytes, None)
+
+    for kw, why in ((dict(ld=4), "strides"), (dict(ldd=32), "overlap"), (dict(ptr=24), "aligned"), (dict(ptr=None), "null"),
+                    (dict(ws_bytes=8), "workspace"), (dict(prefix=16), "prefix")):
+        assert bwd(**kw) == -1 and why in err(), (kw, err())
+    assert lib.mi355_doc_attention_bwd_workspace_bytes(-1, 2) == 0 and lib.mi355_doc_attention_fwd_workspace_bytes(4, 4, 3, 2, 32) == 0
