@@ -1,34 +1,7 @@
-// Attention over packed documents: entry points, and the kernels that give every row (key) a wave of its own.
-#include "doc_attention.h"
+// Attention over packed documents: entry points.
+#include "doc_tiles.h"
 
 namespace {
-
-__global__ __launch_bounds__(256) void rows_fwd_kernel(const DocArgs p) {
-    const size_t r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= (size_t)p.Tq * p.Hq) return;
-    const int i = (int)(r / p.Hq), head = (int)(r % p.Hq);
-    plain_row_out(p, i, head, row_span(p, i));
-}
-
-__global__ __launch_bounds__(256) void rows_dq_kernel(const DocArgs p) {
-    const size_t r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= (size_t)p.Tq * p.Hq) return;
-    const int i = (int)(r / p.Hq), head = (int)(r % p.Hq);
-    const RowSpan s = row_span(p, i);
-    const float delta = plain_delta(p, i, head);
-    const size_t at = (size_t)head * p.Tq + i;
-    plain_dq_row(p, i, head, s, p.lse[at], delta);
-    if ((threadIdx.x & 63) == 0) {
-        p.delta[at] = delta;
-        if (head == 0) p.rows[i] = make_int4(s.lo, s.hi, s.c, 0);
-    }
-}
-
-__global__ __launch_bounds__(256) void keys_dkdv_kernel(const DocArgs p) {
-    const size_t r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= (size_t)p.Tk * p.Hkv) return;
-    plain_dkdv_key(p, (int)(r / p.Hkv), (int)(r % p.Hkv));
-}
 
 static const char* bad_sizes(int docs, int Tq, int Tk, int Hq, int Hkv, int D) {
     if (docs < 1 || Tq < 0 || Tk < 0) return "no document, or a negative number of tokens";
@@ -38,14 +11,15 @@ static const char* bad_sizes(int docs, int Tq, int Tk, int Hq, int Hkv, int D) {
     return nullptr;
 }
 static bool off16(const void* a) { return ((uintptr_t)a & 15) != 0; }
-static bool bad_ld(long long ld) { return ld < 0 || ld % 8 != 0 || ld > (1 << 24); }
+static bool bad_ld(long long ld) { return ld < 0 || ld % 8 != 0 || ld > (1 << 23); }
 
 static int fill(DocArgs& a, const char* who, int docs, int Tq, int Tk, int Hq, int Hkv, int D, const int* q_off, const int* k_off,
                 const int* prefix, const float* slopes, float cap, int causal, int align_start, float scale, float drop_p, unsigned seed) {
     if (const char* why = bad_sizes(docs, Tq, Tk, Hq, Hkv, D)) return mi355_fail(MI355_ERR_ARG, "%s: %s", who, why);
     if (!q_off || !k_off) return mi355_fail(MI355_ERR_ARG, "%s: null pointer", who);
     if (prefix && !causal) return mi355_fail(MI355_ERR_ARG, "%s: a prefix without the causal mask it lifts", who);
-    if (!(cap >= 0.f) || !(cap < 1e30f)) return mi355_fail(MI355_ERR_ARG, "%s: cap %g", who, (double)cap);
+    // the tanh is 1 - 2 / (1 + 2^x), good to 2^-22 of the cap: 2^-12 of a nat at the limit
+    if (!(cap >= 0.f) || !(cap <= 1024.f)) return mi355_fail(MI355_ERR_ARG, "%s: cap %g, not between 0 (none) and 1024", who, (double)cap);
     if (!(drop_p >= 0.f && drop_p < 1.f)) return mi355_fail(MI355_ERR_ARG, "%s: dropout %g", who, (double)drop_p);
     a.docs = docs; a.Tq = Tq; a.Tk = Tk; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.D = D;
     a.q_off = q_off; a.k_off = k_off; a.prefix = prefix; a.slopes = slopes;
@@ -63,7 +37,7 @@ extern "C" {
 
 size_t mi355_doc_attention_fwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D) {
     if (bad_sizes(1, Tq, Tk, Hq, Hkv, D)) return 0;
-    return 16;
+    return doc_fwd_workspace(Tq, Tk, Hq, Hkv, D);
 }
 
 int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int* q_off, const int* k_off, int docs,
@@ -76,15 +50,15 @@ int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* o
     if (!q || !out || !lse || (Tk > 0 && (!k || !v))) return mi355_fail(MI355_ERR_ARG, "doc_attention: null pointer");
     if (off16(q) || off16(k) || off16(v) || off16(out)) return mi355_fail(MI355_ERR_ARG, "doc_attention: operands not 16-byte aligned");
     if (bad_ld(ldq) || bad_ld(ldk) || bad_ld(ldv) || bad_ld(ldo) || ldo < (long long)Hq * D)
-        return mi355_fail(MI355_ERR_ARG, "doc_attention: row strides must be multiples of 8, at most 2^24");
+        return mi355_fail(MI355_ERR_ARG, "doc_attention: row strides must be multiples of 8, at most 2^23");
     const size_t need = mi355_doc_attention_fwd_workspace_bytes(Tq, Tk, Hq, Hkv, D);
     if (!ws || ws_bytes < need || off16(ws)) return mi355_fail(MI355_ERR_ARG, "doc_attention: workspace of %zu bytes, %zu needed, 16-byte aligned", ws ? ws_bytes : 0, need);
     a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.out = (bf16_t*)out; a.lse = lse;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
     const hipStream_t st = (hipStream_t)stream;
     ProfScope prof(FAM_ATTN, st, 4.0 * Tq * (double)Tk / docs * Hq * D);
-    hipLaunchKernelGGL(rows_fwd_kernel, dim3((unsigned)(((size_t)Tq * Hq + 3) / 4)), dim3(256), 0, st, a);
-    return mi355_check_launch("doc_attention_fwd");
+    a.part = (float*)ws;
+    return doc_fwd_tiles(a, st);
 }
 
 size_t mi355_doc_attention_bwd_workspace_bytes(int Tq, int Hq) {
@@ -105,7 +79,7 @@ int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const v
     if (off16(q) || off16(k) || off16(v) || off16(o) || off16(dout) || off16(dq) || off16(dk) || off16(dv))
         return mi355_fail(MI355_ERR_ARG, "doc_attention_bwd: operands not 16-byte aligned");
     if (bad_ld(ldq) || bad_ld(ldk) || bad_ld(ldv) || bad_ld(ldo) || bad_ld(lddo) || bad_ld(lddq) || bad_ld(lddk) || bad_ld(lddv))
-        return mi355_fail(MI355_ERR_ARG, "doc_attention_bwd: row strides must be multiples of 8, at most 2^24");
+        return mi355_fail(MI355_ERR_ARG, "doc_attention_bwd: row strides must be multiples of 8, at most 2^23");
     if (lddq < (long long)Hq * D || lddk < (long long)Hkv * D || lddv < (long long)Hkv * D)
         return mi355_fail(MI355_ERR_ARG, "doc_attention_bwd: rows of a gradient overlap");
     const size_t need = mi355_doc_attention_bwd_workspace_bytes(Tq, Hq);
@@ -117,9 +91,8 @@ int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const v
     a.delta = (float*)((char*)ws + (size_t)Tq * 16);
     const hipStream_t st = (hipStream_t)stream;
     ProfScope prof(FAM_ATTN, st, 10.0 * Tq * (double)Tk / docs * Hq * D);
-    if (Tq > 0) hipLaunchKernelGGL(rows_dq_kernel, dim3((unsigned)(((size_t)Tq * Hq + 3) / 4)), dim3(256), 0, st, a);
-    if (Tk > 0) hipLaunchKernelGGL(keys_dkdv_kernel, dim3((unsigned)(((size_t)Tk * Hkv + 3) / 4)), dim3(256), 0, st, a);
-    return mi355_check_launch("doc_attention_bwd");
+    if (Tq > 0) if (const int rc = doc_bwd_q_tiles(a, st)) return rc;
+    return Tk > 0 ? doc_bwd_kv_tiles(a, st) : MI355_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,179 @@
+// Document attention, dQ, on the matrix units: a lane owns its row as in the forward pass, S^T = K Q^T and dP^T = V dO^T give
+// dS^T in the layout that dQ^T += K^T dS^T takes.  delta = sum dO o of a row, and the row's interval, are left for the dK / dV
+// pass.
+#include "doc_tiles.h"
+
+namespace {
+
+template <int ND, int NO, int KIND>
+__global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p) {
+    constexpr int DP = 16 * ND, KLD = tr_ld(NO), VLD = DP * 2 + 16;
+    constexpr int NCK = (64 * NO * 4 + 255) / 256, NCV = (64 * (DP / 8) + 255) / 256;
+    __shared__ __attribute__((aligned(16))) char smem[64 * KLD + 64 * VLD];
+    __shared__ int range[4][2];
+    char *Ks = smem, *Vs = smem + 64 * KLD;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
+    const int hk = blockIdx.y;
+    const unsigned R = blockIdx.x * 128u + wave * 32 + l31;
+    const bool live = R < (unsigned)p.Tq * (unsigned)p.G;
+    int token, head;
+    row_of(p, live ? R : 0u, hk, token, head);
+    RowSpan span = row_span(p, token);
+    if (live && hh == 0 && head == 0) p.rows[token] = make_int4(span.lo, span.hi, span.c, 0);
+    if (!live) span.lo = span.hi = 0;
+    const bool sees = span.hi > span.lo;
+    const int lo = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.lo : 0x7fffffff));
+    const int hi = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.hi : 0));
+    const int in_lo = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.lo : 0));
+    const int in_hi = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.hi : 0x7fffffff));
+    const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
+    bf16x8 qf[ND], gf[ND];
+    float delta = 0.f;
+    {
+        const bf16_t* q = q_row(p, token, head);
+        const bf16_t* g = p.dout + (size_t)token * p.lddo + (size_t)head * p.D;
+        const bf16_t* o = p.o + (size_t)token * p.ldo + (size_t)head * p.D;
+#pragma unroll
+        for (int ks = 0; ks < ND; ++ks) {
+            const int d = ks * 16 + 8 * hh;
+            const bool ok = sees && d < p.D;
+            qf[ks] = ok ? *(const bf16x8*)(q + d) : zero8;
+            gf[ks] = ok ? *(const bf16x8*)(g + d) : zero8;
+            const bf16x8 ov = ok ? *(const bf16x8*)(o + d) : zero8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = fmaf((float)ov[e], (float)gf[ks][e], delta);
+        }
+        delta += __shfl_xor(delta, 32, 64);
+    }
+    const size_t at = (size_t)head * p.Tq + token;
+    if (live && hh == 0) p.delta[at] = delta;
+    const float lse_raw = sees ? p.lse[at] : -INFINITY;
+    const float lse = lse_raw == -INFINITY ? INFINITY : lse_raw;      // nothing seen: probabilities of 0
+    const float slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;
+    const unsigned drop = drop_row(p, token, head);
+    const Bend bend(p);
+
+    if (lane == 0) { range[wave][0] = lo; range[wave][1] = hi; }
+    __syncthreads();
+    const int klo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
+    const int khi = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
+    f32x16 dqT[NO];
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dqT[i][r] = 0.f;
+    const int tr_row = 4 * hh + ((lane & 15) >> 2);
+    int tr_c0, tr_c1;
+    tr_cols_swz(lane, tr_c0, tr_c1);
+    const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
+    bf16x8 kreg[NCK], vreg[NCV];
+    Fetch<NCK, NO * 4> kf;
+    Fetch<NCV, DP / 8> vf;
+    kf.init(threadIdx.x, p.ldk, p.D);
+    vf.init(threadIdx.x, p.ldv, p.D);
+    if (klo < khi) {
+        kf.load(kreg, kbase, p.ldk, p.D, klo, khi - klo);
+        vf.load(vreg, vbase, p.ldv, p.D, klo, khi - klo);
+    }
+    for (int k0 = klo; k0 < khi; k0 += 64) {
+        __syncthreads();
+        put_tile<NCK, NO * 4, true>(kreg, Ks, KLD, threadIdx.x);
+        put_tile<NCV, DP / 8, false>(vreg, Vs, VLD, threadIdx.x);
+        __syncthreads();
+        if (k0 + 64 < khi) {
+            kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, khi - k0 - 64);
+            vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, khi - k0 - 64);
+        }
+        if (k0 >= hi || k0 + 64 <= lo) continue;
+        const bool masked = k0 < in_lo || k0 + 64 > in_hi;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+            for (int ks = 0; ks < ND; ++ks) {
+                const bf16x8 ak = *(const bf16x8*)(Ks + (kb * 32 + l31) * KLD + ((ks * 2 + hh) ^ ((l31 >> 2) & 3)) * 16);
+                const bf16x8 av = *(const bf16x8*)(Vs + (kb * 32 + l31) * VLD + (ks * 16 + 8 * hh) * 2);
+                s = mfma(ak, qf[ks], s);
+                dp = mfma(av, gf[ks], dp);
+            }
+            if constexpr (KIND == DROPPED) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[r] = drop_keep(p, drop, k0 + kb * 32 + reg_row(r) + 4 * hh) ? dp[r] * p.drop_scale : 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] -= delta;
+            float sl2 = bend.scale2;
+            if constexpr (KIND != PLAIN) {
+                if (bend.capped) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float u = __builtin_amdgcn_rcpf(1.f + EXP2(s[r] * bend.in));       // tanh = 1 - 2 u
+                        s[r] = fmaf(-2.f * bend.cap2, u, bend.cap2);
+                        dp[r] *= 4.f * fmaf(-u, u, u);
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] *= sl2;
+                }
+                if (bend.biased) {
+                    const float cf = (float)(span.c - k0 - kb * 32 - 4 * hh);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope2, fabsf(cf - (float)reg_row(r)), s[r]);
+                }
+                sl2 = 1.f;
+            }
+            bf16x8 dsf[2];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = EXP2(fmaf(s[r], sl2, -lse)) * dp[r];
+            if (masked) {
+                const unsigned rel = (unsigned)(k0 + kb * 32 + 4 * hh - span.lo), len = (unsigned)(span.hi - span.lo);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) if (rel + (unsigned)reg_row(r) >= len) s[r] = 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dsf[r >> 3][r & 7] = (bf16_t)s[r];
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int db = 0; db < NO; ++db) {
+                    const int off = (kb * 32 + 16 * st + tr_row) * KLD + db * 64;
+                    dqT[db] = mfma(cat4(LDS_TR(Ks + off + tr_c0), LDS_TR(Ks + off + 8 * KLD + tr_c1)), dsf[st], dqT[db]);
+                }
+        }
+    }
+    if (live) {
+        bf16_t* dq = p.dq + (size_t)token * p.lddq + (size_t)head * p.D;
+#pragma unroll
+        for (int db = 0; db < NO; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = db * 32 + 8 * g + 4 * hh;
+                if (d < p.D) {
+                    bf16x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = sees ? (bf16_t)(dqT[db][4 * g + e] * p.scale) : (bf16_t)0.f;
+                    *(bf16x4*)(dq + d) = v;
+                }
+            }
+    }
+    for (unsigned bad = bad_rows(sees && !(not_finite(dqT) == 0.f)); bad; bad &= bad - 1) {
+        const int t = __builtin_ctz(bad);
+        const RowSpan s = {__shfl(span.lo, t, 64), __shfl(span.hi, t, 64), __shfl(span.c, t, 64)};
+        plain_dq_row(p, __shfl(token, t, 64), __shfl(head, t, 64), s, __shfl(lse_raw, t, 64), __shfl(delta, t, 64));
+    }
+}
+
+template <int ND, int NO>
+int launch(const DocArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)(((long long)a.Tq * a.G + 127) / 128), a.Hkv);
+    if (a.drop_thresh) hipLaunchKernelGGL((doc_dq_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a);
+    else if (a.cap > 0.f || a.slopes) hipLaunchKernelGGL((doc_dq_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((doc_dq_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a);
+    return mi355_check_launch("doc_attention_dq");
+}
+
+}  // namespace
+
+int doc_bwd_q_tiles(const DocArgs& a, hipStream_t st) { return BY_WIDTH(a.D, launch, a, st); }

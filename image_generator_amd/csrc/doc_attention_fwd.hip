@@ -1,0 +1,221 @@
+// Document attention, forward, on the matrix units.
+//
+// A wave owns 32 rows (a lane its row: S^T = K Q^T leaves a row's scores in two lanes, so the softmax statistics are lane-local
+// plus one exchange), a workgroup four waves that share staged tiles of 64 keys.  One pass over the keys with the running
+// maximum and sum; scores never leave registers.  The key loop runs over the union of the rows' intervals, a wave skips the
+// tiles that none of its rows sees and masks only those that some row sees in part.
+#include "doc_tiles.h"
+
+namespace {
+
+template <int ND, int NO>
+struct Rows {                        // a wave's 32 rows
+    bf16x8 qf[ND];
+    f32x16 o[NO];
+    float m, l;
+    int token, head;
+    bool live;                       // the row exists
+    RowSpan span;
+    float slope2;
+    unsigned drop;
+    int lo, hi;                      // union of the intervals (wave-uniform)
+    int in_lo, in_hi;                // their intersection
+
+    __device__ __forceinline__ void init(const DocArgs& p, unsigned R, int hk) {
+        const int hh = (threadIdx.x & 63) >> 5;
+        live = R < (unsigned)p.Tq * (unsigned)p.G;
+        row_of(p, live ? R : 0u, hk, token, head);
+        span = row_span(p, token);
+        if (!live) span.lo = span.hi = 0;
+        const bool sees = span.hi > span.lo;
+        lo = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.lo : 0x7fffffff));
+        hi = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.hi : 0));
+        // a row without keys asks for no mask: its result is replaced by zeros at the end
+        in_lo = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.lo : 0));
+        in_hi = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.hi : 0x7fffffff));
+        if (lo > hi) lo = hi = 0;
+        const bf16_t* q = q_row(p, token, head);
+        const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < ND; ++ks) {
+            const int d = ks * 16 + 8 * hh;
+            qf[ks] = (sees && d < p.D) ? *(const bf16x8*)(q + d) : zero8;
+        }
+        slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;
+        drop = drop_row(p, token, head);
+#pragma unroll
+        for (int i = 0; i < NO; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+    }
+
+    // one staged tile of keys k0 .. k0 + 63
+    template <int KIND, int KLD, int VLD>
+    __device__ __forceinline__ void tile(const DocArgs& p, const Bend& bend, const char* Ks, const char* Vs, int k0) {
+        const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
+        f32x16 s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < ND; ++ks)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const bf16x8 a = *(const bf16x8*)(Ks + (kb * 32 + l31) * KLD + (ks * 16 + 8 * hh) * 2);
+                s[kb] = mfma(a, qf[ks], s[kb]);
+            }
+        float sl2 = bend.scale2;
+        if constexpr (KIND != PLAIN) {
+            if (bend.capped) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        s[kb][r] = fmaf(-2.f * bend.cap2, __builtin_amdgcn_rcpf(1.f + EXP2(s[kb][r] * bend.in)), bend.cap2);
+            } else {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] *= sl2;
+            }
+            if (bend.biased) {
+                const float cf = (float)(span.c - k0 - 4 * hh);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] = fmaf(-slope2, fabsf(cf - (float)(kb * 32 + reg_row(r))), s[kb][r]);
+            }
+            sl2 = 1.f;
+        }
+        if (k0 < in_lo || k0 + 64 > in_hi) {
+            const unsigned rel = (unsigned)(k0 + 4 * hh - span.lo), len = (unsigned)(span.hi - span.lo);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (rel + (unsigned)(kb * 32 + reg_row(r)) >= len) s[kb][r] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * sl2;
+        const float m_new = fmaxf(m, mx), ref = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = EXP2(m - ref);
+        float sum = 0.f;
+        bf16x8 pf[2][2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float e = EXP2(fmaf(s[kb][r], sl2, -ref));
+                sum += e;
+                if constexpr (KIND == DROPPED) e = drop_keep(p, drop, k0 + kb * 32 + reg_row(r) + 4 * hh) ? e * p.drop_scale : 0.f;
+                pf[kb][r >> 3][r & 7] = (bf16_t)e;
+            }
+        sum += __shfl_xor(sum, 32, 64);
+        l = fmaf(l, alpha, sum);
+        if (__ballot(m_new != m) != 0) {
+#pragma unroll
+            for (int i = 0; i < NO; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+        }
+        m = m_new;
+        const int tr_row = 4 * hh + ((lane & 15) >> 2), tr_col = (((lane >> 4) & 1) * 16 + 4 * (lane & 3)) * 2;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int db = 0; db < NO; ++db) {
+                    const char* a0 = Vs + (kb * 32 + 16 * st + tr_row) * VLD + db * 64 + tr_col;
+                    o[db] = mfma(cat4(LDS_TR(a0), LDS_TR(a0 + 8 * VLD)), pf[kb][st], o[db]);
+                }
+    }
+    // rows whose result is not finite (a NaN maximum included)
+    __device__ __forceinline__ unsigned bad() const {
+        const float z = not_finite(o) + l * 0.f;
+        return bad_rows(span.hi > span.lo && !(z == 0.f));
+    }
+};
+
+template <int ND, int NO, int KIND>
+__global__ __launch_bounds__(256) void doc_fwd_kernel(const DocArgs p) {
+    constexpr int DP = 16 * ND, KLD = DP * 2 + 16, VLD = tr_ld(NO);
+    constexpr int NCK = (64 * (DP / 8) + 255) / 256, NCV = (64 * NO * 4 + 255) / 256;
+    __shared__ __attribute__((aligned(16))) char smem[64 * KLD + 64 * VLD];
+    __shared__ int range[4][2];
+    char *Ks = smem, *Vs = smem + 64 * KLD;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
+    const int hk = blockIdx.y;
+    Rows<ND, NO> w;
+    w.init(p, blockIdx.x * 128u + wave * 32 + l31, hk);
+    if (lane == 0) { range[wave][0] = w.hi > w.lo ? w.lo : 0x7fffffff; range[wave][1] = w.hi; }
+    __syncthreads();
+    const int klo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
+    const int khi = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
+    const Bend bend(p);
+    const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
+    bf16x8 kreg[NCK], vreg[NCV];
+    Fetch<NCK, DP / 8> kf;
+    Fetch<NCV, NO * 4> vf;
+    kf.init(threadIdx.x, p.ldk, p.D);
+    vf.init(threadIdx.x, p.ldv, p.D);
+    if (klo < khi) {
+        kf.load(kreg, kbase, p.ldk, p.D, klo, khi - klo);
+        vf.load(vreg, vbase, p.ldv, p.D, klo, khi - klo);
+    }
+    for (int k0 = klo; k0 < khi; k0 += 64) {
+        __syncthreads();
+        put_tile<NCK, DP / 8, false>(kreg, Ks, KLD, threadIdx.x);
+        put_tile<NCV, NO * 4, false>(vreg, Vs, VLD, threadIdx.x);
+        __syncthreads();
+        if (k0 + 64 < khi) {
+            kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, khi - k0 - 64);
+            vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, khi - k0 - 64);
+        }
+        if (k0 < w.hi && k0 + 64 > w.lo) w.template tile<KIND, KLD, VLD>(p, bend, Ks, Vs, k0);
+    }
+    if (w.live) {
+        const float inv = w.l > 0.f ? 1.f / w.l : 0.f;
+        bf16_t* out = p.out + (size_t)w.token * p.ldo + (size_t)w.head * p.D;
+        const bool none = w.span.hi <= w.span.lo;
+#pragma unroll
+        for (int db = 0; db < NO; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = db * 32 + 8 * g + 4 * hh;
+                if (d < p.D) {
+                    bf16x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = none ? (bf16_t)0.f : (bf16_t)(w.o[db][4 * g + e] * inv);
+                    *(bf16x4*)(out + d) = v;
+                }
+            }
+        if (hh == 0) p.lse[(size_t)w.head * p.Tq + w.token] = none ? -INFINITY : w.m + log2f(w.l);
+    }
+    for (unsigned bad = w.bad(); bad; bad &= bad - 1) {
+        const int t = __builtin_ctz(bad);
+        const RowSpan s = {__shfl(w.span.lo, t, 64), __shfl(w.span.hi, t, 64), __shfl(w.span.c, t, 64)};
+        plain_row_out(p, __shfl(w.token, t, 64), __shfl(w.head, t, 64), s);
+    }
+}
+
+template <int ND, int NO>
+int launch(const DocArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)(((long long)a.Tq * a.G + 127) / 128), a.Hkv);
+    if (a.drop_thresh) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a);
+    else if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a);
+    return mi355_check_launch("doc_attention_fwd");
+}
+
+}  // namespace
+
+int doc_fwd_tiles(const DocArgs& a, hipStream_t st) { return BY_WIDTH(a.D, launch, a, st); }
+size_t doc_fwd_workspace(int, int, int, int, int) { return 16; }

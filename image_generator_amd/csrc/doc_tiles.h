@@ -1,0 +1,118 @@
+// Tiles of the document attention kernels: global -> registers -> LDS, matrix fragments, score modifiers.
+//
+// Products are v_mfma_f32_32x32x16_bf16.  Register r of a 32 x 32 result holds row (r & 3) + 8 (r >> 2) + 4 (lane >> 5) of
+// column lane & 31, which makes the registers of a transposed score tile directly the right operand of the product that
+// contracts over its rows.
+#pragma once
+#include "doc_attention.h"
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+#define EXP2(x) __builtin_amdgcn_exp2f(x)
+#define LDS_TR(ptr) __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(ptr))
+__device__ __forceinline__ bf16x8 cat4(bf16x4 a, bf16x4 b) { return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// Row stride (bytes) of a tile read with transposing reads of 32-column blocks: the four rows that a 16-lane group touches lie
+// 64 bytes apart modulo the 256-byte bank row.
+__host__ __device__ constexpr int tr_ld(int no) { return (no * 64) % 128 == 64 ? no * 64 : no * 64 + 64; }
+
+// kinds of score
+enum { PLAIN = 0, BENT = 1, DROPPED = 2 };      // scale alone; cap / bias; cap / bias / dropout
+
+// NCH 16-byte chunks per thread of a 64-row tile with `cols8` chunks a row (the columns past D and the rows past `valid` read
+// as zeros, by the descriptor's bounds).  A thread's chunks are the same slots of every tile; a tile has a descriptor of its
+// own (a 64-bit base, made from scalars), so no row offset passes 32 bits.
+template <int NCH, int COLS8, int THREADS = 256>
+struct Fetch {
+    int voff[NCH];
+    __device__ __forceinline__ void init(int tid, long long ld, int D) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int idx = tid + THREADS * i, r = idx / COLS8, c = idx % COLS8;
+            voff[i] = (idx < 64 * COLS8 && c * 8 < D) ? (int)(r * ld + c * 8) * 2 : (int)0x80000000;
+        }
+    }
+    // rows row0 .. row0 + 63 of base (row0 >= 0), of which `valid` may be read
+    __device__ __forceinline__ void load(bf16x8 (&reg)[NCH], const bf16_t* base, long long ld, int D, int row0, int valid) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        valid = min(valid, 64);
+        const unsigned bytes = valid > 0 ? (unsigned)(((long long)(valid - 1) * ld + D) * 2) : 0u;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (size_t)row0 * ld), 0, bytes, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) reg[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, voff[i], 0, 0));
+#endif
+    }
+};
+// chunk c of row r goes to chunk c (SWZ: c ^ ((r >> 2) & 3)) of row r
+template <int NCH, int COLS8, bool SWZ, int THREADS = 256>
+__device__ __forceinline__ void put_tile(const bf16x8 (&reg)[NCH], char* dst, int ld, int tid) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int idx = tid + THREADS * i, r = idx / COLS8, c = idx % COLS8;
+        if (64 * COLS8 % THREADS == 0 || idx < 64 * COLS8) *(bf16x8*)(dst + r * ld + (SWZ ? c ^ ((r >> 2) & 3) : c) * 16) = reg[i];
+    }
+}
+// byte offsets inside a row of a swizzled tile for the two transposing reads of a fragment
+__device__ __forceinline__ void tr_cols_swz(int lane, int& c0, int& c1) {
+    const int hh = lane >> 5, chunk = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), b = (lane & 1) * 8;
+    c0 = (chunk ^ hh) * 16 + b;
+    c1 = (chunk ^ (hh + 2)) * 16 + b;
+}
+
+// the row of a result register
+__device__ __forceinline__ constexpr int reg_row(int r) { return (r & 3) + 8 * (r >> 2); }
+
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// q.k -> score in log2 units (cap and bias decided at run time, uniformly).  dist = c - key.
+struct Bend {
+    float scale2, in, cap2;          // scale log2 e;  2 scale log2 e / cap;  cap log2 e
+    bool capped, biased;
+    __device__ __forceinline__ Bend(const DocArgs& p)
+        : scale2(p.scale * LOG2E), in(p.scale * (2.f * LOG2E) * p.rcap), cap2(p.cap * LOG2E), capped(p.cap > 0.f), biased(p.slopes != nullptr) {}
+};
+
+// NaN if any register is not finite, else 0
+template <int NO>
+__device__ __forceinline__ float not_finite(const f32x16 (&a)[NO]) {
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = fmaf(a[i][r], 0.f, z);
+    return z;
+}
+
+// rows of the wave (as bits) of which a lane says `bad`
+__device__ __forceinline__ unsigned bad_rows(bool bad) {
+    const unsigned long long b = __ballot(bad);
+    return (unsigned)b | (unsigned)(b >> 32);
+}
+
+// row R of a key head -> token and query head
+__device__ __forceinline__ void row_of(const DocArgs& p, unsigned R, int hk, int& token, int& head) {
+    if (p.G == 1) { token = (int)R; head = hk; return; }
+    const unsigned t = R / (unsigned)p.G;
+    token = (int)t;
+    head = hk * p.G + (int)(R - t * (unsigned)p.G);
+}
+
+int doc_fwd_tiles(const DocArgs& a, hipStream_t st);
+int doc_bwd_q_tiles(const DocArgs& a, hipStream_t st);
+int doc_bwd_kv_tiles(const DocArgs& a, hipStream_t st);
+size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D);
+
+// FN<ND, NO>(args...) for the head width: ND 16-wide steps of a contraction over it, NO 32-wide blocks of it
+#define BY_WIDTH(D, FN, ...)                              \
+    ((D) <= 32 ? FN<2, 1>(__VA_ARGS__) : (D) <= 48 ? FN<3, 2>(__VA_ARGS__) : (D) <= 64 ? FN<4, 2>(__VA_ARGS__) \
+     : (D) <= 80 ? FN<5, 3>(__VA_ARGS__) : (D) <= 96 ? FN<6, 3>(__VA_ARGS__) : FN<8, 4>(__VA_ARGS__))
