@@ -1,89 +1,132 @@
-// Document attention, dK and dV, on the matrix units: a lane owns its key (S = Q K^T, dP = dO V^T), a wave 32 keys, a workgroup
-// 128, and staged tiles of 64 rows - tokens times the query heads that share the key head - pass by: dV^T += dO^T P,
-// dK^T += Q^T dS.  Nothing is added across workgroups, so there are no atomics and no order to choose.
+// Document attention, dK and dV, on the matrix units: a lane owns its key (S = Q K^T, dP = dO V^T), a wave KB blocks of 32 keys,
+// and staged tiles of 64 rows - tokens times the query heads that share the key head - pass by: dV^T += dO^T P,
+// dK^T += Q^T dS.  -lse and -delta of a row start the accumulators of its scores, so subtracting them costs nothing.
+//
+// Few keys under many rows (captions under image tokens) leave most of the chip idle: the rows of a key tile are then cut
+// into `splits` runs whose fp32 partial gradients a second launch adds, in their order.  No atomics anywhere.
 #include "doc_tiles.h"
 
 namespace {
 
-template <int ND, int NO, int KIND>
-__global__ __launch_bounds__(256) void doc_dkdv_kernel(const DocArgs p) {
+// 64-row tiles of Q and dO: rows are (token, head of the group)
+template <int NCH, int COLS8>
+struct RowFetch {
+    int vq[NCH], vg[NCH];
+    __device__ __forceinline__ void init(const DocArgs& p, unsigned phase) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int idx = threadIdx.x + 256 * i;
+            const unsigned r = idx / COLS8, c = idx % COLS8, x = phase + r, t = p.G == 1 ? x : x / (unsigned)p.G, g = x - t * (unsigned)p.G;
+            const bool in = (64 * COLS8 % 256 == 0 || idx < 64 * COLS8) && (int)c * 8 < p.D;
+            vq[i] = in ? (int)(t * p.ldq + g * p.D + c * 8) * 2 : (int)0x80000000;
+            vg[i] = in ? (int)(t * p.lddo + g * p.D + c * 8) * 2 : (int)0x80000000;
+        }
+    }
+    // rows from token t0 on, tokens below `end`
+    __device__ __forceinline__ void load(bf16x8 (&q)[NCH], bf16x8 (&g)[NCH], const DocArgs& p, int hk, int t0, int end) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const int n = min(end - t0, 65);                // 64 rows lie in at most 64 tokens, one more if they begin inside one
+        const size_t first = (size_t)hk * p.G * p.D;
+        const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(p.q + (size_t)t0 * p.ldq + first), 0, (unsigned)(((long long)(n - 1) * p.ldq + (long long)p.G * p.D) * 2), 0x00020000);
+        const __amdgpu_buffer_rsrc_t rg = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(p.dout + (size_t)t0 * p.lddo + first), 0, (unsigned)(((long long)(n - 1) * p.lddo + (long long)p.G * p.D) * 2), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            q[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rq, vq[i], 0, 0));
+            g[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rg, vg[i], 0, 0));
+        }
+#endif
+    }
+};
+
+struct RowInfo {                     // of the 64 staged rows
+    float lse[64], delta[64];        // PLAIN: -lse / (scale log2 e), else lse;  -delta (DROPPED: delta)
+    int lo[64], count[64], c[64];
+    float slope2[64];
+    unsigned drop[64];
+};
+
+template <int ND, int NO, int KIND, int KB>
+__global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p) {
     constexpr int LD = tr_ld(NO);
     constexpr int NCH = (64 * NO * 4 + 255) / 256;
     __shared__ __attribute__((aligned(16))) char smem[2 * 64 * LD];
-    __shared__ float4 info[64];          // lse, delta, first key and number of keys of a row (as bits)
-    __shared__ float2 place[64];         // its key position (as bits) and slope
-    __shared__ unsigned drops[64];
+    __shared__ __attribute__((aligned(16))) RowInfo info;
     __shared__ int range[4][2];
     char *Qs = smem, *Gs = smem + 64 * LD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
     const int hk = blockIdx.y;
-    const int key = (int)blockIdx.x * 128 + wave * 32 + l31;
-    const bool live = key < p.Tk;
-    int2 span = live ? key_span(p, key) : make_int2(0, 0);
-    const bool seen = span.y > span.x;
-    const int lo = __builtin_amdgcn_readfirstlane(wave_min_i(seen ? span.x : 0x7fffffff));
-    const int hi = __builtin_amdgcn_readfirstlane(wave_max_i(seen ? span.y : 0));
-    if (lane == 0) { range[wave][0] = lo; range[wave][1] = hi; }
+    const int key0 = (int)(blockIdx.x * 4 + wave) * (32 * KB);
     const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
-    bf16x8 kf[ND], vf[ND];
+    bf16x8 kf[KB][ND], vf[KB][ND];
+    bool seen[KB];
+    int lo = 0x7fffffff, hi = 0;
 #pragma unroll
-    for (int ks = 0; ks < ND; ++ks) {
-        const int d = ks * 16 + 8 * hh;
-        const bool ok = seen && d < p.D;
-        kf[ks] = ok ? *(const bf16x8*)(k_row(p, key, hk) + d) : zero8;
-        vf[ks] = ok ? *(const bf16x8*)(v_row(p, key, hk) + d) : zero8;
+    for (int kb = 0; kb < KB; ++kb) {
+        const int key = key0 + kb * 32 + l31;
+        const int2 span = key < p.Tk ? key_span(p, key) : make_int2(0, 0);
+        seen[kb] = span.y > span.x;
+        if (seen[kb]) { lo = min(lo, span.x); hi = max(hi, span.y); }
+#pragma unroll
+        for (int ks = 0; ks < ND; ++ks) {
+            const int d = ks * 16 + 8 * hh;
+            const bool ok = seen[kb] && d < p.D;
+            kf[kb][ks] = ok ? *(const bf16x8*)(k_row(p, key, hk) + d) : zero8;
+            vf[kb][ks] = ok ? *(const bf16x8*)(v_row(p, key, hk) + d) : zero8;
+        }
     }
-    f32x16 dkT[NO], dvT[NO];
+    lo = __builtin_amdgcn_readfirstlane(wave_min_i(lo));
+    hi = __builtin_amdgcn_readfirstlane(wave_max_i(hi));
+    if (lane == 0) { range[wave][0] = lo; range[wave][1] = hi; }
+    f32x16 dkT[KB][NO], dvT[KB][NO];
 #pragma unroll
-    for (int i = 0; i < NO; ++i)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { dkT[i][r] = 0.f; dvT[i][r] = 0.f; }
+        for (int i = 0; i < NO; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) { dkT[kb][i][r] = 0.f; dvT[kb][i][r] = 0.f; }
     const int tr_row = 4 * hh + ((lane & 15) >> 2);
     int tr_c0, tr_c1;
     tr_cols_swz(lane, tr_c0, tr_c1);
     const Bend bend(p);
     __syncthreads();
-    const int tlo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
-    const int thi = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
+    const int tlo = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
+    const int thi = __builtin_amdgcn_readfirstlane(max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])));
     const unsigned G = (unsigned)p.G;
-    const unsigned rlo = tlo < thi ? tlo * G : 0u, rhi = tlo < thi ? thi * G : 0u;
+    unsigned rlo = tlo < thi ? tlo * G : 0u, rhi = tlo < thi ? thi * G : 0u;
+    if (p.splits > 1) {
+        const unsigned tiles = (rhi - rlo + 63) / 64, each = (tiles + p.splits - 1) / p.splits;
+        const unsigned from = rlo + min(tiles, each * blockIdx.z) * 64;
+        rhi = min(rhi, rlo + min(tiles, each * (blockIdx.z + 1)) * 64);
+        rlo = from;
+    }
     const unsigned wlo = lo < hi ? lo * G : 0xffffffffu, whi = lo < hi ? hi * G : 0u;
-    const int kmin = (int)blockIdx.x * 128 + wave * 32;       // the wave's keys: all of them seen in full by a row with
-    const int kmax = min(kmin + 32, p.Tk);                    // lo <= kmin and hi >= kmax
+    const int kmax = min(key0 + 32 * KB, p.Tk);       // the wave's keys: seen whole by a row with lo <= key0 and hi >= kmax
+    const float rsl2 = KIND == PLAIN ? 1.f / bend.scale2 : 0.f;
 
     bf16x8 qreg[NCH], greg[NCH];
-    float4 ireg;
-    float2 preg;
-    unsigned dreg;
-    auto load = [&](unsigned r0) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int idx = threadIdx.x + 256 * i, r = idx / (NO * 4), c = idx % (NO * 4);
-            const unsigned R = r0 + r;
-            const bool ok = (64 * NO * 4 % 256 == 0 || idx < 64 * NO * 4) && R < rhi && c * 8 < p.D;
-            qreg[i] = greg[i] = zero8;
-            if (ok) {
-                int token, head;
-                row_of(p, R, hk, token, head);
-                qreg[i] = *(const bf16x8*)(q_row(p, token, head) + c * 8);
-                greg[i] = *(const bf16x8*)(p.dout + (size_t)token * p.lddo + (size_t)head * p.D + c * 8);
-            }
-        }
+    RowFetch<NCH, NO * 4> f;
+    f.init(p, 0);
+    int4 ireg = {0, 0, 0, 0};
+    float lreg = 0.f, dreg = 0.f, sreg = 0.f;
+    unsigned hreg = 0;
+    bool in = false;
+    auto load = [&](unsigned r0) __attribute__((always_inline)) {
+        const unsigned t0 = G == 1 ? r0 : r0 / G;
+        if (64 % G != 0) f.init(p, r0 - t0 * G);
+        f.load(qreg, greg, p, hk, (int)t0, thi);
         if (threadIdx.x < 64) {
             const unsigned R = r0 + threadIdx.x;
-            ireg = make_float4(INFINITY, 0.f, 0.f, 0.f);
-            preg = make_float2(0.f, 0.f);
-            dreg = 0;
-            if (R < rhi) {
-                int token, head;
-                row_of(p, R, hk, token, head);
-                const int4 s = p.rows[token];
-                const size_t at = (size_t)head * p.Tq + token;
-                const float ls = p.lse[at];
-                ireg = make_float4(ls == -INFINITY ? INFINITY : ls, p.delta[at], __int_as_float(s.x), __int_as_float(s.y - s.x));
-                preg = make_float2(__int_as_float(s.z), p.slopes ? p.slopes[head] * LOG2E : 0.f);
-                dreg = drop_row(p, token, head);
-            }
+            in = R < rhi;
+            int token, head;
+            row_of(p, in ? R : rhi - 1, hk, token, head);
+            const size_t at = (size_t)head * p.Tq + token;
+            ireg = p.rows[token];
+            lreg = p.lse[at];
+            dreg = p.delta[at];
+            if (KIND != PLAIN && p.slopes) sreg = p.slopes[head];
+            if (KIND == DROPPED) hreg = drop_row(p, token, head);
         }
     };
     if (rlo < rhi) load(rlo);
@@ -91,102 +134,218 @@ __global__ __launch_bounds__(256) void doc_dkdv_kernel(const DocArgs p) {
         __syncthreads();
         put_tile<NCH, NO * 4, true>(qreg, Qs, LD, threadIdx.x);
         put_tile<NCH, NO * 4, true>(greg, Gs, LD, threadIdx.x);
-        if (threadIdx.x < 64) { info[threadIdx.x] = ireg; place[threadIdx.x] = preg; drops[threadIdx.x] = dreg; }
+        if (threadIdx.x < 64) {
+            const float ls = !in || lreg == -INFINITY ? INFINITY : lreg;         // rows that see nothing: probabilities of 0
+            info.lse[threadIdx.x] = KIND == PLAIN ? -ls * rsl2 : ls;
+            info.delta[threadIdx.x] = KIND == DROPPED ? dreg : -dreg;
+            info.lo[threadIdx.x] = ireg.x;
+            info.count[threadIdx.x] = in ? ireg.y - ireg.x : 0;
+            if (KIND != PLAIN) { info.c[threadIdx.x] = ireg.z; info.slope2[threadIdx.x] = sreg * LOG2E; }
+            if (KIND == DROPPED) info.drop[threadIdx.x] = hreg;
+        }
         __syncthreads();
         if (r0 + 64 < rhi) load(r0 + 64);
         if (r0 >= whi || r0 + 64 <= wlo) continue;
-        bool masked;
-        {
-            const float4 f = info[lane];
-            const int first = __float_as_int(f.z), count = __float_as_int(f.w);
-            masked = __ballot(first > kmin || first + count < kmax) != 0;
-        }
+        const int first = info.lo[lane], count = info.count[lane];
+        const bool masked = __ballot(first > key0 || first + count < kmax) != 0;
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs) {
             const char *Qt = Qs + qs * 32 * LD, *Gt = Gs + qs * 32 * LD;
-            f32x16 s, dp;
+            f32x16 s[KB], dp[KB];
+            f32x4 ls[4], dl[4];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+            for (int g = 0; g < 4; ++g) {
+                ls[g] = *(const f32x4*)&info.lse[qs * 32 + 8 * g + 4 * hh];
+                dl[g] = *(const f32x4*)&info.delta[qs * 32 + 8 * g + 4 * hh];
+            }
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[kb][r] = KIND == PLAIN ? ls[r >> 2][r & 3] : 0.f;
+                    dp[kb][r] = KIND == DROPPED ? 0.f : dl[r >> 2][r & 3];
+                }
 #pragma unroll
             for (int ks = 0; ks < ND; ++ks) {
                 const int off = l31 * LD + ((ks * 2 + hh) ^ ((l31 >> 2) & 3)) * 16;
-                s = mfma(*(const bf16x8*)(Qt + off), kf[ks], s);
-                dp = mfma(*(const bf16x8*)(Gt + off), vf[ks], dp);
-            }
-            bf16x8 pf[2], dsf[2];
+                const bf16x8 aq = *(const bf16x8*)(Qt + off), ag = *(const bf16x8*)(Gt + off);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = qs * 32 + reg_row(r) + 4 * hh;
-                const float4 f = info[row];
-                float x = s[r] * bend.scale2, turn = 1.f;
+                for (int kb = 0; kb < KB; ++kb) {
+                    s[kb] = mfma(aq, kf[kb][ks], s[kb]);
+                    dp[kb] = mfma(ag, vf[kb][ks], dp[kb]);
+                }
+            }
+            bf16x8 pf[KB][2], dsf[KB][2];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const int key = key0 + kb * 32 + l31;
                 if constexpr (KIND != PLAIN) {
+                    f32x16 turn;
                     if (bend.capped) {
-                        const float u = __builtin_amdgcn_rcpf(1.f + EXP2(s[r] * bend.in));
-                        x = fmaf(-2.f * bend.cap2, u, bend.cap2);
-                        turn = 4.f * fmaf(-u, u, u);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const float u = __builtin_amdgcn_rcpf(1.f + EXP2(s[kb][r] * bend.in));       // tanh = 1 - 2 u
+                            s[kb][r] = fmaf(-2.f * bend.cap2, u, bend.cap2);
+                            turn[r] = fmaf(-4.f * u, u, 4.f * u);
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) { s[kb][r] *= bend.scale2; turn[r] = 1.f; }
                     }
                     if (bend.biased) {
-                        const float2 g = place[row];
-                        x = fmaf(-g.y, fabsf((float)(__float_as_int(g.x) - key)), x);
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const int4 c = *(const int4*)&info.c[qs * 32 + 8 * g + 4 * hh];
+                            const f32x4 sl = *(const f32x4*)&info.slope2[qs * 32 + 8 * g + 4 * hh];
+                            const int cc[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[kb][4 * g + e] = fmaf(-sl[e], fabsf((float)(cc[e] - key)), s[kb][4 * g + e]);
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] = EXP2(s[kb][r] - ls[r >> 2][r & 3]);
+                    if constexpr (KIND == DROPPED) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const bool keep = drop_keep(p, info.drop[qs * 32 + reg_row(r) + 4 * hh], key);
+                            pf[kb][r >> 3][r & 7] = (bf16_t)(keep ? s[kb][r] * p.drop_scale : 0.f);
+                            dp[kb][r] = ((keep ? dp[kb][r] * p.drop_scale : 0.f) - dl[r >> 2][r & 3]) * turn[r];
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) dp[kb][r] *= turn[r];
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] = EXP2(s[kb][r] * bend.scale2);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[kb][r] *= s[kb][r];
+                if (masked) {        // what a row does not see is 0, whatever its scores and gradients are
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int4 a = *(const int4*)&info.lo[qs * 32 + 8 * g + 4 * hh], n = *(const int4*)&info.count[qs * 32 + 8 * g + 4 * hh];
+                        const int lo4[4] = {a.x, a.y, a.z, a.w}, n4[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if ((unsigned)(key - lo4[e]) >= (unsigned)n4[e]) {
+                                s[kb][4 * g + e] = 0.f;
+                                dp[kb][4 * g + e] = 0.f;
+                                if constexpr (KIND == DROPPED) pf[kb][(4 * g + e) >> 3][(4 * g + e) & 7] = (bf16_t)0.f;
+                            }
                     }
                 }
-                float e = EXP2(x - f.x);
-                if (masked && (unsigned)(key - __float_as_int(f.z)) >= (unsigned)__float_as_int(f.w)) e = 0.f;
-                float pd = e, d = dp[r];
-                if constexpr (KIND == DROPPED) {
-                    const bool keep = drop_keep(p, drops[row], key);
-                    pd = keep ? e * p.drop_scale : 0.f;
-                    d = keep ? d * p.drop_scale : 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    if constexpr (KIND != DROPPED) pf[kb][r >> 3][r & 7] = (bf16_t)s[kb][r];
+                    dsf[kb][r >> 3][r & 7] = (bf16_t)dp[kb][r];
                 }
-                float ds = e * (d - f.y);
-                if constexpr (KIND != PLAIN) ds *= turn;
-                // a row that does not see the key: its dO may be anything
-                if (masked && e == 0.f) ds = 0.f;
-                pf[r >> 3][r & 7] = (bf16_t)pd;
-                dsf[r >> 3][r & 7] = (bf16_t)ds;
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int db = 0; db < NO; ++db) {
                     const int off = (16 * st + tr_row) * LD + db * 64;
-                    dvT[db] = mfma(cat4(LDS_TR(Gt + off + tr_c0), LDS_TR(Gt + off + 8 * LD + tr_c1)), pf[st], dvT[db]);
-                    dkT[db] = mfma(cat4(LDS_TR(Qt + off + tr_c0), LDS_TR(Qt + off + 8 * LD + tr_c1)), dsf[st], dkT[db]);
+                    const bf16x8 ag = cat4(LDS_TR(Gt + off + tr_c0), LDS_TR(Gt + off + 8 * LD + tr_c1));
+                    const bf16x8 aq = cat4(LDS_TR(Qt + off + tr_c0), LDS_TR(Qt + off + 8 * LD + tr_c1));
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) {
+                        dvT[kb][db] = mfma(ag, pf[kb][st], dvT[kb][db]);
+                        dkT[kb][db] = mfma(aq, dsf[kb][st], dkT[kb][db]);
+                    }
                 }
         }
     }
-    if (live) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+        const int key = key0 + kb * 32 + l31;
+        if (key >= p.Tk) continue;
         bf16_t *dk = p.dk + (size_t)key * p.lddk + (size_t)hk * p.D, *dv = p.dv + (size_t)key * p.lddv + (size_t)hk * p.D;
+        float* part = p.part + (((size_t)blockIdx.z * p.Tk + key) * p.Hkv + hk) * 2 * p.D;
 #pragma unroll
         for (int db = 0; db < NO; ++db)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int d = db * 32 + 8 * g + 4 * hh;
-                if (d < p.D) {
-                    bf16x4 a, c;
+                if (d >= p.D) continue;
+                const f32x16 &a = dkT[kb][db], &c = dvT[kb][db];
+                if (p.splits > 1) {
+                    *(f32x4*)(part + d) = f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+                    *(f32x4*)(part + p.D + d) = f32x4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
+                } else {
+                    bf16x4 x, y;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        a[e] = seen ? (bf16_t)(dkT[db][4 * g + e] * p.scale) : (bf16_t)0.f;
-                        c[e] = seen ? (bf16_t)dvT[db][4 * g + e] : (bf16_t)0.f;
+                        x[e] = seen[kb] ? (bf16_t)(a[4 * g + e] * p.scale) : (bf16_t)0.f;
+                        y[e] = seen[kb] ? (bf16_t)c[4 * g + e] : (bf16_t)0.f;
                     }
-                    *(bf16x4*)(dk + d) = a;
-                    *(bf16x4*)(dv + d) = c;
+                    *(bf16x4*)(dk + d) = x;
+                    *(bf16x4*)(dv + d) = y;
                 }
             }
     }
-    for (unsigned bad = bad_rows(seen && !(not_finite(dkT) + not_finite(dvT) == 0.f)); bad; bad &= bad - 1)
-        plain_dkdv_key(p, __shfl(key, __builtin_ctz(bad), 64), hk);
+    if (p.splits > 1) return;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+        for (unsigned bad = bad_rows(seen[kb] && !(not_finite(dkT[kb]) + not_finite(dvT[kb]) == 0.f)); bad; bad &= bad - 1)
+            plain_dkdv_key(p, key0 + kb * 32 + __builtin_ctz(bad), hk);
+}
+
+// the partial gradients of a key, added in order: a wave per (key, key head)
+__global__ __launch_bounds__(256) void doc_dkdv_join_kernel(const DocArgs p) {
+    const int lane = threadIdx.x & 63;
+    const size_t u = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (u >= (size_t)p.Tk * p.Hkv) return;
+    const int key = (int)(u / p.Hkv), hk = (int)(u % p.Hkv);
+    const int2 span = key_span(p, key);
+    const bool seen = span.y > span.x;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const int n = 2 * p.D;
+    for (int z = 0; z < p.splits; ++z) {
+        const float* part = p.part + ((size_t)z * p.Tk * p.Hkv + u) * n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (lane + 64 * e < n) acc[e] += part[lane + 64 * e];
+    }
+    bf16_t *dk = p.dk + (size_t)key * p.lddk + (size_t)hk * p.D, *dv = p.dv + (size_t)key * p.lddv + (size_t)hk * p.D;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int d = lane + 64 * e;
+        if (d >= n) continue;
+        bad |= !(acc[e] * 0.f == 0.f);
+        if (d < p.D) dk[d] = seen ? (bf16_t)(acc[e] * p.scale) : (bf16_t)0.f;
+        else dv[d - p.D] = seen ? (bf16_t)acc[e] : (bf16_t)0.f;
+    }
+    if (seen && __ballot(bad) != 0) plain_dkdv_key(p, key, hk);
+}
+
+template <int ND, int NO, int KB>
+void launch_kind(const DocArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)(((long long)a.Tk + 128 * KB - 1) / (128 * KB)), a.Hkv, a.splits);
+    if (a.drop_thresh) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, DROPPED, KB>), grid, dim3(256), 0, st, a);
+    else if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, BENT, KB>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, PLAIN, KB>), grid, dim3(256), 0, st, a);
 }
 
 template <int ND, int NO>
 int launch(const DocArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)(((long long)a.Tk + 127) / 128), a.Hkv);
-    if (a.drop_thresh) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a);
-    else if (a.cap > 0.f || a.slopes) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a);
+    launch_kind<ND, NO, 1>(a, st);
+    if (a.splits > 1) hipLaunchKernelGGL(doc_dkdv_join_kernel, dim3((unsigned)(((size_t)a.Tk * a.Hkv + 3) / 4)), dim3(256), 0, st, a);
     return mi355_check_launch("doc_attention_dkdv");
 }
 
 }  // namespace
+
+// Workgroups without a split: one per 128 keys and key head, each passing about G * (the rows of one document, and of the others
+// that its keys belong to).  Runs of at least 8 tiles, until the chip has about 1024 workgroups.
+int doc_bwd_kv_splits(int Tq, int Tk, int Hq, int Hkv, int docs) {
+    if (Tk < 1) return 1;
+    const double wgs = (double)((Tk + 127) / 128) * Hkv, keys_per_doc = (double)Tk / docs;
+    const double tiles = (double)Tq * (Hq / Hkv) / docs * (1.0 + 127.0 / (keys_per_doc < 1.0 ? 1.0 : keys_per_doc)) / 64.0;
+    const double cap = (double)Tq * (Hq / Hkv) / 64.0;
+    double s = 1024.0 / wgs, most = (tiles < cap ? tiles : cap) / 8.0;
+    if (s > most) s = most;
+    return s < 2.0 ? 1 : s > 64.0 ? 64 : (int)s;
+}
 
 int doc_bwd_kv_tiles(const DocArgs& a, hipStream_t st) { return BY_WIDTH(a.D, launch, a, st); }
