@@ -5,6 +5,7 @@
 // maximum and sum; scores never leave registers.  The key loop runs over the union of the rows' intervals, a wave skips the
 // tiles that none of its rows sees and masks only those that some row sees in part.
 #include "doc_tiles.h"
+#include <mutex>
 
 namespace {
 
@@ -206,16 +207,157 @@ __global__ __launch_bounds__(256) void doc_fwd_kernel(const DocArgs p) {
     }
 }
 
+// Few rows over many keys (single queries over what their documents hold): a wave takes 32 rows and one run of their keys,
+// alone - its own staged tiles, no barrier with the others - and leaves an unnormalised result; the join weighs the runs of a
+// row against each other.  The rows of a tile may belong to many documents, whose keys lie one behind another: a run is read
+// once and only the rows that see a tile take part, so what is bound here is reading K and V.
+template <int ND, int NO, int KIND>
+__global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) {
+    constexpr int DP = 16 * ND, KLD = DP * 2 + 16, VLD = tr_ld(NO);
+    constexpr int NCK = DP / 8, NCV = NO * 4;                     // 64 rows, 64 lanes
+    extern __shared__ __attribute__((aligned(16))) char smem_all[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
+    char *Ks = smem_all + wave * 64 * (KLD + VLD), *Vs = Ks + 64 * KLD;
+    const int hk = blockIdx.y, split = blockIdx.z * 4 + wave;
+    const unsigned R = blockIdx.x * 32u + l31;
+    Rows<ND, NO> w;
+    w.init(p, R, hk);
+    int from, to;
+    {
+        const int tiles = (w.hi - w.lo + 63) / 64, each = (tiles + p.splits - 1) / p.splits;
+        from = w.lo + min(tiles, each * split) * 64;
+        to = min(w.hi, w.lo + min(tiles, each * (split + 1)) * 64);
+    }
+    const Bend bend(p);
+    const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
+    bf16x8 kreg[NCK], vreg[NCV];
+    Fetch<NCK, DP / 8, 64> kf;
+    Fetch<NCV, NO * 4, 64> vf;
+    kf.init(lane, p.ldk, p.D);
+    vf.init(lane, p.ldv, p.D);
+    if (from < to) {
+        kf.load(kreg, kbase, p.ldk, p.D, from, to - from);
+        vf.load(vreg, vbase, p.ldv, p.D, from, to - from);
+    }
+    for (int k0 = from; k0 < to; k0 += 64) {
+        // one wave: its LDS operations complete in order, the fences only keep the compiler from reordering them
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        put_tile<NCK, DP / 8, false, 64>(kreg, Ks, KLD, lane);
+        put_tile<NCV, NO * 4, false, 64>(vreg, Vs, VLD, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (k0 + 64 < to) {
+            kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, to - k0 - 64);
+            vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, to - k0 - 64);
+        }
+        // keys behind this run are another wave's: the tile holds zeros there, and the mask ends with the run
+        w.template tile<KIND, KLD, VLD>(p, bend, Ks, Vs, k0);
+    }
+    const size_t rows = (size_t)gridDim.x * 32, row = ((size_t)hk * rows + R) * p.splits + split;
+    float2* ml = (float2*)p.part;
+    float* part = p.part + (size_t)p.Hkv * rows * p.splits * 2 + row * p.D;
+    // (m = -inf: no key of the run is seen, the values stay unwritten and unread)
+    if (hh == 0) ml[row] = make_float2(w.l == 0.f && w.m == -INFINITY ? -INFINITY : w.m, w.l);
+    const bool any = !(w.m == -INFINITY) && w.live;
+#pragma unroll
+    for (int db = 0; db < NO; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = db * 32 + 8 * g + 4 * hh;
+            if (any && d < p.D) *(f32x4*)(part + d) = f32x4{w.o[db][4 * g], w.o[db][4 * g + 1], w.o[db][4 * g + 2], w.o[db][4 * g + 3]};
+        }
+    for (unsigned bad = from < to ? w.bad() : 0u; bad; bad &= bad - 1) {
+        const int t = __builtin_ctz(bad);
+        const int lo = max(__shfl(w.span.lo, t, 64), from), hi = min(__shfl(w.span.hi, t, 64), to);
+        float m, l, o[2];
+        plain_row(p, __shfl(w.token, t, 64), __shfl(w.head, t, 64), lo, hi, __shfl(w.span.c, t, 64), m, l, o);
+        const size_t at = ((size_t)hk * rows + blockIdx.x * 32u + t) * p.splits + split;
+        if (lane == 0) ml[at] = make_float2(m, l);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (lane + 64 * u < p.D) p.part[(size_t)p.Hkv * rows * p.splits * 2 + at * p.D + lane + 64 * u] = o[u];
+    }
+}
+
+// out = sum o_s 2^(m_s - M) / sum l_s 2^(m_s - M) over the runs of a row: a wave per row, at most 64 runs
+__global__ __launch_bounds__(256) void doc_fwd_join_kernel(const DocArgs p, unsigned rows) {
+    const int lane = threadIdx.x & 63;
+    const unsigned R = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int hk = blockIdx.y;
+    if (R >= (unsigned)p.Tq * (unsigned)p.G) return;
+    int token, head;
+    row_of(p, R, hk, token, head);
+    const size_t row = ((size_t)hk * rows + R) * p.splits;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < p.splits) ml = ((const float2*)p.part)[row + lane];
+    const bool nan = __ballot(ml.x != ml.x) != 0;
+    const float M = wave_max(ml.x);
+    const float w = ml.x == -INFINITY ? 0.f : EXP2(ml.x - M);
+    const float l = wave_sum(ml.y * w);
+    const float* part = p.part + (size_t)p.Hkv * rows * p.splits * 2 + row * p.D;
+    float o[2] = {0.f, 0.f};
+    unsigned long long who = __ballot(ml.x != -INFINITY);
+    while (who) {
+        const int s = __builtin_ctzll(who);
+        who &= who - 1;
+        const float ws = __shfl(w, s, 64);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (lane + 64 * u < p.D) o[u] = fmaf(ws, part[(size_t)s * p.D + lane + 64 * u], o[u]);
+    }
+    const float inv = nan ? NAN : l > 0.f || l != l ? 1.f / l : 0.f;
+    bf16_t* out = p.out + (size_t)token * p.ldo + (size_t)head * p.D;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) if (lane + 64 * u < p.D) out[lane + 64 * u] = (bf16_t)(o[u] * inv);
+    if (lane == 0) p.lse[(size_t)head * p.Tq + token] = nan ? NAN : l == 0.f ? -INFINITY : M + log2f(l);
+}
+
+// Runs per row where the unsplit grid (a workgroup for 128 rows of a key head) leaves most of the chip idle and there are keys to
+// deal out: about 2048 waves, runs of four tiles at least, at most 64 of them.  0: no split.
+static int fwd_splits(int Tq, int Tk, int Hq, int Hkv) {
+    const long long rows = (long long)Tq * (Hq / Hkv);
+    const long long wgs = (rows + 127) / 128 * Hkv;
+    if (wgs >= 256 || Tk < 1024) return 0;
+    long long s = 2048 / ((rows + 31) / 32 * Hkv);
+    const long long most = (Tk + 255) / 256;
+    if (s > most) s = most;
+    if (s > 64) s = 64;
+    s = s / 4 * 4;
+    return s < 4 ? 0 : (int)s;
+}
+
+template <int ND, int NO, int KIND>
+int launch_split(const DocArgs& a, hipStream_t st) {
+    constexpr int LDS = 4 * 64 * (16 * ND * 2 + 16 + tr_ld(NO));
+    static std::once_flag once;
+    static hipError_t set;
+    std::call_once(once, [] { set = hipFuncSetAttribute((const void*)doc_fwd_split_kernel<ND, NO, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
+    if (set != hipSuccess) return mi355_fail(MI355_ERR_LAUNCH, "doc_attention: %s", hipGetErrorString(set));
+    const unsigned tiles = (unsigned)(((long long)a.Tq * a.G + 31) / 32);
+    hipLaunchKernelGGL((doc_fwd_split_kernel<ND, NO, KIND>), dim3(tiles, a.Hkv, a.splits / 4), dim3(256), LDS, st, a);
+    hipLaunchKernelGGL(doc_fwd_join_kernel, dim3((unsigned)(((long long)a.Tq * a.G + 3) / 4), a.Hkv), dim3(256), 0, st, a, tiles * 32);
+    return mi355_check_launch("doc_attention_fwd(split)");
+}
+
 template <int ND, int NO>
 int launch(const DocArgs& a, hipStream_t st) {
+    const bool bent = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
+    if (a.splits)
+        return a.drop_thresh ? launch_split<ND, NO, DROPPED>(a, st) : bent ? launch_split<ND, NO, BENT>(a, st) : launch_split<ND, NO, PLAIN>(a, st);
     const dim3 grid((unsigned)(((long long)a.Tq * a.G + 127) / 128), a.Hkv);
     if (a.drop_thresh) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a);
-    else if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a);
+    else if (bent) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a);
     return mi355_check_launch("doc_attention_fwd");
 }
 
 }  // namespace
 
-int doc_fwd_tiles(const DocArgs& a, hipStream_t st) { return BY_WIDTH(a.D, launch, a, st); }
-size_t doc_fwd_workspace(int, int, int, int, int) { return 16; }
+int doc_fwd_tiles(const DocArgs& a, hipStream_t st) {
+    DocArgs b = a;
+    b.splits = fwd_splits(a.Tq, a.Tk, a.Hq, a.Hkv);
+    return BY_WIDTH(a.D, launch, b, st);
+}
+size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D) {
+    const size_t s = fwd_splits(Tq, Tk, Hq, Hkv), rows = ((size_t)Tq * (Hq / Hkv) + 31) / 32 * 32 * Hkv;
+    return rows * s * (D + 2) * 4 + 16;
+}

@@ -377,3 +377,39 @@ def test_wrong_offsets_stay_in_bounds(docs):
         bad[20], bad[21] = T, -5
         got = run(*x, heads=2, q_offsets=bad)
         assert all(t.shape[0] in (T, 2) for t in got.values())
+
+
+SPLIT = {                                                  # (queries, keys) whose forward pass, or key gradients, run in pieces
+    "few_rows": ([1, 1, 1, 2, 1], [700, 0, 901, 33, 64]), "one_row": ([1], [2500]), "rows_at_the_end": ([3, 30], [1100, 1500]),
+    "few_keys": ([1500, 0, 900], [40, 3, 5]), "one_key": ([3000], [1]), "both": ([600, 1], [7, 1200]),
+}
+
+
+@pytest.mark.parametrize("case", list(SPLIT))
+@pytest.mark.parametrize("how", ["plain", "bent", "dropped"])
+def test_split_work(case, how):
+    ql, kl = SPLIT[case]
+    qo, ko = offsets(ql), offsets(kl)
+    x = inputs(int(qo[-1]), int(ko[-1]), 4, 2, 72, 20)
+    kw = {} if how == "plain" else dict(causal=True, cap=8.0, slopes=torch.tensor([0.01, 0.0, 0.1, 0.003]))
+    drop = dict(drop_p=0.3, seed=99) if how == "dropped" else {}
+    keep = keep_mask(4, x[0].shape[0], x[1].shape[0], 0.3, 99) if drop else None
+    got = run(*x, heads=4, kv_heads=2, q_offsets=qo, k_offsets=ko, **kw, **drop)
+    check(got, reference(*x, 4, 2, qo, ko, keep=keep, drop=0.3, **kw))
+    again = run(*x, heads=4, kv_heads=2, q_offsets=qo, k_offsets=ko, **kw, **drop)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("case", ["few_rows", "few_keys", "both"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("which", ["k", "v", "q", "do"])
+def test_split_work_with_what_is_not_finite(case, value, which):
+    ql, kl = SPLIT[case]
+    qo, ko = offsets(ql), offsets(kl)
+    x = dict(zip(("q", "k", "v", "do"), inputs(int(qo[-1]), int(ko[-1]), 4, 2, 72, 21)))
+    clean = [t.clone() for t in x.values()]
+    x[which][0, 5] = value                                 # document 0
+    got = run(*x.values(), heads=4, kv_heads=2, q_offsets=qo, k_offsets=ko)
+    rows, keys = torch.arange(int(qo[1]), int(qo[-1])), torch.arange(int(ko[1]), int(ko[-1]))
+    check(got, reference(*clean, 4, 2, qo, ko), {"out": rows, "dq": rows, "dk": keys, "dv": keys})
+    assert not torch.isfinite(torch.cat([got[n][:1].float().flatten() for n in ("out", "dq", "dk", "dv")])).all()
