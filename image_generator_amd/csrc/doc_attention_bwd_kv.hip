@@ -48,7 +48,7 @@ struct RowInfo {                     // of the 64 staged rows
 };
 
 template <int ND, int NO, int KIND, int KB>
-__global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p) {
+__global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int tiles) {
     constexpr int LD = tr_ld(NO);
     constexpr int NCH = (64 * NO * 4 + 255) / 256;
     __shared__ __attribute__((aligned(16))) char smem[2 * 64 * LD];
@@ -56,8 +56,10 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p) {
     __shared__ int range[4][2];
     char *Qs = smem, *Gs = smem + 64 * LD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
-    const int hk = blockIdx.y;
-    const int key0 = (int)(blockIdx.x * 4 + wave) * (32 * KB);
+    int unit, hk;
+    if (!unit_of(tiles * p.splits, p.Hkv, unit, hk)) return;
+    const int split = unit / tiles, tile = unit - split * tiles;
+    const int key0 = (tile * 4 + wave) * (32 * KB);
     const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
     bf16x8 kf[KB][ND], vf[KB][ND];
     bool seen[KB];
@@ -96,9 +98,9 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p) {
     const unsigned G = (unsigned)p.G;
     unsigned rlo = tlo < thi ? tlo * G : 0u, rhi = tlo < thi ? thi * G : 0u;
     if (p.splits > 1) {
-        const unsigned tiles = (rhi - rlo + 63) / 64, each = (tiles + p.splits - 1) / p.splits;
-        const unsigned from = rlo + min(tiles, each * blockIdx.z) * 64;
-        rhi = min(rhi, rlo + min(tiles, each * (blockIdx.z + 1)) * 64);
+        const unsigned n = (rhi - rlo + 63) / 64, each = (n + p.splits - 1) / p.splits;
+        const unsigned from = rlo + min(n, each * split) * 64;
+        rhi = min(rhi, rlo + min(n, each * (split + 1)) * 64);
         rlo = from;
     }
     const unsigned wlo = lo < hi ? lo * G : 0xffffffffu, whi = lo < hi ? hi * G : 0u;
@@ -261,7 +263,7 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p) {
         const int key = key0 + kb * 32 + l31;
         if (key >= p.Tk) continue;
         bf16_t *dk = p.dk + (size_t)key * p.lddk + (size_t)hk * p.D, *dv = p.dv + (size_t)key * p.lddv + (size_t)hk * p.D;
-        float* part = p.part + (((size_t)blockIdx.z * p.Tk + key) * p.Hkv + hk) * 2 * p.D;
+        float* part = p.part + (((size_t)split * p.Tk + key) * p.Hkv + hk) * 2 * p.D;
 #pragma unroll
         for (int db = 0; db < NO; ++db)
 #pragma unroll
@@ -321,10 +323,11 @@ __global__ __launch_bounds__(256) void doc_dkdv_join_kernel(const DocArgs p) {
 
 template <int ND, int NO, int KB>
 void launch_kind(const DocArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)(((long long)a.Tk + 128 * KB - 1) / (128 * KB)), a.Hkv, a.splits);
-    if (a.drop_thresh) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, DROPPED, KB>), grid, dim3(256), 0, st, a);
-    else if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, BENT, KB>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, PLAIN, KB>), grid, dim3(256), 0, st, a);
+    const int tiles = (int)(((long long)a.Tk + 128 * KB - 1) / (128 * KB));
+    const dim3 grid(unit_grid((long long)tiles * a.splits, a.Hkv));
+    if (a.drop_thresh) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, DROPPED, KB>), grid, dim3(256), 0, st, a, tiles);
+    else if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, BENT, KB>), grid, dim3(256), 0, st, a, tiles);
+    else hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, PLAIN, KB>), grid, dim3(256), 0, st, a, tiles);
 }
 
 template <int ND, int NO>
@@ -337,13 +340,13 @@ int launch(const DocArgs& a, hipStream_t st) {
 }  // namespace
 
 // Workgroups without a split: one per 128 keys and key head, each passing about G * (the rows of one document, and of the others
-// that its keys belong to).  Runs of at least 8 tiles, until the chip has about 1024 workgroups.
+// that its keys belong to).  Runs of at least 8 tiles, until the chip has about 1536 workgroups.
 int doc_bwd_kv_splits(int Tq, int Tk, int Hq, int Hkv, int docs) {
     if (Tk < 1) return 1;
     const double wgs = (double)((Tk + 127) / 128) * Hkv, keys_per_doc = (double)Tk / docs;
     const double tiles = (double)Tq * (Hq / Hkv) / docs * (1.0 + 127.0 / (keys_per_doc < 1.0 ? 1.0 : keys_per_doc)) / 64.0;
     const double cap = (double)Tq * (Hq / Hkv) / 64.0;
-    double s = 1024.0 / wgs, most = (tiles < cap ? tiles : cap) / 8.0;
+    double s = 1536.0 / wgs, most = (tiles < cap ? tiles : cap) / 8.0;
     if (s > most) s = most;
     return s < 2.0 ? 1 : s > 64.0 ? 64 : (int)s;
 }

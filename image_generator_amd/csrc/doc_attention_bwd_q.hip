@@ -6,15 +6,16 @@
 namespace {
 
 template <int ND, int NO, int KIND>
-__global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p) {
+__global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles) {
     constexpr int DP = 16 * ND, KLD = tr_ld(NO), VLD = DP * 2 + 16;
     constexpr int NCK = (64 * NO * 4 + 255) / 256, NCV = (64 * (DP / 8) + 255) / 256;
     __shared__ __attribute__((aligned(16))) char smem[64 * KLD + 64 * VLD];
     __shared__ int range[4][2];
     char *Ks = smem, *Vs = smem + 64 * KLD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
-    const int hk = blockIdx.y;
-    const unsigned R = blockIdx.x * 128u + wave * 32 + l31;
+    int tile, hk;
+    if (!unit_of(tiles, p.Hkv, tile, hk)) return;
+    const unsigned R = tile * 128u + wave * 32 + l31;
     const bool live = R < (unsigned)p.Tq * (unsigned)p.G;
     int token, head;
     row_of(p, live ? R : 0u, hk, token, head);
@@ -167,10 +168,11 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p) {
 
 template <int ND, int NO>
 int launch(const DocArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)(((long long)a.Tq * a.G + 127) / 128), a.Hkv);
-    if (a.drop_thresh) hipLaunchKernelGGL((doc_dq_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a);
-    else if (a.cap > 0.f || a.slopes) hipLaunchKernelGGL((doc_dq_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((doc_dq_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a);
+    const int tiles = (int)(((long long)a.Tq * a.G + 127) / 128);
+    const dim3 grid(unit_grid(tiles, a.Hkv));
+    if (a.drop_thresh) hipLaunchKernelGGL((doc_dq_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a, tiles);
+    else if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) hipLaunchKernelGGL((doc_dq_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a, tiles);
+    else hipLaunchKernelGGL((doc_dq_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a, tiles);
     return mi355_check_launch("doc_attention_dq");
 }
 

@@ -146,16 +146,17 @@ struct Rows {                        // a wave's 32 rows
 };
 
 template <int ND, int NO, int KIND>
-__global__ __launch_bounds__(256) void doc_fwd_kernel(const DocArgs p) {
+__global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_fwd_kernel(const DocArgs p, int tiles) {
     constexpr int DP = 16 * ND, KLD = DP * 2 + 16, VLD = tr_ld(NO);
     constexpr int NCK = (64 * (DP / 8) + 255) / 256, NCV = (64 * NO * 4 + 255) / 256;
     __shared__ __attribute__((aligned(16))) char smem[64 * KLD + 64 * VLD];
     __shared__ int range[4][2];
     char *Ks = smem, *Vs = smem + 64 * KLD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
-    const int hk = blockIdx.y;
+    int tile, hk;
+    if (!unit_of(tiles, p.Hkv, tile, hk)) return;
     Rows<ND, NO> w;
-    w.init(p, blockIdx.x * 128u + wave * 32 + l31, hk);
+    w.init(p, tile * 128u + wave * 32 + l31, hk);
     if (lane == 0) { range[wave][0] = w.hi > w.lo ? w.lo : 0x7fffffff; range[wave][1] = w.hi; }
     __syncthreads();
     const int klo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
@@ -343,10 +344,11 @@ int launch(const DocArgs& a, hipStream_t st) {
     const bool bent = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
     if (a.splits)
         return a.drop_thresh ? launch_split<ND, NO, DROPPED>(a, st) : bent ? launch_split<ND, NO, BENT>(a, st) : launch_split<ND, NO, PLAIN>(a, st);
-    const dim3 grid((unsigned)(((long long)a.Tq * a.G + 127) / 128), a.Hkv);
-    if (a.drop_thresh) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a);
-    else if (bent) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a);
+    const int tiles = (int)(((long long)a.Tq * a.G + 127) / 128);
+    const dim3 grid(unit_grid(tiles, a.Hkv));
+    if (a.drop_thresh) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a, tiles);
+    else if (bent) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a, tiles);
+    else hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a, tiles);
     return mi355_check_launch("doc_attention_fwd");
 }
 

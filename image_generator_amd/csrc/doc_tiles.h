@@ -107,6 +107,23 @@ __device__ __forceinline__ void row_of(const DocArgs& p, unsigned R, int hk, int
     head = hk * p.G + (int)(R - t * (unsigned)p.G);
 }
 
+// Workgroup -> (unit, key head), a unit being a tile (and one of its runs).  Ids go to the 8 XCDs in turn: the heads of a unit
+// follow each other on one XCD, so the lines and pages that neighbouring heads share (a head's columns are a piece of each
+// row) are fetched once, and neighbouring tiles, whose work grows alike along a causal document, spread over all XCDs.
+// Fewer units than fill the XCDs evenly: heads spread too.
+__device__ __forceinline__ bool unit_of(int units, int heads, int& unit, int& head) {
+    if (units < 64) {
+        unit = (int)blockIdx.x / heads;
+        head = (int)blockIdx.x - unit * heads;
+        return true;
+    }
+    const int slot = (int)(blockIdx.x >> 3), group = slot / heads;
+    head = slot - group * heads;
+    unit = group * 8 + (int)(blockIdx.x & 7);
+    return unit < units;
+}
+inline unsigned unit_grid(long long units, int heads) { return (unsigned)(units < 64 ? units * heads : (units + 7) / 8 * 8 * heads); }
+
 int doc_fwd_tiles(const DocArgs& a, hipStream_t st);
 int doc_bwd_q_tiles(const DocArgs& a, hipStream_t st);
 int doc_bwd_kv_tiles(const DocArgs& a, hipStream_t st);
