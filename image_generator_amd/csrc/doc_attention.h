@@ -45,8 +45,35 @@ __device__ __forceinline__ int doc_of(const int* __restrict__ off, int docs, int
     return a;
 }
 
-__device__ __forceinline__ RowSpan row_span(const DocArgs& p, int i) {
-    const int n = doc_of(p.q_off, p.docs, i);
+// The same for the 64 tokens i of a wave (every lane active), all in a stretch that begins at i0: the document of i0 by a search
+// that probes 64 places a step (two loads for 4096 documents), then the next 64 boundaries in one load and a search among
+// registers.  A lane's own binary search is a chain of loads: it was a third of a caption tile's time.
+__device__ __forceinline__ int doc_of_wave(const int* __restrict__ off, int docs, int i0, int i) {
+    const int lane = threadIdx.x & 63;
+    int a = 0, b = docs;
+    while (b - a > 1) {
+        const int step = (b - a + 63) / 64, at = a + 1 + lane * step;
+        const int count = __popcll(__ballot(at < b && off[min(at, docs)] <= i0));
+        if (count == 0) break;
+        a += 1 + (count - 1) * step;
+        b = min(b, a + step);
+    }
+    const int bound = a + 1 + lane < docs ? off[a + 1 + lane] : 0x7fffffff;
+    int n = 0;
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) if (__shfl(bound, n + s - 1, 64) <= i) n += s;
+    if (n == 63 && __shfl(bound, 63, 64) <= i) {               // past the 64 boundaries: many tiny documents
+        int lo = min(a + 64, docs - 1), hi = docs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (off[mid] <= i) lo = mid; else hi = mid;
+        }
+        return lo;
+    }
+    return a + n;
+}
+
+__device__ __forceinline__ RowSpan row_span_in(const DocArgs& p, int i, int n) {
     const int qb = p.q_off[n], qe = p.q_off[n + 1];
     int kb = max(p.k_off[n], 0), ke = min(p.k_off[n + 1], p.Tk);
     RowSpan s = {0, 0, 0};
@@ -62,9 +89,10 @@ __device__ __forceinline__ RowSpan row_span(const DocArgs& p, int i) {
     return s;
 }
 
-// tokens whose rows may see key j: [first, last)
-__device__ __forceinline__ int2 key_span(const DocArgs& p, int j) {
-    const int n = doc_of(p.k_off, p.docs, j);
+__device__ __forceinline__ RowSpan row_span(const DocArgs& p, int i) { return row_span_in(p, i, doc_of(p.q_off, p.docs, i)); }
+
+// tokens whose rows may see key j of document n: [first, last)
+__device__ __forceinline__ int2 key_span_in(const DocArgs& p, int j, int n) {
     const int kb = max(p.k_off[n], 0), ke = min(p.k_off[n + 1], p.Tk);
     const int qb = p.q_off[n], qe = p.q_off[n + 1];
     if (j < kb || j >= ke || qb >= qe) return make_int2(0, 0);
@@ -77,6 +105,7 @@ __device__ __forceinline__ int2 key_span(const DocArgs& p, int j) {
     const int f = (int)(first < 0 ? 0 : first > last ? last : first);
     return make_int2(f, last);
 }
+__device__ __forceinline__ int2 key_span(const DocArgs& p, int j) { return key_span_in(p, j, doc_of(p.k_off, p.docs, j)); }
 
 __device__ __forceinline__ float tanh_f(float x) {
     return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * LOG2E)));

@@ -65,17 +65,25 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
     bool seen[KB];
     int lo = 0x7fffffff, hi = 0;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-        const int key = key0 + kb * 32 + l31;
-        const int2 span = key < p.Tk ? key_span(p, key) : make_int2(0, 0);
-        seen[kb] = span.y > span.x;
-        if (seen[kb]) { lo = min(lo, span.x); hi = max(hi, span.y); }
+    for (int kb = 0; kb < KB; ++kb) {                 // on their way while the keys' rows are looked up
+        const int key = min(key0 + kb * 32 + l31, p.Tk - 1);
 #pragma unroll
         for (int ks = 0; ks < ND; ++ks) {
             const int d = ks * 16 + 8 * hh;
-            const bool ok = seen[kb] && d < p.D;
-            kf[kb][ks] = ok ? *(const bf16x8*)(k_row(p, key, hk) + d) : zero8;
-            vf[kb][ks] = ok ? *(const bf16x8*)(v_row(p, key, hk) + d) : zero8;
+            kf[kb][ks] = d < p.D ? *(const bf16x8*)(k_row(p, key, hk) + d) : zero8;
+            vf[kb][ks] = d < p.D ? *(const bf16x8*)(v_row(p, key, hk) + d) : zero8;
+        }
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+        const int key = min(key0 + kb * 32 + l31, p.Tk - 1);
+        const int2 span = key_span_in(p, key, doc_of_wave(p.k_off, p.docs, __builtin_amdgcn_readfirstlane(key), key));
+        seen[kb] = key0 + kb * 32 + l31 < p.Tk && span.y > span.x;
+        if (seen[kb]) { lo = min(lo, span.x); hi = max(hi, span.y); }
+#pragma unroll
+        for (int ks = 0; ks < ND; ++ks) {
+            kf[kb][ks] = seen[kb] ? kf[kb][ks] : zero8;
+            vf[kb][ks] = seen[kb] ? vf[kb][ks] : zero8;
         }
     }
     lo = __builtin_amdgcn_readfirstlane(wave_min_i(lo));

@@ -15,11 +15,32 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
     int tile, hk;
     if (!unit_of(tiles, p.Hkv, tile, hk)) return;
-    const unsigned R = tile * 128u + wave * 32 + l31;
-    const bool live = R < (unsigned)p.Tq * (unsigned)p.G;
+    const unsigned rows = (unsigned)p.Tq * (unsigned)p.G, R = tile * 128u + wave * 32 + l31;
+    const bool live = R < rows;
     int token, head;
-    row_of(p, live ? R : 0u, hk, token, head);
-    RowSpan span = row_span(p, token);
+    row_of(p, live ? R : rows - 1, hk, token, head);
+    const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
+    bf16x8 qf[ND], gf[ND];
+    float delta = 0.f;
+    {   // on their way while the intervals are looked up
+        const bf16_t* q = q_row(p, token, head);
+        const bf16_t* g = p.dout + (size_t)token * p.lddo + (size_t)head * p.D;
+        const bf16_t* o = p.o + (size_t)token * p.ldo + (size_t)head * p.D;
+        bf16x8 ov[ND];
+#pragma unroll
+        for (int ks = 0; ks < ND; ++ks) {
+            const int d = ks * 16 + 8 * hh;
+            qf[ks] = d < p.D ? *(const bf16x8*)(q + d) : zero8;
+            gf[ks] = d < p.D ? *(const bf16x8*)(g + d) : zero8;
+            ov[ks] = d < p.D ? *(const bf16x8*)(o + d) : zero8;
+        }
+#pragma unroll
+        for (int ks = 0; ks < ND; ++ks)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = fmaf((float)ov[ks][e], (float)gf[ks][e], delta);
+        delta += __shfl_xor(delta, 32, 64);
+    }
+    RowSpan span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, __builtin_amdgcn_readfirstlane(token), token));
     if (live && hh == 0 && head == 0) p.rows[token] = make_int4(span.lo, span.hi, span.c, 0);
     if (!live) span.lo = span.hi = 0;
     const bool sees = span.hi > span.lo;
@@ -27,24 +48,11 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles)
     const int hi = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.hi : 0));
     const int in_lo = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.lo : 0));
     const int in_hi = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.hi : 0x7fffffff));
-    const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
-    bf16x8 qf[ND], gf[ND];
-    float delta = 0.f;
-    {
-        const bf16_t* q = q_row(p, token, head);
-        const bf16_t* g = p.dout + (size_t)token * p.lddo + (size_t)head * p.D;
-        const bf16_t* o = p.o + (size_t)token * p.ldo + (size_t)head * p.D;
+    if (!sees) delta = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < ND; ++ks) {
-            const int d = ks * 16 + 8 * hh;
-            const bool ok = sees && d < p.D;
-            qf[ks] = ok ? *(const bf16x8*)(q + d) : zero8;
-            gf[ks] = ok ? *(const bf16x8*)(g + d) : zero8;
-            const bf16x8 ov = ok ? *(const bf16x8*)(o + d) : zero8;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) delta = fmaf((float)ov[e], (float)gf[ks][e], delta);
-        }
-        delta += __shfl_xor(delta, 32, 64);
+    for (int ks = 0; ks < ND; ++ks) {
+        qf[ks] = sees ? qf[ks] : zero8;
+        gf[ks] = sees ? gf[ks] : zero8;
     }
     const size_t at = (size_t)head * p.Tq + token;
     if (live && hh == 0) p.delta[at] = delta;

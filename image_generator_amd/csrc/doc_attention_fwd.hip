@@ -22,11 +22,20 @@ struct Rows {                        // a wave's 32 rows
     int lo, hi;                      // union of the intervals (wave-uniform)
     int in_lo, in_hi;                // their intersection
 
-    __device__ __forceinline__ void init(const DocArgs& p, unsigned R, int hk) {
+    // R0: the wave's first row
+    __device__ __forceinline__ void init(const DocArgs& p, unsigned R0, int hk) {
         const int hh = (threadIdx.x & 63) >> 5;
-        live = R < (unsigned)p.Tq * (unsigned)p.G;
-        row_of(p, live ? R : 0u, hk, token, head);
-        span = row_span(p, token);
+        const unsigned rows = (unsigned)p.Tq * (unsigned)p.G, R = R0 + (threadIdx.x & 31);
+        live = R < rows;
+        row_of(p, live ? R : rows - 1, hk, token, head);
+        const bf16_t* q = q_row(p, token, head);
+        const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < ND; ++ks) {             // on their way while the intervals are looked up
+            const int d = ks * 16 + 8 * hh;
+            qf[ks] = d < p.D ? *(const bf16x8*)(q + d) : zero8;
+        }
+        span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, __builtin_amdgcn_readfirstlane(token), token));
         if (!live) span.lo = span.hi = 0;
         const bool sees = span.hi > span.lo;
         lo = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.lo : 0x7fffffff));
@@ -35,13 +44,8 @@ struct Rows {                        // a wave's 32 rows
         in_lo = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.lo : 0));
         in_hi = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.hi : 0x7fffffff));
         if (lo > hi) lo = hi = 0;
-        const bf16_t* q = q_row(p, token, head);
-        const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (int ks = 0; ks < ND; ++ks) {
-            const int d = ks * 16 + 8 * hh;
-            qf[ks] = (sees && d < p.D) ? *(const bf16x8*)(q + d) : zero8;
-        }
+        for (int ks = 0; ks < ND; ++ks) qf[ks] = sees ? qf[ks] : zero8;
         slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;
         drop = drop_row(p, token, head);
 #pragma unroll
@@ -152,11 +156,11 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_fwd_kernel(const Doc
     __shared__ __attribute__((aligned(16))) char smem[64 * KLD + 64 * VLD];
     __shared__ int range[4][2];
     char *Ks = smem, *Vs = smem + 64 * KLD;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
     int tile, hk;
     if (!unit_of(tiles, p.Hkv, tile, hk)) return;
     Rows<ND, NO> w;
-    w.init(p, tile * 128u + wave * 32 + l31, hk);
+    w.init(p, tile * 128u + wave * 32, hk);
     if (lane == 0) { range[wave][0] = w.hi > w.lo ? w.lo : 0x7fffffff; range[wave][1] = w.hi; }
     __syncthreads();
     const int klo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
@@ -222,7 +226,7 @@ __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) 
     const int hk = blockIdx.y, split = blockIdx.z * 4 + wave;
     const unsigned R = blockIdx.x * 32u + l31;
     Rows<ND, NO> w;
-    w.init(p, R, hk);
+    w.init(p, blockIdx.x * 32u, hk);
     int from, to;
     {
         const int tiles = (w.hi - w.lo + 63) / 64, each = (tiles + p.splits - 1) / p.splits;
