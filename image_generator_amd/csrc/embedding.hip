@@ -11,16 +11,19 @@
 
 namespace {
 
-constexpr int SORT1 = 8192;          // ids that one workgroup sorts in LDS
+constexpr int RANKED = 8192;         // ids sorted by counting, for each, those below it
+constexpr int SHARES = 16;           // lanes that count for one id
 constexpr int TILE = 2048;           // ids per workgroup of a radix pass: four waves with 512 consecutive ids each
 constexpr int MAXBINS = 256;
-constexpr int CHUNK = 64;            // sorted positions of one id that are summed ahead when they fill an aligned chunk ...
-constexpr int SUPER = 64;            // ... and aligned runs of so many such chunks
+constexpr int CHUNK = 32;            // sorted positions of one id that are summed ahead when they fill an aligned chunk ...
+constexpr int SUPER = 32;            // ... and aligned runs of so many such chunks
 
 template <typename T> __device__ __forceinline__ float ldf(const T* p) { return (float)*p; }
 template <typename T> struct Vec4;
 template <> struct Vec4<float> { typedef f32x4 t; };
 template <> struct Vec4<bf16_t> { typedef bf16x4 t; };
+template <typename T, int VEC> struct Raw { typedef typename Vec4<T>::t t; };
+template <typename T> struct Raw<T, 1> { typedef T t; };
 template <typename T> __device__ __forceinline__ f32x4 ld4(const T* p) {
     const typename Vec4<T>::t v = *(const typename Vec4<T>::t*)p;
     return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
@@ -37,7 +40,7 @@ __device__ __forceinline__ long long load_id(const void* ids, int ids64, size_t 
 }
 
 // ---- rows -------------------------------------------------------------------------------------------------------
-// One thread per 4 (or, for odd widths and unaligned tensors, 1) elements of the output; bound by the bytes of the rows.
+// One thread per 8 (or, for odd widths and unaligned tensors, 1) elements of the output; bound by the bytes of the rows.
 template <typename TI, typename TO, int VEC>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const void* __restrict__ ids, int ids64, const TI* __restrict__ table,
                                                          TO* __restrict__ out, unsigned total, unsigned per_row, long long rows,
@@ -49,44 +52,40 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const void* __restrict_
     const bool ok = id >= 0 && id < rows;
     const TI* src = table + (size_t)(ok ? id : 0) * width + c;
     TO* dst = out + (size_t)row * width + c;
-    if constexpr (VEC == 4) {
-        f32x4 v = {NAN, NAN, NAN, NAN};
-        if (ok) v = ld4(src) * scale;
-        st4(dst, v);
+    if constexpr (VEC == 8) {
+        const float f = ok ? scale : NAN;
+        f32x4 a = ld4(src), b = ld4(src + 4);
+        a = ok ? a * f : f32x4{NAN, NAN, NAN, NAN};
+        b = ok ? b * f : f32x4{NAN, NAN, NAN, NAN};
+        if constexpr (sizeof(TO) == 2)
+            *(bf16x8*)dst = bf16x8{(bf16_t)a[0], (bf16_t)a[1], (bf16_t)a[2], (bf16_t)a[3], (bf16_t)b[0], (bf16_t)b[1], (bf16_t)b[2], (bf16_t)b[3]};
+        else { st4(dst, a); st4(dst + 4, b); }
     } else {
         *dst = ok ? (TO)(ldf(src) * scale) : (TO)NAN;
     }
 }
 
-// ---- sort: up to SORT1 ids by one workgroup -----------------------------------------------------------------------
-// Bitonic network over id * 2^posbits + position: unique keys, so the order is that of a stable sort.
-template <typename KEY>
-__global__ __launch_bounds__(1024) void sort_small_kernel(const void* __restrict__ ids, int ids64, int n, int n2, int posbits,
-                                                          unsigned rows, unsigned* __restrict__ keys, unsigned* __restrict__ pos) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    KEY* s = (KEY*)smem;
-    for (int i = threadIdx.x; i < n2; i += blockDim.x) {
-        KEY k = ~(KEY)0;
-        if (i < n) {
-            const long long id = load_id(ids, ids64, i);
-            k = ((KEY)(id >= 0 && id < (long long)rows ? (unsigned)id : rows) << posbits) | (KEY)i;
-        }
-        s[i] = k;
+// ---- sort: up to RANKED ids ---------------------------------------------------------------------------------------
+// The place of an id in the sorted list is the number of (id, position) pairs below its own.  That is n^2 comparisons, but
+// spread over the chip (16 lanes for each id, every workgroup with the whole list in LDS) they take 2 us at 8192 ids, where a
+// sort by one workgroup is a chain of 91 steps (19 us at 2048 ids).
+__global__ __launch_bounds__(256) void rank_sort_kernel(const void* __restrict__ ids, int ids64, int n, unsigned rows,
+                                                        unsigned* __restrict__ keys, unsigned* __restrict__ pos) {
+    extern __shared__ __attribute__((aligned(16))) unsigned list[];
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const long long id = load_id(ids, ids64, i);
+        list[i] = id >= 0 && id < (long long)rows ? (unsigned)id : rows;
     }
     __syncthreads();
-    for (int size = 2; size <= n2; size <<= 1)
-        for (int step = size >> 1; step > 0; step >>= 1) {
-            for (int t = threadIdx.x; t < n2 / 2; t += blockDim.x) {
-                const int i = ((t & ~(step - 1)) << 1) | (t & (step - 1)), j = i + step;
-                const KEY a = s[i], b = s[j];
-                if ((a > b) == ((i & size) == 0)) { s[i] = b; s[j] = a; }
-            }
-            __syncthreads();
-        }
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        keys[i] = (unsigned)(s[i] >> posbits);
-        pos[i] = (unsigned)(s[i] & (((KEY)1 << posbits) - 1));
-    }
+    const int mine = blockIdx.x * (256 / SHARES) + threadIdx.x / SHARES, share = threadIdx.x % SHARES;
+    if (mine >= n) return;                       // whole groups of SHARES lanes
+    const unsigned key = list[mine];
+    int below = 0;
+#pragma unroll 8
+    for (int j = share; j < n; j += SHARES) below += list[j] < key || (list[j] == key && j < mine) ? 1 : 0;
+#pragma unroll
+    for (int o = 1; o < SHARES; o <<= 1) below += __shfl_xor(below, o, 64);
+    if (share == 0) { keys[below] = key; pos[below] = mine; }
 }
 
 // ---- sort: any number of ids, least significant digit first ---------------------------------------------------------
@@ -115,43 +114,36 @@ __global__ __launch_bounds__(256) void radix_count_kernel(const void* __restrict
     if (threadIdx.x <= mask) counts[(size_t)threadIdx.x * tiles + blockIdx.x] = hist[threadIdx.x];
 }
 
-// In place: counts -> exclusive prefix sums, one workgroup, 4096 consecutive entries per round.
-__global__ __launch_bounds__(1024) void scan_kernel(unsigned* __restrict__ counts, int total) {
-    __shared__ unsigned wsum[16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// counts[bin][tile] -> exclusive prefix sums along the tiles, and the bin's total: a wave per bin.
+__global__ __launch_bounds__(256) void scan_kernel(unsigned* __restrict__ counts, unsigned* __restrict__ totals, int bins, int tiles) {
+    const int lane = threadIdx.x & 63, bin = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (bin >= bins) return;
+    unsigned* row = counts + (size_t)bin * tiles;
     unsigned carry = 0;
-    for (int base = 0; base < total; base += 4096) {
-        const int i = base + threadIdx.x * 4;
-        unsigned v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = i + e < total ? counts[i + e] : 0u;
-        const unsigned mine = v[0] + v[1] + v[2] + v[3];
-        unsigned inc = mine;
+    for (int base = 0; base < tiles; base += 64) {
+        const int i = base + lane;
+        const unsigned v = i < tiles ? row[i] : 0u;
+        unsigned inc = v;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const unsigned t = __shfl_up(inc, o, 64);
             if (lane >= o) inc += t;
         }
-        if (lane == 63) wsum[wave] = inc;
-        __syncthreads();
-        unsigned before = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < 16; ++w) { if (w < wave) before += wsum[w]; all += wsum[w]; }
-        unsigned run = carry + before + inc - mine;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { if (i + e < total) counts[i + e] = run; run += v[e]; }
-        carry += all;
-        __syncthreads();
+        if (i < tiles) row[i] = carry + inc - v;
+        carry += __shfl(inc, 63, 64);
     }
+    if (lane == 0) totals[bin] = carry;
 }
 
 template <bool FIRST>
 __global__ __launch_bounds__(256) void radix_scatter_kernel(const void* __restrict__ ids, int ids64, const unsigned* __restrict__ keys,
                                                             const unsigned* __restrict__ pos, int n, unsigned rows, int shift, int bits,
                                                             int tiles, const unsigned* __restrict__ starts,
+                                                            const unsigned* __restrict__ totals,
                                                             unsigned* __restrict__ keys_out, unsigned* __restrict__ pos_out) {
     constexpr int ROUNDS = TILE / 256;
     __shared__ unsigned cnt[4][MAXBINS];
+    __shared__ unsigned wsum[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned mask = (1u << bits) - 1;
 #pragma unroll
@@ -179,8 +171,18 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(const void* __restri
     }
     __syncthreads();
     {   // counts of the four waves -> where each wave's first entry of a digit goes
-        const unsigned d = threadIdx.x;
-        unsigned at = d <= mask ? starts[(size_t)d * tiles + blockIdx.x] : 0u;
+        const unsigned d = threadIdx.x, total = d <= mask ? totals[d] : 0u;
+        unsigned inc = total;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned t = __shfl_up(inc, o, 64);
+            if (lane >= o) inc += t;
+        }
+        if (lane == 63) wsum[wave] = inc;
+        __syncthreads();
+        unsigned at = inc - total + (d <= mask ? starts[(size_t)d * tiles + blockIdx.x] : 0u);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) if (w < wave) at += wsum[w];
 #pragma unroll
         for (int w = 0; w < 4; ++w) { const unsigned c = cnt[w][d]; cnt[w][d] = at; at += c; }
     }
@@ -197,39 +199,41 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(const void* __restri
 }
 
 // ---- sums -----------------------------------------------------------------------------------------------------------
-// Adds `count` rows src[idx(j)][col0 ..] to acc: a wave, four columns per lane and sweep, four rows in flight.
-constexpr int SWEEPS = 4;            // 256 columns each
+// Adds `count` rows src[idx(j)][col0 ..] to acc in order: a wave, VEC columns per lane and sweep, eight rows in flight.  Every
+// load is issued (lanes past the row's end repeat its last columns, what they add up is not stored): a load behind a
+// condition is waited for on the spot.
+constexpr int SWEEPS = 3;            // of 64 * VEC columns
 template <int VEC, typename T, typename IDX>
 __device__ __forceinline__ void add_rows(f32x4 (&acc)[SWEEPS], const T* __restrict__ src, int width, int col0, int count, IDX idx) {
     const int lane = threadIdx.x & 63;
-    int j = 0;
-    for (; j + 4 <= count; j += 4) {
-        const T* r[4];
+    constexpr int FLY = 8;
+    int col[SWEEPS];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = src + (size_t)idx(j + e) * width;
+    for (int s = 0; s < SWEEPS; ++s) col[s] = min(col0 + (s * 64 + lane) * VEC, width - VEC);
+    const int sweeps = min(SWEEPS, (width - col0 + 64 * VEC - 1) / (64 * VEC));
+    for (int b = 0; b < count; b += 64) {
+        const int n = min(64, count - b);
+        const unsigned mine = idx(b + min(lane, n - 1));
+        for (int j = 0; j < n; j += FLY) {
+            const T* r[FLY];
 #pragma unroll
-        for (int s = 0; s < SWEEPS; ++s) {
-            const int c = col0 + s * 64 * VEC + lane * VEC;
-            if (c < width) {
-                if constexpr (VEC == 4) {
-                    const f32x4 a = ld4(r[0] + c), b = ld4(r[1] + c), d = ld4(r[2] + c), e = ld4(r[3] + c);
-                    acc[s] = acc[s] + a; acc[s] = acc[s] + b; acc[s] = acc[s] + d; acc[s] = acc[s] + e;
-                } else {
-                    const float a = ldf(r[0] + c), b = ldf(r[1] + c), d = ldf(r[2] + c), e = ldf(r[3] + c);
-                    acc[s][0] += a; acc[s][0] += b; acc[s][0] += d; acc[s][0] += e;
+            for (int e = 0; e < FLY; ++e) r[e] = src + (size_t)(unsigned)__builtin_amdgcn_readlane((int)mine, min(j + e, n - 1)) * width;
+            typename Raw<T, VEC>::t v[FLY][SWEEPS];
+#pragma unroll
+            for (int s = 0; s < SWEEPS; ++s)
+                if (s < sweeps) {
+#pragma unroll
+                    for (int e = 0; e < FLY; ++e) v[e][s] = *(const typename Raw<T, VEC>::t*)(r[e] + col[s]);
                 }
-            }
-        }
-    }
-    for (; j < count; ++j) {
-        const T* r = src + (size_t)idx(j) * width;
 #pragma unroll
-        for (int s = 0; s < SWEEPS; ++s) {
-            const int c = col0 + s * 64 * VEC + lane * VEC;
-            if (c < width) {
-                if constexpr (VEC == 4) acc[s] = acc[s] + ld4(r + c);
-                else acc[s][0] += ldf(r + c);
-            }
+            for (int e = 0; e < FLY; ++e)
+                if (j + e < n)
+#pragma unroll
+                    for (int s = 0; s < SWEEPS; ++s)
+                        if (s < sweeps) {
+                            if constexpr (VEC == 4) acc[s] = acc[s] + f32x4{(float)v[e][s][0], (float)v[e][s][1], (float)v[e][s][2], (float)v[e][s][3]};
+                            else acc[s][0] += (float)v[e][s];
+                        }
         }
     }
 }
@@ -250,7 +254,7 @@ __device__ __forceinline__ void put_row(T* __restrict__ dst, const f32x4 (&acc)[
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void chunk_sum_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ pos, int n,
                                                         unsigned rows, const T* __restrict__ dy, int width, float* __restrict__ part) {
-    const int c = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int c = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const int lo = c * CHUNK;
     if (lo + CHUNK > n) return;
     const unsigned k = keys[lo];
@@ -276,7 +280,7 @@ __global__ __launch_bounds__(64) void super_sum_kernel(const unsigned* __restric
 
 // Every row of the table, written once: a wave takes the sorted positions of its id (found by binary search) in order, whole
 // aligned chunks and runs of chunks from their sums; an id without positions gets zeros.
-constexpr int ROWS_PER_WG = 8;
+constexpr int ROWS_PER_WG = 7;       // eight boundaries: two rounds of the workgroup's four waves
 template <typename T, typename TO, int VEC>
 __global__ __launch_bounds__(256) void table_grad_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ pos, int n,
                                                          unsigned rows, const T* __restrict__ dy, int width, float scale,
@@ -284,14 +288,20 @@ __global__ __launch_bounds__(256) void table_grad_kernel(const unsigned* __restr
                                                          TO* __restrict__ dtable) {
     __shared__ int start[ROWS_PER_WG + 1];
     const unsigned v0 = blockIdx.x * ROWS_PER_WG;
-    if (threadIdx.x <= ROWS_PER_WG) {
-        const unsigned v = v0 + threadIdx.x;
-        int lo = 0, hi = n;                                   // first index with keys[index] >= v
+    // first index with keys[index] >= v, for each v of the workgroup: a wave per v and round probes 64 places a step
+    for (int r = threadIdx.x >> 6; r <= ROWS_PER_WG; r += 4) {
+        const unsigned v = v0 + r;
+        const int lane = threadIdx.x & 63;
+        int lo = 0, hi = n;
         while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (keys[mid] < v) lo = mid + 1; else hi = mid;
+            const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+            const int below = __popcll(__ballot(at < hi && keys[min(at, n - 1)] < v));
+            if (below == 0) break;                            // keys[lo] >= v
+            const int last = lo + (below - 1) * step;         // keys[last] < v
+            lo = last + 1;
+            hi = min(hi, last + step);
         }
-        start[threadIdx.x] = lo;
+        if (lane == 0) start[r] = lo;
     }
     __syncthreads();
     for (int r = threadIdx.x >> 6; r < ROWS_PER_WG; r += 4) {
@@ -328,7 +338,7 @@ __global__ __launch_bounds__(256) void table_grad_kernel(const unsigned* __restr
 
 struct GradPlan {
     int n, tiles, passes, bits, keybits;
-    size_t keys, pos, keys2, pos2, counts, part, part2, bytes;   // byte offsets into the workspace
+    size_t keys, pos, keys2, pos2, counts, totals, part, part2, bytes;   // byte offsets into the workspace
 };
 static GradPlan grad_plan(long long n, long long rows, int width) {
     GradPlan g = {};
@@ -342,10 +352,11 @@ static GradPlan grad_plan(long long n, long long rows, int width) {
     auto take = [&](size_t b) { const size_t o = at; at += (b + 255) / 256 * 256; return o; };
     g.keys = take((size_t)n * 4);
     g.pos = take((size_t)n * 4);
-    if (n > SORT1) {
+    if (n > RANKED) {
         g.keys2 = take((size_t)n * 4);
         g.pos2 = take((size_t)n * 4);
         g.counts = take((size_t)g.tiles * MAXBINS * 4);
+        g.totals = take(MAXBINS * 4);
     }
     g.part = take((size_t)(n / CHUNK) * width * 4);
     g.part2 = take((size_t)(n / (CHUNK * SUPER)) * width * 4);
@@ -376,9 +387,9 @@ static void launch_grad(const GradPlan& g, char* ws, const unsigned* keys, const
 template <typename TI, typename TO>
 static void launch_rows(const void* ids, int ids64, long long n, const void* table, long long rows, int width, float scale, void* out,
                         bool vec, hipStream_t st) {
-    const unsigned per_row = vec ? width / 4 : width, total = (unsigned)(n * per_row);
+    const unsigned per_row = vec ? width / 8 : width, total = (unsigned)(n * per_row);
     const dim3 grid((unsigned)(((size_t)total + 255) / 256)), blk(256);
-    if (vec) hipLaunchKernelGGL((embed_rows_kernel<TI, TO, 4>), grid, blk, 0, st, ids, ids64, (const TI*)table, (TO*)out, total, per_row, rows, width, scale);
+    if (vec) hipLaunchKernelGGL((embed_rows_kernel<TI, TO, 8>), grid, blk, 0, st, ids, ids64, (const TI*)table, (TO*)out, total, per_row, rows, width, scale);
     else hipLaunchKernelGGL((embed_rows_kernel<TI, TO, 1>), grid, blk, 0, st, ids, ids64, (const TI*)table, (TO*)out, total, per_row, rows, width, scale);
 }
 
@@ -392,7 +403,7 @@ int mi355_embedding_fwd(const void* ids, int ids64, long long n, const void* tab
     if (n == 0) return MI355_OK;
     if (!ids || !table || !out) return mi355_fail(MI355_ERR_ARG, "embedding: null pointer");
     const hipStream_t st = (hipStream_t)stream;
-    const bool vec = width % 4 == 0 && (uintptr_t)table % (table_bf16 ? 8 : 16) == 0 && (uintptr_t)out % (out_bf16 ? 8 : 16) == 0;
+    const bool vec = width % 8 == 0 && (uintptr_t)table % 16 == 0 && (uintptr_t)out % 16 == 0;
     ProfScope prof(FAM_ELEM, st, (double)n * width * ((table_bf16 ? 2 : 4) + (out_bf16 ? 2 : 4)));
     if (table_bf16) {
         if (out_bf16) launch_rows<bf16_t, bf16_t>(ids, ids64, n, table, rows, width, scale, out, vec, st);
@@ -421,19 +432,13 @@ int mi355_embedding_bwd(const void* ids, int ids64, long long n, const void* dy,
     char* w = (char*)ws;
     unsigned *keys = (unsigned*)(w + g.keys), *pos = (unsigned*)(w + g.pos);
     const unsigned R = (unsigned)rows;
-    if (n > 0 && n <= SORT1) {
-        int n2 = 2, posbits = 1;
-        while (n2 < n) { n2 <<= 1; ++posbits; }
-        const int threads = n2 / 2 < 64 ? 64 : n2 / 2 > 1024 ? 1024 : n2 / 2;
-        if (g.keybits + posbits <= 31)      // all ones stays free for the padding
-            hipLaunchKernelGGL((sort_small_kernel<unsigned>), dim3(1), dim3(threads), n2 * 4, st, ids, ids64, (int)n, n2, posbits, R, keys, pos);
-        else
-            hipLaunchKernelGGL((sort_small_kernel<unsigned long long>), dim3(1), dim3(threads), n2 * 8, st, ids, ids64, (int)n, n2, posbits, R, keys, pos);
+    if (n > 0 && n <= RANKED) {
+        hipLaunchKernelGGL(rank_sort_kernel, dim3((unsigned)((n + 256 / SHARES - 1) / (256 / SHARES))), dim3(256), (size_t)n * 4, st, ids, ids64, (int)n, R, keys, pos);
     } else if (n > 0) {
         unsigned* counts = (unsigned*)(w + g.counts);
         unsigned *k2 = (unsigned*)(w + g.keys2), *p2 = (unsigned*)(w + g.pos2);
         const unsigned mask = (1u << g.bits) - 1;
-        const int total = (int)(mask + 1) * g.tiles;
+        unsigned* totals = (unsigned*)(w + g.totals);
         for (int p = 0; p < g.passes; ++p) {
             const bool into2 = ((g.passes - p) & 1) == 0;        // the last pass ends in (keys, pos)
             const unsigned *ki = into2 ? keys : k2, *pi = into2 ? pos : p2;
@@ -441,9 +446,9 @@ int mi355_embedding_bwd(const void* ids, int ids64, long long n, const void* dy,
             const int shift = p * g.bits;
             if (p == 0) hipLaunchKernelGGL((radix_count_kernel<true>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, g.n, R, shift, mask, g.tiles, counts);
             else hipLaunchKernelGGL((radix_count_kernel<false>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, g.n, R, shift, mask, g.tiles, counts);
-            hipLaunchKernelGGL(scan_kernel, dim3(1), dim3(1024), 0, st, counts, total);
-            if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<true>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, pi, g.n, R, shift, g.bits, g.tiles, counts, ko, po);
-            else hipLaunchKernelGGL((radix_scatter_kernel<false>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, pi, g.n, R, shift, g.bits, g.tiles, counts, ko, po);
+            hipLaunchKernelGGL(scan_kernel, dim3((mask + 4) / 4), dim3(256), 0, st, counts, totals, (int)(mask + 1), g.tiles);
+            if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<true>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, pi, g.n, R, shift, g.bits, g.tiles, counts, totals, ko, po);
+            else hipLaunchKernelGGL((radix_scatter_kernel<false>), dim3(g.tiles), dim3(256), 0, st, ids, ids64, ki, pi, g.n, R, shift, g.bits, g.tiles, counts, totals, ko, po);
         }
     }
     const bool vec = width % 4 == 0 && (uintptr_t)dy % (dy_bf16 ? 8 : 16) == 0 && (uintptr_t)dtable % (out_bf16 ? 8 : 16) == 0;
