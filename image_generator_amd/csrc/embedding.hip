@@ -199,14 +199,36 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(const void* __restri
 }
 
 // ---- sums -----------------------------------------------------------------------------------------------------------
-// Adds `count` rows src[idx(j)][col0 ..] to acc in order: a wave, VEC columns per lane and sweep, eight rows in flight.  Every
-// load is issued (lanes past the row's end repeat its last columns, what they add up is not stored): a load behind a
-// condition is waited for on the spot.
+// Adds `count` rows src[idx(j)][col0 ..] to acc in order: a wave, VEC columns per lane and sweep, up to FLY rows in flight.  A
+// batch issues all its loads (lanes past the row's end repeat its last columns, what they add up is not stored): a load
+// behind a condition is waited for on the spot.
 constexpr int SWEEPS = 3;            // of 64 * VEC columns
+template <int FLY, int VEC, typename T>
+__device__ __forceinline__ void add_batch(f32x4 (&acc)[SWEEPS], const T* __restrict__ src, int width, const int (&col)[SWEEPS], int sweeps,
+                                          unsigned mine, int j) {
+    const T* r[FLY];
+#pragma unroll
+    for (int e = 0; e < FLY; ++e) r[e] = src + (size_t)(unsigned)__builtin_amdgcn_readlane((int)mine, j + e) * width;
+    typename Raw<T, VEC>::t v[FLY][SWEEPS];
+#pragma unroll
+    for (int s = 0; s < SWEEPS; ++s)
+        if (s < sweeps) {
+#pragma unroll
+            for (int e = 0; e < FLY; ++e) v[e][s] = *(const typename Raw<T, VEC>::t*)(r[e] + col[s]);
+        }
+#pragma unroll
+    for (int s = 0; s < SWEEPS; ++s)
+        if (s < sweeps) {
+#pragma unroll
+            for (int e = 0; e < FLY; ++e) {
+                if constexpr (VEC == 4) acc[s] = acc[s] + f32x4{(float)v[e][s][0], (float)v[e][s][1], (float)v[e][s][2], (float)v[e][s][3]};
+                else acc[s][0] += (float)v[e][s];
+            }
+        }
+}
 template <int VEC, typename T, typename IDX>
 __device__ __forceinline__ void add_rows(f32x4 (&acc)[SWEEPS], const T* __restrict__ src, int width, int col0, int count, IDX idx) {
     const int lane = threadIdx.x & 63;
-    constexpr int FLY = 8;
     int col[SWEEPS];
 #pragma unroll
     for (int s = 0; s < SWEEPS; ++s) col[s] = min(col0 + (s * 64 + lane) * VEC, width - VEC);
@@ -214,27 +236,12 @@ __device__ __forceinline__ void add_rows(f32x4 (&acc)[SWEEPS], const T* __restri
     for (int b = 0; b < count; b += 64) {
         const int n = min(64, count - b);
         const unsigned mine = idx(b + min(lane, n - 1));
-        for (int j = 0; j < n; j += FLY) {
-            const T* r[FLY];
-#pragma unroll
-            for (int e = 0; e < FLY; ++e) r[e] = src + (size_t)(unsigned)__builtin_amdgcn_readlane((int)mine, min(j + e, n - 1)) * width;
-            typename Raw<T, VEC>::t v[FLY][SWEEPS];
-#pragma unroll
-            for (int s = 0; s < SWEEPS; ++s)
-                if (s < sweeps) {
-#pragma unroll
-                    for (int e = 0; e < FLY; ++e) v[e][s] = *(const typename Raw<T, VEC>::t*)(r[e] + col[s]);
-                }
-#pragma unroll
-            for (int e = 0; e < FLY; ++e)
-                if (j + e < n)
-#pragma unroll
-                    for (int s = 0; s < SWEEPS; ++s)
-                        if (s < sweeps) {
-                            if constexpr (VEC == 4) acc[s] = acc[s] + f32x4{(float)v[e][s][0], (float)v[e][s][1], (float)v[e][s][2], (float)v[e][s][3]};
-                            else acc[s][0] += (float)v[e][s];
-                        }
-        }
+        int j = 0;
+        for (; j + 16 <= n; j += 16) add_batch<16, VEC>(acc, src, width, col, sweeps, mine, j);
+        if (n & 8) { add_batch<8, VEC>(acc, src, width, col, sweeps, mine, j); j += 8; }
+        if (n & 4) { add_batch<4, VEC>(acc, src, width, col, sweeps, mine, j); j += 4; }
+        if (n & 2) { add_batch<2, VEC>(acc, src, width, col, sweeps, mine, j); j += 2; }
+        if (n & 1) add_batch<1, VEC>(acc, src, width, col, sweeps, mine, j);
     }
 }
 template <int VEC, typename T>
