@@ -60,21 +60,41 @@ __global__ __launch_bounds__(1024) void multi_sumsq_kernel(const Rec* __restrict
     __shared__ double red[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double acc = 0.0;
-    for (int e = blockIdx.x * 16 + wave; e < n_wg; e += PARTS * 16) {
-        const int2 at = map[e];
-        const long long g = grads[at.x];
+    const int e0 = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 16 + wave);
+    int2 at = e0 < n_wg ? map[e0] : make_int2(0, 0);
+    for (int e = e0; e < n_wg; e += PARTS * 16) {
+        const int2 now = at;
+        if (e + PARTS * 16 < n_wg) at = map[e + PARTS * 16];
+        const long long g = grads[now.x];
         if (g == 0) continue;
-        const size_t n = (size_t)recs[at.x].n, i0 = (size_t)at.y * BLK + lane * 4;
-        f32x4 v[WG_BLOCKS];
+        const size_t n = (size_t)recs[now.x].n, i0 = (size_t)now.y * BLK;
+        if (i0 + WG_BLOCKS * BLK <= n && (g & 15) == 0) {          // a whole run of fp32: every load issued before the first use
+            const f32x4* src = (const f32x4*)g + i0 / 4 + lane;
+            f32x4 v[WG_BLOCKS];
 #pragma unroll
-        for (int u = 0; u < WG_BLOCKS; ++u) {
-            const size_t i = i0 + u * BLK;
-            v[u] = i < n ? load_grad(g, i, n) : f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int u = 0; u < WG_BLOCKS; ++u) v[u] = src[u * (BLK / 4)];
+#pragma unroll
+            for (int u = 0; u < WG_BLOCKS; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc = fma((double)v[u][k], (double)v[u][k], acc);
+        } else if (i0 + WG_BLOCKS * BLK <= n && (g & 15) == 1) {   // of bf16
+            const bf16x8* src = (const bf16x8*)(g & ~1ll) + i0 / 8 + lane;
+            bf16x8 v[WG_BLOCKS / 2];
+#pragma unroll
+            for (int u = 0; u < WG_BLOCKS / 2; ++u) v[u] = src[u * (BLK / 4)];
+#pragma unroll
+            for (int u = 0; u < WG_BLOCKS / 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc = fma((double)(float)v[u][k], (double)(float)v[u][k], acc);
+        } else {
+            for (int u = 0; u < WG_BLOCKS; ++u) {
+                const size_t i = i0 + u * BLK + lane * 4;
+                if (i >= n) break;
+                const f32x4 v = load_grad(g, i, n);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc = fma((double)v[k], (double)v[k], acc);
+            }
         }
-#pragma unroll
-        for (int u = 0; u < WG_BLOCKS; ++u)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc = fma((double)v[u][k], (double)v[u][k], acc);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o, 64);
@@ -87,15 +107,44 @@ __global__ __launch_bounds__(1024) void multi_sumsq_kernel(const Rec* __restrict
     }
 }
 
+// Reductions over a wave by DPP: within rows of 16 lanes, then across them; lane 63 holds the result.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ float wave_max_pos(float x) {          // of values >= 0, whose bits order like whole numbers
+    int v = __float_as_int(x);
+    v = max(v, dpp<0x111, 0xf>(v, v));
+    v = max(v, dpp<0x112, 0xf>(v, v));
+    v = max(v, dpp<0x114, 0xf>(v, v));
+    v = max(v, dpp<0x118, 0xf>(v, v));
+    v = max(v, dpp<0x142, 0xa>(v, v));
+    v = max(v, dpp<0x143, 0xc>(v, v));
+    return __int_as_float(__builtin_amdgcn_readlane(v, 63));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double x) {             // lanes without a source add 0
+    const long long b = __double_as_longlong(x);
+    const unsigned lo = (unsigned)dpp<CTRL, ROWS>(0, (int)b), hi = (unsigned)dpp<CTRL, ROWS>(0, (int)(b >> 32));
+    return x + __longlong_as_double(((long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_sum_d(double x) {
+    x = dpp_add<0x111, 0xf>(x);
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);
+    x = dpp_add<0x143, 0xc>(x);
+    const long long b = __double_as_longlong(x);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)b, 63), hi = (unsigned)__builtin_amdgcn_readlane((int)(b >> 32), 63);
+    return __longlong_as_double(((long long)hi << 32) | lo);
+}
+
 // every wave sums the partials in the same order
 __device__ __forceinline__ double total_sumsq(const double* __restrict__ partial) {
     const int lane = threadIdx.x & 63;
     double t = 0.0;
 #pragma unroll
     for (int k = 0; k < PARTS / 64; ++k) t += partial[k * 64 + lane];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
-    return t;
+    return wave_sum_d(t);
 }
 
 // sqrt(x) to about 2^-45, x >= 0
@@ -198,26 +247,43 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
                                                            float* __restrict__ m_scales, unsigned* __restrict__ u_codes,
                                                            float* __restrict__ u_scales, const double* __restrict__ partial,
                                                            const double* __restrict__ hyper, float* __restrict__ state) {
+    constexpr int MINE = WG_BLOCKS / 4;                               // blocks of a wave, all of them on their way at once
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double norm;
-    if (!norm_of(partial, state, norm)) return;
     const int2 at = map[blockIdx.x];
     const long long g = grads[at.x];
-    if (g == 0) return;
     const Rec t = recs[at.x];
+    f32x4 pvs[MINE], gvs[MINE];
+    unsigned mcs[MINE], ucs[MINE];
+    float mss[MINE], uss[MINE];
+    if (g != 0) {
+#pragma unroll
+        for (int u = 0; u < MINE; ++u) {
+            const size_t tb = (size_t)(at.y + u * 4 + wave), i = tb * BLK + lane * 4;
+            const size_t blk = (size_t)t.block0 + (tb * BLK < (size_t)t.n ? tb : 0);
+            pvs[u] = gvs[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (i < (size_t)t.n) { pvs[u] = load_param(t, i); gvs[u] = load_grad(g, i, (size_t)t.n); }
+            mcs[u] = m_codes[blk * (BLK / 4) + lane];
+            ucs[u] = u_codes[blk * (BLK / 4) + lane];
+            mss[u] = m_scales[blk];
+            uss[u] = u_scales[blk];
+        }
+    }
+    double norm;
+    if (!norm_of(partial, state, norm) || g == 0) return;
     const double b1 = hyper[H_B1], b2 = hyper[H_B2], omb1 = hyper[H_OMB1], omb2 = hyper[H_OMB2];
     const float eps = (float)hyper[H_EPS], decay = (float)hyper[H_DECAY], step = (float)hyper[H_STEP], rbc2 = (float)hyper[H_RBC2];
     double c = 1.0;
     if (hyper[H_MAX] > 0.0) { c = hyper[H_MAX] / (norm + 1e-6); if (c > 1.0) c = 1.0; }
-    for (int u = 0; u < WG_BLOCKS / 4; ++u) {
+#pragma unroll
+    for (int u = 0; u < MINE; ++u) {
         const size_t tb = (size_t)(at.y + u * 4 + wave);             // block within the tensor
         if (tb * BLK >= (size_t)t.n) return;
         const size_t i = tb * BLK + lane * 4, blk = (size_t)t.block0 + tb, w = blk * (BLK / 4) + lane;
         const bool in = i < (size_t)t.n;
-        f32x4 pv = {0.f, 0.f, 0.f, 0.f}, gv = pv;
-        if (in) { pv = load_param(t, i); gv = load_grad(g, i, (size_t)t.n); }
-        const unsigned mc = m_codes[w], uc = u_codes[w];
-        const double md = (double)m_scales[blk] * (1.0 / 16129.0), ud = (double)u_scales[blk] * (1.0 / 65025.0);
+        f32x4 pv = pvs[u];
+        const f32x4 gv = gvs[u];
+        const unsigned mc = mcs[u], uc = ucs[u];
+        const double md = (double)mss[u] * (1.0 / 16129.0), ud = (double)uss[u] * (1.0 / 65025.0);
         double me[4], ue[4];
         float mmax = 0.f, umax = 0.f;
 #pragma unroll
@@ -233,8 +299,8 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
             pv[e] = pv[e] * decay - step * (mf / (uf * rbc2 + eps));
         }
         if (in) store_param(t, i, pv);
-        mmax = wave_max(mmax);
-        umax = wave_max(umax);
+        mmax = wave_max_pos(mmax);
+        umax = wave_max_pos(umax);
         // a scale below the normal range is held as 0, with its codes: nothing of that size moves a parameter
         mmax = mmax >= 0x1p-126f ? mmax : 0.f;
         umax = umax >= 0x1p-126f ? umax : 0.f;

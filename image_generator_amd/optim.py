@@ -7,6 +7,7 @@ for every 256 elements of a tensor: 2.03 instead of 8 bytes of state for a param
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 
@@ -15,6 +16,7 @@ from .ops import BF16, F32, PinnedRing, _stream
 
 BLOCK = 256            # elements that share a scale
 _WG_BLOCKS = 8         # blocks per workgroup of the update
+_SHAPE, _DEVICE, _DTYPE = (operator.attrgetter(n) for n in ("shape", "device", "dtype"))
 _HYPER = 16            # doubles in front of the gradient addresses in the step's upload
 
 
@@ -41,6 +43,7 @@ class TensorAdamW:
             if p.dtype != F32 or not p.is_contiguous():
                 raise ValueError("TensorAdamW: parameters must be contiguous fp32 tensors")
         _disjoint(self.params, "parameters")
+        self._shapes = [p.shape for p in self.params]
         self.lr, self.betas, self.eps, self.wd, self.max_norm = lr, tuple(betas), eps, weight_decay, max_grad_norm
         self.bits, self.device, self.t = state_bits, dev, 0
         blocks = [-(-p.numel() // BLOCK) for p in self.params]
@@ -76,6 +79,7 @@ class TensorAdamW:
                 raise ValueError("TensorAdamW: a copy must be a contiguous bf16 tensor of its parameter's size on its device")
         _disjoint([c for c in copies if c is not None], "copies")
         self.copies = copies
+        self._written = [t for t in self.params + copies if t is not None]
         rows = [[p.data_ptr(), 0 if c is None else c.data_ptr(), p.numel(), s] for p, c, s in zip(self.params, copies, self.starts)]
         self._recs = torch.tensor(rows, dtype=torch.int64).to(self.device)
 
@@ -88,6 +92,33 @@ class TensorAdamW:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"TensorAdamW: {len(grads)} gradients of {len(self.params)} parameters")
+        words, kept = self._addresses(grads)
+        if lr is not None:
+            self.lr = lr
+        self.t += 1
+        b1, b2 = self.betas
+        c1, c2 = 1 - b1 ** self.t, 1 - b2 ** self.t
+        hyper = (self.lr, b1, b2, self.eps, self.wd, c1, c2, self.max_norm or 0.0, 1 - self.lr * self.wd, self.lr / c1, 1 / math.sqrt(c2),
+                 1 - b1, 1 - b2)
+        h = self._ring.acquire().numpy()
+        h[:_HYPER].view("float64")[:len(hyper)] = hyper
+        h[_HYPER:] = words
+        self._upload.copy_(self._ring.acquire(), non_blocking=True)
+        self._ring.copied()
+        self._ring.release()
+        self._kept, self._bound = kept, True
+
+    def _addresses(self, grads):
+        """(what the device table holds for each gradient, copies made here)."""
+        try:      # every gradient there, in one sweep for each question
+            if (list(map(_SHAPE, grads)) == self._shapes and set(map(_DEVICE, grads)) == {self.device} and all(map(torch.Tensor.is_contiguous, grads))):
+                kinds = set(map(_DTYPE, grads))
+                if kinds == {F32}:
+                    return list(map(torch.Tensor.data_ptr, grads)), []
+                if kinds == {BF16}:
+                    return [a | 1 for a in map(torch.Tensor.data_ptr, grads)], []
+        except AttributeError:
+            pass
         words, kept = [], []
         for i, (p, g) in enumerate(zip(self.params, grads)):
             if g is None:
@@ -104,20 +135,7 @@ class TensorAdamW:
                 words.append(g.data_ptr() | 1)
             else:
                 raise ValueError(f"TensorAdamW: gradient {i} is {g.dtype}, neither fp32 nor bf16")
-        if lr is not None:
-            self.lr = lr
-        self.t += 1
-        b1, b2 = self.betas
-        c1, c2 = 1 - b1 ** self.t, 1 - b2 ** self.t
-        hyper = (self.lr, b1, b2, self.eps, self.wd, c1, c2, self.max_norm or 0.0, 1 - self.lr * self.wd, self.lr / c1, 1 / math.sqrt(c2),
-                 1 - b1, 1 - b2)
-        h = self._ring.acquire().numpy()
-        h[:_HYPER].view("float64")[:len(hyper)] = hyper
-        h[_HYPER:] = words
-        self._upload.copy_(self._ring.acquire(), non_blocking=True)
-        self._ring.copied()
-        self._ring.release()
-        self._kept, self._bound = kept, True
+        return words, kept
 
     def apply(self):
         """The launches of the step that `bind` began (capturable)."""
@@ -132,7 +150,7 @@ class TensorAdamW:
                                          self._map.shape[0], self.bits, m.data_ptr(), ptr(ms), v.data_ptr(), ptr(us),
                                          self._partial.data_ptr(), self._upload.data_ptr(), self.state.data_ptr(), self._elements,
                                          _stream()), "multi_adamw")
-        torch.autograd.graph.increment_version([t for t in self.params + self.copies if t is not None])
+        torch.autograd.graph.increment_version(self._written)
 
     def step(self, grads=None, lr=None):
         self.bind(grads, lr)
