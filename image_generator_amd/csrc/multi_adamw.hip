@@ -61,13 +61,18 @@ __global__ __launch_bounds__(1024) void multi_sumsq_kernel(const Rec* __restrict
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double acc = 0.0;
     const int e0 = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 16 + wave);
-    int2 at = e0 < n_wg ? map[e0] : make_int2(0, 0);
-    for (int e = e0; e < n_wg; e += PARTS * 16) {
-        const int2 now = at;
-        if (e + PARTS * 16 < n_wg) at = map[e + PARTS * 16];
-        const long long g = grads[now.x];
+    // addresses two entries ahead: place -> gradient -> values is a chain of three loads
+    constexpr int STEP = PARTS * 16;
+    int2 next = e0 < n_wg ? map[e0] : make_int2(0, 0), after = e0 + STEP < n_wg ? map[e0 + STEP] : make_int2(0, 0);
+    long long g_next = e0 < n_wg ? grads[next.x] : 0, n_next = e0 < n_wg ? recs[next.x].n : 0;
+    for (int e = e0; e < n_wg; e += STEP) {
+        const int2 now = next;
+        const long long g = g_next;
+        const size_t n = (size_t)n_next, i0 = (size_t)now.y * BLK;
+        next = after;
+        if (e + STEP < n_wg) { g_next = grads[next.x]; n_next = recs[next.x].n; }
+        if (e + 2 * STEP < n_wg) after = map[e + 2 * STEP];
         if (g == 0) continue;
-        const size_t n = (size_t)recs[now.x].n, i0 = (size_t)now.y * BLK;
         if (i0 + WG_BLOCKS * BLK <= n && (g & 15) == 0) {          // a whole run of fp32: every load issued before the first use
             const f32x4* src = (const f32x4*)g + i0 / 4 + lane;
             f32x4 v[WG_BLOCKS];

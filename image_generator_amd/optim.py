@@ -16,7 +16,7 @@ from .ops import BF16, F32, PinnedRing, _stream
 
 BLOCK = 256            # elements that share a scale
 _WG_BLOCKS = 8         # blocks per workgroup of the update
-_SHAPE, _DEVICE, _DTYPE = (operator.attrgetter(n) for n in ("shape", "device", "dtype"))
+_SHAPE, _DTYPE = operator.attrgetter("shape"), operator.attrgetter("dtype")
 _HYPER = 16            # doubles in front of the gradient addresses in the step's upload
 
 
@@ -89,10 +89,11 @@ class TensorAdamW:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("TensorAdamW: bind() before the capture (and before every replay); only apply() can be captured")
         self._on_device()
-        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        owned = grads is None
+        grads = [p.grad for p in self.params] if owned else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"TensorAdamW: {len(grads)} gradients of {len(self.params)} parameters")
-        words, kept = self._addresses(grads)
+        words, kept = self._addresses(grads, owned)
         if lr is not None:
             self.lr = lr
         self.t += 1
@@ -108,17 +109,17 @@ class TensorAdamW:
         self._ring.release()
         self._kept, self._bound = kept, True
 
-    def _addresses(self, grads):
+    def _addresses(self, grads, owned):
         """(what the device table holds for each gradient, copies made here)."""
-        try:      # every gradient there, in one sweep for each question
-            if (list(map(_SHAPE, grads)) == self._shapes and set(map(_DEVICE, grads)) == {self.device} and all(map(torch.Tensor.is_contiguous, grads))):
+        # the common case in a few sweeps: every gradient there, of its parameter's shape, contiguous, one type, this device
+        # (a parameter's own `.grad` has its shape and device already)
+        if not any(g is None for g in grads) and all(map(torch.Tensor.is_contiguous, grads)):
+            if owned or (list(map(_SHAPE, grads)) == self._shapes and set(map(torch.Tensor.get_device, grads)) == {self.device.index}):
                 kinds = set(map(_DTYPE, grads))
                 if kinds == {F32}:
                     return list(map(torch.Tensor.data_ptr, grads)), []
                 if kinds == {BF16}:
                     return [a | 1 for a in map(torch.Tensor.data_ptr, grads)], []
-        except AttributeError:
-            pass
         words, kept = [], []
         for i, (p, g) in enumerate(zip(self.params, grads)):
             if g is None:
