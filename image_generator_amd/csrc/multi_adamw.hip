@@ -10,9 +10,8 @@
 // code did.  The largest magnitude of a block is held exactly, as its scale; the
 // others move with it.
 //
-// The arithmetic between reading and writing 8-bit codes is fp64.  Vector fp64 runs at the rate of vector fp32 on this chip, one
-// Newton step on the hardware's reciprocal root is cheaper than a correctly rounded fp32 root, and a code then does not depend
-// on the order in which a compiler rounds the steps before it.  States of 32 bits are stepped in fp32, by the expressions of
+// Moments between reading and writing 8-bit codes are fp64 (vector fp64 runs at the rate of vector fp32 on this chip), so a code
+// does not depend on the order in which a compiler rounds the steps before it.  States of 32 bits are stepped in fp32, by the expressions of
 // the flat-buffer update, whose bits they reproduce.
 #include "common.h"
 
@@ -20,7 +19,7 @@ namespace {
 
 constexpr int BLK = 256;             // elements that share a scale; one wave
 constexpr int WG_BLOCKS = 8;         // blocks per workgroup of four waves
-constexpr int PARTS = 256;           // partial sums of the norm
+constexpr int PARTS = 512;           // partial sums of the norm: two workgroups of eight waves per CU
 
 // A code is the nearest whole number, the lower one of a tie: bf16 gradients from zero states do meet ties (a quarter of the
 // largest magnitude, at 127 / 2), and the margin keeps the fp64 steps' own rounding from deciding them.
@@ -55,14 +54,14 @@ __device__ __forceinline__ f32x4 load_grad(long long g, size_t i, size_t n) {
 }
 
 // ---- norm: partial[b] = sum of the squares of a fixed share of the gradients, fp64, in a fixed order --------------------
-__global__ __launch_bounds__(1024) void multi_sumsq_kernel(const Rec* __restrict__ recs, const long long* __restrict__ grads,
+__global__ __launch_bounds__(512) void multi_sumsq_kernel(const Rec* __restrict__ recs, const long long* __restrict__ grads,
                                                            const int2* __restrict__ map, int n_wg, double* __restrict__ partial) {
-    __shared__ double red[16];
+    __shared__ double red[8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double acc = 0.0;
-    const int e0 = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 16 + wave);
+    const int e0 = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 8 + wave);
     // addresses two entries ahead: place -> gradient -> values is a chain of three loads
-    constexpr int STEP = PARTS * 16;
+    constexpr int STEP = PARTS * 8;
     int2 next = e0 < n_wg ? map[e0] : make_int2(0, 0), after = e0 + STEP < n_wg ? map[e0 + STEP] : make_int2(0, 0);
     long long g_next = e0 < n_wg ? grads[next.x] : 0, n_next = e0 < n_wg ? recs[next.x].n : 0;
     for (int e = e0; e < n_wg; e += STEP) {
@@ -107,7 +106,7 @@ __global__ __launch_bounds__(1024) void multi_sumsq_kernel(const Rec* __restrict
     __syncthreads();
     if (threadIdx.x == 0) {
         double t = 0.0;
-        for (int w = 0; w < 16; ++w) t += red[w];
+        for (int w = 0; w < 8; ++w) t += red[w];
         partial[blockIdx.x] = t;
     }
 }
@@ -126,21 +125,33 @@ __device__ __forceinline__ float wave_max_pos(float x) {          // of values >
     return __int_as_float(__builtin_amdgcn_readlane(v, 63));
 }
 template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp_add(double x) {             // lanes without a source add 0
+__device__ __forceinline__ double dpp_d(double x) {               // lanes without a source get 0
     const long long b = __double_as_longlong(x);
     const unsigned lo = (unsigned)dpp<CTRL, ROWS>(0, (int)b), hi = (unsigned)dpp<CTRL, ROWS>(0, (int)(b >> 32));
-    return x + __longlong_as_double(((long long)hi << 32) | lo);
+    return __longlong_as_double(((long long)hi << 32) | lo);
 }
-__device__ __forceinline__ double wave_sum_d(double x) {
-    x = dpp_add<0x111, 0xf>(x);
-    x = dpp_add<0x112, 0xf>(x);
-    x = dpp_add<0x114, 0xf>(x);
-    x = dpp_add<0x118, 0xf>(x);
-    x = dpp_add<0x142, 0xa>(x);
-    x = dpp_add<0x143, 0xc>(x);
+__device__ __forceinline__ double lane63(double x) {
     const long long b = __double_as_longlong(x);
     const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)b, 63), hi = (unsigned)__builtin_amdgcn_readlane((int)(b >> 32), 63);
     return __longlong_as_double(((long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_max_pos(double x) {
+    x = fmax(x, dpp_d<0x111, 0xf>(x));
+    x = fmax(x, dpp_d<0x112, 0xf>(x));
+    x = fmax(x, dpp_d<0x114, 0xf>(x));
+    x = fmax(x, dpp_d<0x118, 0xf>(x));
+    x = fmax(x, dpp_d<0x142, 0xa>(x));
+    x = fmax(x, dpp_d<0x143, 0xc>(x));
+    return lane63(x);
+}
+__device__ __forceinline__ double wave_sum_d(double x) {
+    x += dpp_d<0x111, 0xf>(x);
+    x += dpp_d<0x112, 0xf>(x);
+    x += dpp_d<0x114, 0xf>(x);
+    x += dpp_d<0x118, 0xf>(x);
+    x += dpp_d<0x142, 0xa>(x);
+    x += dpp_d<0x143, 0xc>(x);
+    return lane63(x);
 }
 
 // every wave sums the partials in the same order
@@ -279,6 +290,7 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
     const float eps = (float)hyper[H_EPS], decay = (float)hyper[H_DECAY], step = (float)hyper[H_STEP], rbc2 = (float)hyper[H_RBC2];
     double c = 1.0;
     if (hyper[H_MAX] > 0.0) { c = hyper[H_MAX] / (norm + 1e-6); if (c > 1.0) c = 1.0; }
+    const double omb1c = omb1 * c, omb2c = omb2 * c * c;
 #pragma unroll
     for (int u = 0; u < MINE; ++u) {
         const size_t tb = (size_t)(at.y + u * 4 + wave);             // block within the tensor
@@ -288,39 +300,68 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
         f32x4 pv = pvs[u];
         const f32x4 gv = gvs[u];
         const unsigned mc = mcs[u], uc = ucs[u];
-        const double md = (double)mss[u] * (1.0 / 16129.0), ud = (double)uss[u] * (1.0 / 65025.0);
-        double me[4], ue[4];
-        float mmax = 0.f, umax = 0.f;
+        // m = b1 md q|q| + (1 - b1) c g;  v = b2 (ud q^2)^2 + (1 - b2) (c g)^2, with the factors of a block made once
+        const double md = (double)mss[u] * (b1 / 16129.0), ud = (double)uss[u] * (1.0 / 65025.0), vd = b2 * ud * ud;
+        typedef double f64x4 __attribute__((ext_vector_type(4)));
+        f64x4 me, ve;
+        double vmax = 0.0;
+        float mf[4], mmax = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const double gg = (double)gv[e] * c;
-            const int qm = sbyte(mc, e), qu = ubyte(uc, e);
-            const double u0 = (double)(qu * qu) * ud;
-            me[e] = b1 * ((double)(qm * abs(qm)) * md) + omb1 * gg;
-            ue[e] = root(b2 * (u0 * u0) + omb2 * (gg * gg));
-            const float mf = (float)me[e], uf = (float)ue[e];
-            mmax = fmaxf(mmax, fabsf(mf));
-            umax = fmaxf(umax, uf);
-            pv[e] = pv[e] * decay - step * (mf / (uf * rbc2 + eps));
+            const double gg = (double)gv[e];
+            const float qm = (float)sbyte(mc, e), qu = (float)ubyte(uc, e);        // squares of codes are exact in fp32
+            const double qu2 = (double)(qu * qu);
+            me[e] = fma((double)(qm * fabsf(qm)), md, omb1c * gg);
+            ve[e] = fma(qu2 * qu2, vd, omb2c * (gg * gg));
+            mf[e] = (float)me[e];
+            mmax = fmaxf(mmax, fabsf(mf[e]));
+            vmax = fmax(vmax, ve[e]);
         }
-        if (in) store_param(t, i, pv);
         mmax = wave_max_pos(mmax);
-        umax = wave_max_pos(umax);
+        float umax = (float)root(wave_max_pos(vmax));
         // a scale below the normal range is held as 0, with its codes: nothing of that size moves a parameter
         mmax = mmax >= 0x1p-126f ? mmax : 0.f;
         umax = umax >= 0x1p-126f ? umax : 0.f;
-        const double rm = inverse(mmax), ru = inverse(umax);
+        const double rm = inverse(mmax), ru = inverse(umax), ru2 = ru * ru;
+        // Codes from fp32 roots, whose positions are good to 6.3e-5 (two roots of 1 ulp each on a ratio rounded once, times 255);
+        // a lane with a position within twice that of the border of two codes takes the fp64 roots: one wave and block in ten.
+        constexpr float SURE = 0.5f - 1.25e-4f;
+        int qm[4], qu[4];
+        f32x4 uf;
+        bool near = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float tm = 127.f * __builtin_amdgcn_sqrtf((float)(fabs(me[e]) * rm));
+            const float ratio = __builtin_amdgcn_sqrtf((float)(ve[e] * ru2)), tu = 255.f * __builtin_amdgcn_sqrtf(ratio);
+            const float fm = floorf(tm + 0.5f), fu = floorf(tu + 0.5f);
+            near |= fabsf(tm - fm) > SURE || fabsf(tu - fu) > SURE;
+            qm[e] = (int)fm;
+            qu[e] = (int)fu;
+            uf[e] = ratio * umax;
+        }
+        if (umax == 0.f) {                                           // (uniform) roots too small to be held still divide
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) uf[e] = (float)root(ve[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pv[e] = fmaf(pv[e], decay, -step * (mf[e] * __builtin_amdgcn_rcpf(fmaf(uf[e], rbc2, eps))));
+        if (near) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                qm[e] = (int)fma(127.0, root(fabs(me[e]) * rm), HALF);
+                qu[e] = (int)fma(255.0, root(root(ve[e] * ru2)), HALF);
+            }
+        }
+        if (in) store_param(t, i, pv);
         unsigned mo = 0, uo = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            int qm = (int)fma(127.0, root(fabs(me[e]) * rm), HALF);
-            int qu = (int)fma(255.0, root(ue[e] * ru), HALF);
-            qm = min(qm, 127);
-            qu = min(qu, 255);
-            if (ue[e] > 0.0 && umax > 0.f) qu = max(qu, 1);
-            if (me[e] < 0.0) qm = -qm;
-            mo |= (unsigned)(qm & 255) << (8 * e);
-            uo |= (unsigned)qu << (8 * e);
+            int q = min(qm[e], 127);
+            if (mf[e] < 0.f) q = -q;
+            mo |= (unsigned)(q & 255) << (8 * e);
+            q = min(qu[e], 255);
+            if (ve[e] > 0.0 && umax > 0.f) q = max(q, 1);
+            uo |= (unsigned)q << (8 * e);
         }
         m_codes[w] = mo;
         u_codes[w] = uo;
@@ -366,7 +407,7 @@ int mi355_multi_adamw_step(const long long* recs, const long long* grads, const 
     if (n_wg == 0) return MI355_OK;
     const hipStream_t st = (hipStream_t)stream;
     ProfScope prof(FAM_ELEM, st, elements * (bits == 8 ? 22.0 : 34.0));
-    hipLaunchKernelGGL(multi_sumsq_kernel, dim3(PARTS), dim3(1024), 0, st, (const Rec*)recs, grads, (const int2*)map, n_wg, partial);
+    hipLaunchKernelGGL(multi_sumsq_kernel, dim3(PARTS), dim3(512), 0, st, (const Rec*)recs, grads, (const int2*)map, n_wg, partial);
     if (bits == 32)
         hipLaunchKernelGGL(multi_adamw32_kernel, dim3(n_wg), dim3(256), 0, st, (const Rec*)recs, grads, (const int2*)map, (float*)m,
                            (float*)v, partial, hyper, state);
