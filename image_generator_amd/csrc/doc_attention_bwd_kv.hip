@@ -41,9 +41,9 @@ struct RowFetch {
 };
 
 struct RowInfo {                     // of the 64 staged rows
-    float lse[64], delta[64];        // PLAIN: -lse / (scale log2 e), else lse;  -delta (DROPPED: delta)
-    int lo[64], count[64], c[64];
-    float slope2[64];
+    float lse[64], delta[64];        // -lse, PLAIN: -lse / (scale log2 e);  -delta (DROPPED: delta)
+    int lo[64], count[64];
+    float c[64], slope2[64];         // key position, from the workgroup's first key;  -slope log2 e
     unsigned drop[64];
 };
 
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
     int unit, hk;
     if (!unit_of(tiles * p.splits, p.Hkv, unit, hk)) return;
     const int split = unit / tiles, tile = unit - split * tiles;
-    const int key0 = (tile * 4 + wave) * (32 * KB);
+    const int base = tile * 128 * KB, key0 = base + wave * 32 * KB;
     const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
     bf16x8 kf[KB][ND], vf[KB][ND];
     bool seen[KB];
@@ -146,11 +146,11 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
         put_tile<NCH, NO * 4, true>(greg, Gs, LD, threadIdx.x);
         if (threadIdx.x < 64) {
             const float ls = !in || lreg == -INFINITY ? INFINITY : lreg;         // rows that see nothing: probabilities of 0
-            info.lse[threadIdx.x] = KIND == PLAIN ? -ls * rsl2 : ls;
+            info.lse[threadIdx.x] = KIND == PLAIN ? -ls * rsl2 : -ls;
             info.delta[threadIdx.x] = KIND == DROPPED ? dreg : -dreg;
             info.lo[threadIdx.x] = ireg.x;
             info.count[threadIdx.x] = in ? ireg.y - ireg.x : 0;
-            if (KIND != PLAIN) { info.c[threadIdx.x] = ireg.z; info.slope2[threadIdx.x] = sreg * LOG2E; }
+            if (KIND != PLAIN) { info.c[threadIdx.x] = (float)(ireg.z - base); info.slope2[threadIdx.x] = -sreg * LOG2E; }
             if (KIND == DROPPED) info.drop[threadIdx.x] = hreg;
         }
         __syncthreads();
@@ -191,29 +191,32 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
                 const int key = key0 + kb * 32 + l31;
                 if constexpr (KIND != PLAIN) {
                     f32x16 turn;
+                    float gain = bend.scale2;
                     if (bend.capped) {
+                        bend.tanh16(s[kb]);
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float u = __builtin_amdgcn_rcpf(1.f + EXP2(s[kb][r] * bend.in));       // tanh = 1 - 2 u
-                            s[kb][r] = fmaf(-2.f * bend.cap2, u, bend.cap2);
-                            turn[r] = fmaf(-4.f * u, u, 4.f * u);
+                        for (int r = 0; r < 16; ++r) turn[r] = fmaf(-s[kb][r], s[kb][r], 1.f);
+                        gain = bend.cap2;
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) turn[r] = 1.f;
+                    }
+                    if (bend.biased) {
+                        const float keyf = (float)(key - base);
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const f32x4 c = *(const f32x4*)&info.c[qs * 32 + 8 * g + 4 * hh];
+                            const f32x4 sl = *(const f32x4*)&info.slope2[qs * 32 + 8 * g + 4 * hh];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                s[kb][4 * g + e] = fmaf(s[kb][4 * g + e], gain, fmaf(sl[e], fabsf(c[e] - keyf), ls[g][e]));
                         }
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) { s[kb][r] *= bend.scale2; turn[r] = 1.f; }
-                    }
-                    if (bend.biased) {
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const int4 c = *(const int4*)&info.c[qs * 32 + 8 * g + 4 * hh];
-                            const f32x4 sl = *(const f32x4*)&info.slope2[qs * 32 + 8 * g + 4 * hh];
-                            const int cc[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) s[kb][4 * g + e] = fmaf(-sl[e], fabsf((float)(cc[e] - key)), s[kb][4 * g + e]);
-                        }
+                        for (int r = 0; r < 16; ++r) s[kb][r] = fmaf(s[kb][r], gain, ls[r >> 2][r & 3]);
                     }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kb][r] = EXP2(s[kb][r] - ls[r >> 2][r & 3]);
+                    for (int r = 0; r < 16; ++r) s[kb][r] = EXP2(s[kb][r]);
                     if constexpr (KIND == DROPPED) {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {

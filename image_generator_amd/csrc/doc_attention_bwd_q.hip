@@ -48,6 +48,7 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles)
     const int hi = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.hi : 0));
     const int in_lo = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.lo : 0));
     const int in_hi = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.hi : 0x7fffffff));
+    const int c_min = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.c : 0x7fffffff));
     if (!sees) delta = 0.f;
 #pragma unroll
     for (int ks = 0; ks < ND; ++ks) {
@@ -61,6 +62,7 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles)
     const float slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;
     const unsigned drop = drop_row(p, token, head);
     const Bend bend(p);
+    const float s0 = KIND == PLAIN ? -lse / bend.scale2 : 0.f;
 
     if (lane == 0) { range[wave][0] = lo; range[wave][1] = hi; }
     __syncthreads();
@@ -97,9 +99,9 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles)
         const bool masked = k0 < in_lo || k0 + 64 > in_hi;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            f32x16 s, dp;
+            f32x16 s, dp;                 // started at -lse and -delta, which saves subtracting them
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+            for (int r = 0; r < 16; ++r) { s[r] = s0; dp[r] = KIND == DROPPED ? 0.f : -delta; }
 #pragma unroll
             for (int ks = 0; ks < ND; ++ks) {
                 const bf16x8 ak = *(const bf16x8*)(Ks + (kb * 32 + l31) * KLD + ((ks * 2 + hh) ^ ((l31 >> 2) & 3)) * 16);
@@ -109,33 +111,31 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles)
             }
             if constexpr (KIND == DROPPED) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) dp[r] = drop_keep(p, drop, k0 + kb * 32 + reg_row(r) + 4 * hh) ? dp[r] * p.drop_scale : 0.f;
+                for (int r = 0; r < 16; ++r) dp[r] = (drop_keep(p, drop, k0 + kb * 32 + reg_row(r) + 4 * hh) ? dp[r] * p.drop_scale : 0.f) - delta;
             }
+            if constexpr (KIND == PLAIN) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) dp[r] -= delta;
-            float sl2 = bend.scale2;
-            if constexpr (KIND != PLAIN) {
+                for (int r = 0; r < 16; ++r) s[r] = EXP2(s[r] * bend.scale2) * dp[r];
+            } else {
+                float gain = bend.scale2;
                 if (bend.capped) {
+                    bend.tanh16(s);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float u = __builtin_amdgcn_rcpf(1.f + EXP2(s[r] * bend.in));       // tanh = 1 - 2 u
-                        s[r] = fmaf(-2.f * bend.cap2, u, bend.cap2);
-                        dp[r] *= 4.f * fmaf(-u, u, u);
-                    }
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] *= sl2;
+                    for (int r = 0; r < 16; ++r) dp[r] *= fmaf(-s[r], s[r], 1.f);
+                    gain = bend.cap2;
                 }
                 if (bend.biased) {
-                    const float cf = (float)(span.c - k0 - kb * 32 - 4 * hh);
+                    const f32x16 y = bias16(slope2, (float)(span.c - k0 - kb * 32 - 4 * hh), -lse, k0 + 63 <= c_min);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope2, fabsf(cf - (float)reg_row(r)), s[r]);
+                    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], gain, y[r]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], gain, -lse);
                 }
-                sl2 = 1.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = EXP2(s[r]) * dp[r];
             }
             bf16x8 dsf[2];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = EXP2(fmaf(s[r], sl2, -lse)) * dp[r];
             if (masked) {
                 const unsigned rel = (unsigned)(k0 + kb * 32 + 4 * hh - span.lo), len = (unsigned)(span.hi - span.lo);
 #pragma unroll

@@ -6,6 +6,7 @@
 // tiles that none of its rows sees and masks only those that some row sees in part.
 #include "doc_tiles.h"
 #include <mutex>
+#include <type_traits>
 
 namespace {
 
@@ -21,6 +22,7 @@ struct Rows {                        // a wave's 32 rows
     unsigned drop;
     int lo, hi;                      // union of the intervals (wave-uniform)
     int in_lo, in_hi;                // their intersection
+    int c_min;                       // first key position of a row
 
     // R0: the wave's first row
     __device__ __forceinline__ void init(const DocArgs& p, unsigned R0, int hk) {
@@ -44,20 +46,18 @@ struct Rows {                        // a wave's 32 rows
         in_lo = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.lo : 0));
         in_hi = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.hi : 0x7fffffff));
         if (lo > hi) lo = hi = 0;
+        c_min = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.c : 0x7fffffff));
 #pragma unroll
         for (int ks = 0; ks < ND; ++ks) qf[ks] = sees ? qf[ks] : zero8;
         slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;
         drop = drop_row(p, token, head);
-#pragma unroll
-        for (int i = 0; i < NO; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-        m = -INFINITY;
-        l = 0.f;
     }
 
-    // one staged tile of keys k0 .. k0 + 63
-    template <int KIND, int KLD, int VLD>
+    // One staged tile of keys k0 .. k0 + 63.  FAST: no running maximum, p = 2^x against the fixed reference 0.  Floating point
+    // does not mind the common factor while nothing leaves the normal range, and bf16 probabilities have fp32's exponents; a
+    // row whose sum (`fits`) is not within 2^-100 .. 2^100 - scores beyond some 70 nats, or a distance bias on every key it
+    // sees - sends its workgroup through the loop again with the maximum.
+    template <int KIND, bool FAST, int KLD, int VLD>
     __device__ __forceinline__ void tile(const DocArgs& p, const Bend& bend, const char* Ks, const char* Vs, int k0) {
         const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
         f32x16 s[2];
@@ -74,24 +74,12 @@ struct Rows {                        // a wave's 32 rows
             }
         float sl2 = bend.scale2;
         if constexpr (KIND != PLAIN) {
-            if (bend.capped) {
+            const bool before = k0 + 63 <= c_min;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        s[kb][r] = fmaf(-2.f * bend.cap2, __builtin_amdgcn_rcpf(1.f + EXP2(s[kb][r] * bend.in)), bend.cap2);
-            } else {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kb][r] *= sl2;
-            }
-            if (bend.biased) {
-                const float cf = (float)(span.c - k0 - 4 * hh);
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kb][r] = fmaf(-slope2, fabsf(cf - (float)(kb * 32 + reg_row(r))), s[kb][r]);
+            for (int kb = 0; kb < 2; ++kb) {
+                f32x16 y = {};
+                if (bend.biased) y = bias16(slope2, (float)(span.c - k0 - kb * 32 - 4 * hh), 0.f, before);
+                bend.score16(s[kb], y);
             }
             sl2 = 1.f;
         }
@@ -103,34 +91,38 @@ struct Rows {                        // a wave's 32 rows
                 for (int r = 0; r < 16; ++r)
                     if (rel + (unsigned)(kb * 32 + reg_row(r)) >= len) s[kb][r] = -INFINITY;
         }
-        float mx = -INFINITY;
+        float ref = 0.f;
+        if constexpr (!FAST) {
+            float mx = -INFINITY;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * sl2;
-        const float m_new = fmaxf(m, mx), ref = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = EXP2(m - ref);
-        float sum = 0.f;
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * sl2;
+            const float m_new = fmaxf(m, mx);
+            ref = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = EXP2(m - ref);
+            l *= alpha;
+            if (__ballot(m_new != m) != 0) {
+#pragma unroll
+                for (int i = 0; i < NO; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+            }
+            m = m_new;
+        }
         bf16x8 pf[2][2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float e = EXP2(fmaf(s[kb][r], sl2, -ref));
-                sum += e;
+                float e;
+                if constexpr (FAST) e = EXP2(KIND == PLAIN ? s[kb][r] * sl2 : s[kb][r]);
+                else e = EXP2(fmaf(s[kb][r], sl2, -ref));
+                l += e;
                 if constexpr (KIND == DROPPED) e = drop_keep(p, drop, k0 + kb * 32 + reg_row(r) + 4 * hh) ? e * p.drop_scale : 0.f;
                 pf[kb][r >> 3][r & 7] = (bf16_t)e;
             }
-        sum += __shfl_xor(sum, 32, 64);
-        l = fmaf(l, alpha, sum);
-        if (__ballot(m_new != m) != 0) {
-#pragma unroll
-            for (int i = 0; i < NO; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
-        }
-        m = m_new;
         const int tr_row = 4 * hh + ((lane & 15) >> 2), tr_col = (((lane >> 4) & 1) * 16 + 4 * (lane & 3)) * 2;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -142,7 +134,18 @@ struct Rows {                        // a wave's 32 rows
                     o[db] = mfma(cat4(LDS_TR(a0), LDS_TR(a0 + 8 * VLD)), pf[kb][st], o[db]);
                 }
     }
-    // rows whose result is not finite (a NaN maximum included)
+    __device__ __forceinline__ void reset(float reference) {
+#pragma unroll
+        for (int i = 0; i < NO; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+        m = reference;
+        l = 0.f;
+    }
+    // the two lanes of a row hold the sums of the keys whose scores they hold
+    __device__ __forceinline__ void join() { l += __shfl_xor(l, 32, 64); }
+    __device__ __forceinline__ bool fits() const { return span.hi <= span.lo || (l > 0x1p-100f && l < 0x1p100f); }
+    // rows whose result is not finite
     __device__ __forceinline__ unsigned bad() const {
         const float z = not_finite(o) + l * 0.f;
         return bad_rows(span.hi > span.lo && !(z == 0.f));
@@ -150,7 +153,7 @@ struct Rows {                        // a wave's 32 rows
 };
 
 template <int ND, int NO, int KIND>
-__global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_fwd_kernel(const DocArgs p, int tiles) {
+__global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd_kernel(const DocArgs p, int tiles) {
     constexpr int DP = 16 * ND, KLD = DP * 2 + 16, VLD = tr_ld(NO);
     constexpr int NCK = (64 * (DP / 8) + 255) / 256, NCV = (64 * NO * 4 + 255) / 256;
     __shared__ __attribute__((aligned(16))) char smem[64 * KLD + 64 * VLD];
@@ -172,21 +175,27 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_fwd_kernel(const Doc
     Fetch<NCV, NO * 4> vf;
     kf.init(threadIdx.x, p.ldk, p.D);
     vf.init(threadIdx.x, p.ldv, p.D);
-    if (klo < khi) {
-        kf.load(kreg, kbase, p.ldk, p.D, klo, khi - klo);
-        vf.load(vreg, vbase, p.ldv, p.D, klo, khi - klo);
-    }
-    for (int k0 = klo; k0 < khi; k0 += 64) {
-        __syncthreads();
-        put_tile<NCK, DP / 8, false>(kreg, Ks, KLD, threadIdx.x);
-        put_tile<NCV, NO * 4, false>(vreg, Vs, VLD, threadIdx.x);
-        __syncthreads();
-        if (k0 + 64 < khi) {
-            kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, khi - k0 - 64);
-            vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, khi - k0 - 64);
+    auto pass = [&](auto fast) __attribute__((always_inline)) {
+        w.reset(decltype(fast)::value ? 0.f : -INFINITY);
+        if (klo < khi) {
+            kf.load(kreg, kbase, p.ldk, p.D, klo, khi - klo);
+            vf.load(vreg, vbase, p.ldv, p.D, klo, khi - klo);
         }
-        if (k0 < w.hi && k0 + 64 > w.lo) w.template tile<KIND, KLD, VLD>(p, bend, Ks, Vs, k0);
-    }
+        for (int k0 = klo; k0 < khi; k0 += 64) {
+            __syncthreads();
+            put_tile<NCK, DP / 8, false>(kreg, Ks, KLD, threadIdx.x);
+            put_tile<NCV, NO * 4, false>(vreg, Vs, VLD, threadIdx.x);
+            __syncthreads();
+            if (k0 + 64 < khi) {
+                kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, khi - k0 - 64);
+                vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, khi - k0 - 64);
+            }
+            if (k0 < w.hi && k0 + 64 > w.lo) w.template tile<KIND, decltype(fast)::value, KLD, VLD>(p, bend, Ks, Vs, k0);
+        }
+        w.join();
+    };
+    pass(std::true_type{});
+    if (__syncthreads_or(!w.fits())) pass(std::false_type{});      // (the loop has barriers: the workgroup decides as one)
     if (w.live) {
         const float inv = w.l > 0.f ? 1.f / w.l : 0.f;
         bf16_t* out = p.out + (size_t)w.token * p.ldo + (size_t)w.head * p.D;
@@ -240,29 +249,34 @@ __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) 
     Fetch<NCV, NO * 4, 64> vf;
     kf.init(lane, p.ldk, p.D);
     vf.init(lane, p.ldv, p.D);
-    if (from < to) {
-        kf.load(kreg, kbase, p.ldk, p.D, from, to - from);
-        vf.load(vreg, vbase, p.ldv, p.D, from, to - from);
-    }
-    for (int k0 = from; k0 < to; k0 += 64) {
-        // one wave: its LDS operations complete in order, the fences only keep the compiler from reordering them
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        put_tile<NCK, DP / 8, false, 64>(kreg, Ks, KLD, lane);
-        put_tile<NCV, NO * 4, false, 64>(vreg, Vs, VLD, lane);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (k0 + 64 < to) {
-            kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, to - k0 - 64);
-            vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, to - k0 - 64);
+    w.reset(-INFINITY);
+    {   // (with the running maximum: what bounds this loop is memory, and a distance bias makes far runs tiny)
+        if (from < to) {
+            kf.load(kreg, kbase, p.ldk, p.D, from, to - from);
+            vf.load(vreg, vbase, p.ldv, p.D, from, to - from);
         }
-        // keys behind this run are another wave's: the tile holds zeros there, and the mask ends with the run
-        w.template tile<KIND, KLD, VLD>(p, bend, Ks, Vs, k0);
+        for (int k0 = from; k0 < to; k0 += 64) {
+            // one wave: its LDS operations complete in order, the fences only keep the compiler from reordering them
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            put_tile<NCK, DP / 8, false, 64>(kreg, Ks, KLD, lane);
+            put_tile<NCV, NO * 4, false, 64>(vreg, Vs, VLD, lane);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (k0 + 64 < to) {
+                kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, to - k0 - 64);
+                vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, to - k0 - 64);
+            }
+            // a run ends with whole tiles, or where the last of the rows' intervals does
+            w.template tile<KIND, false, KLD, VLD>(p, bend, Ks, Vs, k0);
+        }
+        w.join();
     }
+    const bool some = max(w.span.lo, from) < min(w.span.hi, to);     // the row sees keys of this run
     const size_t rows = (size_t)gridDim.x * 32, row = ((size_t)hk * rows + R) * p.splits + split;
     float2* ml = (float2*)p.part;
     float* part = p.part + (size_t)p.Hkv * rows * p.splits * 2 + row * p.D;
     // (m = -inf: no key of the run is seen, the values stay unwritten and unread)
-    if (hh == 0) ml[row] = make_float2(w.l == 0.f && w.m == -INFINITY ? -INFINITY : w.m, w.l);
-    const bool any = !(w.m == -INFINITY) && w.live;
+    const bool any = some && !(w.l == 0.f);
+    if (hh == 0) ml[row] = make_float2(any ? w.m : -INFINITY, any ? w.l : 0.f);
 #pragma unroll
     for (int db = 0; db < NO; ++db)
 #pragma unroll

@@ -17,6 +17,9 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __
 // 64 bytes apart modulo the 256-byte bank row.
 __host__ __device__ constexpr int tr_ld(int no) { return (no * 64) % 128 == 64 ? no * 64 : no * 64 + 64; }
 
+// the row of a result register
+__device__ __forceinline__ constexpr int reg_row(int r) { return (r & 3) + 8 * (r >> 2); }
+
 // kinds of score
 enum { PLAIN = 0, BENT = 1, DROPPED = 2 };      // scale alone; cap / bias; cap / bias / dropout
 
@@ -60,9 +63,6 @@ __device__ __forceinline__ void tr_cols_swz(int lane, int& c0, int& c1) {
     c1 = (chunk ^ (hh + 2)) * 16 + b;
 }
 
-// the row of a result register
-__device__ __forceinline__ constexpr int reg_row(int r) { return (r & 3) + 8 * (r >> 2); }
-
 __device__ __forceinline__ int wave_min_i(int v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
@@ -74,13 +74,75 @@ __device__ __forceinline__ int wave_max_i(int v) {
     return v;
 }
 
-// q.k -> score in log2 units (cap and bias decided at run time, uniformly).  dist = c - key.
+// q.k -> score in log2 units (cap and bias decided at run time, uniformly).
+//
+// The cap's tanh costs an exponential and a reciprocal beside a probability's own exponential, and what bounds these kernels
+// is vector issue.  Scores are mostly small against their cap, and for |z| <= 0.625 tanh z = z P(z^2) with P of degree 4
+// (fitted to the largest error of z P on that range: 8e-8, less than the 2.4e-7 of the other form): in s = q.k, with the
+// scale folded into the coefficients, five multiply-adds and two products.  A block of scores that are all that small - one
+// wave-uniform test of its largest magnitude - uses it.
 struct Bend {
-    float scale2, in, cap2;          // scale log2 e;  2 scale log2 e / cap;  cap log2 e
+    float scale2, cap2;              // scale log2 e;  cap log2 e
+    float in, small;                 // 2 scale log2 e / cap;  |s| below which |z| <= 0.625
+    float c0, c1, c2, c3, c4;        // tanh(s scale / cap) = s (c0 + c1 s^2 + ...)
     bool capped, biased;
     __device__ __forceinline__ Bend(const DocArgs& p)
-        : scale2(p.scale * LOG2E), in(p.scale * (2.f * LOG2E) * p.rcap), cap2(p.cap * LOG2E), capped(p.cap > 0.f), biased(p.slopes != nullptr) {}
+        : scale2(p.scale * LOG2E), cap2(p.cap * LOG2E), in(p.scale * (2.f * LOG2E) * p.rcap), small(0.625f * p.cap / fabsf(p.scale)),
+          capped(p.cap > 0.f), biased(p.slopes != nullptr) {
+        const float z = p.scale * p.rcap, zz = z * z;
+        c0 = z * 0.999999463558197f;
+        c1 = z * zz * -0.33330482244491577f;
+        c2 = z * zz * zz * 0.13291031122207642f;
+        c3 = z * zz * zz * zz * -0.051362864673137665f;
+        c4 = z * zz * zz * zz * zz * 0.014530063606798649f;
+    }
+    __device__ __forceinline__ bool all_small(const f32x16& s) const {
+        float top = fabsf(s[0]);
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, fabsf(s[r]));
+        return __ballot(!(top <= small)) == 0;
+    }
+    __device__ __forceinline__ float poly(float s) const {           // tanh(s scale / cap) / s
+        const float w = s * s;
+        return fmaf(w, fmaf(w, fmaf(w, fmaf(w, c4, c3), c2), c1), c0);
+    }
+    __device__ __forceinline__ float any(float s) const { return fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + EXP2(s * in)), 1.f); }
+    // s -> tanh(s scale / cap)
+    __device__ __forceinline__ void tanh16(f32x16& s) const {
+        if (all_small(s)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= poly(s[r]);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = any(s[r]);
+        }
+    }
+    // s -> score + y, in log2 units
+    __device__ __forceinline__ void score16(f32x16& s, const f32x16& y) const {
+        if (!capped) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], scale2, y[r]);
+            return;
+        }
+        tanh16(s);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], cap2, y[r]);
+    }
 };
+// -slope |c - key| + rest over the registers of a block whose first key lies cf keys before c.  `before`: every key is at or
+// before c, which leaves one multiply-add for each.
+__device__ __forceinline__ f32x16 bias16(float slope2, float cf, float rest, bool before) {
+    f32x16 y;
+    if (before) {
+        const float first = fmaf(-slope2, cf, rest);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[r] = fmaf(slope2, (float)reg_row(r), first);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[r] = fmaf(-slope2, fabsf(cf - (float)reg_row(r)), rest);
+    }
+    return y;
+}
 
 // NaN if any register is not finite, else 0
 template <int NO>
