@@ -9,21 +9,22 @@
 namespace {
 
 // 64-row tiles of Q and dO: rows are (token, head of the group)
-template <int NCH, int COLS8>
+template <int NO>
 struct RowFetch {
-    int vq[NCH], vg[NCH];
+    static constexpr int N = Fetch<NO, 4>::N;
+    int vq[N], vg[N];
     __device__ __forceinline__ void init(const DocArgs& p, unsigned phase) {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int idx = threadIdx.x + 256 * i;
-            const unsigned r = idx / COLS8, c = idx % COLS8, x = phase + r, t = p.G == 1 ? x : x / (unsigned)p.G, g = x - t * (unsigned)p.G;
-            const bool in = (64 * COLS8 % 256 == 0 || idx < 64 * COLS8) && (int)c * 8 < p.D;
-            vq[i] = in ? (int)(t * p.ldq + g * p.D + c * 8) * 2 : (int)0x80000000;
-            vg[i] = in ? (int)(t * p.lddo + g * p.D + c * 8) * 2 : (int)0x80000000;
+        for (int i = 0; i < N; ++i) {
+            const unsigned x = phase + Fetch<NO, 4>::row_of_slot(i), c = Fetch<NO, 4>::col_of_slot(i);
+            const unsigned t = p.G == 1 ? x : x / (unsigned)p.G, g = x - t * (unsigned)p.G;
+            const bool in = (int)c * 8 < p.D;
+            vq[i] = in ? (int)(t * p.ldq + g * p.D + c * 8) * 2 : NOWHERE;
+            vg[i] = in ? (int)(t * p.lddo + g * p.D + c * 8) * 2 : NOWHERE;
         }
     }
     // rows from token t0 on, tokens below `end`
-    __device__ __forceinline__ void load(bf16x8 (&q)[NCH], bf16x8 (&g)[NCH], const DocArgs& p, int hk, int t0, int end) const {
+    __device__ __forceinline__ void dma(char* q, char* g, const DocArgs& p, int hk, int t0, int end) const {
 #if defined(__HIP_DEVICE_COMPILE__)
         const int n = min(end - t0, 65);                // 64 rows lie in at most 64 tokens, one more if they begin inside one
         const size_t first = (size_t)hk * p.G * p.D;
@@ -31,10 +32,11 @@ struct RowFetch {
             (void*)(p.q + (size_t)t0 * p.ldq + first), 0, (unsigned)(((long long)(n - 1) * p.ldq + (long long)p.G * p.D) * 2), 0x00020000);
         const __amdgpu_buffer_rsrc_t rg = __builtin_amdgcn_make_buffer_rsrc(
             (void*)(p.dout + (size_t)t0 * p.lddo + first), 0, (unsigned)(((long long)(n - 1) * p.lddo + (long long)p.G * p.D) * 2), 0x00020000);
+        const int piece = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * N * 1024;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            q[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rq, vq[i], 0, 0));
-            g[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rg, vg[i], 0, 0));
+        for (int i = 0; i < N; ++i) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, LDS_PTR(q + piece + i * 1024), 16, vq[i], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rg, LDS_PTR(g + piece + i * 1024), 16, vg[i], 0, 0, 0);
         }
 #endif
     }
@@ -48,13 +50,10 @@ struct RowInfo {                     // of the 64 staged rows
 };
 
 template <int ND, int NO, int KIND, int KB>
-__global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int tiles) {
-    constexpr int LD = tr_ld(NO);
-    constexpr int NCH = (64 * NO * 4 + 255) / 256;
-    __shared__ __attribute__((aligned(16))) char smem[2 * 64 * LD];
-    __shared__ __attribute__((aligned(16))) RowInfo info;
+__global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1) void doc_dkdv_kernel(const DocArgs p, int tiles) {
+    __shared__ __attribute__((aligned(16))) char smem[4 * TILE_BYTES<NO>];      // Q and dO, twice
+    __shared__ __attribute__((aligned(16))) RowInfo infos[2];
     __shared__ int range[4][2];
-    char *Qs = smem, *Gs = smem + 64 * LD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
     int unit, hk;
     if (!unit_of(tiles * p.splits, p.Hkv, unit, hk)) return;
@@ -96,9 +95,7 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
         for (int i = 0; i < NO; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) { dkT[kb][i][r] = 0.f; dvT[kb][i][r] = 0.f; }
-    const int tr_row = 4 * hh + ((lane & 15) >> 2);
-    int tr_c0, tr_c1;
-    tr_cols_swz(lane, tr_c0, tr_c1);
+    const Reads<ND, NO> rd;
     const Bend bend(p);
     __syncthreads();
     const int tlo = __builtin_amdgcn_readfirstlane(min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])));
@@ -115,17 +112,17 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
     const int kmax = min(key0 + 32 * KB, p.Tk);       // the wave's keys: seen whole by a row with lo <= key0 and hi >= kmax
     const float rsl2 = KIND == PLAIN ? 1.f / bend.scale2 : 0.f;
 
-    bf16x8 qreg[NCH], greg[NCH];
-    RowFetch<NCH, NO * 4> f;
+    RowFetch<NO> f;
     f.init(p, 0);
     int4 ireg = {0, 0, 0, 0};
     float lreg = 0.f, dreg = 0.f, sreg = 0.f;
     unsigned hreg = 0;
     bool in = false;
-    auto load = [&](unsigned r0) __attribute__((always_inline)) {
+    auto request = [&](unsigned r0) __attribute__((always_inline)) {
         const unsigned t0 = G == 1 ? r0 : r0 / G;
         if (64 % G != 0) f.init(p, r0 - t0 * G);
-        f.load(qreg, greg, p, hk, (int)t0, thi);
+        char* to = smem + (((r0 - rlo) >> 6) & 1) * 2 * TILE_BYTES<NO>;
+        f.dma(to, to + TILE_BYTES<NO>, p, hk, (int)t0, thi);
         if (threadIdx.x < 64) {
             const unsigned R = r0 + threadIdx.x;
             in = R < rhi;
@@ -139,12 +136,9 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
             if (KIND == DROPPED) hreg = drop_row(p, token, head);
         }
     };
-    if (rlo < rhi) load(rlo);
-    for (unsigned r0 = rlo; r0 < rhi; r0 += 64) {
-        __syncthreads();
-        put_tile<NCH, NO * 4, true>(qreg, Qs, LD, threadIdx.x);
-        put_tile<NCH, NO * 4, true>(greg, Gs, LD, threadIdx.x);
+    auto note = [&](unsigned r0) __attribute__((always_inline)) {      // what request() read of the rows, into the LDS
         if (threadIdx.x < 64) {
+            RowInfo& info = infos[((r0 - rlo) >> 6) & 1];
             const float ls = !in || lreg == -INFINITY ? INFINITY : lreg;         // rows that see nothing: probabilities of 0
             info.lse[threadIdx.x] = KIND == PLAIN ? -ls * rsl2 : -ls;
             info.delta[threadIdx.x] = KIND == DROPPED ? dreg : -dreg;
@@ -153,14 +147,22 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
             if (KIND != PLAIN) { info.c[threadIdx.x] = (float)(ireg.z - base); info.slope2[threadIdx.x] = -sreg * LOG2E; }
             if (KIND == DROPPED) info.drop[threadIdx.x] = hreg;
         }
-        __syncthreads();
-        if (r0 + 64 < rhi) load(r0 + 64);
-        if (r0 >= whi || r0 + 64 <= wlo) continue;
+    };
+    if (rlo < rhi) {
+        request(rlo);
+        note(rlo);
+    }
+    for (unsigned r0 = rlo; r0 < rhi; r0 += 64) {
+        tiles_landed();
+        const bool more = r0 + 64 < rhi;
+        if (more) request(r0 + 64);
+        const char *Qs = smem + (((r0 - rlo) >> 6) & 1) * 2 * TILE_BYTES<NO>, *Gs = Qs + TILE_BYTES<NO>;
+        const RowInfo& info = infos[((r0 - rlo) >> 6) & 1];
+        if (r0 < whi && r0 + 64 > wlo) {
         const int first = info.lo[lane], count = info.count[lane];
         const bool masked = __ballot(first > key0 || first + count < kmax) != 0;
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs) {
-            const char *Qt = Qs + qs * 32 * LD, *Gt = Gs + qs * 32 * LD;
             f32x16 s[KB], dp[KB];
             f32x4 ls[4], dl[4];
 #pragma unroll
@@ -177,8 +179,7 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
                 }
 #pragma unroll
             for (int ks = 0; ks < ND; ++ks) {
-                const int off = l31 * LD + ((ks * 2 + hh) ^ ((l31 >> 2) & 3)) * 16;
-                const bf16x8 aq = *(const bf16x8*)(Qt + off), ag = *(const bf16x8*)(Gt + off);
+                const bf16x8 aq = rd.frag(Qs, ks, qs), ag = rd.frag(Gs, ks, qs);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
                     s[kb] = mfma(aq, kf[kb][ks], s[kb]);
@@ -258,9 +259,7 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
             for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int db = 0; db < NO; ++db) {
-                    const int off = (16 * st + tr_row) * LD + db * 64;
-                    const bf16x8 ag = cat4(LDS_TR(Gt + off + tr_c0), LDS_TR(Gt + off + 8 * LD + tr_c1));
-                    const bf16x8 aq = cat4(LDS_TR(Qt + off + tr_c0), LDS_TR(Qt + off + 8 * LD + tr_c1));
+                    const bf16x8 ag = rd.frag_t(Gs, db, qs * 2 + st), aq = rd.frag_t(Qs, db, qs * 2 + st);
 #pragma unroll
                     for (int kb = 0; kb < KB; ++kb) {
                         dvT[kb][db] = mfma(ag, pf[kb][st], dvT[kb][db]);
@@ -268,6 +267,8 @@ __global__ __launch_bounds__(256, 1) void doc_dkdv_kernel(const DocArgs p, int t
                     }
                 }
         }
+        }
+        if (more) note(r0 + 64);
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {

@@ -6,12 +6,9 @@
 namespace {
 
 template <int ND, int NO, int KIND>
-__global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles) {
-    constexpr int DP = 16 * ND, KLD = tr_ld(NO), VLD = DP * 2 + 16;
-    constexpr int NCK = (64 * NO * 4 + 255) / 256, NCV = (64 * (DP / 8) + 255) / 256;
-    __shared__ __attribute__((aligned(16))) char smem[64 * KLD + 64 * VLD];
+__global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocArgs p, int tiles) {
+    __shared__ __attribute__((aligned(16))) char smem[4 * TILE_BYTES<NO>];      // K and V, twice
     __shared__ int range[4][2];
-    char *Ks = smem, *Vs = smem + 64 * KLD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
     int tile, hk;
     if (!unit_of(tiles, p.Hkv, tile, hk)) return;
@@ -73,28 +70,21 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles)
     for (int i = 0; i < NO; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dqT[i][r] = 0.f;
-    const int tr_row = 4 * hh + ((lane & 15) >> 2);
-    int tr_c0, tr_c1;
-    tr_cols_swz(lane, tr_c0, tr_c1);
     const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
-    bf16x8 kreg[NCK], vreg[NCV];
-    Fetch<NCK, NO * 4> kf;
-    Fetch<NCV, DP / 8> vf;
-    kf.init(threadIdx.x, p.ldk, p.D);
-    vf.init(threadIdx.x, p.ldv, p.D);
-    if (klo < khi) {
-        kf.load(kreg, kbase, p.ldk, p.D, klo, khi - klo);
-        vf.load(vreg, vbase, p.ldv, p.D, klo, khi - klo);
-    }
+    const Reads<ND, NO> rd;
+    Fetch<NO, 4> kf, vf;
+    kf.init(p.ldk, p.D);
+    vf.init(p.ldv, p.D);
+    auto request = [&](int k0) __attribute__((always_inline)) {
+        char* to = smem + (((k0 - klo) >> 6) & 1) * 2 * TILE_BYTES<NO>;
+        kf.dma(to, kbase, p.ldk, p.D, k0, khi - k0);
+        vf.dma(to + TILE_BYTES<NO>, vbase, p.ldv, p.D, k0, khi - k0);
+    };
+    if (klo < khi) request(klo);
     for (int k0 = klo; k0 < khi; k0 += 64) {
-        __syncthreads();
-        put_tile<NCK, NO * 4, true>(kreg, Ks, KLD, threadIdx.x);
-        put_tile<NCV, DP / 8, false>(vreg, Vs, VLD, threadIdx.x);
-        __syncthreads();
-        if (k0 + 64 < khi) {
-            kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, khi - k0 - 64);
-            vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, khi - k0 - 64);
-        }
+        tiles_landed();
+        if (k0 + 64 < khi) request(k0 + 64);
+        const char *Ks = smem + (((k0 - klo) >> 6) & 1) * 2 * TILE_BYTES<NO>, *Vs = Ks + TILE_BYTES<NO>;
         if (k0 >= hi || k0 + 64 <= lo) continue;
         const bool masked = k0 < in_lo || k0 + 64 > in_hi;
 #pragma unroll
@@ -104,10 +94,8 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles)
             for (int r = 0; r < 16; ++r) { s[r] = s0; dp[r] = KIND == DROPPED ? 0.f : -delta; }
 #pragma unroll
             for (int ks = 0; ks < ND; ++ks) {
-                const bf16x8 ak = *(const bf16x8*)(Ks + (kb * 32 + l31) * KLD + ((ks * 2 + hh) ^ ((l31 >> 2) & 3)) * 16);
-                const bf16x8 av = *(const bf16x8*)(Vs + (kb * 32 + l31) * VLD + (ks * 16 + 8 * hh) * 2);
-                s = mfma(ak, qf[ks], s);
-                dp = mfma(av, gf[ks], dp);
+                s = mfma(rd.frag(Ks, ks, kb), qf[ks], s);
+                dp = mfma(rd.frag(Vs, ks, kb), gf[ks], dp);
             }
             if constexpr (KIND == DROPPED) {
 #pragma unroll
@@ -146,10 +134,7 @@ __global__ __launch_bounds__(256) void doc_dq_kernel(const DocArgs p, int tiles)
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
-                for (int db = 0; db < NO; ++db) {
-                    const int off = (kb * 32 + 16 * st + tr_row) * KLD + db * 64;
-                    dqT[db] = mfma(cat4(LDS_TR(Ks + off + tr_c0), LDS_TR(Ks + off + 8 * KLD + tr_c1)), dsf[st], dqT[db]);
-                }
+                for (int db = 0; db < NO; ++db) dqT[db] = mfma(rd.frag_t(Ks, db, kb * 2 + st), dsf[st], dqT[db]);
         }
     }
     if (live) {

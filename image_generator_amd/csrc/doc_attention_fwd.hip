@@ -57,9 +57,9 @@ struct Rows {                        // a wave's 32 rows
     // does not mind the common factor while nothing leaves the normal range, and bf16 probabilities have fp32's exponents; a
     // row whose sum (`fits`) is not within 2^-100 .. 2^100 - scores beyond some 70 nats, or a distance bias on every key it
     // sees - sends its workgroup through the loop again with the maximum.
-    template <int KIND, bool FAST, int KLD, int VLD>
-    __device__ __forceinline__ void tile(const DocArgs& p, const Bend& bend, const char* Ks, const char* Vs, int k0) {
-        const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
+    template <int KIND, bool FAST>
+    __device__ __forceinline__ void tile(const DocArgs& p, const Bend& bend, const Reads<ND, NO>& at, const char* Ks, const char* Vs, int k0) {
+        const int hh = (threadIdx.x & 63) >> 5;
         f32x16 s[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -68,10 +68,7 @@ struct Rows {                        // a wave's 32 rows
 #pragma unroll
         for (int ks = 0; ks < ND; ++ks)
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                const bf16x8 a = *(const bf16x8*)(Ks + (kb * 32 + l31) * KLD + (ks * 16 + 8 * hh) * 2);
-                s[kb] = mfma(a, qf[ks], s[kb]);
-            }
+            for (int kb = 0; kb < 2; ++kb) s[kb] = mfma(at.frag(Ks, ks, kb), qf[ks], s[kb]);
         float sl2 = bend.scale2;
         if constexpr (KIND != PLAIN) {
             const bool before = k0 + 63 <= c_min;
@@ -123,16 +120,12 @@ struct Rows {                        // a wave's 32 rows
                 if constexpr (KIND == DROPPED) e = drop_keep(p, drop, k0 + kb * 32 + reg_row(r) + 4 * hh) ? e * p.drop_scale : 0.f;
                 pf[kb][r >> 3][r & 7] = (bf16_t)e;
             }
-        const int tr_row = 4 * hh + ((lane & 15) >> 2), tr_col = (((lane >> 4) & 1) * 16 + 4 * (lane & 3)) * 2;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
-                for (int db = 0; db < NO; ++db) {
-                    const char* a0 = Vs + (kb * 32 + 16 * st + tr_row) * VLD + db * 64 + tr_col;
-                    o[db] = mfma(cat4(LDS_TR(a0), LDS_TR(a0 + 8 * VLD)), pf[kb][st], o[db]);
-                }
+                for (int db = 0; db < NO; ++db) o[db] = mfma(at.frag_t(Vs, db, kb * 2 + st), pf[kb][st], o[db]);
     }
     __device__ __forceinline__ void reset(float reference) {
 #pragma unroll
@@ -154,11 +147,8 @@ struct Rows {                        // a wave's 32 rows
 
 template <int ND, int NO, int KIND>
 __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd_kernel(const DocArgs p, int tiles) {
-    constexpr int DP = 16 * ND, KLD = DP * 2 + 16, VLD = tr_ld(NO);
-    constexpr int NCK = (64 * (DP / 8) + 255) / 256, NCV = (64 * NO * 4 + 255) / 256;
-    __shared__ __attribute__((aligned(16))) char smem[64 * KLD + 64 * VLD];
+    __shared__ __attribute__((aligned(16))) char smem[4 * TILE_BYTES<NO>];      // K and V, twice: one tile arrives under the other
     __shared__ int range[4][2];
-    char *Ks = smem, *Vs = smem + 64 * KLD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
     int tile, hk;
     if (!unit_of(tiles, p.Hkv, tile, hk)) return;
@@ -170,27 +160,23 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
     const int khi = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
     const Bend bend(p);
     const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
-    bf16x8 kreg[NCK], vreg[NCV];
-    Fetch<NCK, DP / 8> kf;
-    Fetch<NCV, NO * 4> vf;
-    kf.init(threadIdx.x, p.ldk, p.D);
-    vf.init(threadIdx.x, p.ldv, p.D);
+    const Reads<ND, NO> at;
+    Fetch<NO, 4> kf, vf;
+    kf.init(p.ldk, p.D);
+    vf.init(p.ldv, p.D);
+    auto request = [&](int k0) __attribute__((always_inline)) {
+        char* to = smem + (((k0 - klo) >> 6) & 1) * 2 * TILE_BYTES<NO>;
+        kf.dma(to, kbase, p.ldk, p.D, k0, khi - k0);
+        vf.dma(to + TILE_BYTES<NO>, vbase, p.ldv, p.D, k0, khi - k0);
+    };
     auto pass = [&](auto fast) __attribute__((always_inline)) {
         w.reset(decltype(fast)::value ? 0.f : -INFINITY);
-        if (klo < khi) {
-            kf.load(kreg, kbase, p.ldk, p.D, klo, khi - klo);
-            vf.load(vreg, vbase, p.ldv, p.D, klo, khi - klo);
-        }
+        if (klo < khi) request(klo);
         for (int k0 = klo; k0 < khi; k0 += 64) {
-            __syncthreads();
-            put_tile<NCK, DP / 8, false>(kreg, Ks, KLD, threadIdx.x);
-            put_tile<NCV, NO * 4, false>(vreg, Vs, VLD, threadIdx.x);
-            __syncthreads();
-            if (k0 + 64 < khi) {
-                kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, khi - k0 - 64);
-                vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, khi - k0 - 64);
-            }
-            if (k0 < w.hi && k0 + 64 > w.lo) w.template tile<KIND, decltype(fast)::value, KLD, VLD>(p, bend, Ks, Vs, k0);
+            tiles_landed();                        // ... and every wave has left the tile before
+            if (k0 + 64 < khi) request(k0 + 64);
+            const char* Ks = smem + (((k0 - klo) >> 6) & 1) * 2 * TILE_BYTES<NO>;
+            if (k0 < w.hi && k0 + 64 > w.lo) w.template tile<KIND, decltype(fast)::value>(p, bend, at, Ks, Ks + TILE_BYTES<NO>, k0);
         }
         w.join();
     };
@@ -227,11 +213,9 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
 // once and only the rows that see a tile take part, so what is bound here is reading K and V.
 template <int ND, int NO, int KIND>
 __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) {
-    constexpr int DP = 16 * ND, KLD = DP * 2 + 16, VLD = tr_ld(NO);
-    constexpr int NCK = DP / 8, NCV = NO * 4;                     // 64 rows, 64 lanes
     extern __shared__ __attribute__((aligned(16))) char smem_all[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
-    char *Ks = smem_all + wave * 64 * (KLD + VLD), *Vs = Ks + 64 * KLD;
+    char *Ks = smem_all + wave * 2 * TILE_BYTES<NO>, *Vs = Ks + TILE_BYTES<NO>;
     const int hk = blockIdx.y, split = blockIdx.z * 4 + wave;
     const unsigned R = blockIdx.x * 32u + l31;
     Rows<ND, NO> w;
@@ -244,11 +228,11 @@ __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) 
     }
     const Bend bend(p);
     const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
-    bf16x8 kreg[NCK], vreg[NCV];
-    Fetch<NCK, DP / 8, 64> kf;
-    Fetch<NCV, NO * 4, 64> vf;
-    kf.init(lane, p.ldk, p.D);
-    vf.init(lane, p.ldv, p.D);
+    const Reads<ND, NO> at;
+    Fetch<NO, 1> kf, vf;
+    bf16x8 kreg[kf.N], vreg[vf.N];
+    kf.init(p.ldk, p.D);
+    vf.init(p.ldv, p.D);
     w.reset(-INFINITY);
     {   // (with the running maximum: what bounds this loop is memory, and a distance bias makes far runs tiny)
         if (from < to) {
@@ -258,15 +242,15 @@ __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) 
         for (int k0 = from; k0 < to; k0 += 64) {
             // one wave: its LDS operations complete in order, the fences only keep the compiler from reordering them
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            put_tile<NCK, DP / 8, false, 64>(kreg, Ks, KLD, lane);
-            put_tile<NCV, NO * 4, false, 64>(vreg, Vs, VLD, lane);
+            kf.put(kreg, Ks);
+            vf.put(vreg, Vs);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             if (k0 + 64 < to) {
                 kf.load(kreg, kbase, p.ldk, p.D, k0 + 64, to - k0 - 64);
                 vf.load(vreg, vbase, p.ldv, p.D, k0 + 64, to - k0 - 64);
             }
             // a run ends with whole tiles, or where the last of the rows' intervals does
-            w.template tile<KIND, false, KLD, VLD>(p, bend, Ks, Vs, k0);
+            w.template tile<KIND, false>(p, bend, at, Ks, Vs, k0);
         }
         w.join();
     }
@@ -346,7 +330,7 @@ static int fwd_splits(int Tq, int Tk, int Hq, int Hkv) {
 
 template <int ND, int NO, int KIND>
 int launch_split(const DocArgs& a, hipStream_t st) {
-    constexpr int LDS = 4 * 64 * (16 * ND * 2 + 16 + tr_ld(NO));
+    constexpr int LDS = 4 * 2 * TILE_BYTES<NO>;
     static std::once_flag once;
     static hipError_t set;
     std::call_once(once, [] { set = hipFuncSetAttribute((const void*)doc_fwd_split_kernel<ND, NO, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });

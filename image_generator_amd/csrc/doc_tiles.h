@@ -13,9 +13,40 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ bf16x8 cat4(bf16x4 a, bf16x4 b) { return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-// Row stride (bytes) of a tile read with transposing reads of 32-column blocks: the four rows that a 16-lane group touches lie
-// 64 bytes apart modulo the 256-byte bank row.
-__host__ __device__ constexpr int tr_ld(int no) { return (no * 64) % 128 == 64 ? no * 64 : no * 64 + 64; }
+// A staged tile: 64 rows of NO * 4 chunks of 16 bytes, without padding (the LDS-DMA writes a wave's 64 chunks one behind
+// another), chunk c of row r at place c ^ swz(r).  Read by rows, 16 consecutive rows at one c cover all 16 bank slots of the
+// 256-byte bank row; read by ds_read_b64_tr_b16, the four rows of a 16-lane group lie in four different 64-byte blocks of it.
+template <int NO>
+__host__ __device__ constexpr int swz(int r) {
+    return NO == 2 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1 | ((r >> 3) & 1)
+         : NO == 4 ? (r & 3) << 2 | ((r >> 2) & 3) : (r >> 2) & 3;
+}
+template <int NO> constexpr int TILE_LD = NO * 64;
+template <int NO> constexpr int TILE_BYTES = 64 * NO * 64;
+
+// offsets of a lane's reads inside a tile
+template <int ND, int NO>
+struct Reads {
+    int row[ND];                     // chunk of contraction step ks in row lane & 31 (rows 32 apart: + 32 * TILE_LD)
+    int tr[NO][2];                   // transposing reads of column block db: rows 0 .. 7 and 8 .. 15 of a 16-row block
+    __device__ __forceinline__ Reads() {
+        const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
+#pragma unroll
+        for (int ks = 0; ks < ND; ++ks) row[ks] = l31 * TILE_LD<NO> + ((ks * 2 + hh) ^ swz<NO>(l31)) * 16;
+        const int r = 4 * hh + ((lane & 15) >> 2), c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+#pragma unroll
+        for (int db = 0; db < NO; ++db)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) tr[db][h] = (r + 8 * h) * TILE_LD<NO> + ((db * 4 + c) ^ swz<NO>(r + 8 * h)) * 16 + (lane & 1) * 8;
+    }
+    __device__ __forceinline__ bf16x8 frag(const char* tile, int ks, int block32) const {
+        return *(const bf16x8*)(tile + row[ks] + block32 * 32 * TILE_LD<NO>);
+    }
+    __device__ __forceinline__ bf16x8 frag_t(const char* tile, int db, int block16) const {
+        const char* t = tile + block16 * 16 * TILE_LD<NO>;
+        return cat4(LDS_TR(t + tr[db][0]), LDS_TR(t + tr[db][1]));
+    }
+};
 
 // the row of a result register
 __device__ __forceinline__ constexpr int reg_row(int r) { return (r & 3) + 8 * (r >> 2); }
@@ -23,44 +54,56 @@ __device__ __forceinline__ constexpr int reg_row(int r) { return (r & 3) + 8 * (
 // kinds of score
 enum { PLAIN = 0, BENT = 1, DROPPED = 2 };      // scale alone; cap / bias; cap / bias / dropout
 
-// NCH 16-byte chunks per thread of a 64-row tile with `cols8` chunks a row (the columns past D and the rows past `valid` read
-// as zeros, by the descriptor's bounds).  A thread's chunks are the same slots of every tile; a tile has a descriptor of its
-// own (a 64-bit base, made from scalars), so no row offset passes 32 bits.
-template <int NCH, int COLS8, int THREADS = 256>
+#define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
+constexpr int NOWHERE = (int)0x80000000;        // a buffer offset that reads as zeros
+
+// The part of a 64-row tile that one of WAVES waves brings: chunks per lane, and where they come from.  A lane's chunks are the
+// same places of every tile; a tile has a descriptor of its own (a 64-bit base, made from scalars), so no row offset passes 32
+// bits, and its bound turns the rows past `valid` and the columns past D into zeros.
+template <int NO, int WAVES>
 struct Fetch {
-    int voff[NCH];
-    __device__ __forceinline__ void init(int tid, long long ld, int D) {
+    static constexpr int N = NO * 4 / WAVES;
+    int voff[N];
+    __device__ __forceinline__ static int slot(int i) { return (((int)(threadIdx.x >> 6) % WAVES) * N + i) * 64 + (int)(threadIdx.x & 63); }
+    __device__ __forceinline__ static int row_of_slot(int i) { return slot(i) / (NO * 4); }
+    __device__ __forceinline__ static int col_of_slot(int i) { const int s = slot(i), r = s / (NO * 4); return (s - r * (NO * 4)) ^ swz<NO>(r); }
+    __device__ __forceinline__ void init(long long ld, int D) {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int idx = tid + THREADS * i, r = idx / COLS8, c = idx % COLS8;
-            voff[i] = (idx < 64 * COLS8 && c * 8 < D) ? (int)(r * ld + c * 8) * 2 : (int)0x80000000;
-        }
+        for (int i = 0; i < N; ++i) voff[i] = col_of_slot(i) * 8 < D ? (int)(row_of_slot(i) * ld + col_of_slot(i) * 8) * 2 : NOWHERE;
     }
-    // rows row0 .. row0 + 63 of base (row0 >= 0), of which `valid` may be read
-    __device__ __forceinline__ void load(bf16x8 (&reg)[NCH], const bf16_t* base, long long ld, int D, int row0, int valid) const {
 #if defined(__HIP_DEVICE_COMPILE__)
+    __device__ __forceinline__ static __amdgpu_buffer_rsrc_t rsrc(const bf16_t* base, long long ld, int D, int row0, int valid) {
         valid = min(valid, 64);
         const unsigned bytes = valid > 0 ? (unsigned)(((long long)(valid - 1) * ld + D) * 2) : 0u;
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (size_t)row0 * ld), 0, bytes, 0x00020000);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (size_t)row0 * ld), 0, bytes, 0x00020000);
+    }
+#endif
+    // rows row0 .. row0 + 63 of base straight into the LDS; whoever reads them waits (tiles_landed) and meets at a barrier first
+    __device__ __forceinline__ void dma(char* tile, const bf16_t* base, long long ld, int D, int row0, int valid) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const __amdgpu_buffer_rsrc_t rs = rsrc(base, ld, D, row0, valid);
+        char* to = tile + (int)__builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % WAVES) * N * 1024;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) reg[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, voff[i], 0, 0));
+        for (int i = 0; i < N; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LDS_PTR(to + i * 1024), 16, voff[i], 0, 0, 0);
 #endif
     }
-};
-// chunk c of row r goes to chunk c (SWZ: c ^ ((r >> 2) & 3)) of row r
-template <int NCH, int COLS8, bool SWZ, int THREADS = 256>
-__device__ __forceinline__ void put_tile(const bf16x8 (&reg)[NCH], char* dst, int ld, int tid) {
+    // ... or by way of registers
+    __device__ __forceinline__ void load(bf16x8 (&reg)[N], const bf16_t* base, long long ld, int D, int row0, int valid) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const __amdgpu_buffer_rsrc_t rs = rsrc(base, ld, D, row0, valid);
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-        const int idx = tid + THREADS * i, r = idx / COLS8, c = idx % COLS8;
-        if (64 * COLS8 % THREADS == 0 || idx < 64 * COLS8) *(bf16x8*)(dst + r * ld + (SWZ ? c ^ ((r >> 2) & 3) : c) * 16) = reg[i];
+        for (int i = 0; i < N; ++i) reg[i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, voff[i], 0, 0));
+#endif
     }
-}
-// byte offsets inside a row of a swizzled tile for the two transposing reads of a fragment
-__device__ __forceinline__ void tr_cols_swz(int lane, int& c0, int& c1) {
-    const int hh = lane >> 5, chunk = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), b = (lane & 1) * 8;
-    c0 = (chunk ^ hh) * 16 + b;
-    c1 = (chunk ^ (hh + 2)) * 16 + b;
+    __device__ __forceinline__ static void put(const bf16x8 (&reg)[N], char* tile) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) *(bf16x8*)(tile + slot(i) * 16) = reg[i];
+    }
+};
+// every request of this wave has landed, and every wave is here
+__device__ __forceinline__ void tiles_landed() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
 }
 
 __device__ __forceinline__ int wave_min_i(int v) {
