@@ -313,22 +313,29 @@ __global__ __launch_bounds__(256) void doc_dkdv_join_kernel(const DocArgs p) {
     const int key = (int)(u / p.Hkv), hk = (int)(u % p.Hkv);
     const int2 span = key_span(p, key);
     const bool seen = span.y > span.x;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int n = 2 * p.D;
-    for (int z = 0; z < p.splits; ++z) {
-        const float* part = p.part + ((size_t)z * p.Tk * p.Hkv + u) * n;
+    const int n = 2 * p.D, at = min(lane * 4, n - 4);      // dK then dV: at most 256 values, four a lane
+    const float* part = p.part + u * n + at;
+    const size_t step = (size_t)p.Tk * p.Hkv * n;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    int z = 0;
+    for (; z + 8 <= p.splits; z += 8) {
+        f32x4 v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (lane + 64 * e < n) acc[e] += part[lane + 64 * e];
+        for (int e = 0; e < 8; ++e) v[e] = *(const f32x4*)(part + (z + e) * step);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc += v[e];
     }
-    bf16_t *dk = p.dk + (size_t)key * p.lddk + (size_t)hk * p.D, *dv = p.dv + (size_t)key * p.lddv + (size_t)hk * p.D;
+    for (; z < p.splits; ++z) acc += *(const f32x4*)(part + z * step);
     bool bad = false;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int d = lane + 64 * e;
-        if (d >= n) continue;
-        bad |= !(acc[e] * 0.f == 0.f);
-        if (d < p.D) dk[d] = seen ? (bf16_t)(acc[e] * p.scale) : (bf16_t)0.f;
-        else dv[d - p.D] = seen ? (bf16_t)acc[e] : (bf16_t)0.f;
+    for (int e = 0; e < 4; ++e) bad |= !(acc[e] * 0.f == 0.f);
+    if (lane * 4 < n) {
+        const bool v = at >= p.D;
+        bf16_t* to = v ? p.dv + (size_t)key * p.lddv + (size_t)hk * p.D + at - p.D : p.dk + (size_t)key * p.lddk + (size_t)hk * p.D + at;
+        bf16x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = seen ? (bf16_t)(v ? acc[e] : acc[e] * p.scale) : (bf16_t)0.f;
+        *(bf16x4*)to = y;
     }
     if (seen && __ballot(bad) != 0) plain_dkdv_key(p, key, hk);
 }

@@ -297,15 +297,28 @@ __global__ __launch_bounds__(256) void doc_fwd_join_kernel(const DocArgs p, unsi
     const float w = ml.x == -INFINITY ? 0.f : EXP2(ml.x - M);
     const float l = wave_sum(ml.y * w);
     const float* part = p.part + (size_t)p.Hkv * rows * p.splits * 2 + row * p.D;
+    // runs with something to add, eight loads at a time (a run that adds nothing is not read: its values were not written)
     float o[2] = {0.f, 0.f};
+    const int d0 = min(lane, p.D - 1), d1 = min(lane + 64, p.D - 1);
     unsigned long long who = __ballot(ml.x != -INFINITY);
     while (who) {
-        const int s = __builtin_ctzll(who);
-        who &= who - 1;
-        const float ws = __shfl(w, s, 64);
+        float ws[8], v0[8], v1[8];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-            if (lane + 64 * u < p.D) o[u] = fmaf(ws, part[(size_t)s * p.D + lane + 64 * u], o[u]);
+        for (int e = 0; e < 8; ++e) {
+            const int s = who ? __builtin_ctzll(who) : -1;
+            who &= who - 1;
+            ws[e] = s < 0 ? 0.f : __shfl(w, s < 0 ? 0 : s, 64);
+            v0[e] = v1[e] = 0.f;
+            if (s >= 0) {                                  // (uniform)
+                v0[e] = part[(size_t)s * p.D + d0];
+                v1[e] = part[(size_t)s * p.D + d1];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            o[0] = fmaf(ws[e], v0[e], o[0]);
+            o[1] = fmaf(ws[e], v1[e], o[1]);
+        }
     }
     const float inv = nan ? NAN : l > 0.f || l != l ? 1.f / l : 0.f;
     bf16_t* out = p.out + (size_t)token * p.ldo + (size_t)head * p.D;
