@@ -25,7 +25,8 @@ constexpr int PARTS = 512;           // partial sums of the norm: two workgroups
 // largest magnitude, at 127 / 2), and the margin keeps the fp64 steps' own rounding from deciding them.
 constexpr double HALF = 0.5 - 0x1p-30;
 
-// record of a tensor: parameter, bf16 copy (or 0), elements, first block in the flat moment arrays
+// record of a tensor: parameter (0: its gradient counts in the norm, nothing is stepped), bf16 copy (or 0), elements, first block
+// in the flat moment arrays
 struct Rec { long long p, p16, n, block0; };
 // hyper: lr, beta1, beta2, eps, weight decay, bc1, bc2, max norm, 1 - lr wd, lr / bc1, 1 / sqrt(bc2), 1 - beta1, 1 - beta2
 enum { H_LR, H_B1, H_B2, H_EPS, H_WD, H_BC1, H_BC2, H_MAX, H_DECAY, H_STEP, H_RBC2, H_OMB1, H_OMB2 };
@@ -207,7 +208,7 @@ __device__ __forceinline__ bool norm_of(const double* __restrict__ partial, floa
     const bool fine = sq <= 3.4028234663852886e38;            // false for NaN; beyond fp32 is where the flat-buffer update skips
     norm = sqrt(sq);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
-        state[0] = (float)norm;
+        state[0] = fine ? (float)norm : sq == sq ? INFINITY : NAN;
         if (!fine) state[1] += 1.f;
     }
     return fine;
@@ -222,9 +223,9 @@ __global__ __launch_bounds__(256) void multi_adamw32_kernel(const Rec* __restric
     double norm;
     if (!norm_of(partial, state, norm)) return;
     const int2 at = map[blockIdx.x];
-    const long long g = grads[at.x];
-    if (g == 0) return;
     const Rec t = recs[at.x];
+    const long long g = t.p ? grads[at.x] : 0;
+    if (g == 0) return;
     const float lr = (float)hyper[H_LR], b1 = (float)hyper[H_B1], b2 = (float)hyper[H_B2], eps = (float)hyper[H_EPS];
     const float wd = (float)hyper[H_WD], bc1 = (float)hyper[H_BC1], bc2 = (float)hyper[H_BC2];
     float scale = 1.f;
@@ -266,8 +267,8 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
     constexpr int MINE = WG_BLOCKS / 4;                               // blocks of a wave, all of them on their way at once
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int2 at = map[blockIdx.x];
-    const long long g = grads[at.x];
     const Rec t = recs[at.x];
+    const long long g = t.p ? grads[at.x] : 0;
     f32x4 pvs[MINE], gvs[MINE];
     unsigned mcs[MINE], ucs[MINE];
     float mss[MINE], uss[MINE];

@@ -9,12 +9,15 @@ What is different on purpose:
   * the image tower (`encoder/image_encoder.py`: a pretrained CLIP ViT fetched by name) is not part of this package; the
     step takes its output, the image embeddings, as an input and returns their gradient for whoever owns that tower;
   * bf16 compute with fp32 masters instead of fp16 autocast + GradScaler (train_encoder.py:51,103-109).  What the
-    GradScaler also does - leave every parameter untouched when a gradient is not finite - is kept: one table-driven
-    launch sums the squares of all gradients (the temperature's included), the update kernels skip on a non-finite sum
-    and count the skip, and the temperature's own update is gated by the same device flag.  No host synchronisation;
+    GradScaler also does - leave every parameter untouched when a gradient is not finite - is kept: the optimizer's norm
+    covers all gradients (the temperature's included), its update skips on a non-finite one and counts the skip, and the
+    temperature's own update is gated by the same device value.  No host synchronisation;
   * every matrix product, the attention (mask and dropout inside the flash kernels), the normalisations, the loss and
-    the parameter update run in libmi355_denoiser.so; the update is `mi355_adamw_step` per parameter tensor, which also
-    writes the bf16 operand copy the next forward pass multiplies with.
+    the parameter update run in libmi355_denoiser.so; the update is `optim.TensorAdamW`, two launches for all tensors,
+    which also write the bf16 operand copies the next forward pass multiplies with.  `state_bits=8` holds its moments in
+    8 bits;
+  * `train_step_packed` takes captions without padding (tokens one behind another, documents by offsets) through
+    `TextEncoder.forward_packed`.
 """
 from __future__ import annotations
 
@@ -22,81 +25,54 @@ import torch
 
 from ._lib import lib, check
 from .ops import F32, _stream
+from .optim import TensorAdamW
 
 
 class ContrastiveTrainer:
-    def __init__(self, text_encoder, criterion, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    def __init__(self, text_encoder, criterion, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
         self.enc, self.crit = text_encoder, criterion
         self.lr, self.betas, self.eps, self.wd = lr, betas, eps, weight_decay
         self.t = 0
         dev = next(text_encoder.parameters()).device
         if dev.type != "cuda":
             raise RuntimeError("ContrastiveTrainer: parameters must live on the HIP device (no CPU path)")
-        self.params = [p for p in text_encoder.parameters() if p.requires_grad]
-        if any(p.numel() % 4 for p in self.params):
-            raise ValueError("ContrastiveTrainer: parameter sizes must be multiples of 4")
-        self.m = [torch.zeros_like(p) for p in self.params]
-        self.v = [torch.zeros_like(p) for p in self.params]
-        self.hyper = torch.zeros(9, dtype=F32, device=dev)
-        # [0] = sum of squared gradients of the step (no clipping: only its finiteness is used), [1] = skip count
-        self.state = torch.zeros(4, dtype=F32, device=dev)
-        self._hyper_host = None
-        self._table_host = None
-        self._table = torch.zeros((len(self.params) + 1, 2), dtype=torch.int64, device=dev)
-        # the loss's single scalar (the library's update works on multiples of 4): AdamW in a few one-element tensor
-        # ops, lr 0.1 x the encoder's (train_encoder.py:42-49), gated by the same non-finite flag
+        self.names, self.params = zip(*((n, p) for n, p in text_encoder.named_parameters() if p.requires_grad))
+        # the loss's single scalar: AdamW in a few one-element tensor ops, lr 0.1 x the encoder's (train_encoder.py:42-49),
+        # gated by the optimizer's norm, in which its gradient counts
         self.temp = [p for p in criterion.parameters() if p.requires_grad]
         self.temp_m = [torch.zeros_like(p) for p in self.temp]
         self.temp_v = [torch.zeros_like(p) for p in self.temp]
+        self.opt = TensorAdamW(self.params, lr, betas, eps, weight_decay, state_bits=state_bits, watched=[p.numel() for p in self.temp])
+        self.state = self.opt.state            # [0] = norm of the step's gradients (no clipping: only its finiteness is used)
+        if state_bits == 32:
+            self.m, self.v = self.opt.split(self.opt.m), self.opt.split(self.opt.v)
         self.step_count = 0
-        self._updates_per_step = 1
-
-    def _set_hyper(self):
-        from .ops import PinnedRing
-        if self._hyper_host is None:
-            self._hyper_host = PinnedRing(lambda: torch.zeros(9, dtype=F32).pin_memory(), 8)
-        self.t += 1
-        h = self._hyper_host.acquire()
-        h[0], h[1], h[2], h[3], h[4] = self.lr, self.betas[0], self.betas[1], self.eps, self.wd
-        h[5], h[6] = 1 - self.betas[0] ** self.t, 1 - self.betas[1] ** self.t
-        h[7], h[8] = 0.0, 1.0
-        self.hyper.copy_(h, non_blocking=True)
-        self._hyper_host.copied()
-        self._hyper_host.release()
 
     def train_step(self, input_ids, attention_mask, image_embeds):
         """Returns (loss, gradient of the loss with respect to image_embeds)."""
+        return self._train_step(lambda: self.enc(input_ids, attention_mask, return_pooled=True), image_embeds)
+
+    def train_step_packed(self, input_ids, offsets, image_embeds):
+        """`train_step` on captions without padding: input_ids [tokens], offsets int32 [captions + 1]."""
+        return self._train_step(lambda: self.enc.forward_packed(input_ids, offsets, return_pooled=True), image_embeds)
+
+    def _train_step(self, encode, image_embeds):
         self.enc.train()
         img = image_embeds.detach().to(F32).requires_grad_(True)
         for p in self.params:
             p.grad = None
         for p in self.temp:
             p.grad = None
-        text = self.enc(input_ids, attention_mask, return_pooled=True)
-        loss = self.crit(text, img)
+        loss = self.crit(encode(), img)
         loss.backward()
-        self._set_hyper()
         packs = self.enc._train_packs()
-        names = {id(p): n for n, p in self.enc.named_parameters()}
-        s = _stream()
-        grads = []
-        for p in self.params:
-            g = p.grad
-            if g is not None and not (g.dtype == F32 and g.is_contiguous()):
-                g = g.to(F32).contiguous()
-            grads.append(g)
+        copies = [packs[n].w16 if n in packs else None for n in self.names]
+        if [c is not None and c.data_ptr() for c in copies] != [c is not None and c.data_ptr() for c in self.opt.copies]:
+            self.opt.set_copies(copies)
         tgrads = [None if p.grad is None else p.grad.to(F32).contiguous() for p in self.temp]
-        self._sum_squares([g for g in grads + tgrads if g is not None], s)
-        n_upd = 0
-        for p, g, m, v in zip(self.params, grads, self.m, self.v):
-            if g is None:
-                continue
-            pk = packs.get(names[id(p)])
-            p16 = None if pk is None else pk.w16.data_ptr()
-            check(lib.mi355_adamw_step(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p16, self.hyper.data_ptr(),
-                                       self.state.data_ptr(), p.numel(), s), "adamw")
-            n_upd += 1
-        self._updates_per_step = max(n_upd, 1)
+        self.t += 1
+        self.opt.step([None if p.grad is None else p.grad.to(F32) for p in self.params], lr=self.lr, watched=tgrads)
+        s = _stream()
         for pk in packs.values():        # the data-gradient operands of the next step
             check(lib.mi355_transpose_bf16(pk.w16.data_ptr(), pk.w16_t.data_ptr(), 1, pk.n, pk.k, s), "transpose")
         self.enc.operands_current()
@@ -104,29 +80,11 @@ class ContrastiveTrainer:
         self.step_count += 1
         return loss.detach(), img.grad
 
-    def _sum_squares(self, grads, s):
-        """state[0] = sum of the squares of every gradient of this step: one table (address, count) through a pinned
-        ring, one launch."""
-        from .ops import PinnedRing
-        n = len(grads)
-        if self._table_host is None:
-            rows = self._table.shape[0]
-            self._table_host = PinnedRing(lambda: torch.zeros((rows, 2), dtype=torch.int64).pin_memory(), 8)
-        h = self._table_host.acquire()
-        for i, g in enumerate(grads):
-            h[i, 0], h[i, 1] = g.data_ptr(), g.numel()
-        self._table.copy_(h, non_blocking=True)
-        self._table_host.copied()
-        self._table_host.release()
-        check(lib.mi355_zero_f32(self.state.data_ptr(), 1, s), "zero")
-        if n:
-            check(lib.mi355_sumsq_ranges(self._table.data_ptr(), n, self.state.data_ptr(), s), "sumsq_ranges")
-
     def _temperature_step(self, tgrads):
         b1, b2 = self.betas
         lr = self.lr * 0.1
         bc1, bc2 = 1 - b1 ** self.t, 1 - b2 ** self.t
-        ok = torch.isfinite(self.state[0])                      # device flag: nothing moves on a non-finite step
+        ok = torch.isfinite(self.state[0])                      # device value: nothing moves on a non-finite step
         with torch.no_grad():
             for p, g, m, v in zip(self.temp, tgrads, self.temp_m, self.temp_v):
                 if g is None:
@@ -141,4 +99,4 @@ class ContrastiveTrainer:
 
     def skipped_steps(self) -> int:
         """Steps whose gradients were not finite and that therefore changed nothing (host synchronisation)."""
-        return int(round(float(self.state[1]) / self._updates_per_step))
+        return self.opt.skipped_steps()

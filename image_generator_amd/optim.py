@@ -25,10 +25,14 @@ class TensorAdamW:
     max_grad_norm: global norm to clip to (0: none).  A step whose gradients are not finite changes nothing and is counted
     (`skipped_steps`), as in `trainer.FusedAdamW`; like there, its number still advances the bias correction.
 
+    watched: sizes of further gradients, stepped by someone else, that count in the norm (and in the test for finite values); they
+    follow as `bind(..., watched=[...])`.
+
     `step(grads)` uploads what changes (addresses, bias corrections) and launches.  For a captured graph: `bind(grads)` before
     the capture and before every replay, `apply()` inside it; the gradients stay the caller's to keep."""
 
-    def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=0.0, state_bits=32, copies=None):
+    def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=0.0, state_bits=32, copies=None,
+                 watched=()):
         self.params = list(params)
         if not self.params:
             raise ValueError("TensorAdamW: no parameters")
@@ -46,6 +50,7 @@ class TensorAdamW:
         self._shapes = [p.shape for p in self.params]
         self.lr, self.betas, self.eps, self.wd, self.max_norm = lr, tuple(betas), eps, weight_decay, max_grad_norm
         self.bits, self.device, self.t = state_bits, dev, 0
+        self.watched = list(watched)
         blocks = [-(-p.numel() // BLOCK) for p in self.params]
         self.starts = [0]
         for b in blocks:
@@ -58,12 +63,12 @@ class TensorAdamW:
             self.u_codes = torch.zeros(total * BLOCK, dtype=torch.uint8, device=dev)
             self.m_scales, self.u_scales = (torch.zeros(total, dtype=F32, device=dev) for _ in range(2))
         parts = [torch.stack((torch.full((-(-b // _WG_BLOCKS),), i, dtype=torch.int32),
-                              torch.arange(0, b, _WG_BLOCKS, dtype=torch.int32)), 1) for i, b in enumerate(blocks) if b]
+                              torch.arange(0, b, _WG_BLOCKS, dtype=torch.int32)), 1) for i, b in enumerate(blocks + [-(-n // BLOCK) for n in self.watched]) if b]
         self._map = torch.cat(parts).to(dev) if parts else torch.zeros((0, 2), dtype=torch.int32, device=dev)
         self._elements = float(sum(p.numel() for p in self.params))
         self._partial = torch.zeros(int(lib.mi355_multi_adamw_parts()), dtype=torch.float64, device=dev)
         self.state = torch.zeros(2, dtype=F32, device=dev)          # norm of the last step, skipped steps
-        n = len(self.params)
+        n = len(self.params) + len(self.watched)
         self._upload = torch.zeros(_HYPER + n, dtype=torch.int64, device=dev)
         self._ring = PinnedRing(lambda: torch.zeros(_HYPER + n, dtype=torch.int64).pin_memory(), 8)
         self._kept, self._bound = [], False
@@ -81,9 +86,10 @@ class TensorAdamW:
         self.copies = copies
         self._written = [t for t in self.params + copies if t is not None]
         rows = [[p.data_ptr(), 0 if c is None else c.data_ptr(), p.numel(), s] for p, c, s in zip(self.params, copies, self.starts)]
+        rows += [[0, 0, n, 0] for n in self.watched]
         self._recs = torch.tensor(rows, dtype=torch.int64).to(self.device)
 
-    def bind(self, grads=None, lr=None):
+    def bind(self, grads=None, lr=None, watched=None):
         """Begin a step: gradients (default: the parameters' own `.grad`; None leaves a parameter alone) and learning rate.
         Addresses and scalars go to the device in one asynchronous copy on the current stream."""
         if torch.cuda.is_current_stream_capturing():
@@ -94,6 +100,13 @@ class TensorAdamW:
         if len(grads) != len(self.params):
             raise ValueError(f"TensorAdamW: {len(grads)} gradients of {len(self.params)} parameters")
         words, kept = self._addresses(grads, owned)
+        watched = [None] * len(self.watched) if watched is None else list(watched)
+        if len(watched) != len(self.watched):
+            raise ValueError(f"TensorAdamW: {len(watched)} watched gradients, {len(self.watched)} announced")
+        for n, g in zip(self.watched, watched):
+            if g is not None and (g.numel() != n or g.device != self.device or g.dtype not in (F32, BF16) or not g.is_contiguous()):
+                raise ValueError("TensorAdamW: a watched gradient must be a contiguous fp32 or bf16 tensor of the announced size")
+            words.append(0 if g is None else g.data_ptr() | (g.dtype == BF16))
         if lr is not None:
             self.lr = lr
         self.t += 1
@@ -153,8 +166,8 @@ class TensorAdamW:
                                          _stream()), "multi_adamw")
         torch.autograd.graph.increment_version(self._written)
 
-    def step(self, grads=None, lr=None):
-        self.bind(grads, lr)
+    def step(self, grads=None, lr=None, watched=None):
+        self.bind(grads, lr, watched)
         self.apply()
 
     def _on_device(self):

@@ -92,6 +92,19 @@ class _AttnTrainFn(torch.autograd.Function):
         return dqkv, None, None, None, None
 
 
+class _QueriesAndKeysFn(torch.autograd.Function):
+    """[q | k | v] as q and [k | v], copies of their own; the gradients go back into one matrix."""
+
+    @staticmethod
+    def forward(ctx, qkv, width):
+        ctx.width = width
+        return qkv[:, :width].contiguous(), qkv[:, width:].contiguous()
+
+    @staticmethod
+    def backward(ctx, dq, dkv):
+        return torch.cat((dq, dkv), 1), None
+
+
 class _DropoutAddFn(torch.autograd.Function):
     """y = residual + dropout_p(x): the dropout behind the attention / feed-forward output projection and the residual
     add in one pass."""
@@ -323,6 +336,71 @@ class TextEncoder(nn.Module):
         x = LayerNormFn.apply(x, self.norm.weight, self.norm.bias, self.norm.eps)
         y = LinearFn.apply(x, packs["projection.weight"], self.projection.bias, None, True, self.projection.weight)
         return self._poison(y.view(B, T, -1), bad)
+
+    # ---- captions without padding ---------------------------------------------------------------
+    # Options of the packed path that the reference does not have (its encoder attends without positions or caps): scores
+    # capped by a tanh, and a bias that falls with the distance of two tokens (slope per head), which gives the encoder the
+    # order of the words without a parameter.  None / 0 leave the reference's arithmetic.
+    score_cap = 0.0
+    distance_slopes = None
+
+    def forward_packed(self, input_ids, offsets, return_pooled=True):
+        """The encoder on captions that lie one behind another: input_ids [tokens] (int32 / int64), caption n the tokens
+        offsets[n] .. offsets[n + 1] (int32 on the device, any layout that `ops.doc_attention_fwd` takes).  Returns the
+        pooled, normalised rows [captions, projection_dim], or every token's projected state [tokens, projection_dim].
+        The arithmetic of `forward` on the same captions, right-padded (encoder/text_encoder.py:25-43), without the
+        padding rows: dropout included when `self.training`, with masks of its own.  An empty caption comes back as NaN,
+        and so does an id outside the vocabulary; tokens of no caption attend to nothing."""
+        from . import ops
+        from .ops import LinearFn, LayerNormFn
+        self._require_kernels(input_ids)
+        if input_ids.dim() != 1 or offsets.dim() != 1:
+            raise ValueError("TextEncoder.forward_packed: input_ids and offsets are vectors")
+        packs = self._train_packs()
+        layers = self.transformer.layers
+        H = layers[0].self_attn.num_heads
+        D = self.embedding.embedding_dim
+        p = float(layers[0].p) if self.training else 0.0
+        seed = int(torch.randint(0, 2 ** 31 - 1, (1,))) if p > 0 else 0     # CPU generator: no device synchronisation
+        how = dict(heads=H, cap=self.score_cap, slopes=self.distance_slopes, drop_p=p)
+        x = ops.embedding(input_ids, self.embedding.weight)
+        if return_pooled:        # one query for each caption, its first token: position 0 (no row for an empty caption)
+            first = torch.where(offsets[1:] > offsets[:-1], offsets[:-1], -1)
+            singles = torch.arange(offsets.numel(), dtype=torch.int32, device=offsets.device)
+
+        def behind(x, a, layer, pre, s0):        # everything behind a layer's attention, row by row
+            sa = layer.self_attn
+            if p > 0:
+                a = LinearFn.apply(a, packs[pre + "self_attn.out_proj.weight"], sa.out_proj.bias, None, False, sa.out_proj.weight)
+                h = _DropoutAddFn.apply(a, x, p, s0 + 1)
+            else:
+                h = LinearFn.apply(a, packs[pre + "self_attn.out_proj.weight"], sa.out_proj.bias, x, False, sa.out_proj.weight)
+            x = LayerNormFn.apply(h, layer.norm1.weight, layer.norm1.bias, layer.norm1.eps)
+            f = LinearFn.apply(x, packs[pre + "linear1.weight"], layer.linear1.bias, None, False, layer.linear1.weight)
+            f = _GeluDropoutFn.apply(f, p, s0 + 2)
+            if p > 0:
+                f = LinearFn.apply(f, packs[pre + "linear2.weight"], layer.linear2.bias, None, False, layer.linear2.weight)
+                h = _DropoutAddFn.apply(f, x, p, s0 + 3)
+            else:
+                h = LinearFn.apply(f, packs[pre + "linear2.weight"], layer.linear2.bias, x, False, layer.linear2.weight)
+            return LayerNormFn.apply(h, layer.norm2.weight, layer.norm2.bias, layer.norm2.eps)
+
+        for i, layer in enumerate(layers):
+            pre = f"transformer.layers.{i}."
+            sa = layer.self_attn
+            s0 = (seed + 7919 * (4 * i + 1)) & 0x7FFFFFFF
+            qkv = LinearFn.apply(x, packs[pre + "self_attn.in_proj_weight"], sa.in_proj_bias, None, False, sa.in_proj_weight)
+            if return_pooled and i == len(layers) - 1:
+                # the last layer's other rows reach nothing: gather the first tokens' queries and states
+                q, kv = _QueriesAndKeysFn.apply(qkv, D)
+                q, x = ops.embedding(first, q), ops.embedding(first, x)
+                a = ops.doc_attention(q, kv, q_offsets=singles, k_offsets=offsets, align="start", seed=s0, **how)
+            else:
+                a = ops.doc_attention(qkv, q_offsets=offsets, seed=s0, **how)
+            x = behind(x, a, layer, pre, s0)
+        x = LayerNormFn.apply(x, self.norm.weight, self.norm.bias, self.norm.eps)
+        y = LinearFn.apply(x, packs["projection.weight"], self.projection.bias, None, True, self.projection.weight)
+        return _L2NormFn.apply(y) if return_pooled else y
 
     def _require_kernels(self, input_ids):
         d = self.embedding.embedding_dim

@@ -465,7 +465,8 @@ int mi355_embedding_bwd(const void* ids, int ids64, long long n, const void* dy,
  * min(1, max_norm / (norm + 1e-6)) and the bf16 operand copies.  A step whose gradients' sum of squares is not a finite fp32
  * number changes nothing but the skip count.
  * recs: per tensor {parameter (fp32), bf16 copy or 0, elements, first block} (int64, device memory), a block being 256
- * elements and a tensor's blocks following each other in the moment arrays (the last one padded).
+ * elements and a tensor's blocks following each other in the moment arrays (the last one padded).  Parameter 0: the gradient
+ * counts in the norm and nothing else happens.
  * grads: per tensor the gradient's address, fp32, or bf16 with the lowest bit set; 0 leaves the tensor alone.
  * map: per workgroup {tensor, first block within it} (int32), eight blocks each, n_wg of them covering every tensor.
  * bits 32: m, v fp32 arrays.  bits 8: m int8 codes, v uint8 codes of its root, fp32 scales per block (csrc/multi_adamw.hip
