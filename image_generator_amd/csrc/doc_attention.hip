@@ -53,7 +53,7 @@ int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* o
     if (bad_ld(ldq) || bad_ld(ldk) || bad_ld(ldv) || bad_ld(ldo) || ldo < (long long)Hq * D)
         return mi355_fail(MI355_ERR_ARG, "doc_attention: row strides must be multiples of 8, at most 2^23");
     const size_t need = mi355_doc_attention_fwd_workspace_bytes(Tq, Tk, Hq, Hkv, D);
-    if (!ws || ws_bytes < need || off16(ws)) return mi355_fail(MI355_ERR_ARG, "doc_attention: workspace of %zu bytes, %zu needed, 16-byte aligned", ws ? ws_bytes : 0, need);
+    if (need && (!ws || ws_bytes < need || off16(ws))) return mi355_fail(MI355_ERR_ARG, "doc_attention: workspace of %zu bytes, %zu needed, 16-byte aligned", ws ? ws_bytes : 0, need);
     a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.out = (bf16_t*)out; a.lse = lse;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
     const hipStream_t st = (hipStream_t)stream;

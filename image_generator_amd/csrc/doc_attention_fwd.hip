@@ -376,5 +376,5 @@ int doc_fwd_tiles(const DocArgs& a, hipStream_t st) {
 }
 size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D) {
     const size_t s = fwd_splits(Tq, Tk, Hq, Hkv), rows = ((size_t)Tq * (Hq / Hkv) + 31) / 32 * 32 * Hkv;
-    return rows * s * (D + 2) * 4 + 16;
+    return rows * s * (D + 2) * 4;
 }

@@ -612,45 +612,59 @@ def attention_bwd(q, k, v, o, do, lse, heads, dq, dk, dv):
 
 
 def _here(*tensors):
-    """Operands of one launch: all on the current device (a launch goes to its stream)."""
-    dev = torch.cuda.current_device() if tensors[0].is_cuda else None
+    """Operands of one launch: all on the current device (a launch goes to its stream).  Returns that device's index."""
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("HIP device tensors required (no CPU path)")
-        if t.device.index != dev:
-            raise RuntimeError(f"a tensor on {t.device}, the current device is {dev}")
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError(f"tensors on {tensors[0].device} and {t.device}; HIP device tensors required (no CPU path)")
+    if dev < 0:
+        raise RuntimeError("HIP device tensors required (no CPU path)")
+    if torch._C._cuda_getDevice() != dev:
+        raise RuntimeError(f"tensors on {tensors[0].device}, the current device is {torch._C._cuda_getDevice()}")
+    return dev
+
+
+def _doc_offsets(name, t, n, dtype):
+    if t is not None and (t.numel() != n or t.dtype != dtype or not t.is_contiguous()):
+        raise ValueError(f"doc_attention: {name} must be {n} contiguous {dtype} values, got {t.numel()} {t.dtype}")
+
+
+def _doc_matrix(name, t, heads, width):
+    if t.dtype != BF16 or t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1:
+        raise RuntimeError(f"doc_attention: {name} must be a bf16 matrix [tokens, heads * width] with adjacent columns")
+    if t.shape[1] != heads * width:
+        raise ValueError(f"doc_attention: {name} {tuple(t.shape)} for {heads} heads of width {width}")
 
 
 def _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed):
-    """Checks shared by the two directions of the document attention; (leading arguments, trailing arguments, sizes)."""
-    kv_heads = heads if kv_heads is None else kv_heads
-    k_offsets = q_offsets if k_offsets is None else k_offsets
-    _here(q, k, v, q_offsets, k_offsets, prefix, slopes)
+    """Checks shared by the two directions of the document attention; (leading arguments, trailing arguments, sizes, device)."""
+    if kv_heads is None:
+        kv_heads = heads
+    if k_offsets is None:
+        k_offsets = q_offsets
+    dev = _here(q, k, v, q_offsets, k_offsets, prefix, slopes)
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"doc_attention: {heads} query heads on {kv_heads} key heads")
-    for name, t, h in (("q", q, heads), ("k", k, kv_heads), ("v", v, kv_heads)):
-        if t.dim() != 2 or t.dtype != BF16 or t.stride(1) != 1 and t.shape[1] > 1:
-            raise RuntimeError(f"doc_attention: {name} must be a bf16 matrix [tokens, heads * width] with adjacent columns")
-        if t.shape[1] % h or t.shape[1] // h != q.shape[1] // heads:
-            raise ValueError(f"doc_attention: {name} {tuple(t.shape)} for {h} heads of width {q.shape[1] // heads}")
+    width = q.shape[-1] // heads
+    _doc_matrix("q", q, heads, width)
+    _doc_matrix("k", k, kv_heads, width)
+    _doc_matrix("v", v, kv_heads, width)
     if k.shape[0] != v.shape[0]:
         raise ValueError(f"doc_attention: {k.shape[0]} keys, {v.shape[0]} values")
     docs = q_offsets.numel() - 1
-    for name, t, n, dt in (("q_offsets", q_offsets, docs + 1, torch.int32), ("k_offsets", k_offsets, docs + 1, torch.int32),
-                           ("prefix", prefix, docs, torch.int32), ("slopes", slopes, heads, F32)):
-        if t is not None and (t.dtype != dt or t.numel() != n or not t.is_contiguous()):
-            raise ValueError(f"doc_attention: {name} must be {n} contiguous {dt} values, got {t.numel()} {t.dtype}")
     if docs < 1:
         raise ValueError("doc_attention: offsets hold at least two entries")
+    _doc_offsets("q_offsets", q_offsets, docs + 1, torch.int32)
+    if k_offsets is not q_offsets:
+        _doc_offsets("k_offsets", k_offsets, docs + 1, torch.int32)
+    _doc_offsets("prefix", prefix, docs, torch.int32)
+    _doc_offsets("slopes", slopes, heads, F32)
     if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("doc_attention: no gradient reaches the slopes (detach them)")
     if align not in ("end", "start"):
         raise ValueError(f"doc_attention: align {align!r} is neither 'end' nor 'start'")
-    D = q.shape[1] // heads
     head = (q_offsets.data_ptr(), k_offsets.data_ptr(), docs, _ptr(prefix), _ptr(slopes), cap or 0.0, causal, align == "start")
-    return head, (1.0 / math.sqrt(D) if scale is None else scale, drop_p, seed), (q.shape[0], k.shape[0], heads, kv_heads, D)
+    return head, (width ** -0.5 if scale is None else scale, drop_p, seed), (q.shape[0], k.shape[0], heads, kv_heads, width), dev
 
 
 def doc_attention_fwd(q, k, v, heads, q_offsets, k_offsets=None, kv_heads=None, causal=False, prefix=None, slopes=None, cap=0.0,
@@ -661,13 +675,14 @@ def doc_attention_fwd(q, k, v, heads, q_offsets, k_offsets=None, kv_heads=None, 
     their starts, and sees its document's keys; with `causal` those up to c and the document's first `prefix[n]`.  `cap`:
     scores become cap tanh(s / cap); `slopes` [heads]: minus slope times |c - j|.  Returns (out [Tq, heads * d],
     lse [heads, Tq]); a query that sees nothing gets zeros and -inf."""
-    head, tail, sizes = _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed)
+    head, tail, sizes, dev = _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed)
     out = torch.empty(q.shape, dtype=BF16, device=q.device)
     lse = torch.empty((heads, q.shape[0]), dtype=F32, device=q.device)
-    ws = torch.empty(int(lib.mi355_doc_attention_fwd_workspace_bytes(*sizes)), dtype=torch.uint8, device=q.device)
+    need = lib.mi355_doc_attention_fwd_workspace_bytes(*sizes)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     check(lib.mi355_doc_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *head, *sizes,
-                                      q.stride(0), k.stride(0), v.stride(0), out.stride(0), *tail, ws.data_ptr(), ws.numel(), _stream()),
-          "doc_attention_fwd")
+                                      q.stride(0), k.stride(0), v.stride(0), out.stride(0), *tail, _ptr(ws), need,
+                                      torch._C._cuda_getCurrentRawStream(dev)), "doc_attention_fwd")
     return out, lse
 
 
@@ -675,8 +690,8 @@ def doc_attention_bwd(do, q, k, v, o, lse, heads, q_offsets, k_offsets=None, kv_
                       cap=0.0, scale=None, align="end", drop_p=0.0, seed=0, dq=None, dk=None, dv=None):
     """(dq, dk, dv) of `doc_attention_fwd` for the gradient `do` of its output; `o`, `lse` are what it returned.  dq / dk / dv:
     bf16 matrices to write (slices of one buffer, say); new ones by default."""
-    head, tail, sizes = _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed)
-    _here(do, o, lse, dq, dk, dv)
+    head, tail, sizes, _ = _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed)
+    _here(q, do, o, lse, dq, dk, dv)
     dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=q.device) if d is None else d for t, d in ((q, dq), (k, dk), (v, dv)))
     for name, t, like in (("do", do, q), ("o", o, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
         if t.shape != like.shape or t.dtype != BF16 or t.stride(1) != 1 and t.shape[1] > 1:

@@ -57,7 +57,7 @@ def test_doc_attention_refusals():
     for kw, why in ((dict(docs=0), "document"), (dict(Tq=-1), "document"), (dict(Hq=3), "multiple"), (dict(D=36), "multiple of 8"),
                     (dict(D=136), "128"), (dict(prefix=16), "prefix"), (dict(cap=-1.0), "cap"), (dict(cap=2000.0), "cap"), (dict(ld=(1 << 23) + 8), "strides"), (dict(cap=float("nan")), "cap"),
                     (dict(drop=1.0), "dropout"), (dict(ld=60), "strides"), (dict(ldo=32), "strides"), (dict(ptr=8), "aligned"),
-                    (dict(ptr=None), "null"), (dict(off=None), "null"), (dict(ws=None), "workspace"), (dict(ws_bytes=0), "workspace"),
+                    (dict(ptr=None), "null"), (dict(off=None), "null"), (dict(ws=None, Tk=5000), "workspace"), (dict(ws_bytes=0, Tk=5000), "workspace"),
                     (dict(Tq=1 << 30), "2^31"), (dict(ld=-64), "strides")):
         assert fwd(**kw) == -1 and why in err(), (kw, err())
     assert fwd(Tq=0) == 0
