@@ -62,9 +62,9 @@ int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* o
     return doc_fwd_tiles(a, st);
 }
 
-size_t mi355_doc_attention_bwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D, int docs) {
+size_t mi355_doc_attention_bwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D, int docs, int causal) {
     if (bad_sizes(docs, Tq, Tk, Hq, Hkv, D)) return 0;
-    const int splits = doc_bwd_kv_splits(Tq, Tk, Hq, Hkv, docs);
+    const int splits = doc_bwd_kv_splits(Tq, Tk, Hq, Hkv, docs, causal != 0);
     return bwd_rows_bytes(Tq, Hq) + (splits > 1 ? (size_t)splits * Tk * Hkv * 2 * D * 4 : 0) + 16;
 }
 
@@ -84,7 +84,7 @@ int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const v
         return mi355_fail(MI355_ERR_ARG, "doc_attention_bwd: row strides must be multiples of 8, at most 2^23");
     if (lddq < (long long)Hq * D || lddk < (long long)Hkv * D || lddv < (long long)Hkv * D)
         return mi355_fail(MI355_ERR_ARG, "doc_attention_bwd: rows of a gradient overlap");
-    const size_t need = mi355_doc_attention_bwd_workspace_bytes(Tq, Tk, Hq, Hkv, D, docs);
+    const size_t need = mi355_doc_attention_bwd_workspace_bytes(Tq, Tk, Hq, Hkv, D, docs, causal);
     if (!ws || ws_bytes < need || off16(ws)) return mi355_fail(MI355_ERR_ARG, "doc_attention_bwd: workspace of %zu bytes, %zu needed, 16-byte aligned", ws ? ws_bytes : 0, need);
     a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.o = (const bf16_t*)o; a.dout = (const bf16_t*)dout;
     a.dq = (bf16_t*)dq; a.dk = (bf16_t*)dk; a.dv = (bf16_t*)dv; a.lse = (float*)lse;
@@ -92,7 +92,7 @@ int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const v
     a.rows = (int4*)ws;
     a.delta = (float*)((char*)ws + (size_t)Tq * 16);
     a.part = (float*)((char*)ws + bwd_rows_bytes(Tq, Hq));
-    a.splits = doc_bwd_kv_splits(Tq, Tk, Hq, Hkv, docs);
+    a.splits = doc_bwd_kv_splits(Tq, Tk, Hq, Hkv, docs, a.causal);
     const hipStream_t st = (hipStream_t)stream;
     ProfScope prof(FAM_ATTN, st, 10.0 * Tq * (double)Tk / docs * Hq * D);
     if (Tq > 0) if (const int rc = doc_bwd_q_tiles(a, st)) return rc;

@@ -232,7 +232,7 @@ inline unsigned unit_grid(long long units, int heads) { return (unsigned)(units 
 int doc_fwd_tiles(const DocArgs& a, hipStream_t st);
 int doc_bwd_q_tiles(const DocArgs& a, hipStream_t st);
 int doc_bwd_kv_tiles(const DocArgs& a, hipStream_t st);
-int doc_bwd_kv_splits(int Tq, int Tk, int Hq, int Hkv, int docs);
+int doc_bwd_kv_splits(int Tq, int Tk, int Hq, int Hkv, int docs, int causal);
 size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D);
 
 // FN<ND, NO>(args...) for the head width: ND 16-wide steps of a contraction over it, NO 32-wide blocks of it

@@ -698,7 +698,7 @@ def doc_attention_bwd(do, q, k, v, o, lse, heads, q_offsets, k_offsets=None, kv_
             raise RuntimeError(f"doc_attention_bwd: {name} must be a bf16 matrix {tuple(like.shape)} with adjacent columns")
     if lse.shape != (heads, q.shape[0]) or lse.dtype != F32 or not lse.is_contiguous():
         raise RuntimeError("doc_attention_bwd: lse is not the forward pass's")
-    ws = torch.empty(int(lib.mi355_doc_attention_bwd_workspace_bytes(*sizes, q_offsets.numel() - 1)), dtype=torch.uint8, device=q.device)
+    ws = torch.empty(int(lib.mi355_doc_attention_bwd_workspace_bytes(*sizes, q_offsets.numel() - 1, causal)), dtype=torch.uint8, device=q.device)
     check(lib.mi355_doc_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), dq.data_ptr(),
                                       dk.data_ptr(), dv.data_ptr(), *head, *sizes, q.stride(0), k.stride(0), v.stride(0), o.stride(0),
                                       do.stride(0), dq.stride(0), dk.stride(0), dv.stride(0), *tail, ws.data_ptr(), ws.numel(), _stream()),

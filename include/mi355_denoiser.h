@@ -439,7 +439,7 @@ int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* o
                             int Tk, int Hq, int Hkv, int D, long long ldq, long long ldk, long long ldv, long long ldo,
                             float scale, float drop_p, unsigned seed, void* ws, size_t ws_bytes, void* stream);
 /* o, lse: the forward pass's; dout like o with its own row stride lddo.  dq, dk, dv are written whole. */
-size_t mi355_doc_attention_bwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D, int docs);
+size_t mi355_doc_attention_bwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D, int docs, int causal);
 int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq,
                             void* dk, void* dv, const int* q_off, const int* k_off, int docs, const int* prefix,
                             const float* slopes, float cap, int causal, int align_start, int Tq, int Tk, int Hq, int Hkv, int D,
