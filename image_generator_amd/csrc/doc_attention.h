@@ -45,59 +45,76 @@ __device__ __forceinline__ int doc_of(const int* __restrict__ off, int docs, int
     return a;
 }
 
-// The same for the 64 tokens i of a wave (every lane active), all in a stretch that begins at i0: the document of i0 by a search
-// that probes 64 places a step (two loads for 4096 documents), then the next 64 boundaries in one load and a search among
-// registers.  A lane's own binary search is a chain of loads: it was a third of a caption tile's time.
-__device__ __forceinline__ int doc_of_wave(const int* __restrict__ off, int docs, int i0, int i) {
-    const int lane = threadIdx.x & 63;
-    int a = 0, b = docs;
-    while (b - a > 1) {
-        const int step = (b - a + 63) / 64, at = a + 1 + lane * step;
-        const int count = __popcll(__ballot(at < b && off[min(at, docs)] <= i0));
-        if (count == 0) break;
-        a += 1 + (count - 1) * step;
-        b = min(b, a + step);
-    }
-    const int bound = a + 1 + lane < docs ? off[a + 1 + lane] : 0x7fffffff;
-    int n = 0;
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) if (__shfl(bound, n + s - 1, 64) <= i) n += s;
-    if (n == 63 && __shfl(bound, 63, 64) <= i) {               // past the 64 boundaries: many tiny documents
-        int lo = min(a + 64, docs - 1), hi = docs;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (off[mid] <= i) lo = mid; else hi = mid;
-        }
-        return lo;
-    }
-    return a + n;
+// A document's queries [qb, qe) and its number; qb > qe: none
+struct Doc { int n, b, e; };
+
+// The document of token i by itself.
+__device__ __forceinline__ Doc doc_at(const int* __restrict__ off, int docs, int i) {
+    const int n = doc_of(off, docs, i);
+    return {n, off[n], off[n + 1]};
 }
 
-__device__ __forceinline__ RowSpan row_span_in(const DocArgs& p, int i, int n) {
-    const int qb = p.q_off[n], qe = p.q_off[n + 1];
-    int kb = max(p.k_off[n], 0), ke = min(p.k_off[n + 1], p.Tk);
+// The same for the tokens i of a wave (every lane active, ascending from i0 to i1), out of `total`.  A lane's own binary search is a
+// chain of loads, a third of a caption tile's time; here the 64 offsets around the place where documents of equal length would
+// have this one are loaded at once and usually hold it - if not, a search that probes 64 places a step says where they are -
+// and the lanes take their documents from those registers.
+__device__ __forceinline__ Doc doc_of_wave(const int* __restrict__ off, int docs, int total, int i0, int i1, int i) {
+    const int lane = threadIdx.x & 63;
+    int w = max(0, (int)((float)i0 * (float)docs / (float)total) - 24);       // first offset of the window
+    int val = w + lane <= docs ? off[w + lane] : 0x7fffffff;
+    int k = __popcll(__ballot(val <= i0));                                      // offsets of the window up to i0
+    if ((k == 0 && w > 0) || k == 64) {
+        int a = 0, b = docs;
+        while (b - a > 1) {
+            const int step = (b - a + 63) / 64, at = a + 1 + lane * step;
+            const int count = __popcll(__ballot(at < b && off[min(at, docs)] <= i0));
+            if (count == 0) break;
+            a += 1 + (count - 1) * step;
+            b = min(b, a + step);
+        }
+        w = a;
+        val = w + lane <= docs ? off[w + lane] : 0x7fffffff;
+        k = __popcll(__ballot(val <= i0));
+    }
+    Doc d = {w + max(k - 1, 0), __builtin_amdgcn_readlane(val, max(k - 1, 0)), __builtin_amdgcn_readlane(val, max(min(k, 63), 1))};
+    for (; k < 64; ++k) {                                                       // documents that begin behind i0
+        const int b = __builtin_amdgcn_readlane(val, k);
+        if (b > i1) break;
+        const int e = __builtin_amdgcn_readlane(val, min(k + 1, 63));
+        if (b <= i) d = {w + k, b, e};
+    }
+    if (d.n - w >= 63 && d.n < docs) return doc_at(off, docs, i);               // past the window: many tiny documents
+    if (d.n >= docs) d = {docs - 1, 1, 0};
+    return d;
+}
+
+__device__ __forceinline__ RowSpan row_span_in(const DocArgs& p, int i, const Doc& q) {
+    int kb = q.b, ke = q.e;
+    if (p.k_off != p.q_off) { kb = p.k_off[q.n]; ke = p.k_off[q.n + 1]; }
+    kb = max(kb, 0);
+    ke = min(ke, p.Tk);
     RowSpan s = {0, 0, 0};
-    if (i < qb || i >= qe || kb >= ke) return s;
-    s.c = (int)((long long)i + (p.align_start ? (long long)kb - qb : (long long)ke - qe));
+    if (i < q.b || i >= q.e || kb >= ke) return s;
+    s.c = (int)((long long)i + (p.align_start ? (long long)kb - q.b : (long long)ke - q.e));
     s.lo = kb;
     s.hi = ke;
     if (p.causal) {
         int seen = s.c < kb ? kb : s.c >= ke ? ke : s.c + 1;
-        if (p.prefix) seen = max(seen, kb + min(max(p.prefix[n], 0), ke - kb));
+        if (p.prefix) seen = max(seen, kb + min(max(p.prefix[q.n], 0), ke - kb));
         s.hi = seen;
     }
     return s;
 }
+__device__ __forceinline__ RowSpan row_span(const DocArgs& p, int i) { return row_span_in(p, i, doc_at(p.q_off, p.docs, i)); }
 
-__device__ __forceinline__ RowSpan row_span(const DocArgs& p, int i) { return row_span_in(p, i, doc_of(p.q_off, p.docs, i)); }
-
-// tokens whose rows may see key j of document n: [first, last)
-__device__ __forceinline__ int2 key_span_in(const DocArgs& p, int j, int n) {
-    const int kb = max(p.k_off[n], 0), ke = min(p.k_off[n + 1], p.Tk);
-    const int qb = p.q_off[n], qe = p.q_off[n + 1];
+// tokens whose rows may see key j of document k: [first, last)
+__device__ __forceinline__ int2 key_span_in(const DocArgs& p, int j, const Doc& k) {
+    const int kb = max(k.b, 0), ke = min(k.e, p.Tk);
+    int qb = k.b, qe = k.e;
+    if (p.k_off != p.q_off) { qb = p.q_off[k.n]; qe = p.q_off[k.n + 1]; }
     if (j < kb || j >= ke || qb >= qe) return make_int2(0, 0);
     long long first = qb;
-    if (p.causal && !(p.prefix && j < kb + min(max(p.prefix[n], 0), ke - kb))) {
+    if (p.causal && !(p.prefix && j < kb + min(max(p.prefix[k.n], 0), ke - kb))) {
         const long long at = (long long)j - (p.align_start ? (long long)kb - qb : (long long)ke - qe);   // c >= j
         if (at > first) first = at;
     }
@@ -105,7 +122,7 @@ __device__ __forceinline__ int2 key_span_in(const DocArgs& p, int j, int n) {
     const int f = (int)(first < 0 ? 0 : first > last ? last : first);
     return make_int2(f, last);
 }
-__device__ __forceinline__ int2 key_span(const DocArgs& p, int j) { return key_span_in(p, j, doc_of(p.k_off, p.docs, j)); }
+__device__ __forceinline__ int2 key_span(const DocArgs& p, int j) { return key_span_in(p, j, doc_at(p.k_off, p.docs, j)); }
 
 __device__ __forceinline__ float tanh_f(float x) {
     return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * LOG2E)));

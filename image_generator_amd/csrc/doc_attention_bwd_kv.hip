@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
         const int key = min(key0 + kb * 32 + l31, p.Tk - 1);
-        const int2 span = key_span_in(p, key, doc_of_wave(p.k_off, p.docs, __builtin_amdgcn_readfirstlane(key), key));
+        const int2 span = key_span_in(p, key, doc_of_wave(p.k_off, p.docs, p.Tk, __builtin_amdgcn_readfirstlane(key), __builtin_amdgcn_readlane(key, 31), key));
         seen[kb] = key0 + kb * 32 + l31 < p.Tk && span.y > span.x;
         if (seen[kb]) { lo = min(lo, span.x); hi = max(hi, span.y); }
 #pragma unroll
@@ -85,8 +85,8 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
             vf[kb][ks] = seen[kb] ? vf[kb][ks] : zero8;
         }
     }
-    lo = __builtin_amdgcn_readfirstlane(wave_min_i(lo));
-    hi = __builtin_amdgcn_readfirstlane(wave_max_i(hi));
+    lo = wave_min_i(lo);
+    hi = wave_max_i(hi);
     if (lane == 0) { range[wave][0] = lo; range[wave][1] = hi; }
     f32x16 dkT[KB][NO], dvT[KB][NO];
 #pragma unroll

@@ -37,15 +37,15 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
             for (int e = 0; e < 8; ++e) delta = fmaf((float)ov[ks][e], (float)gf[ks][e], delta);
         delta += __shfl_xor(delta, 32, 64);
     }
-    RowSpan span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, __builtin_amdgcn_readfirstlane(token), token));
+    RowSpan span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, p.Tq, __builtin_amdgcn_readfirstlane(token), __builtin_amdgcn_readlane(token, 31), token));
     if (live && hh == 0 && head == 0) p.rows[token] = make_int4(span.lo, span.hi, span.c, 0);
     if (!live) span.lo = span.hi = 0;
     const bool sees = span.hi > span.lo;
-    const int lo = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.lo : 0x7fffffff));
-    const int hi = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.hi : 0));
-    const int in_lo = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.lo : 0));
-    const int in_hi = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.hi : 0x7fffffff));
-    const int c_min = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.c : 0x7fffffff));
+    const int lo = wave_min_i(sees ? span.lo : 0x7fffffff);
+    const int hi = wave_max_i(sees ? span.hi : 0);
+    const int in_lo = wave_max_i(sees ? span.lo : 0);
+    const int in_hi = wave_min_i(sees ? span.hi : 0x7fffffff);
+    const int c_min = wave_min_i(sees ? span.c : 0x7fffffff);
     if (!sees) delta = 0.f;
 #pragma unroll
     for (int ks = 0; ks < ND; ++ks) {

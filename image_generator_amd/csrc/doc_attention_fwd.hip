@@ -37,16 +37,16 @@ struct Rows {                        // a wave's 32 rows
             const int d = ks * 16 + 8 * hh;
             qf[ks] = d < p.D ? *(const bf16x8*)(q + d) : zero8;
         }
-        span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, __builtin_amdgcn_readfirstlane(token), token));
+        span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, p.Tq, __builtin_amdgcn_readfirstlane(token), __builtin_amdgcn_readlane(token, 31), token));
         if (!live) span.lo = span.hi = 0;
         const bool sees = span.hi > span.lo;
-        lo = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.lo : 0x7fffffff));
-        hi = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.hi : 0));
+        lo = wave_min_i(sees ? span.lo : 0x7fffffff);
+        hi = wave_max_i(sees ? span.hi : 0);
         // a row without keys asks for no mask: its result is replaced by zeros at the end
-        in_lo = __builtin_amdgcn_readfirstlane(wave_max_i(sees ? span.lo : 0));
-        in_hi = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.hi : 0x7fffffff));
+        in_lo = wave_max_i(sees ? span.lo : 0);
+        in_hi = wave_min_i(sees ? span.hi : 0x7fffffff);
         if (lo > hi) lo = hi = 0;
-        c_min = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? span.c : 0x7fffffff));
+        c_min = wave_min_i(sees ? span.c : 0x7fffffff);
 #pragma unroll
         for (int ks = 0; ks < ND; ++ks) qf[ks] = sees ? qf[ks] : zero8;
         slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;

@@ -106,15 +106,19 @@ __device__ __forceinline__ void tiles_landed() {
     __syncthreads();
 }
 
+// Reductions over a wave by DPP: within rows of 16 lanes, then across them; lane 63 holds the result.  (By way of the LDS, as
+// __shfl_xor goes, the five of a tile were a chain of 3000 cycles.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, ROWS, 0xf, false); }
 __device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-    return v;
+    v = min(v, dpp<0x111, 0xf>(v)); v = min(v, dpp<0x112, 0xf>(v)); v = min(v, dpp<0x114, 0xf>(v)); v = min(v, dpp<0x118, 0xf>(v));
+    v = min(v, dpp<0x142, 0xa>(v)); v = min(v, dpp<0x143, 0xc>(v));
+    return __builtin_amdgcn_readlane(v, 63);
 }
 __device__ __forceinline__ int wave_max_i(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-    return v;
+    v = max(v, dpp<0x111, 0xf>(v)); v = max(v, dpp<0x112, 0xf>(v)); v = max(v, dpp<0x114, 0xf>(v)); v = max(v, dpp<0x118, 0xf>(v));
+    v = max(v, dpp<0x142, 0xa>(v)); v = max(v, dpp<0x143, 0xc>(v));
+    return __builtin_amdgcn_readlane(v, 63);
 }
 
 // q.k -> score in log2 units (cap and bias decided at run time, uniformly).
