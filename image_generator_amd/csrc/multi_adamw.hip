@@ -230,7 +230,8 @@ __global__ __launch_bounds__(256) void multi_adamw32_kernel(const Rec* __restric
     const float wd = (float)hyper[H_WD], bc1 = (float)hyper[H_BC1], bc2 = (float)hyper[H_BC2];
     float scale = 1.f;
     if (hyper[H_MAX] > 0.0) { const double c = hyper[H_MAX] / (norm + 1e-6); if (c < 1.0) scale = (float)c; }
-    const float decay = fmaf(-lr, wd, 1.f), rbc2 = 1.f / sqrtf(bc2), step = lr / bc1, omb1 = 1.f - b1, omb2 = 1.f - b2;
+    const float decay = fmaf(-lr, wd, 1.f), rbc2 = 1.f / sqrtf(bc2), step = lr / bc1;
+    const float omb1 = (float)hyper[H_OMB1], omb2 = (float)hyper[H_OMB2];
 #pragma unroll
     for (int u = 0; u < WG_BLOCKS / 4; ++u) {
         const size_t i = (size_t)(at.y + u * 4 + wave) * BLK + lane * 4;

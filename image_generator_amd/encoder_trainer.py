@@ -42,7 +42,8 @@ class ContrastiveTrainer:
         self.temp = [p for p in criterion.parameters() if p.requires_grad]
         self.temp_m = [torch.zeros_like(p) for p in self.temp]
         self.temp_v = [torch.zeros_like(p) for p in self.temp]
-        self.opt = TensorAdamW(self.params, lr, betas, eps, weight_decay, state_bits=state_bits, watched=[p.numel() for p in self.temp])
+        self.opt = TensorAdamW(self.params, lr, betas, eps, weight_decay, state_bits=state_bits, watched=[p.numel() for p in self.temp],
+                               fp32_betas=state_bits == 32)
         self.state = self.opt.state            # [0] = norm of the step's gradients (no clipping: only its finiteness is used)
         if state_bits == 32:
             self.m, self.v = self.opt.split(self.opt.m), self.opt.split(self.opt.v)

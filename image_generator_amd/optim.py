@@ -28,11 +28,14 @@ class TensorAdamW:
     watched: sizes of further gradients, stepped by someone else, that count in the norm (and in the test for finite values); they
     follow as `bind(..., watched=[...])`.
 
+    fp32_betas: a new gradient's weights are 1 - beta of betas rounded to fp32, as `trainer.FusedAdamW` forms them (1 - 0.999 is
+    7e-6 off then), instead of 1 - beta rounded itself; an option of 32-bit states.
+
     `step(grads)` uploads what changes (addresses, bias corrections) and launches.  For a captured graph: `bind(grads)` before
     the capture and before every replay, `apply()` inside it; the gradients stay the caller's to keep."""
 
     def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=0.0, state_bits=32, copies=None,
-                 watched=()):
+                 watched=(), fp32_betas=False):
         self.params = list(params)
         if not self.params:
             raise ValueError("TensorAdamW: no parameters")
@@ -50,6 +53,7 @@ class TensorAdamW:
         self._shapes = [p.shape for p in self.params]
         self.lr, self.betas, self.eps, self.wd, self.max_norm = lr, tuple(betas), eps, weight_decay, max_grad_norm
         self.bits, self.device, self.t = state_bits, dev, 0
+        self._new = tuple(float(1 - torch.tensor(b, dtype=F32).double()) if fp32_betas else 1 - b for b in self.betas)
         self.watched = list(watched)
         blocks = [-(-p.numel() // BLOCK) for p in self.params]
         self.starts = [0]
@@ -113,7 +117,7 @@ class TensorAdamW:
         b1, b2 = self.betas
         c1, c2 = 1 - b1 ** self.t, 1 - b2 ** self.t
         hyper = (self.lr, b1, b2, self.eps, self.wd, c1, c2, self.max_norm or 0.0, 1 - self.lr * self.wd, self.lr / c1, 1 / math.sqrt(c2),
-                 1 - b1, 1 - b2)
+                 *self._new)
         h = self._ring.acquire().numpy()
         h[:_HYPER].view("float64")[:len(hyper)] = hyper
         h[_HYPER:] = words
