@@ -1,5 +1,5 @@
-// Document attention, dK and dV, on the matrix units: a lane owns its key (S = Q K^T, dP = dO V^T), a wave KB blocks of 32 keys,
-// and staged tiles of 64 rows - tokens times the query heads that share the key head - pass by: dV^T += dO^T P,
+// Document attention, dK and dV, on the matrix units: a lane owns its key (S = Q K^T, dP = dO V^T), a wave 32 keys, and
+// staged tiles of 64 rows - tokens times the query heads that share the key head - pass by: dV^T += dO^T P,
 // dK^T += Q^T dS.  -lse and -delta of a row start the accumulators of its scores, so subtracting them costs nothing.
 //
 // Few keys under many rows (captions under image tokens) leave most of the chip idle: the rows of a key tile are then cut
@@ -49,7 +49,7 @@ struct RowInfo {                     // of the 64 staged rows
     unsigned drop[64];
 };
 
-template <int ND, int NO, int KIND, int KB>
+template <int ND, int NO, int KIND>
 __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1) void doc_dkdv_kernel(const DocArgs p, int tiles) {
     __shared__ __attribute__((aligned(16))) char smem[4 * TILE_BYTES<NO>];      // Q and dO, twice
     __shared__ __attribute__((aligned(16))) RowInfo infos[2];
@@ -58,43 +58,32 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
     int unit, hk;
     if (!unit_of(tiles * p.splits, p.Hkv, unit, hk)) return;
     const int split = unit / tiles, tile = unit - split * tiles;
-    const int base = tile * 128 * KB, key0 = base + wave * 32 * KB;
+    const int base = tile * 128, key0 = base + wave * 32, key = key0 + l31;
     const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
-    bf16x8 kf[KB][ND], vf[KB][ND];
-    bool seen[KB];
-    int lo = 0x7fffffff, hi = 0;
+    bf16x8 kf[ND], vf[ND];
+    const int mine = min(key, p.Tk - 1);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {                 // on their way while the keys' rows are looked up
-        const int key = min(key0 + kb * 32 + l31, p.Tk - 1);
-#pragma unroll
-        for (int ks = 0; ks < ND; ++ks) {
-            const int d = ks * 16 + 8 * hh;
-            kf[kb][ks] = d < p.D ? *(const bf16x8*)(k_row(p, key, hk) + d) : zero8;
-            vf[kb][ks] = d < p.D ? *(const bf16x8*)(v_row(p, key, hk) + d) : zero8;
-        }
+    for (int ks = 0; ks < ND; ++ks) {                 // on their way while the keys' rows are looked up
+        const int d = ks * 16 + 8 * hh;
+        kf[ks] = d < p.D ? *(const bf16x8*)(k_row(p, mine, hk) + d) : zero8;
+        vf[ks] = d < p.D ? *(const bf16x8*)(v_row(p, mine, hk) + d) : zero8;
     }
+    const int2 span = key_span_in(p, mine, doc_of_wave(p.k_off, p.docs, p.Tk, __builtin_amdgcn_readfirstlane(mine), __builtin_amdgcn_readlane(mine, 31), mine));
+    const bool seen = key < p.Tk && span.y > span.x;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-        const int key = min(key0 + kb * 32 + l31, p.Tk - 1);
-        const int2 span = key_span_in(p, key, doc_of_wave(p.k_off, p.docs, p.Tk, __builtin_amdgcn_readfirstlane(key), __builtin_amdgcn_readlane(key, 31), key));
-        seen[kb] = key0 + kb * 32 + l31 < p.Tk && span.y > span.x;
-        if (seen[kb]) { lo = min(lo, span.x); hi = max(hi, span.y); }
-#pragma unroll
-        for (int ks = 0; ks < ND; ++ks) {
-            kf[kb][ks] = seen[kb] ? kf[kb][ks] : zero8;
-            vf[kb][ks] = seen[kb] ? vf[kb][ks] : zero8;
-        }
+    for (int ks = 0; ks < ND; ++ks) {
+        kf[ks] = seen ? kf[ks] : zero8;
+        vf[ks] = seen ? vf[ks] : zero8;
     }
+    int lo = seen ? span.x : 0x7fffffff, hi = seen ? span.y : 0;
     lo = wave_min_i(lo);
     hi = wave_max_i(hi);
     if (lane == 0) { range[wave][0] = lo; range[wave][1] = hi; }
-    f32x16 dkT[KB][NO], dvT[KB][NO];
+    f32x16 dkT[NO], dvT[NO];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int i = 0; i < NO; ++i)
 #pragma unroll
-        for (int i = 0; i < NO; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) { dkT[kb][i][r] = 0.f; dvT[kb][i][r] = 0.f; }
+        for (int r = 0; r < 16; ++r) { dkT[i][r] = 0.f; dvT[i][r] = 0.f; }
     const Reads<ND, NO> rd;
     const Bend bend(p);
     __syncthreads();
@@ -109,7 +98,7 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
         rlo = from;
     }
     const unsigned wlo = lo < hi ? lo * G : 0xffffffffu, whi = lo < hi ? hi * G : 0u;
-    const int kmax = min(key0 + 32 * KB, p.Tk);       // the wave's keys: seen whole by a row with lo <= key0 and hi >= kmax
+    const int kmax = min(key0 + 32, p.Tk);       // the wave's keys: seen whole by a row with lo <= key0 and hi >= kmax
     const float rsl2 = KIND == PLAIN ? 1.f / bend.scale2 : 0.f;
 
     RowFetch<NO> f;
@@ -163,7 +152,7 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
         const bool masked = __ballot(first > key0 || first + count < kmax) != 0;
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs) {
-            f32x16 s[KB], dp[KB];
+            f32x16 s, dp;
             f32x4 ls[4], dl[4];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -171,32 +160,25 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
                 dl[g] = *(const f32x4*)&info.delta[qs * 32 + 8 * g + 4 * hh];
             }
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[kb][r] = KIND == PLAIN ? ls[r >> 2][r & 3] : 0.f;
-                    dp[kb][r] = KIND == DROPPED ? 0.f : dl[r >> 2][r & 3];
-                }
+            for (int r = 0; r < 16; ++r) {
+                s[r] = KIND == PLAIN ? ls[r >> 2][r & 3] : 0.f;
+                dp[r] = KIND == DROPPED ? 0.f : dl[r >> 2][r & 3];
+            }
 #pragma unroll
             for (int ks = 0; ks < ND; ++ks) {
                 const bf16x8 aq = rd.frag(Qs, ks, qs), ag = rd.frag(Gs, ks, qs);
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    s[kb] = mfma(aq, kf[kb][ks], s[kb]);
-                    dp[kb] = mfma(ag, vf[kb][ks], dp[kb]);
-                }
+                s = mfma(aq, kf[ks], s);
+                dp = mfma(ag, vf[ks], dp);
             }
-            bf16x8 pf[KB][2], dsf[KB][2];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                const int key = key0 + kb * 32 + l31;
+            bf16x8 pf[2], dsf[2];
+            {
                 if constexpr (KIND != PLAIN) {
                     f32x16 turn;
                     float gain = bend.scale2;
                     if (bend.capped) {
-                        bend.tanh16(s[kb]);
+                        bend.tanh16(s);
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) turn[r] = fmaf(-s[kb][r], s[kb][r], 1.f);
+                        for (int r = 0; r < 16; ++r) turn[r] = fmaf(-s[r], s[r], 1.f);
                         gain = bend.cap2;
                     } else {
 #pragma unroll
@@ -210,31 +192,31 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
                             const f32x4 sl = *(const f32x4*)&info.slope2[qs * 32 + 8 * g + 4 * hh];
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                s[kb][4 * g + e] = fmaf(s[kb][4 * g + e], gain, fmaf(sl[e], fabsf(c[e] - keyf), ls[g][e]));
+                                s[4 * g + e] = fmaf(s[4 * g + e], gain, fmaf(sl[e], fabsf(c[e] - keyf), ls[g][e]));
                         }
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[kb][r] = fmaf(s[kb][r], gain, ls[r >> 2][r & 3]);
+                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], gain, ls[r >> 2][r & 3]);
                     }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kb][r] = EXP2(s[kb][r]);
+                    for (int r = 0; r < 16; ++r) s[r] = EXP2(s[r]);
                     if constexpr (KIND == DROPPED) {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const bool keep = drop_keep(p, info.drop[qs * 32 + reg_row(r) + 4 * hh], key);
-                            pf[kb][r >> 3][r & 7] = (bf16_t)(keep ? s[kb][r] * p.drop_scale : 0.f);
-                            dp[kb][r] = ((keep ? dp[kb][r] * p.drop_scale : 0.f) - dl[r >> 2][r & 3]) * turn[r];
+                            pf[r >> 3][r & 7] = (bf16_t)(keep ? s[r] * p.drop_scale : 0.f);
+                            dp[r] = ((keep ? dp[r] * p.drop_scale : 0.f) - dl[r >> 2][r & 3]) * turn[r];
                         }
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) dp[kb][r] *= turn[r];
+                        for (int r = 0; r < 16; ++r) dp[r] *= turn[r];
                     }
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kb][r] = EXP2(s[kb][r] * bend.scale2);
+                    for (int r = 0; r < 16; ++r) s[r] = EXP2(s[r] * bend.scale2);
                 }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) dp[kb][r] *= s[kb][r];
+                for (int r = 0; r < 16; ++r) dp[r] *= s[r];
                 if (masked) {        // what a row does not see is 0, whatever its scores and gradients are
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
@@ -243,16 +225,16 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if ((unsigned)(key - lo4[e]) >= (unsigned)n4[e]) {
-                                s[kb][4 * g + e] = 0.f;
-                                dp[kb][4 * g + e] = 0.f;
-                                if constexpr (KIND == DROPPED) pf[kb][(4 * g + e) >> 3][(4 * g + e) & 7] = (bf16_t)0.f;
+                                s[4 * g + e] = 0.f;
+                                dp[4 * g + e] = 0.f;
+                                if constexpr (KIND == DROPPED) pf[(4 * g + e) >> 3][(4 * g + e) & 7] = (bf16_t)0.f;
                             }
                     }
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    if constexpr (KIND != DROPPED) pf[kb][r >> 3][r & 7] = (bf16_t)s[kb][r];
-                    dsf[kb][r >> 3][r & 7] = (bf16_t)dp[kb][r];
+                    if constexpr (KIND != DROPPED) pf[r >> 3][r & 7] = (bf16_t)s[r];
+                    dsf[r >> 3][r & 7] = (bf16_t)dp[r];
                 }
             }
 #pragma unroll
@@ -260,20 +242,14 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
 #pragma unroll
                 for (int db = 0; db < NO; ++db) {
                     const bf16x8 ag = rd.frag_t(Gs, db, qs * 2 + st), aq = rd.frag_t(Qs, db, qs * 2 + st);
-#pragma unroll
-                    for (int kb = 0; kb < KB; ++kb) {
-                        dvT[kb][db] = mfma(ag, pf[kb][st], dvT[kb][db]);
-                        dkT[kb][db] = mfma(aq, dsf[kb][st], dkT[kb][db]);
-                    }
+                    dvT[db] = mfma(ag, pf[st], dvT[db]);
+                    dkT[db] = mfma(aq, dsf[st], dkT[db]);
                 }
         }
         }
         if (more) note(r0 + 64);
     }
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-        const int key = key0 + kb * 32 + l31;
-        if (key >= p.Tk) continue;
+    if (key < p.Tk) {
         bf16_t *dk = p.dk + (size_t)key * p.lddk + (size_t)hk * p.D, *dv = p.dv + (size_t)key * p.lddv + (size_t)hk * p.D;
         float* part = p.part + (((size_t)split * p.Tk + key) * p.Hkv + hk) * 2 * p.D;
 #pragma unroll
@@ -282,7 +258,7 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
             for (int g = 0; g < 4; ++g) {
                 const int d = db * 32 + 8 * g + 4 * hh;
                 if (d >= p.D) continue;
-                const f32x16 &a = dkT[kb][db], &c = dvT[kb][db];
+                const f32x16 &a = dkT[db], &c = dvT[db];
                 if (p.splits > 1) {
                     *(f32x4*)(part + d) = f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
                     *(f32x4*)(part + p.D + d) = f32x4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
@@ -290,8 +266,8 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
                     bf16x4 x, y;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        x[e] = seen[kb] ? (bf16_t)(a[4 * g + e] * p.scale) : (bf16_t)0.f;
-                        y[e] = seen[kb] ? (bf16_t)c[4 * g + e] : (bf16_t)0.f;
+                        x[e] = seen ? (bf16_t)(a[4 * g + e] * p.scale) : (bf16_t)0.f;
+                        y[e] = seen ? (bf16_t)c[4 * g + e] : (bf16_t)0.f;
                     }
                     *(bf16x4*)(dk + d) = x;
                     *(bf16x4*)(dv + d) = y;
@@ -299,10 +275,8 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
             }
     }
     if (p.splits > 1) return;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-        for (unsigned bad = bad_rows(seen[kb] && !(not_finite(dkT[kb]) + not_finite(dvT[kb]) == 0.f)); bad; bad &= bad - 1)
-            plain_dkdv_key(p, key0 + kb * 32 + __builtin_ctz(bad), hk);
+    for (unsigned bad = bad_rows(seen && !(not_finite(dkT) + not_finite(dvT) == 0.f)); bad; bad &= bad - 1)
+        plain_dkdv_key(p, key0 + __builtin_ctz(bad), hk);
 }
 
 // the partial gradients of a key, added in order: a wave per (key, key head)
@@ -340,18 +314,13 @@ __global__ __launch_bounds__(256) void doc_dkdv_join_kernel(const DocArgs p) {
     if (seen && __ballot(bad) != 0) plain_dkdv_key(p, key, hk);
 }
 
-template <int ND, int NO, int KB>
-void launch_kind(const DocArgs& a, hipStream_t st) {
-    const int tiles = (int)(((long long)a.Tk + 128 * KB - 1) / (128 * KB));
-    const dim3 grid(unit_grid((long long)tiles * a.splits, a.Hkv));
-    if (a.drop_thresh) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, DROPPED, KB>), grid, dim3(256), 0, st, a, tiles);
-    else if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, BENT, KB>), grid, dim3(256), 0, st, a, tiles);
-    else hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, PLAIN, KB>), grid, dim3(256), 0, st, a, tiles);
-}
-
 template <int ND, int NO>
 int launch(const DocArgs& a, hipStream_t st) {
-    launch_kind<ND, NO, 1>(a, st);
+    const int tiles = (int)(((long long)a.Tk + 127) / 128);
+    const dim3 grid(unit_grid((long long)tiles * a.splits, a.Hkv));
+    if (a.drop_thresh) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a, tiles);
+    else if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a, tiles);
+    else hipLaunchKernelGGL((doc_dkdv_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a, tiles);
     if (a.splits > 1) hipLaunchKernelGGL(doc_dkdv_join_kernel, dim3((unsigned)(((size_t)a.Tk * a.Hkv + 3) / 4)), dim3(256), 0, st, a);
     return mi355_check_launch("doc_attention_dkdv");
 }

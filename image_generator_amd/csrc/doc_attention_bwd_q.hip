@@ -12,6 +12,7 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
     int tile, hk;
     if (!unit_of(tiles, p.Hkv, tile, hk)) return;
+    if (p.causal) tile = tiles - 1 - tile;       // the last rows of a document see most: the longest work first
     const unsigned rows = (unsigned)p.Tq * (unsigned)p.G, R = tile * 128u + wave * 32 + l31;
     const bool live = R < rows;
     int token, head;

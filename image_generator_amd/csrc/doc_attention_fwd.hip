@@ -152,6 +152,7 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
     int tile, hk;
     if (!unit_of(tiles, p.Hkv, tile, hk)) return;
+    if (p.causal) tile = tiles - 1 - tile;       // the last rows of a document see most: the longest work first
     Rows<ND, NO> w;
     w.init(p, tile * 128u + wave * 32, hk);
     if (lane == 0) { range[wave][0] = w.hi > w.lo ? w.lo : 0x7fffffff; range[wave][1] = w.hi; }
