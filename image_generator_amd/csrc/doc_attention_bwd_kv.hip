@@ -46,6 +46,7 @@ struct RowInfo {                     // of the 64 staged rows
     float lse[64], delta[64];        // -lse, PLAIN: -lse / (scale log2 e);  -delta (DROPPED: delta)
     int lo[64], count[64];
     float c[64], slope2[64];         // key position, from the workgroup's first key;  -slope log2 e
+    float shift[64];                 // -lse - slope c log2 e
     unsigned drop[64];
 };
 
@@ -133,7 +134,12 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
             info.delta[threadIdx.x] = KIND == DROPPED ? dreg : -dreg;
             info.lo[threadIdx.x] = ireg.x;
             info.count[threadIdx.x] = in ? ireg.y - ireg.x : 0;
-            if (KIND != PLAIN) { info.c[threadIdx.x] = (float)(ireg.z - base); info.slope2[threadIdx.x] = -sreg * LOG2E; }
+            if (KIND != PLAIN) {
+                const float c = (float)(ireg.z - base), slope2 = -sreg * LOG2E;
+                info.c[threadIdx.x] = c;
+                info.slope2[threadIdx.x] = slope2;
+                info.shift[threadIdx.x] = fmaf(slope2, c, -ls);
+            }
             if (KIND == DROPPED) info.drop[threadIdx.x] = hreg;
         }
     };
@@ -150,6 +156,8 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
         if (r0 < whi && r0 + 64 > wlo) {
         const int first = info.lo[lane], count = info.count[lane];
         const bool masked = __ballot(first > key0 || first + count < kmax) != 0;
+        const bool before = KIND != PLAIN && __ballot(info.c[lane] < (float)(key0 + 31 - base)) == 0;
+        const float keyf = (float)(key - base);
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs) {
             f32x16 s, dp;
@@ -170,72 +178,69 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
                 s = mfma(aq, kf[ks], s);
                 dp = mfma(ag, vf[ks], dp);
             }
-            bf16x8 pf[2], dsf[2];
-            {
-                if constexpr (KIND != PLAIN) {
-                    f32x16 turn;
-                    float gain = bend.scale2;
-                    if (bend.capped) {
-                        bend.tanh16(s);
+            unsigned kept = 0;           // DROPPED: one bit for each register
+            if constexpr (KIND == DROPPED) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) turn[r] = fmaf(-s[r], s[r], 1.f);
-                        gain = bend.cap2;
-                    } else {
+                for (int r = 0; r < 16; ++r) {
+                    const bool keep = drop_keep(p, info.drop[qs * 32 + reg_row(r) + 4 * hh], key);
+                    kept |= keep ? 1u << r : 0u;
+                    dp[r] = (keep ? dp[r] * p.drop_scale : 0.f) - dl[r >> 2][r & 3];
+                }
+            }
+            if constexpr (KIND == PLAIN) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) turn[r] = 1.f;
-                    }
-                    if (bend.biased) {
-                        const float keyf = (float)(key - base);
+                for (int r = 0; r < 16; ++r) s[r] = EXP2(s[r] * bend.scale2);
+            } else {
+                float gain = bend.scale2;
+                if (bend.capped) {
+                    bend.tanh16(s);
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const f32x4 c = *(const f32x4*)&info.c[qs * 32 + 8 * g + 4 * hh];
-                            const f32x4 sl = *(const f32x4*)&info.slope2[qs * 32 + 8 * g + 4 * hh];
+                    for (int r = 0; r < 16; ++r) dp[r] *= fmaf(-s[r], s[r], 1.f);
+                    gain = bend.cap2;
+                }
+                if (!bend.biased) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                s[4 * g + e] = fmaf(s[4 * g + e], gain, fmaf(sl[e], fabsf(c[e] - keyf), ls[g][e]));
-                        }
-                    } else {
+                    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], gain, ls[r >> 2][r & 3]);
+                } else if (before) {     // every key at or before every row's position: -slope (c - key) - lse = slope key + shift
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], gain, ls[r >> 2][r & 3]);
-                    }
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 shift = *(const f32x4*)&info.shift[qs * 32 + 8 * g + 4 * hh];
+                        const f32x4 sl = *(const f32x4*)&info.slope2[qs * 32 + 8 * g + 4 * hh];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = EXP2(s[r]);
-                    if constexpr (KIND == DROPPED) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const bool keep = drop_keep(p, info.drop[qs * 32 + reg_row(r) + 4 * hh], key);
-                            pf[r >> 3][r & 7] = (bf16_t)(keep ? s[r] * p.drop_scale : 0.f);
-                            dp[r] = ((keep ? dp[r] * p.drop_scale : 0.f) - dl[r >> 2][r & 3]) * turn[r];
-                        }
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) dp[r] *= turn[r];
+                        for (int e = 0; e < 4; ++e) s[4 * g + e] = fmaf(s[4 * g + e], gain, fmaf(-sl[e], keyf, shift[e]));
                     }
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = EXP2(s[r] * bend.scale2);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) dp[r] *= s[r];
-                if (masked) {        // what a row does not see is 0, whatever its scores and gradients are
-#pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const int4 a = *(const int4*)&info.lo[qs * 32 + 8 * g + 4 * hh], n = *(const int4*)&info.count[qs * 32 + 8 * g + 4 * hh];
-                        const int lo4[4] = {a.x, a.y, a.z, a.w}, n4[4] = {n.x, n.y, n.z, n.w};
+                        const f32x4 c = *(const f32x4*)&info.c[qs * 32 + 8 * g + 4 * hh];
+                        const f32x4 sl = *(const f32x4*)&info.slope2[qs * 32 + 8 * g + 4 * hh];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if ((unsigned)(key - lo4[e]) >= (unsigned)n4[e]) {
-                                s[4 * g + e] = 0.f;
-                                dp[4 * g + e] = 0.f;
-                                if constexpr (KIND == DROPPED) pf[(4 * g + e) >> 3][(4 * g + e) & 7] = (bf16_t)0.f;
-                            }
+                        for (int e = 0; e < 4; ++e) s[4 * g + e] = fmaf(s[4 * g + e], gain, fmaf(sl[e], fabsf(c[e] - keyf), ls[g][e]));
                     }
                 }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    if constexpr (KIND != DROPPED) pf[r >> 3][r & 7] = (bf16_t)s[r];
-                    dsf[r >> 3][r & 7] = (bf16_t)dp[r];
+                for (int r = 0; r < 16; ++r) s[r] = EXP2(s[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+            if (masked) {        // what a row does not see is 0, whatever its scores and gradients are
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int4 a = *(const int4*)&info.lo[qs * 32 + 8 * g + 4 * hh], n = *(const int4*)&info.count[qs * 32 + 8 * g + 4 * hh];
+                    const int lo4[4] = {a.x, a.y, a.z, a.w}, n4[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if ((unsigned)(key - lo4[e]) >= (unsigned)n4[e]) {
+                            s[4 * g + e] = 0.f;
+                            dp[4 * g + e] = 0.f;
+                        }
                 }
+            }
+            bf16x8 pf[2], dsf[2];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                pf[r >> 3][r & 7] = (bf16_t)(KIND != DROPPED ? s[r] : kept >> r & 1 ? s[r] * p.drop_scale : 0.f);
+                dsf[r >> 3][r & 7] = (bf16_t)dp[r];
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st)
