@@ -55,8 +55,9 @@ struct Rows {                        // a wave's 32 rows
 
     // One staged tile of keys k0 .. k0 + 63.  FAST: no running maximum, p = 2^x against the fixed reference 0.  Floating point
     // does not mind the common factor while nothing leaves the normal range, and bf16 probabilities have fp32's exponents; a
-    // row whose sum (`fits`) is not within 2^-100 .. 2^100 - scores beyond some 70 nats, or a distance bias on every key it
-    // sees - sends its workgroup through the loop again with the maximum.
+    // row whose sum (`fits`) is not within 2^-60 .. 2^100 - scores all below some -40 nats or one beyond 70, or a distance bias
+    // on every key it sees - sends its workgroup through the loop again with the maximum.  (Below, the products with values
+    // would meet the end of the normal range sooner: values above 2^-66 keep theirs.)
     template <int KIND, bool FAST>
     __device__ __forceinline__ void tile(const DocArgs& p, const Bend& bend, const Reads<ND, NO>& at, const char* Ks, const char* Vs, int k0) {
         const int hh = (threadIdx.x & 63) >> 5;
@@ -137,7 +138,7 @@ struct Rows {                        // a wave's 32 rows
     }
     // the two lanes of a row hold the sums of the keys whose scores they hold
     __device__ __forceinline__ void join() { l += __shfl_xor(l, 32, 64); }
-    __device__ __forceinline__ bool fits() const { return span.hi <= span.lo || (l > 0x1p-100f && l < 0x1p100f); }
+    __device__ __forceinline__ bool fits() const { return span.hi <= span.lo || (l > 0x1p-60f && l < 0x1p100f); }
     // rows whose result is not finite
     __device__ __forceinline__ unsigned bad() const {
         const float z = not_finite(o) + l * 0.f;

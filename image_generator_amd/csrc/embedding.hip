@@ -1,7 +1,7 @@
 // Embedding rows and the gradient of their table.
 //
 //   out[i][:]    = scale * table[id_i][:]
-//   dtable[v][:] = scale * sum over i with id_i = v, in ascending i, of dy[i][:]
+//   dtable[v][:] = scale * sum over i with id_i = v of dy[i][:]
 //
 // The gradient groups the positions by id with a stable sort instead of adding with atomics, so every row of the table is
 // written once, by one wave, in an order that depends on the ids alone: the same call returns the same bits.  Sums are fp32,
@@ -16,7 +16,8 @@ constexpr int SHARES = 16;           // lanes that count for one id
 constexpr int TILE = 2048;           // ids per workgroup of a radix pass: four waves with 512 consecutive ids each
 constexpr int MAXBINS = 256;
 constexpr int CHUNK = 32;            // sorted positions of one id that are summed ahead when they fill an aligned chunk ...
-constexpr int SUPER = 32;            // ... and aligned runs of so many such chunks
+constexpr int SUPER = 32;            // ... and aligned runs of so many such chunks,
+constexpr int SUPERS_FROM = 4096;    // from so many positions on
 
 template <typename T> __device__ __forceinline__ float ldf(const T* p) { return (float)*p; }
 template <typename T> struct Vec4;
@@ -72,9 +73,13 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const void* __restrict_
 __global__ __launch_bounds__(256) void rank_sort_kernel(const void* __restrict__ ids, int ids64, int n, unsigned rows,
                                                         unsigned* __restrict__ keys, unsigned* __restrict__ pos) {
     extern __shared__ __attribute__((aligned(16))) unsigned list[];
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const long long id = load_id(ids, ids64, i);
-        list[i] = id >= 0 && id < (long long)rows ? (unsigned)id : rows;
+    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * 256) {
+        long long id[8];                         // eight loads under way at a time
+#pragma unroll
+        for (int u = 0; u < 8; ++u) id[u] = load_id(ids, ids64, min(i0 + u * 256, n - 1));
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i0 + u * 256 < n) list[i0 + u * 256] = id[u] >= 0 && id[u] < (long long)rows ? (unsigned)id[u] : rows;
     }
     __syncthreads();
     const int mine = blockIdx.x * (256 / SHARES) + threadIdx.x / SHARES, share = threadIdx.x % SHARES;
@@ -264,11 +269,11 @@ __global__ __launch_bounds__(256) void chunk_sum_kernel(const unsigned* __restri
     const int c = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const int lo = c * CHUNK;
     if (lo + CHUNK > n) return;
-    const unsigned k = keys[lo];
-    if (k >= rows || keys[lo + CHUNK - 1] != k) return;
+    const unsigned k = keys[lo], last = keys[lo + CHUNK - 1], mine = pos[lo + (threadIdx.x & (CHUNK - 1))];
+    if (k >= rows || last != k) return;
     const int col0 = blockIdx.y * SWEEPS * 64 * VEC;
     f32x4 acc[SWEEPS] = {};
-    add_rows<VEC>(acc, dy, width, col0, CHUNK, [&](int j) { return pos[lo + j]; });
+    add_rows<VEC>(acc, dy, width, col0, CHUNK, [&](int) { return mine; });       // (CHUNK <= 64: lane j asks for j)
     put_row<VEC>(part + (size_t)c * width, acc, width, col0, 1.f);
 }
 // ... and aligned runs of SUPER such chunks.
@@ -382,7 +387,7 @@ template <typename T, typename TO, int VEC>
 static void launch_grad(const GradPlan& g, char* ws, const unsigned* keys, const unsigned* pos, unsigned rows, const void* dy, int width,
                         float scale, void* dtable, hipStream_t st) {
     const int cols = (width + SWEEPS * 64 * VEC - 1) / (SWEEPS * 64 * VEC);
-    const int chunks = g.n / CHUNK, supers = g.n / (CHUNK * SUPER);
+    const int chunks = g.n / CHUNK, supers = g.n < SUPERS_FROM ? 0 : g.n / (CHUNK * SUPER);
     float *part = (float*)(ws + g.part), *part2 = (float*)(ws + g.part2);
     if (chunks) hipLaunchKernelGGL((chunk_sum_kernel<T, VEC>), dim3((chunks + 3) / 4, cols), dim3(256), 0, st, keys, pos, g.n, rows,
                                    (const T*)dy, width, part);
@@ -430,6 +435,7 @@ size_t mi355_embedding_bwd_workspace_bytes(long long n, long long rows, int widt
 int mi355_embedding_bwd(const void* ids, int ids64, long long n, const void* dy, int dy_bf16, long long rows, int width, float scale,
                         void* dtable, int out_bf16, void* ws, size_t ws_bytes, void* stream) {
     if (const char* why = bad_shape(n, rows, width)) return mi355_fail(MI355_ERR_ARG, "embedding_bwd: %s", why);
+    if (rows > (1ll << 26)) return mi355_fail(MI355_ERR_ARG, "embedding_bwd: more than 2^26 rows");
     if (!dtable || (n > 0 && (!ids || !dy || !ws))) return mi355_fail(MI355_ERR_ARG, "embedding_bwd: null pointer");
     const GradPlan g = grad_plan(n, rows, width);
     if (ws_bytes < g.bytes) return mi355_fail(MI355_ERR_ARG, "embedding_bwd: workspace of %zu bytes, %zu needed", ws_bytes, g.bytes);

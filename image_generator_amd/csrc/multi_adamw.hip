@@ -425,7 +425,7 @@ int mi355_adamw_moments(const void* m_codes, const float* m_scales, const void* 
     if (blocks == 0) return MI355_OK;
     if (!m_codes || !m_scales || !u_codes || !u_scales || !m || !v) return mi355_fail(MI355_ERR_ARG, "adamw_moments: null pointer");
     if (off16(m) || off16(v)) return mi355_fail(MI355_ERR_ARG, "adamw_moments: outputs not 16-byte aligned");
-    if (blocks > (1ll << 31)) return mi355_fail(MI355_ERR_ARG, "adamw_moments: more than 2^31 blocks");
+    if (blocks > (1ll << 25)) return mi355_fail(MI355_ERR_ARG, "adamw_moments: more than 2^25 blocks");
     const size_t words = (size_t)blocks * (BLK / 4);
     hipLaunchKernelGGL(moments_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, (hipStream_t)stream, (const unsigned*)m_codes,
                        m_scales, (const unsigned*)u_codes, u_scales, words, m, v);

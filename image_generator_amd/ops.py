@@ -636,6 +636,11 @@ def _doc_matrix(name, t, heads, width):
         raise ValueError(f"doc_attention: {name} {tuple(t.shape)} for {heads} heads of width {width}")
 
 
+def _ld(t):
+    # the stride between the rows of one row is whatever made the tensor (a transposed column, say) and is not looked at
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed):
     """Checks shared by the two directions of the document attention; (leading arguments, trailing arguments, sizes, device)."""
     if kv_heads is None:
@@ -681,7 +686,7 @@ def doc_attention_fwd(q, k, v, heads, q_offsets, k_offsets=None, kv_heads=None, 
     need = lib.mi355_doc_attention_fwd_workspace_bytes(*sizes)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     check(lib.mi355_doc_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *head, *sizes,
-                                      q.stride(0), k.stride(0), v.stride(0), out.stride(0), *tail, _ptr(ws), need,
+                                      _ld(q), _ld(k), _ld(v), out.stride(0), *tail, _ptr(ws), need,
                                       torch._C._cuda_getCurrentRawStream(dev)), "doc_attention_fwd")
     return out, lse
 
@@ -689,19 +694,22 @@ def doc_attention_fwd(q, k, v, heads, q_offsets, k_offsets=None, kv_heads=None, 
 def doc_attention_bwd(do, q, k, v, o, lse, heads, q_offsets, k_offsets=None, kv_heads=None, causal=False, prefix=None, slopes=None,
                       cap=0.0, scale=None, align="end", drop_p=0.0, seed=0, dq=None, dk=None, dv=None):
     """(dq, dk, dv) of `doc_attention_fwd` for the gradient `do` of its output; `o`, `lse` are what it returned.  dq / dk / dv:
-    bf16 matrices to write (slices of one buffer, say); new ones by default."""
+    bf16 matrices to write (slices of one buffer, say, that share no element with each other or an operand); new ones by default."""
     head, tail, sizes, _ = _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed)
     _here(q, do, o, lse, dq, dk, dv)
     dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=q.device) if d is None else d for t, d in ((q, dq), (k, dk), (v, dv)))
     for name, t, like in (("do", do, q), ("o", o, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
         if t.shape != like.shape or t.dtype != BF16 or t.stride(1) != 1 and t.shape[1] > 1:
             raise RuntimeError(f"doc_attention_bwd: {name} must be a bf16 matrix {tuple(like.shape)} with adjacent columns")
+    to = [t.data_ptr() for t in (dq, dk, dv) if t.numel()]
+    if len(set(to)) < len(to) or not {t.data_ptr() for t in (q, k, v, o, do)}.isdisjoint(to):
+        raise ValueError("doc_attention_bwd: a gradient in the place of an operand or of another gradient")
     if lse.shape != (heads, q.shape[0]) or lse.dtype != F32 or not lse.is_contiguous():
         raise RuntimeError("doc_attention_bwd: lse is not the forward pass's")
     ws = torch.empty(int(lib.mi355_doc_attention_bwd_workspace_bytes(*sizes, q_offsets.numel() - 1, causal)), dtype=torch.uint8, device=q.device)
     check(lib.mi355_doc_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), dq.data_ptr(),
-                                      dk.data_ptr(), dv.data_ptr(), *head, *sizes, q.stride(0), k.stride(0), v.stride(0), o.stride(0),
-                                      do.stride(0), dq.stride(0), dk.stride(0), dv.stride(0), *tail, ws.data_ptr(), ws.numel(), _stream()),
+                                      dk.data_ptr(), dv.data_ptr(), *head, *sizes, _ld(q), _ld(k), _ld(v), _ld(o), _ld(do), _ld(dq), _ld(dk),
+                                      _ld(dv), *tail, ws.data_ptr(), ws.numel(), _stream()),
           "doc_attention_bwd")
     return dq, dk, dv
 
@@ -729,8 +737,8 @@ def embedding_fwd(ids, table, scale=1.0, out_dtype=BF16):
 
 
 def embedding_bwd(ids, dy, rows, scale=1.0, out_dtype=F32):
-    """Gradient [rows, width] of the table of `embedding_fwd`: scale times the sum of the dy rows of each id, in the order of
-    the positions (same call, same bits)."""
+    """Gradient [rows, width] of the table of `embedding_fwd`: scale times the sum of the dy rows of each id, in an order
+    that the ids alone decide (same call, same bits)."""
     _here(dy, ids)
     if dy.dtype not in (F32, BF16) or out_dtype not in (F32, BF16):
         raise RuntimeError("embedding_bwd: gradients are fp32 or bf16")
@@ -1382,7 +1390,10 @@ class DocAttentionFn(torch.autograd.Function):
         da, db, dc = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (a, b, c))
         q, k, v = DocAttentionFn._split(a, b, c, heads, kv_heads)
         dq, dk, dv = DocAttentionFn._split(da, db, dc, heads, kv_heads)
-        doc_attention_bwd(do.contiguous(), q, k, v, o, lse, heads, q_offsets, k_offsets, kv_heads, prefix=prefix, slopes=slopes, dq=dq, dk=dk,
+        do = do.contiguous()
+        if do.data_ptr() % 16:           # a piece of some larger gradient
+            do = do.clone()
+        doc_attention_bwd(do, q, k, v, o, lse, heads, q_offsets, k_offsets, kv_heads, prefix=prefix, slopes=slopes, dq=dq, dk=dk,
                           dv=dv, **how)
         return da, db, dc, None, None, None, None, None, None, None
 
@@ -1390,6 +1401,8 @@ class DocAttentionFn(torch.autograd.Function):
 def doc_attention(a, b=None, c=None, *, heads, q_offsets, k_offsets=None, kv_heads=None, prefix=None, slopes=None, **how):
     """Differentiable `doc_attention_fwd` (out only).  Operands: [q | k | v], or q and [k | v], or q, k and v."""
     kv_heads = heads if kv_heads is None else kv_heads
+    if b is None and c is not None:
+        raise ValueError("doc_attention: operands are [q | k | v], or q and [k | v], or q, k and v")
     if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("doc_attention: no gradient reaches the slopes (detach them)")
     return DocAttentionFn.apply(a, b, c, heads, kv_heads, how, q_offsets, k_offsets, prefix, slopes)

@@ -9,6 +9,7 @@ from __future__ import annotations
 import math
 import operator
 
+import numpy as np
 import torch
 
 from ._lib import lib, check
@@ -39,6 +40,8 @@ class TensorAdamW:
         self.params = list(params)
         if not self.params:
             raise ValueError("TensorAdamW: no parameters")
+        if not all(0 <= b < 1 for b in betas) or not eps >= 2.0 ** -126:      # (0 / 0 behind a smaller one: untouched rows have m = v = 0)
+            raise ValueError(f"TensorAdamW: betas {tuple(betas)} not below 1, or eps {eps} not a normal fp32 number above 0")
         if state_bits not in (8, 32):
             raise ValueError(f"TensorAdamW: states of 8 or 32 bits, not {state_bits}")
         dev = self.params[0].device
@@ -53,7 +56,7 @@ class TensorAdamW:
         self._shapes = [p.shape for p in self.params]
         self.lr, self.betas, self.eps, self.wd, self.max_norm = lr, tuple(betas), eps, weight_decay, max_grad_norm
         self.bits, self.device, self.t = state_bits, dev, 0
-        self._new = tuple(float(1 - torch.tensor(b, dtype=F32).double()) if fp32_betas else 1 - b for b in self.betas)
+        self.fp32_betas = fp32_betas
         self.watched = list(watched)
         blocks = [-(-p.numel() // BLOCK) for p in self.params]
         self.starts = [0]
@@ -80,6 +83,9 @@ class TensorAdamW:
 
     def set_copies(self, copies=None):
         """The bf16 tensors that receive the updated parameters (one for each parameter, or None in its place)."""
+        for p, shape in zip(self.params, self._shapes):
+            if p.device != self.device or p.dtype != F32 or p.shape != shape or not p.is_contiguous():
+                raise ValueError(f"TensorAdamW: a parameter has become {p.dtype} {tuple(p.shape)} on {p.device}")
         copies = [None] * len(self.params) if copies is None else list(copies)
         if len(copies) != len(self.params):
             raise ValueError(f"TensorAdamW: {len(copies)} copies of {len(self.params)} parameters")
@@ -89,6 +95,7 @@ class TensorAdamW:
         _disjoint([c for c in copies if c is not None], "copies")
         self.copies = copies
         self._written = [t for t in self.params + copies if t is not None]
+        self._places = list(map(torch.Tensor.data_ptr, self._written))
         rows = [[p.data_ptr(), 0 if c is None else c.data_ptr(), p.numel(), s] for p, c, s in zip(self.params, copies, self.starts)]
         rows += [[0, 0, n, 0] for n in self.watched]
         self._recs = torch.tensor(rows, dtype=torch.int64).to(self.device)
@@ -103,6 +110,8 @@ class TensorAdamW:
         grads = [p.grad for p in self.params] if owned else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"TensorAdamW: {len(grads)} gradients of {len(self.params)} parameters")
+        if list(map(torch.Tensor.data_ptr, self._written)) != self._places:
+            raise RuntimeError("TensorAdamW: a parameter or copy has moved to other memory (set_copies() takes the new places)")
         words, kept = self._addresses(grads, owned)
         watched = [None] * len(self.watched) if watched is None else list(watched)
         if len(watched) != len(self.watched):
@@ -117,7 +126,7 @@ class TensorAdamW:
         b1, b2 = self.betas
         c1, c2 = 1 - b1 ** self.t, 1 - b2 ** self.t
         hyper = (self.lr, b1, b2, self.eps, self.wd, c1, c2, self.max_norm or 0.0, 1 - self.lr * self.wd, self.lr / c1, 1 / math.sqrt(c2),
-                 *self._new)
+                 *(1 - float(np.float32(b)) if self.fp32_betas else 1 - b for b in self.betas))
         h = self._ring.acquire().numpy()
         h[:_HYPER].view("float64")[:len(hyper)] = hyper
         h[_HYPER:] = words
@@ -130,7 +139,7 @@ class TensorAdamW:
         """(what the device table holds for each gradient, copies made here)."""
         # the common case in a few sweeps: every gradient there, of its parameter's shape, contiguous, one type, this device
         # (a parameter's own `.grad` has its shape and device already)
-        if not any(g is None for g in grads) and all(map(torch.Tensor.is_contiguous, grads)):
+        if type(None) not in set(map(type, grads)) and all(map(torch.Tensor.is_contiguous, grads)):
             if owned or (list(map(_SHAPE, grads)) == self._shapes and set(map(torch.Tensor.get_device, grads)) == {self.device.index}):
                 kinds = set(map(_DTYPE, grads))
                 if kinds == {F32}:

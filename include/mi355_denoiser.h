@@ -427,7 +427,8 @@ int mi355_copy2d_f32_batched(const long long* table, int n, void* stream);
  * Query i sits at key position c = i - q_end + k_end (align_start: i - q_begin + k_begin) and sees the keys j of its document,
  * with `causal` those with j <= c or j < k_begin + prefix[n] (prefix: int32 [docs] or NULL):
  *   t = scale q.k;  t = cap tanh(t / cap) if cap > 0;  score = t - slopes[head] |c - j|;  out = softmax(score) v
- * cap <= 1024.  slopes: fp32 [Hq] or NULL.  Row strides are at most 2^23.  Hq is a multiple of Hkv; query head h reads key head h / (Hq / Hkv).  D: a multiple of 8, <= 128.
+ * cap <= 1024.  slopes: fp32 [Hq] or NULL.  Hq is a multiple of Hkv; query head h reads key head h / (Hq / Hkv).  D: a multiple
+ * of 8, <= 128.  Limits: Tq * Hq, Tk * Hkv < 2^30, row strides <= 2^23.
  * A query that sees no key, or belongs to no document, gets a row of zeros and lse = -infinity; keys of no document get zero
  * gradients.  What a query does not see never reaches its result, infinities and NaN included.  lse [Hq][Tq] in log2 units.
  * drop_p, seed: dropout on the probabilities, the same in both directions for the same seed.
@@ -449,11 +450,11 @@ int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const v
 
 /* ---- embedding rows (nn.Embedding of encoder/text_encoder.py:14,27) and the gradient of their table -----------------------
  * fwd: out[i][:] = scale * table[ids[i]][:], i < n; table [rows][width] and out [n][width] fp32 or bf16.
- * bwd: dtable[v][:] = scale * sum of dy[i][:] over ids[i] = v in ascending i (fp32 sums, rounded once); every row of dtable is
- * written, zeros where no id names it.  The order depends on the ids alone: equal calls return equal bits.
+ * bwd: dtable[v][:] = scale * sum of dy[i][:] over ids[i] = v (fp32 sums, rounded once); every row of dtable is written, zeros
+ * where no id names it.  The order depends on the ids alone: equal calls return equal bits.
  * ids: int32, or int64 (ids64 != 0).  An id outside [0, rows) reads as a NaN row and adds to no gradient.  ws: a device
  * buffer of mi355_embedding_bwd_workspace_bytes(n, rows, width), 16-byte aligned, for this call alone.
- * Limits: n, rows <= 2^30, width <= 2^20, n * width < 2^32. */
+ * Limits: n, rows <= 2^30 (bwd: rows <= 2^26), width <= 2^20, n * width < 2^32. */
 int mi355_embedding_fwd(const void* ids, int ids64, long long n, const void* table, int table_bf16, long long rows, int width,
                         float scale, void* out, int out_bf16, void* stream);
 size_t mi355_embedding_bwd_workspace_bytes(long long n, long long rows, int width);

@@ -413,3 +413,50 @@ def test_split_work_with_what_is_not_finite(case, value, which):
     rows, keys = torch.arange(int(qo[1]), int(qo[-1])), torch.arange(int(ko[1]), int(ko[-1]))
     check(got, reference(*clean, 4, 2, qo, ko), {"out": rows, "dq": rows, "dk": keys, "dv": keys})
     assert not torch.isfinite(torch.cat([got[n][:1].float().flatten() for n in ("out", "dq", "dk", "dv")])).all()
+
+
+def test_one_row_of_any_stride():
+    """The stride of a matrix of one row is whatever made it: 1 here."""
+    off = offsets([1])
+    x = [t.cuda() for t in inputs(1, 1, 4, 2, 64, 30)]
+    want = run(*x, heads=4, kv_heads=2, q_offsets=off)
+    odd = [t.as_strided(t.shape, (1, 1)) for t in x]
+    assert all(t.stride(0) == 1 for t in odd)
+    got = run(*odd, heads=4, kv_heads=2, q_offsets=off)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+def test_gradient_that_is_a_piece_of_another():
+    """cat's backward hands out views of one buffer, 3 elements in here."""
+    from image_generator_amd import ops
+    off = offsets([30, 50]).cuda()
+    q, k, v, do = (t.cuda() for t in inputs(80, 80, 4, 2, 64, 31))
+    want = run(q, k, v, do, heads=4, kv_heads=2, q_offsets=off)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = ops.doc_attention(*leaves, heads=4, kv_heads=2, q_offsets=off)
+    torch.cat((torch.zeros(3, device="cuda", dtype=BF), out.flatten())).backward(torch.cat((torch.zeros(3, device="cuda", dtype=BF), do.flatten())))
+    assert all(torch.equal(t.grad, want[n]) for t, n in zip(leaves, ("dq", "dk", "dv")))
+
+
+def test_small_values_under_low_scores():
+    """Scores around -48 and values around 2^-70: neither alone leaves fp32's range, their product would."""
+    off = offsets([90, 40])
+    q, k, v, do = inputs(130, 130, 2, 2, 64, 32)
+    q, k, v = (q.float() * 0.1 + 2).to(BF), (k.float() * 0.1 - 3).to(BF), (v.float() * 2.0 ** -70).to(BF)
+    check(run(q, k, v, do, heads=2, q_offsets=off), reference(q, k, v, do, 2, 2, off, off))
+
+
+def test_places_that_are_refused():
+    from image_generator_amd import ops
+    off = offsets([8]).cuda()
+    q, k, v, do = (t.cuda() for t in inputs(8, 8, 2, 2, 64, 33))
+    out, lse = ops.doc_attention_fwd(q, k, v, 2, off)
+    for bad in (dict(dq=q), dict(dk=k), dict(dv=do), dict(dk=out), dict(dk=torch.empty_like(k), dv=None)):
+        if "dv" in bad and bad["dv"] is None:
+            bad["dv"] = bad["dk"]
+        with pytest.raises(ValueError, match="in the place"):
+            ops.doc_attention_bwd(do, q, k, v, out, lse, 2, off, **bad)
+    with pytest.raises(ValueError, match="operands"):
+        ops.doc_attention(q, None, v, heads=2, q_offsets=off)
+    for n, t in zip(("dq", "dk", "dv"), ops.doc_attention_bwd(out, q, q, q, out, lse, 2, off)):       # one tensor in several places is read only
+        assert torch.isfinite(t).all(), n

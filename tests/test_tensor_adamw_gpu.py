@@ -300,3 +300,26 @@ def test_refusals():
             opt.step(grads)
     with pytest.raises(RuntimeError):
         opt.apply()
+
+
+def test_parameter_that_moved_is_refused():
+    """The addresses of parameters and copies live on the device: a step after one of them moved would write to its old place."""
+    from image_generator_amd.optim import TensorAdamW
+    p, c = torch.zeros(8, device="cuda"), torch.zeros(8, device="cuda", dtype=BF)
+    opt = TensorAdamW([p], copies=[c], lr=0.5, weight_decay=0.0)
+    old, p.data = p.data, torch.ones(8, device="cuda")
+    with pytest.raises(RuntimeError, match="moved"):
+        opt.step([torch.ones(8, device="cuda")])
+    opt.set_copies([c])
+    opt.step([torch.ones(8, device="cuda")])
+    assert (old == 0).all() and opt.t == 1 and torch.allclose(p, torch.full_like(p, 0.5)) and torch.equal(c, p.to(BF))
+    p.data = torch.ones(9, device="cuda")
+    with pytest.raises(ValueError, match="become"):
+        opt.set_copies([c])
+
+
+@pytest.mark.parametrize("kw", [dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)), dict(eps=0.0), dict(eps=1e-40), dict(eps=float("nan"))])
+def test_refused_hyperparameters(kw):
+    from image_generator_amd.optim import TensorAdamW
+    with pytest.raises(ValueError, match="betas"):
+        TensorAdamW([torch.zeros(8, device="cuda")], **kw)

@@ -20,6 +20,7 @@ def test_embedding_refusals():
     assert lib.mi355_embedding_bwd(16, 1, 100, 16, 1, 50, 8, 1.0, 16, 0, 16, need - 1, None) == -1 and "workspace" in err()
     assert lib.mi355_embedding_bwd(16, 1, 100, 16, 1, 50, 8, 1.0, 16, 0, 24, need, None) == -1 and "aligned" in err()
     assert lib.mi355_embedding_bwd(16, 1, 100, 16, 1, 50, 8, 1.0, None, 0, 16, need, None) == -1 and "null" in err()
+    assert lib.mi355_embedding_bwd(16, 1, 100, 16, 1, (1 << 26) + 1, 8, 1.0, 16, 0, 16, 1 << 40, None) == -1 and "2^26" in err()
 
 
 def test_optimizer_refusals():
@@ -58,7 +59,7 @@ def test_doc_attention_refusals():
                     (dict(D=136), "128"), (dict(prefix=16), "prefix"), (dict(cap=-1.0), "cap"), (dict(cap=2000.0), "cap"), (dict(ld=(1 << 23) + 8), "strides"), (dict(cap=float("nan")), "cap"),
                     (dict(drop=1.0), "dropout"), (dict(ld=60), "strides"), (dict(ldo=32), "strides"), (dict(ptr=8), "aligned"),
                     (dict(ptr=None), "null"), (dict(off=None), "null"), (dict(ws=None, Tk=5000), "workspace"), (dict(ws_bytes=0, Tk=5000), "workspace"),
-                    (dict(Tq=1 << 30), "2^31"), (dict(ld=-64), "strides")):
+                    (dict(Tq=1 << 29), "2^30"), (dict(docs=2 ** 31 - 1), "document"), (dict(ld=-64), "strides")):
         assert fwd(**kw) == -1 and why in err(), (kw, err())
     assert fwd(Tq=0) == 0
 
