@@ -242,8 +242,9 @@ __device__ __forceinline__ void add_rows(f32x4 (&acc)[SWEEPS], const T* __restri
         const int n = min(64, count - b);
         const unsigned mine = idx(b + min(lane, n - 1));
         int j = 0;
-        for (; j + 16 <= n; j += 16) add_batch<16, VEC>(acc, src, width, col, sweeps, mine, j);
-        if (n & 8) { add_batch<8, VEC>(acc, src, width, col, sweeps, mine, j); j += 8; }
+        constexpr int FLY = 16;
+        for (; j + FLY <= n; j += FLY) add_batch<FLY, VEC>(acc, src, width, col, sweeps, mine, j);
+        if (FLY == 16 && (n & 8)) { add_batch<8, VEC>(acc, src, width, col, sweeps, mine, j); j += 8; }
         if (n & 4) { add_batch<4, VEC>(acc, src, width, col, sweeps, mine, j); j += 4; }
         if (n & 2) { add_batch<2, VEC>(acc, src, width, col, sweeps, mine, j); j += 2; }
         if (n & 1) add_batch<1, VEC>(acc, src, width, col, sweeps, mine, j);
@@ -300,20 +301,30 @@ __global__ __launch_bounds__(256) void table_grad_kernel(const unsigned* __restr
                                                          TO* __restrict__ dtable) {
     __shared__ int start[ROWS_PER_WG + 1];
     const unsigned v0 = blockIdx.x * ROWS_PER_WG;
-    // first index with keys[index] >= v, for each v of the workgroup: a wave per v and round probes 64 places a step
-    for (int r = threadIdx.x >> 6; r <= ROWS_PER_WG; r += 4) {
-        const unsigned v = v0 + r;
-        const int lane = threadIdx.x & 63;
-        int lo = 0, hi = n;
-        while (lo < hi) {
-            const int step = (hi - lo + 63) / 64, at = lo + lane * step;
-            const int below = __popcll(__ballot(at < hi && keys[min(at, n - 1)] < v));
-            if (below == 0) break;                            // keys[lo] >= v
-            const int last = lo + (below - 1) * step;         // keys[last] < v
-            lo = last + 1;
-            hi = min(hi, last + step);
+    // first index with keys[index] >= v, for each v of the workgroup: a wave takes two v and probes 64 places a step for each
+    static_assert(ROWS_PER_WG == 7, "two boundaries for each of four waves");
+    {
+        const int lane = threadIdx.x & 63, r = threadIdx.x >> 6;
+        int lo[2] = {0, 0}, hi[2] = {n, n};
+        while (lo[0] < hi[0] || lo[1] < hi[1]) {
+            unsigned key[2];
+            int step[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                step[q] = (hi[q] - lo[q] + 63) / 64;
+                key[q] = keys[min(lo[q] + lane * step[q], n - 1)];
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (lo[q] >= hi[q]) continue;
+                const int below = __popcll(__ballot(lo[q] + lane * step[q] < hi[q] && key[q] < v0 + r + 4 * q));
+                if (below == 0) { hi[q] = lo[q]; continue; }      // keys[lo] >= v
+                const int last = lo[q] + (below - 1) * step[q];   // keys[last] < v
+                lo[q] = last + 1;
+                hi[q] = min(hi[q], last + step[q]);
+            }
         }
-        if (lane == 0) start[r] = lo;
+        if (lane == 0) { start[r] = lo[0]; start[r + 4] = lo[1]; }
     }
     __syncthreads();
     for (int r = threadIdx.x >> 6; r < ROWS_PER_WG; r += 4) {
