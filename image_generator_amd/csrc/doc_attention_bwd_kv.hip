@@ -52,7 +52,7 @@ struct RowInfo {                     // of the 64 staged rows
 
 template <int ND, int NO, int KIND>
 __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1) void doc_dkdv_kernel(const DocArgs p, int tiles) {
-    __shared__ __attribute__((aligned(16))) char smem[4 * TILE_BYTES<NO>];      // Q and dO, twice
+    __shared__ __attribute__((aligned(16))) char even[2 * TILE_BYTES<NO>], odd[2 * TILE_BYTES<NO>];      // Q and dO, twice
     __shared__ __attribute__((aligned(16))) RowInfo infos[2];
     __shared__ int range[4][2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
@@ -108,10 +108,9 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
     float lreg = 0.f, dreg = 0.f, sreg = 0.f;
     unsigned hreg = 0;
     bool in = false;
-    auto request = [&](unsigned r0) __attribute__((always_inline)) {
+    auto request = [&](char* to, unsigned r0) __attribute__((always_inline)) {
         const unsigned t0 = G == 1 ? r0 : r0 / G;
         if (64 % G != 0) f.init(p, r0 - t0 * G);
-        char* to = smem + (((r0 - rlo) >> 6) & 1) * 2 * TILE_BYTES<NO>;
         f.dma(to, to + TILE_BYTES<NO>, p, hk, (int)t0, thi);
         if (threadIdx.x < 64) {
             const unsigned R = r0 + threadIdx.x;
@@ -126,9 +125,8 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
             if (KIND == DROPPED) hreg = drop_row(p, token, head);
         }
     };
-    auto note = [&](unsigned r0) __attribute__((always_inline)) {      // what request() read of the rows, into the LDS
+    auto note = [&](RowInfo& info) __attribute__((always_inline)) {      // what request() read of the rows, into the LDS
         if (threadIdx.x < 64) {
-            RowInfo& info = infos[((r0 - rlo) >> 6) & 1];
             const float ls = !in || lreg == -INFINITY ? INFINITY : lreg;         // rows that see nothing: probabilities of 0
             info.lse[threadIdx.x] = KIND == PLAIN ? -ls * rsl2 : -ls;
             info.delta[threadIdx.x] = KIND == DROPPED ? dreg : -dreg;
@@ -143,17 +141,9 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
             if (KIND == DROPPED) info.drop[threadIdx.x] = hreg;
         }
     };
-    if (rlo < rhi) {
-        request(rlo);
-        note(rlo);
-    }
-    for (unsigned r0 = rlo; r0 < rhi; r0 += 64) {
-        tiles_landed();
-        const bool more = r0 + 64 < rhi;
-        if (more) request(r0 + 64);
-        const char *Qs = smem + (((r0 - rlo) >> 6) & 1) * 2 * TILE_BYTES<NO>, *Gs = Qs + TILE_BYTES<NO>;
-        const RowInfo& info = infos[((r0 - rlo) >> 6) & 1];
-        if (r0 < whi && r0 + 64 > wlo) {
+    auto visit = [&](const char* Qs, const RowInfo& info, unsigned r0) __attribute__((always_inline)) {
+        if (r0 >= whi || r0 + 64 <= wlo) return;
+        const char* Gs = Qs + TILE_BYTES<NO>;
         const int first = info.lo[lane], count = info.count[lane];
         const bool masked = __ballot(first > key0 || first + count < kmax) != 0;
         const bool before = KIND != PLAIN && __ballot(info.c[lane] < (float)(key0 + 31 - base)) == 0;
@@ -251,8 +241,22 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
                     dkT[db] = mfma(aq, dsf[st], dkT[db]);
                 }
         }
-        }
-        if (more) note(r0 + 64);
+    };
+    if (rlo < rhi) {
+        request(even, rlo);
+        note(infos[0]);
+    }
+    for (unsigned r0 = rlo; r0 < rhi; r0 += 128) {
+        tiles_landed();
+        const bool second = r0 + 64 < rhi, more = r0 + 128 < rhi;
+        if (second) request(odd, r0 + 64);
+        visit(even, infos[0], r0);
+        if (!second) break;
+        note(infos[1]);
+        tiles_landed();
+        if (more) request(even, r0 + 128);
+        visit(odd, infos[1], r0 + 64);
+        if (more) note(infos[0]);
     }
     if (key < p.Tk) {
         bf16_t *dk = p.dk + (size_t)key * p.lddk + (size_t)hk * p.D, *dv = p.dv + (size_t)key * p.lddv + (size_t)hk * p.D;

@@ -7,7 +7,7 @@ namespace {
 
 template <int ND, int NO, int KIND>
 __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocArgs p, int tiles) {
-    __shared__ __attribute__((aligned(16))) char smem[4 * TILE_BYTES<NO>];      // K and V, twice
+    __shared__ __attribute__((aligned(16))) char even[2 * TILE_BYTES<NO>], odd[2 * TILE_BYTES<NO>];      // K and V, twice
     __shared__ int range[4][2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
     int tile, hk;
@@ -76,17 +76,13 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     Fetch<NO, 4> kf, vf;
     kf.init(p.ldk, p.D);
     vf.init(p.ldv, p.D);
-    auto request = [&](int k0) __attribute__((always_inline)) {
-        char* to = smem + (((k0 - klo) >> 6) & 1) * 2 * TILE_BYTES<NO>;
+    auto request = [&](char* to, int k0) __attribute__((always_inline)) {
         kf.dma(to, kbase, p.ldk, p.D, k0, khi - k0);
         vf.dma(to + TILE_BYTES<NO>, vbase, p.ldv, p.D, k0, khi - k0);
     };
-    if (klo < khi) request(klo);
-    for (int k0 = klo; k0 < khi; k0 += 64) {
-        tiles_landed();
-        if (k0 + 64 < khi) request(k0 + 64);
-        const char *Ks = smem + (((k0 - klo) >> 6) & 1) * 2 * TILE_BYTES<NO>, *Vs = Ks + TILE_BYTES<NO>;
-        if (k0 >= hi || k0 + 64 <= lo) continue;
+    auto visit = [&](const char* Ks, int k0) __attribute__((always_inline)) {
+        const char* Vs = Ks + TILE_BYTES<NO>;
+        if (k0 >= hi || k0 + 64 <= lo) return;
         const bool masked = k0 < in_lo || k0 + 64 > in_hi;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -137,6 +133,16 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
 #pragma unroll
                 for (int db = 0; db < NO; ++db) dqT[db] = mfma(rd.frag_t(Ks, db, kb * 2 + st), dsf[st], dqT[db]);
         }
+    };
+    if (klo < khi) request(even, klo);
+    for (int k0 = klo; k0 < khi; k0 += 128) {
+        tiles_landed();
+        if (k0 + 64 < khi) request(odd, k0 + 64);
+        visit(even, k0);
+        if (k0 + 64 >= khi) break;
+        tiles_landed();
+        if (k0 + 128 < khi) request(even, k0 + 128);
+        visit(odd, k0 + 64);
     }
     if (live) {
         bf16_t* dq = p.dq + (size_t)token * p.lddq + (size_t)head * p.D;

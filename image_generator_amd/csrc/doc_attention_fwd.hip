@@ -148,7 +148,7 @@ struct Rows {                        // a wave's 32 rows
 
 template <int ND, int NO, int KIND>
 __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd_kernel(const DocArgs p, int tiles) {
-    __shared__ __attribute__((aligned(16))) char smem[4 * TILE_BYTES<NO>];      // K and V, twice: one tile arrives under the other
+    __shared__ __attribute__((aligned(16))) char even[2 * TILE_BYTES<NO>], odd[2 * TILE_BYTES<NO>];      // K and V, twice
     __shared__ int range[4][2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
     int tile, hk;
@@ -166,19 +166,24 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
     Fetch<NO, 4> kf, vf;
     kf.init(p.ldk, p.D);
     vf.init(p.ldv, p.D);
-    auto request = [&](int k0) __attribute__((always_inline)) {
-        char* to = smem + (((k0 - klo) >> 6) & 1) * 2 * TILE_BYTES<NO>;
+    auto request = [&](char* to, int k0) __attribute__((always_inline)) {
         kf.dma(to, kbase, p.ldk, p.D, k0, khi - k0);
         vf.dma(to + TILE_BYTES<NO>, vbase, p.ldv, p.D, k0, khi - k0);
     };
     auto pass = [&](auto fast) __attribute__((always_inline)) {
-        w.reset(decltype(fast)::value ? 0.f : -INFINITY);
-        if (klo < khi) request(klo);
-        for (int k0 = klo; k0 < khi; k0 += 64) {
-            tiles_landed();                        // ... and every wave has left the tile before
-            if (k0 + 64 < khi) request(k0 + 64);
-            const char* Ks = smem + (((k0 - klo) >> 6) & 1) * 2 * TILE_BYTES<NO>;
+        auto visit = [&](const char* Ks, int k0) __attribute__((always_inline)) {
             if (k0 < w.hi && k0 + 64 > w.lo) w.template tile<KIND, decltype(fast)::value>(p, bend, at, Ks, Ks + TILE_BYTES<NO>, k0);
+        };
+        w.reset(decltype(fast)::value ? 0.f : -INFINITY);
+        if (klo < khi) request(even, klo);
+        for (int k0 = klo; k0 < khi; k0 += 128) {
+            tiles_landed();                        // ... and every wave has left the tile before
+            if (k0 + 64 < khi) request(odd, k0 + 64);
+            visit(even, k0);
+            if (k0 + 64 >= khi) break;
+            tiles_landed();
+            if (k0 + 128 < khi) request(even, k0 + 128);
+            visit(odd, k0 + 64);
         }
         w.join();
     };

@@ -100,7 +100,10 @@ struct Fetch {
         for (int i = 0; i < N; ++i) *(bf16x8*)(tile + slot(i) * 16) = reg[i];
     }
 };
-// every request of this wave has landed, and every wave is here
+// Every request of this wave has landed, and every wave is here.
+// The buffers that take turns are LDS variables of their own, in code unrolled over them: the compiler, which keeps reads of the
+// LDS behind DMA writes that may alias, then sees that they do not.  With one array and an offset it waited for the next tile's
+// arrival before it read the present one (captions 434 -> 406 us, long documents 1440 -> 1333 us).
 __device__ __forceinline__ void tiles_landed() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
