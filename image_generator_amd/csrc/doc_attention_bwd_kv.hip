@@ -258,8 +258,8 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
         visit(odd, infos[1], r0 + 64);
         if (more) note(infos[0]);
     }
-    if (key < p.Tk) {
-        bf16_t *dk = p.dk + (size_t)key * p.lddk + (size_t)hk * p.D, *dv = p.dv + (size_t)key * p.lddv + (size_t)hk * p.D;
+    if (p.splits > 1) {
+        if (key >= p.Tk) return;
         float* part = p.part + (((size_t)split * p.Tk + key) * p.Hkv + hk) * 2 * p.D;
 #pragma unroll
         for (int db = 0; db < NO; ++db)
@@ -268,22 +268,14 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
                 const int d = db * 32 + 8 * g + 4 * hh;
                 if (d >= p.D) continue;
                 const f32x16 &a = dkT[db], &c = dvT[db];
-                if (p.splits > 1) {
-                    *(f32x4*)(part + d) = f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
-                    *(f32x4*)(part + p.D + d) = f32x4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
-                } else {
-                    bf16x4 x, y;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[e] = seen ? (bf16_t)(a[4 * g + e] * p.scale) : (bf16_t)0.f;
-                        y[e] = seen ? (bf16_t)c[4 * g + e] : (bf16_t)0.f;
-                    }
-                    *(bf16x4*)(dk + d) = x;
-                    *(bf16x4*)(dv + d) = y;
-                }
+                *(f32x4*)(part + d) = f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+                *(f32x4*)(part + p.D + d) = f32x4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
             }
+        return;
     }
-    if (p.splits > 1) return;
+    __syncthreads();
+    put_rows<NO>(even + wave * 32 * TILE_LD<NO>, dkT, p.scale, !seen, key < p.Tk ? p.dk + (size_t)key * p.lddk + (size_t)hk * p.D : nullptr, p.D);
+    put_rows<NO>(odd + wave * 32 * TILE_LD<NO>, dvT, 1.f, !seen, key < p.Tk ? p.dv + (size_t)key * p.lddv + (size_t)hk * p.D : nullptr, p.D);
     for (unsigned bad = bad_rows(seen && !(not_finite(dkT) + not_finite(dvT) == 0.f)); bad; bad &= bad - 1)
         plain_dkdv_key(p, key0 + __builtin_ctz(bad), hk);
 }

@@ -144,21 +144,8 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
         if (k0 + 128 < khi) request(even, k0 + 128);
         visit(odd, k0 + 64);
     }
-    if (live) {
-        bf16_t* dq = p.dq + (size_t)token * p.lddq + (size_t)head * p.D;
-#pragma unroll
-        for (int db = 0; db < NO; ++db)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int d = db * 32 + 8 * g + 4 * hh;
-                if (d < p.D) {
-                    bf16x4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = sees ? (bf16_t)(dqT[db][4 * g + e] * p.scale) : (bf16_t)0.f;
-                    *(bf16x4*)(dq + d) = v;
-                }
-            }
-    }
+    __syncthreads();
+    put_rows<NO>(even + wave * 32 * TILE_LD<NO>, dqT, p.scale, !sees, live ? p.dq + (size_t)token * p.lddq + (size_t)head * p.D : nullptr, p.D);
     for (unsigned bad = bad_rows(sees && !(not_finite(dqT) == 0.f)); bad; bad &= bad - 1) {
         const int t = __builtin_ctz(bad);
         const RowSpan s = {__shfl(span.lo, t, 64), __shfl(span.hi, t, 64), __shfl(span.c, t, 64)};

@@ -188,25 +188,14 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
         w.join();
     };
     pass(std::true_type{});
-    if (__syncthreads_or(!w.fits())) pass(std::false_type{});      // (the loop has barriers: the workgroup decides as one)
-    if (w.live) {
-        const float inv = w.l > 0.f ? 1.f / w.l : 0.f;
-        bf16_t* out = p.out + (size_t)w.token * p.ldo + (size_t)w.head * p.D;
-        const bool none = w.span.hi <= w.span.lo;
-#pragma unroll
-        for (int db = 0; db < NO; ++db)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int d = db * 32 + 8 * g + 4 * hh;
-                if (d < p.D) {
-                    bf16x4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = none ? (bf16_t)0.f : (bf16_t)(w.o[db][4 * g + e] * inv);
-                    *(bf16x4*)(out + d) = v;
-                }
-            }
-        if (hh == 0) p.lse[(size_t)w.head * p.Tq + w.token] = none ? -INFINITY : w.m + log2f(w.l);
+    if (__syncthreads_or(!w.fits())) {           // (the loop has barriers: the workgroup decides as one)
+        pass(std::false_type{});
+        __syncthreads();
     }
+    const bool none = w.span.hi <= w.span.lo;
+    put_rows<NO>(even + wave * 32 * TILE_LD<NO>, w.o, w.l > 0.f ? 1.f / w.l : 0.f, none,
+                 w.live ? p.out + (size_t)w.token * p.ldo + (size_t)w.head * p.D : nullptr, p.D);
+    if (w.live && hh == 0) p.lse[(size_t)w.head * p.Tq + w.token] = none ? -INFINITY : w.m + log2f(w.l);
     for (unsigned bad = w.bad(); bad; bad &= bad - 1) {
         const int t = __builtin_ctz(bad);
         const RowSpan s = {__shfl(w.span.lo, t, 64), __shfl(w.span.hi, t, 64), __shfl(w.span.c, t, 64)};

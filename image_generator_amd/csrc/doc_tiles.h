@@ -194,6 +194,33 @@ __device__ __forceinline__ f32x16 bias16(float slope2, float cf, float rest, boo
     return y;
 }
 
+// A wave's 32 rows of a result, a lane its row, out by way of the LDS (`own`: 32 * TILE_LD bytes of this wave's, that nobody
+// reads any more): 16-byte pieces, a row's side by side.  Straight from the registers a store would touch 16 bytes in each of
+// 32 rows, eight times the requests.  `to`: where the lane's row goes, nullptr: nowhere; `zero`: as zeros.
+template <int NO>
+__device__ __forceinline__ void put_rows(char* own, const f32x16 (&a)[NO], float scale, bool zero, bf16_t* to, int D) {
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int db = 0; db < NO; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            bf16x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = zero ? (bf16_t)0.f : (bf16_t)(a[db][4 * g + e] * scale);
+            *(bf16x4*)(own + l31 * TILE_LD<NO> + ((db * 4 + g) ^ swz<NO>(l31)) * 16 + hh * 8) = v;
+        }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // one wave: its LDS operations complete in order
+    const unsigned lo = (unsigned)(uintptr_t)to, hi = (unsigned)((uintptr_t)to >> 32);
+#pragma unroll
+    for (int i = 0; i < 2 * NO; ++i) {
+        const int s = i * 64 + lane, r = s / (NO * 4), c = s - r * (NO * 4);
+        const bf16x8 v = *(const bf16x8*)(own + r * TILE_LD<NO> + (c ^ swz<NO>(r)) * 16);
+        bf16_t* row = (bf16_t*)((uintptr_t)(unsigned)__shfl((int)hi, r, 64) << 32 | (unsigned)__shfl((int)lo, r, 64));
+        if (row && c * 8 < D) *(bf16x8*)(row + c * 8) = v;
+    }
+}
+
 // NaN if any register is not finite, else 0
 template <int NO>
 __device__ __forceinline__ float not_finite(const f32x16 (&a)[NO]) {
