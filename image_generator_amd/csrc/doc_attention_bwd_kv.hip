@@ -60,22 +60,14 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
     if (!unit_of(tiles * p.splits, p.Hkv, unit, hk)) return;
     const int split = unit / tiles, tile = unit - split * tiles;
     const int base = tile * 128, key0 = base + wave * 32, key = key0 + l31;
-    const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
     bf16x8 kf[ND], vf[ND];
     const int mine = min(key, p.Tk - 1);
-#pragma unroll
-    for (int ks = 0; ks < ND; ++ks) {                 // on their way while the keys' rows are looked up
-        const int d = ks * 16 + 8 * hh;
-        kf[ks] = d < p.D ? *(const bf16x8*)(k_row(p, mine, hk) + d) : zero8;
-        vf[ks] = d < p.D ? *(const bf16x8*)(v_row(p, mine, hk) + d) : zero8;
-    }
+    load_row(kf, k_row(p, mine, hk), p.D);            // on their way while the keys' rows are looked up
+    load_row(vf, v_row(p, mine, hk), p.D);
     const int2 span = key_span_in(p, mine, doc_of_wave(p.k_off, p.docs, p.Tk, __builtin_amdgcn_readfirstlane(mine), __builtin_amdgcn_readlane(mine, 31), mine));
     const bool seen = key < p.Tk && span.y > span.x;
-#pragma unroll
-    for (int ks = 0; ks < ND; ++ks) {
-        kf[ks] = seen ? kf[ks] : zero8;
-        vf[ks] = seen ? vf[ks] : zero8;
-    }
+    keep_row(kf, seen, p.D);
+    keep_row(vf, seen, p.D);
     int lo = seen ? span.x : 0x7fffffff, hi = seen ? span.y : 0;
     lo = wave_min_i(lo);
     hi = wave_max_i(hi);

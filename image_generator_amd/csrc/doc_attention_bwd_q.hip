@@ -17,21 +17,15 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     const bool live = R < rows;
     int token, head;
     row_of(p, live ? R : rows - 1, hk, token, head);
-    const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
     bf16x8 qf[ND], gf[ND];
     float delta = 0.f;
     {   // on their way while the intervals are looked up
-        const bf16_t* q = q_row(p, token, head);
-        const bf16_t* g = p.dout + (size_t)token * p.lddo + (size_t)head * p.D;
-        const bf16_t* o = p.o + (size_t)token * p.ldo + (size_t)head * p.D;
         bf16x8 ov[ND];
-#pragma unroll
-        for (int ks = 0; ks < ND; ++ks) {
-            const int d = ks * 16 + 8 * hh;
-            qf[ks] = d < p.D ? *(const bf16x8*)(q + d) : zero8;
-            gf[ks] = d < p.D ? *(const bf16x8*)(g + d) : zero8;
-            ov[ks] = d < p.D ? *(const bf16x8*)(o + d) : zero8;
-        }
+        load_row(gf, p.dout + (size_t)token * p.lddo + (size_t)head * p.D, p.D);
+        load_row(ov, p.o + (size_t)token * p.ldo + (size_t)head * p.D, p.D);
+        load_row(qf, q_row(p, token, head), p.D);
+        keep_row(gf, true, p.D);
+        keep_row(ov, true, p.D);
 #pragma unroll
         for (int ks = 0; ks < ND; ++ks)
 #pragma unroll
@@ -48,11 +42,8 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     const int in_hi = wave_min_i(sees ? span.hi : 0x7fffffff);
     const int c_min = wave_min_i(sees ? span.c : 0x7fffffff);
     if (!sees) delta = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < ND; ++ks) {
-        qf[ks] = sees ? qf[ks] : zero8;
-        gf[ks] = sees ? gf[ks] : zero8;
-    }
+    keep_row(qf, sees, p.D);
+    keep_row(gf, sees, p.D);
     const size_t at = (size_t)head * p.Tq + token;
     if (live && hh == 0) p.delta[at] = delta;
     const float lse_raw = sees ? p.lse[at] : -INFINITY;

@@ -26,17 +26,10 @@ struct Rows {                        // a wave's 32 rows
 
     // R0: the wave's first row
     __device__ __forceinline__ void init(const DocArgs& p, unsigned R0, int hk) {
-        const int hh = (threadIdx.x & 63) >> 5;
         const unsigned rows = (unsigned)p.Tq * (unsigned)p.G, R = R0 + (threadIdx.x & 31);
         live = R < rows;
         row_of(p, live ? R : rows - 1, hk, token, head);
-        const bf16_t* q = q_row(p, token, head);
-        const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-        for (int ks = 0; ks < ND; ++ks) {             // on their way while the intervals are looked up
-            const int d = ks * 16 + 8 * hh;
-            qf[ks] = d < p.D ? *(const bf16x8*)(q + d) : zero8;
-        }
+        load_row(qf, q_row(p, token, head), p.D);     // on its way while the intervals are looked up
         span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, p.Tq, __builtin_amdgcn_readfirstlane(token), __builtin_amdgcn_readlane(token, 31), token));
         if (!live) span.lo = span.hi = 0;
         const bool sees = span.hi > span.lo;
@@ -47,8 +40,7 @@ struct Rows {                        // a wave's 32 rows
         in_hi = wave_min_i(sees ? span.hi : 0x7fffffff);
         if (lo > hi) lo = hi = 0;
         c_min = wave_min_i(sees ? span.c : 0x7fffffff);
-#pragma unroll
-        for (int ks = 0; ks < ND; ++ks) qf[ks] = sees ? qf[ks] : zero8;
+        keep_row(qf, sees, p.D);
         slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;
         drop = drop_row(p, token, head);
     }

@@ -48,6 +48,26 @@ struct Reads {
     }
 };
 
+// A lane's row as the right operand of ND steps: 16-byte pieces at columns 16 ks + 8 (lane >> 5), zeros past D.  One tensor at a time
+// and without branches: the pieces of a 128-byte line are asked for in a row, while it is in the first-level cache.  (Three tensors
+// taken in turn were four times the requests to the second-level cache.)
+template <int ND>
+__device__ __forceinline__ void load_row(bf16x8 (&f)[ND], const bf16_t* row, int D) {
+    const int hh = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int ks = 0; ks < ND; ++ks) {
+        const int d = ks * 16 + 8 * hh;
+        f[ks] = *(const bf16x8*)(row + (d < D ? d : 0));
+    }
+}
+template <int ND>
+__device__ __forceinline__ void keep_row(bf16x8 (&f)[ND], bool keep, int D) {
+    const int hh = (threadIdx.x & 63) >> 5;
+    const bf16x8 zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < ND; ++ks) f[ks] = keep && ks * 16 + 8 * hh < D ? f[ks] : zero8;
+}
+
 // the row of a result register
 __device__ __forceinline__ constexpr int reg_row(int r) { return (r & 3) + 8 * (r >> 2); }
 
