@@ -58,10 +58,16 @@ __device__ __forceinline__ Doc doc_at(const int* __restrict__ off, int docs, int
 // chain of loads, a third of a caption tile's time; here the 64 offsets around the place where documents of equal length would
 // have this one are loaded at once and usually hold it - if not, a search that probes 64 places a step says where they are -
 // and the lanes take their documents from those registers.
-__device__ __forceinline__ Doc doc_of_wave(const int* __restrict__ off, int docs, int total, int i0, int i1, int i) {
+// Loads return in order: the window is asked for before the rows' own operands, behind which it would wait (OffWindow).
+struct OffWindow { int w, val; };        // first offset; the lane's
+__device__ __forceinline__ OffWindow off_window(const int* __restrict__ off, int docs, int total, int i0) {
+    const int w = max(0, (int)((float)i0 * (float)docs / (float)total) - 24), at = w + (int)(threadIdx.x & 63);
+    return {w, off[min(at, docs)]};
+}
+__device__ __forceinline__ Doc doc_of_wave(const int* __restrict__ off, int docs, const OffWindow& window, int i0, int i1, int i) {
     const int lane = threadIdx.x & 63;
-    int w = max(0, (int)((float)i0 * (float)docs / (float)total) - 24);       // first offset of the window
-    int val = w + lane <= docs ? off[w + lane] : 0x7fffffff;
+    int w = window.w;
+    int val = w + lane <= docs ? window.val : 0x7fffffff;
     int k = __popcll(__ballot(val <= i0));                                      // offsets of the window up to i0
     if ((k == 0 && w > 0) || k == 64) {
         int a = 0, b = docs;

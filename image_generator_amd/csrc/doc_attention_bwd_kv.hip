@@ -62,9 +62,11 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
     const int base = tile * 128, key0 = base + wave * 32, key = key0 + l31;
     bf16x8 kf[ND], vf[ND];
     const int mine = min(key, p.Tk - 1);
+    const int first_key = __builtin_amdgcn_readfirstlane(mine);
+    const OffWindow window = off_window(p.k_off, p.docs, p.Tk, first_key);
     load_row(kf, k_row(p, mine, hk), p.D);            // on their way while the keys' rows are looked up
     load_row(vf, v_row(p, mine, hk), p.D);
-    const int2 span = key_span_in(p, mine, doc_of_wave(p.k_off, p.docs, p.Tk, __builtin_amdgcn_readfirstlane(mine), __builtin_amdgcn_readlane(mine, 31), mine));
+    const int2 span = key_span_in(p, mine, doc_of_wave(p.k_off, p.docs, window, first_key, __builtin_amdgcn_readlane(mine, 31), mine));
     const bool seen = key < p.Tk && span.y > span.x;
     keep_row(kf, seen, p.D);
     keep_row(vf, seen, p.D);

@@ -17,22 +17,14 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     const bool live = R < rows;
     int token, head;
     row_of(p, live ? R : rows - 1, hk, token, head);
+    const int first = __builtin_amdgcn_readfirstlane(token);
+    const OffWindow window = off_window(p.q_off, p.docs, p.Tq, first);
     bf16x8 qf[ND], gf[ND];
-    float delta = 0.f;
-    {   // on their way while the intervals are looked up
-        bf16x8 ov[ND];
-        load_row(gf, p.dout + (size_t)token * p.lddo + (size_t)head * p.D, p.D);
-        load_row(ov, p.o + (size_t)token * p.ldo + (size_t)head * p.D, p.D);
-        load_row(qf, q_row(p, token, head), p.D);
-        keep_row(gf, true, p.D);
-        keep_row(ov, true, p.D);
-#pragma unroll
-        for (int ks = 0; ks < ND; ++ks)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) delta = fmaf((float)ov[ks][e], (float)gf[ks][e], delta);
-        delta += __shfl_xor(delta, 32, 64);
-    }
-    RowSpan span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, p.Tq, __builtin_amdgcn_readfirstlane(token), __builtin_amdgcn_readlane(token, 31), token));
+    bf16x8 ov[ND];                               // on their way while the intervals are looked up
+    load_row(gf, p.dout + (size_t)token * p.lddo + (size_t)head * p.D, p.D);
+    load_row(ov, p.o + (size_t)token * p.ldo + (size_t)head * p.D, p.D);
+    load_row(qf, q_row(p, token, head), p.D);
+    RowSpan span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, window, first, __builtin_amdgcn_readlane(token, 31), token));
     if (live && hh == 0 && head == 0) p.rows[token] = make_int4(span.lo, span.hi, span.c, 0);
     if (!live) span.lo = span.hi = 0;
     const bool sees = span.hi > span.lo;
@@ -41,9 +33,15 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     const int in_lo = wave_max_i(sees ? span.lo : 0);
     const int in_hi = wave_min_i(sees ? span.hi : 0x7fffffff);
     const int c_min = wave_min_i(sees ? span.c : 0x7fffffff);
-    if (!sees) delta = 0.f;
-    keep_row(qf, sees, p.D);
     keep_row(gf, sees, p.D);
+    keep_row(ov, sees, p.D);
+    float delta = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < ND; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf((float)ov[ks][e], (float)gf[ks][e], delta);
+    delta += __shfl_xor(delta, 32, 64);
+    keep_row(qf, sees, p.D);
     const size_t at = (size_t)head * p.Tq + token;
     if (live && hh == 0) p.delta[at] = delta;
     const float lse_raw = sees ? p.lse[at] : -INFINITY;

@@ -29,8 +29,10 @@ struct Rows {                        // a wave's 32 rows
         const unsigned rows = (unsigned)p.Tq * (unsigned)p.G, R = R0 + (threadIdx.x & 31);
         live = R < rows;
         row_of(p, live ? R : rows - 1, hk, token, head);
+        const int first = __builtin_amdgcn_readfirstlane(token);
+        const OffWindow window = off_window(p.q_off, p.docs, p.Tq, first);
         load_row(qf, q_row(p, token, head), p.D);     // on its way while the intervals are looked up
-        span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, p.Tq, __builtin_amdgcn_readfirstlane(token), __builtin_amdgcn_readlane(token, 31), token));
+        span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, window, first, __builtin_amdgcn_readlane(token, 31), token));
         if (!live) span.lo = span.hi = 0;
         const bool sees = span.hi > span.lo;
         lo = wave_min_i(sees ? span.lo : 0x7fffffff);
