@@ -68,8 +68,6 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
     load_row(vf, v_row(p, mine, hk), p.D);
     const int2 span = key_span_in(p, mine, doc_of_wave(p.k_off, p.docs, window, first_key, __builtin_amdgcn_readlane(mine, 31), mine));
     const bool seen = key < p.Tk && span.y > span.x;
-    keep_row(kf, seen, p.D);
-    keep_row(vf, seen, p.D);
     int lo = seen ? span.x : 0x7fffffff, hi = seen ? span.y : 0;
     lo = wave_min_i(lo);
     hi = wave_max_i(hi);
@@ -240,6 +238,8 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
         request(even, rlo);
         note(infos[0]);
     }
+    keep_row(kf, seen, p.D);
+    keep_row(vf, seen, p.D);
     for (unsigned r0 = rlo; r0 < rhi; r0 += 128) {
         tiles_landed();
         const bool second = r0 + 64 < rhi, more = r0 + 128 < rhi;

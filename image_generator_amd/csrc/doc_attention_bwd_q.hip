@@ -19,6 +19,8 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     row_of(p, live ? R : rows - 1, hk, token, head);
     const int first = __builtin_amdgcn_readfirstlane(token);
     const OffWindow window = off_window(p.q_off, p.docs, p.Tq, first);
+    const size_t at = (size_t)head * p.Tq + token;
+    const float lse_at = p.lse[at], slope = p.slopes ? p.slopes[head] : 0.f;
     bf16x8 qf[ND], gf[ND];
     bf16x8 ov[ND];                               // on their way while the intervals are looked up
     load_row(gf, p.dout + (size_t)token * p.lddo + (size_t)head * p.D, p.D);
@@ -33,6 +35,19 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     const int in_lo = wave_max_i(sees ? span.lo : 0);
     const int in_hi = wave_min_i(sees ? span.hi : 0x7fffffff);
     const int c_min = wave_min_i(sees ? span.c : 0x7fffffff);
+    if (lane == 0) { range[wave][0] = lo; range[wave][1] = hi; }
+    __syncthreads();
+    const int klo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
+    const int khi = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
+    const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
+    Fetch<NO, 4> kf, vf;
+    kf.init(p.ldk, p.D);
+    vf.init(p.ldv, p.D);
+    auto request = [&](char* to, int k0) __attribute__((always_inline)) {
+        kf.dma(to, kbase, p.ldk, p.D, k0, khi - k0);
+        vf.dma(to + TILE_BYTES<NO>, vbase, p.ldv, p.D, k0, khi - k0);
+    };
+    if (klo < khi) request(even, klo);
     keep_row(gf, sees, p.D);
     keep_row(ov, sees, p.D);
     float delta = 0.f;
@@ -42,33 +57,19 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
         for (int e = 0; e < 8; ++e) delta = fmaf((float)ov[ks][e], (float)gf[ks][e], delta);
     delta += __shfl_xor(delta, 32, 64);
     keep_row(qf, sees, p.D);
-    const size_t at = (size_t)head * p.Tq + token;
     if (live && hh == 0) p.delta[at] = delta;
-    const float lse_raw = sees ? p.lse[at] : -INFINITY;
+    const float lse_raw = sees ? lse_at : -INFINITY;
     const float lse = lse_raw == -INFINITY ? INFINITY : lse_raw;      // nothing seen: probabilities of 0
-    const float slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;
+    const float slope2 = slope * LOG2E;
     const unsigned drop = drop_row(p, token, head);
     const Bend bend(p);
     const float s0 = KIND == PLAIN ? -lse / bend.scale2 : 0.f;
-
-    if (lane == 0) { range[wave][0] = lo; range[wave][1] = hi; }
-    __syncthreads();
-    const int klo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
-    const int khi = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
+    const Reads<ND, NO> rd;
     f32x16 dqT[NO];
 #pragma unroll
     for (int i = 0; i < NO; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dqT[i][r] = 0.f;
-    const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
-    const Reads<ND, NO> rd;
-    Fetch<NO, 4> kf, vf;
-    kf.init(p.ldk, p.D);
-    vf.init(p.ldv, p.D);
-    auto request = [&](char* to, int k0) __attribute__((always_inline)) {
-        kf.dma(to, kbase, p.ldk, p.D, k0, khi - k0);
-        vf.dma(to + TILE_BYTES<NO>, vbase, p.ldv, p.D, k0, khi - k0);
-    };
     auto visit = [&](const char* Ks, int k0) __attribute__((always_inline)) {
         const char* Vs = Ks + TILE_BYTES<NO>;
         if (k0 >= hi || k0 + 64 <= lo) return;
@@ -123,7 +124,6 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
                 for (int db = 0; db < NO; ++db) dqT[db] = mfma(rd.frag_t(Ks, db, kb * 2 + st), dsf[st], dqT[db]);
         }
     };
-    if (klo < khi) request(even, klo);
     for (int k0 = klo; k0 < khi; k0 += 128) {
         tiles_landed();
         if (k0 + 64 < khi) request(odd, k0 + 64);

@@ -42,10 +42,11 @@ struct Rows {                        // a wave's 32 rows
         in_hi = wave_min_i(sees ? span.hi : 0x7fffffff);
         if (lo > hi) lo = hi = 0;
         c_min = wave_min_i(sees ? span.c : 0x7fffffff);
-        keep_row(qf, sees, p.D);
         slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;
         drop = drop_row(p, token, head);
     }
+    // the rest of it, which waits for the rows: once the first keys are on their way
+    __device__ __forceinline__ void settle(const DocArgs& p) { keep_row(qf, span.hi > span.lo, p.D); }
 
     // One staged tile of keys k0 .. k0 + 63.  FAST: no running maximum, p = 2^x against the fixed reference 0.  Floating point
     // does not mind the common factor while nothing leaves the normal range, and bf16 probabilities have fp32's exponents; a
@@ -170,6 +171,7 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
         };
         w.reset(decltype(fast)::value ? 0.f : -INFINITY);
         if (klo < khi) request(even, klo);
+        if constexpr (decltype(fast)::value) w.settle(p);
         for (int k0 = klo; k0 < khi; k0 += 128) {
             tiles_landed();                        // ... and every wave has left the tile before
             if (k0 + 64 < khi) request(odd, k0 + 64);
@@ -224,6 +226,7 @@ __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) 
     kf.init(p.ldk, p.D);
     vf.init(p.ldv, p.D);
     w.reset(-INFINITY);
+    w.settle(p);
     {   // (with the running maximum: what bounds this loop is memory, and a distance bias makes far runs tiny)
         if (from < to) {
             kf.load(kreg, kbase, p.ldk, p.D, from, to - from);
