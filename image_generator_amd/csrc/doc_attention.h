@@ -266,14 +266,6 @@ __device__ inline void plain_dq_row(const DocArgs& p, int i, int head, const Row
     for (int u = 0; u < 2; ++u) if (lane + 64 * u < p.D) dq[lane + 64 * u] = (bf16_t)(acc[u] * p.scale);
 }
 
-// delta = sum of dO o over a row
-__device__ inline float plain_delta(const DocArgs& p, int i, int head) {
-    const bf16_t *a = p.o + (size_t)i * p.ldo + (size_t)head * p.D, *b = p.dout + (size_t)i * p.lddo + (size_t)head * p.D;
-    float t = 0.f;
-    for (int d = threadIdx.x & 63; d < p.D; d += 64) t = fmaf((float)a[d], (float)b[d], t);
-    return wave_sum(t);
-}
-
 // dK and dV of one key of one key head, every query head of its group
 __device__ inline void plain_dkdv_key(const DocArgs& p, int j, int hk) {
     const int lane = threadIdx.x & 63;

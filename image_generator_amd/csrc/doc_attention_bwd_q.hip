@@ -1,14 +1,25 @@
 // Document attention, dQ, on the matrix units: a lane owns its row as in the forward pass, S^T = K Q^T and dP^T = V dO^T give
-// dS^T in the layout that dQ^T += K^T dS^T takes.  delta = sum dO o of a row, and the row's interval, are left for the dK / dV
-// pass.
+// dS^T in the layout that dQ^T += K^T dS^T takes.  delta and the interval of a row are left for the dK / dV pass.
+//
+// dS is rounded to bf16 (the matrix units' type): 2^-9 of each entry at most beside the result's own rounding, 0.24 % instead of
+// 0.17 % in the 2-norm; -lse and -delta start the accumulators, in fp32.
+//
+// Measured, with what bounds it: 58 254 caption tokens, 8 heads of 96 (537 MB): 149 us, 3.6 TB/s, bound by the chain of a short
+// workgroup (offsets, rows, keys, three tiles, store) at two workgroups per CU.  Four documents of 4001 .. 8191 tokens, 8 heads on 2
+// of 64, causal with prefix, cap and bias (223 GFLOP): 409 us, 545 TFLOP/s, bound by vector issue (80 % of the cycles: tanh, bias,
+// exp2 and the conversions of a score against three products).  32768 image rows over 328 keys, 8 heads of 40: 34 us, 2.5 TB/s.
 #include "doc_tiles.h"
 
 namespace {
 
+constexpr int FEW = 32;              // keys of a row whose delta is summed over them
+
 template <int ND, int NO, int KIND>
 __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocArgs p, int tiles) {
-    __shared__ __attribute__((aligned(16))) char even[2 * TILE_BYTES<NO>], odd[2 * TILE_BYTES<NO>];      // K and V, twice
-    __shared__ int range[4][2];
+    // three: captions' tiles stay in place for both walks; of the widest heads they would leave one workgroup to a CU
+    constexpr int BUFS = NO <= 3 && KIND == PLAIN ? 3 : 2;
+    __shared__ __attribute__((aligned(16))) char ring0[2 * TILE_BYTES<NO>], ring1[2 * TILE_BYTES<NO>], ring2[BUFS == 3 ? 2 * TILE_BYTES<NO> : 16];
+    __shared__ __attribute__((aligned(16))) int range[4][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
     int tile, hk;
     if (!unit_of(tiles, p.Hkv, tile, hk)) return;
@@ -35,10 +46,13 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     const int in_lo = wave_max_i(sees ? span.lo : 0);
     const int in_hi = wave_min_i(sees ? span.hi : 0x7fffffff);
     const int c_min = wave_min_i(sees ? span.c : 0x7fffffff);
-    if (lane == 0) { range[wave][0] = lo; range[wave][1] = hi; }
+    const bool few = sees && span.hi - span.lo <= FEW;
+    const int few_lo = wave_min_i(few ? span.lo : 0x7fffffff), few_hi = wave_max_i(few ? span.hi : 0);
+    if (lane == 0) *(int4*)range[wave] = make_int4(lo, hi, few_lo, few_hi);
     __syncthreads();
-    const int klo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
-    const int khi = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
+    auto least = [&](int i) { return min(min(range[0][i], range[1][i]), min(range[2][i], range[3][i])); };
+    auto most = [&](int i) { return max(max(range[0][i], range[1][i]), max(range[2][i], range[3][i])); };
+    const int klo = least(0), khi = most(1), flo = least(2), fhi = most(3);
     const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
     Fetch<NO, 4> kf, vf;
     kf.init(p.ldk, p.D);
@@ -47,7 +61,15 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
         kf.dma(to, kbase, p.ldk, p.D, k0, khi - k0);
         vf.dma(to + TILE_BYTES<NO>, vbase, p.ldv, p.D, k0, khi - k0);
     };
-    if (klo < khi) request(even, klo);
+    // up to BUFS tiles stay where they are; of more, all but one buffer are filled ahead
+    const bool resident = klo >= khi || khi - klo <= BUFS * 64;
+    auto start = [&](int from, int to) __attribute__((always_inline)) {
+        if (from >= to) return;                  // (rows that see nothing leave `from` at the largest int)
+        request(ring0, from);
+        if ((BUFS == 3 || resident) && from + 64 < to) request(ring1, from + 64);
+        if (BUFS == 3 && resident && from + 128 < to) request(ring2, from + 128);
+    };
+    start(klo, khi);
     keep_row(gf, sees, p.D);
     keep_row(ov, sees, p.D);
     float delta = 0.f;
@@ -57,7 +79,6 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
         for (int e = 0; e < 8; ++e) delta = fmaf((float)ov[ks][e], (float)gf[ks][e], delta);
     delta += __shfl_xor(delta, 32, 64);
     keep_row(qf, sees, p.D);
-    if (live && hh == 0) p.delta[at] = delta;
     const float lse_raw = sees ? lse_at : -INFINITY;
     const float lse = lse_raw == -INFINITY ? INFINITY : lse_raw;      // nothing seen: probabilities of 0
     const float slope2 = slope * LOG2E;
@@ -65,14 +86,70 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     const Bend bend(p);
     const float s0 = KIND == PLAIN ? -lse / bend.scale2 : 0.f;
     const Reads<ND, NO> rd;
+    auto each_tile = [&](int from, int to, int wave_lo, int wave_hi, auto visit) __attribute__((always_inline)) {
+        auto step = [&](const char* now, char* free, int k0) __attribute__((always_inline)) {
+            if (!resident) {
+                tile_landed<(BUFS - 2) * 2 * kf.N>(k0 + 64 < to);
+                if (k0 + (BUFS - 1) * 64 < to) request(free, k0 + (BUFS - 1) * 64);
+            }
+            if (k0 < wave_hi && k0 + 64 > wave_lo) visit(now, k0);
+        };
+        for (int k0 = from; k0 < to; k0 += BUFS * 64) {
+            step(ring0, BUFS == 3 ? ring2 : ring1, k0);
+            if (k0 + 64 < to) step(ring1, ring0, k0 + 64);
+            if constexpr (BUFS == 3) if (k0 + 128 < to) step(ring2, ring1, k0 + 128);
+        }
+    };
+    // delta = sum dO o of the result as it was handed out carries its rounding, some 2^-9 of |dO| |o|.  Over many keys that is lost
+    // in dP - delta; over few it is not (gradients 1.2 % off in the 2-norm with two keys, 0.25 % with 32, where the rounding of dS is
+    // what counts), so rows of few keys take the sum over their keys instead, delta = sum P dP, in a walk of its own over the tiles
+    // that such rows see: captions 128 -> 149 us, where the tiles are still in place, long documents nothing.
+    if (resident) tiles_landed();
+    if (flo < fhi) {
+        float sum = 0.f;
+        if (!resident) {
+            tiles_landed();
+            start(flo, fhi);
+        }
+        each_tile(resident ? klo : flo, resident ? khi : fhi, few_lo, few_hi, [&](const char* Ks, int k0) __attribute__((always_inline)) {
+            const char* Vs = Ks + TILE_BYTES<NO>;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                f32x16 s, dp;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) { s[r] = s0; dp[r] = 0.f; }
+#pragma unroll
+                for (int ks = 0; ks < ND; ++ks) {
+                    s = mfma(rd.frag(Ks, ks, kb), qf[ks], s);
+                    dp = mfma(rd.frag(Vs, ks, kb), gf[ks], dp);
+                }
+                const f32x16 y = KIND != PLAIN && bend.biased ? bias16(slope2, (float)(span.c - k0 - kb * 32 - 4 * hh), -lse, false) : f32x16{} - lse;
+                if (KIND != PLAIN) bend.score16(s, y);
+                const unsigned rel = (unsigned)(k0 + kb * 32 + 4 * hh - span.lo), len = (unsigned)(span.hi - span.lo);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float d = dp[r];
+                    if constexpr (KIND == DROPPED) d = drop_keep(p, drop, k0 + kb * 32 + reg_row(r) + 4 * hh) ? d * p.drop_scale : 0.f;
+                    const float w = EXP2(KIND == PLAIN ? s[r] * bend.scale2 : s[r]);
+                    sum = rel + (unsigned)reg_row(r) < len ? fmaf(w, d, sum) : sum;
+                }
+            }
+        });
+        sum += __shfl_xor(sum, 32, 64);
+        if (few) delta = sum;
+        if (!resident) {
+            __syncthreads();
+            start(klo, khi);
+        }
+    }
+    if (live && hh == 0) p.delta[at] = delta;
     f32x16 dqT[NO];
 #pragma unroll
     for (int i = 0; i < NO; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dqT[i][r] = 0.f;
-    auto visit = [&](const char* Ks, int k0) __attribute__((always_inline)) {
+    each_tile(klo, khi, lo, hi, [&](const char* Ks, int k0) __attribute__((always_inline)) {
         const char* Vs = Ks + TILE_BYTES<NO>;
-        if (k0 >= hi || k0 + 64 <= lo) return;
         const bool masked = k0 < in_lo || k0 + 64 > in_hi;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -123,18 +200,9 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
 #pragma unroll
                 for (int db = 0; db < NO; ++db) dqT[db] = mfma(rd.frag_t(Ks, db, kb * 2 + st), dsf[st], dqT[db]);
         }
-    };
-    for (int k0 = klo; k0 < khi; k0 += 128) {
-        tiles_landed();
-        if (k0 + 64 < khi) request(odd, k0 + 64);
-        visit(even, k0);
-        if (k0 + 64 >= khi) break;
-        tiles_landed();
-        if (k0 + 128 < khi) request(even, k0 + 128);
-        visit(odd, k0 + 64);
-    }
+    });
     __syncthreads();
-    put_rows<NO>(even + wave * 32 * TILE_LD<NO>, dqT, p.scale, !sees, live ? p.dq + (size_t)token * p.lddq + (size_t)head * p.D : nullptr, p.D);
+    put_rows<NO>(ring0 + wave * 32 * TILE_LD<NO>, dqT, p.scale, !sees, live ? p.dq + (size_t)token * p.lddq + (size_t)head * p.D : nullptr, p.D);
     for (unsigned bad = bad_rows(sees && !(not_finite(dqT) == 0.f)); bad; bad &= bad - 1) {
         const int t = __builtin_ctz(bad);
         const RowSpan s = {__shfl(span.lo, t, 64), __shfl(span.hi, t, 64), __shfl(span.c, t, 64)};

@@ -129,6 +129,14 @@ __device__ __forceinline__ void tiles_landed() {
     __syncthreads();
 }
 
+// the same for all but the last N requests, if there are any behind the one waited for
+template <int N>
+__device__ __forceinline__ void tile_landed(bool more) {
+    if (N > 0 && more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // Reductions over a wave by DPP: within rows of 16 lanes, then across them; lane 63 holds the result.  (By way of the LDS, as
 // __shfl_xor goes, the five of a tile were a chain of 3000 cycles.)
 template <int CTRL, int ROWS>

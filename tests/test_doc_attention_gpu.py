@@ -460,3 +460,39 @@ def test_places_that_are_refused():
         ops.doc_attention(q, None, v, heads=2, q_offsets=off)
     for n, t in zip(("dq", "dk", "dv"), ops.doc_attention_bwd(out, q, q, q, out, lse, 2, off)):       # one tensor in several places is read only
         assert torch.isfinite(t).all(), n
+
+
+@pytest.mark.parametrize("lens", [[2, 3, 1, 32, 7, 16, 2], [2, 300, 2, 1], [1] * 9])
+@pytest.mark.parametrize("d,cap", [(64, 0.0), (40, 5.0), (128, 0.0)])
+def test_gradients_of_few_keys_do_not_carry_the_rounding_of_the_result(lens, d, cap):
+    """Values that differ by little beside their size: delta = sum dO o of the bf16 result would be off by 2^-8 sum |dO| |o|, far more
+    than dP - delta.  Rows of at most 32 keys sum P dP instead:  |d delta| <= sum_j P (D u sum |dO v| + r |dP|)  and, as above,
+    tol_dS = P (|d delta| + D u sum |dO v| + 2^-19 |dP - delta|) + (2^-8 + r) |dS|."""
+    off = offsets(lens)
+    T = int(off[-1])
+    q, k, v, do = inputs(T, T, 1, 1, d, 34)
+    v = (v.float() * 0.25 + 100).to(BF)
+    got = run(q, k, v, do, heads=1, q_offsets=off, cap=cap)
+    for n, size in enumerate(lens):
+        if size > 32:
+            continue
+        rows = slice(int(off[n]), int(off[n + 1]))
+        Q, K, V, G = (t[rows].double() for t in (q, k, v, do))
+        scale = d ** -0.5
+        t = Q @ K.T * scale
+        e = (d + 4) * U * scale * (Q.abs() @ K.abs().T) + 2.0 ** -20 * cap + 4 * U * t.abs()
+        bend = torch.ones_like(t)
+        if cap:
+            bend = 1 - torch.tanh(t / cap) ** 2
+            t = cap * torch.tanh(t / cap)
+        P = torch.softmax(t, 1)
+        r = e + (P * e).sum(1, keepdim=True) + 2.0 ** -20
+        dP = G @ V.T
+        rough = d * U * (G.abs() @ V.abs().T)
+        delta = (P * dP).sum(1, keepdim=True)
+        ddelta = (P * (rough + r * dP.abs())).sum(1, keepdim=True)
+        dS = P * (dP - delta) * bend
+        tol = P * (ddelta + rough + 2.0 ** -19 * (dP - delta).abs()) + (2.0 ** -8 + r) * dS.abs()
+        for name, want, bound in (("dq", scale * dS @ K, scale * tol @ K.abs()), ("dk", scale * dS.T @ Q, scale * tol.T @ Q.abs())):
+            x = got[name][rows].cpu().double()
+            assert ((x - want).abs() <= 1.05 * (bound + 2.0 ** -8 * want.abs()) + 1e-30).all(), (name, n, float((x - want).abs().max()), float(want.abs().max()))
