@@ -4,10 +4,10 @@
 //
 // P and dS are rounded to bf16 for their products, as in the other passes; sums over rows and heads are fp32.
 //
-// Measured, with what bounds it: 58 254 caption tokens, 8 heads of 96 (537 MB): 160 us, 3.4 TB/s, a chain per workgroup as in the
+// Measured, with what bounds it: 58 255 caption tokens, 8 heads of 96 (537 MB): 160 us, 3.4 TB/s, a chain per workgroup as in the
 // dQ pass with four products instead of three.  Four documents of 4001 .. 8191 tokens, 8 heads on 2 of 64, causal with prefix, cap and
 // bias (298 GFLOP): 673 us, 443 TFLOP/s: 229 registers leave two waves per SIMD, whose scores and products follow each other
-// (vector issue 57 %, matrix units 25 % of the cycles), and 30 us for the join.  32768 image rows over 328 keys, 8 heads of 40:
+// (vector issue 57 %, matrix units 25 % of the cycles), and 30 us for the join.  32768 image rows over 210 keys, 8 heads of 40:
 // 33 us and 6 us for the join.
 //
 // Few keys under many rows (captions under image tokens) leave most of the chip idle: the rows of a key tile are then cut
@@ -332,7 +332,7 @@ int launch(const DocArgs& a, hipStream_t st) {
 
 // Workgroups without a split: one per 128 keys and key head, each passing about G * (the rows of one document, and of the others
 // that its keys belong to).  Runs of at least 8 tiles; without a causal mask as many as are resident at once (two workgroups
-// per CU: 8 x 4096 rows over 328 keys took 48 us with three times as many, 36 us with these), with one four times as many, which
+// per CU: 8 x 4096 rows over 210 keys took 48 us with three times as many, 36 us with these), with one four times as many, which
 // evens out that the first keys of a document are passed by all its rows and the last by few (twice as many were slower).
 int doc_bwd_kv_splits(int Tq, int Tk, int Hq, int Hkv, int docs, int causal) {
     if (Tk < 1) return 1;

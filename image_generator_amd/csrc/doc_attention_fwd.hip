@@ -8,10 +8,10 @@
 // Probabilities are rounded to bf16, the matrix units' type, the sum is of the fp32 values: 0.24 % instead of 0.17 % in the 2-norm
 // of a result that is itself rounded to bf16.
 //
-// Measured, with what bounds it: 58 254 caption tokens, 8 heads of 96 (358 MB): 87 us, 4.1 TB/s against 5.2 for a copy, the rest is
+// Measured, with what bounds it: 58 255 caption tokens, 8 heads of 96 (358 MB): 87 us, 4.1 TB/s against 5.2 for a copy, the rest is
 // the chain of a short workgroup (offsets, rows, keys, store).  Four documents of 4001 .. 8191 tokens, 8 heads on 2 of 64, causal
 // with prefix, cap and bias (149 GFLOP): 349 us, 427 TFLOP/s, bound by vector issue (81 % of the cycles, a score's tanh, bias,
-// exp2, sum and conversion against two products).  32768 image rows over 328 keys, 8 heads of 40: 21 us.
+// exp2, sum and conversion against two products).  32768 image rows over 210 keys, 8 heads of 40: 21 us.
 #include "doc_tiles.h"
 #include <mutex>
 #include <type_traits>
@@ -210,8 +210,8 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
 // Few rows over many keys (single queries over what their documents hold): a wave takes 32 rows and one run of their keys,
 // alone - its own staged tiles, no barrier with the others - and leaves an unnormalised result; the join weighs the runs of a
 // row against each other.  The rows of a tile may belong to many documents, whose keys lie one behind another: a run is read
-// once and only the rows that see a tile take part, so what is bound here is reading K and V: 48 queries over 339 761 keys, 8
-// heads on 2 of 96 (261 MB), 74 us, 3.5 TB/s, and 5.5 us for the join (whole rows of 97 x 64 runs read twice).
+// once and only the rows that see a tile take part, so what is bound here is reading K and V: 48 queries over 339 602 keys, 8
+// heads on 2 of 96 (261 MB), 74 us, 3.5 TB/s, and 5.5 us for the join.
 template <int ND, int NO, int KIND>
 __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem_all[];

@@ -78,33 +78,43 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const void* __restrict_
 }
 
 // ---- sort: up to RANKED ids ---------------------------------------------------------------------------------------
-// The place of an id in the sorted list is the number of (id, position) pairs below its own.  That is n^2 comparisons, but
-// spread over the chip (16 lanes for each id, every workgroup with the whole list in LDS) they take 2 us at 8192 ids, where a
-// sort by one workgroup is a chain of 91 steps (19 us at 2048 ids).
+// The place of an id in the sorted list is the number of (id, position) pairs below its own: ids up to its own in front of it,
+// ids below it behind.  That is n^2 comparisons, but spread over the chip (16 lanes for each id, every workgroup with the whole
+// list in LDS, four ids a read) they beat the passes below, whose six launches wait for each other: 17.6 against 32 us of
+// kernels at 8192 ids, 5.2 us at 2048 (two trips to memory and a launch).
 __global__ __launch_bounds__(256) void rank_sort_kernel(const void* __restrict__ ids, int ids64, int n, unsigned rows,
                                                         unsigned* __restrict__ keys, unsigned* __restrict__ pos) {
     extern __shared__ __attribute__((aligned(16))) unsigned list[];
-    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * 256) {
+    const int padded = (n + 4 * SHARES - 1) / (4 * SHARES) * (4 * SHARES);       // (the padding is above every id)
+    for (int i0 = threadIdx.x; i0 < padded; i0 += 8 * 256) {
         long long id[8];                         // eight loads under way at a time
 #pragma unroll
         for (int u = 0; u < 8; ++u) id[u] = load_id(ids, ids64, min(i0 + u * 256, n - 1));
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (i0 + u * 256 < n) list[i0 + u * 256] = id[u] >= 0 && id[u] < (long long)rows ? (unsigned)id[u] : rows;
+            if (i0 + u * 256 < padded) list[i0 + u * 256] = i0 + u * 256 >= n ? 0xffffffffu : id[u] >= 0 && id[u] < (long long)rows ? (unsigned)id[u] : rows;
     }
     __syncthreads();
     const int mine = blockIdx.x * (256 / SHARES) + threadIdx.x / SHARES, share = threadIdx.x % SHARES;
     if (mine >= n) return;                       // whole groups of SHARES lanes
     const unsigned key = list[mine];
     int below = 0;
-#pragma unroll 8
-    for (int j = share; j < n; j += SHARES) below += list[j] < key || (list[j] == key && j < mine) ? 1 : 0;
+#pragma unroll 4
+    for (int j = share * 4; j < padded; j += 4 * SHARES) {
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        const u32x4 x = *(const u32x4*)&list[j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) below += x[e] < key + (j + e < mine ? 1u : 0u) ? 1 : 0;
+    }
 #pragma unroll
     for (int o = 1; o < SHARES; o <<= 1) below += __shfl_xor(below, o, 64);
     if (share == 0) { keys[below] = key; pos[below] = mine; }
 }
 
 // ---- sort: any number of ids, least significant digit first ---------------------------------------------------------
+// Bits of a pass: as even as at most 8 a pass allow.  Each is three launches - digits of a tile counted, prefix sums over the tiles,
+// entries moved to their places, in order within a tile by ballots over the waves' digits - bound by their chains, not by bytes:
+// 262143 ids of 16384 rows, two passes: 45 us, of it 10 us each move.  No atomic decides an order.
 // FIRST: the input is the id list itself (position = index); else (keys, pos) of the previous pass.
 template <bool FIRST>
 __device__ __forceinline__ unsigned pass_key(const void* ids, int ids64, const unsigned* keys, size_t i, unsigned rows) {
@@ -274,7 +284,9 @@ __device__ __forceinline__ void put_row(T* __restrict__ dst, const f32x4 (&acc)[
     }
 }
 
-// Aligned chunks whose CHUNK positions all belong to one id: a wave sums each (blockIdx.y: 256 * VEC columns).
+// Ids that make up much of a batch would leave one wave with most of the work, so aligned chunks whose CHUNK positions all belong
+// to one id are summed ahead, by a wave each (blockIdx.y: SWEEPS * 64 * VEC columns), wherever they lie.  Bound by reading rows:
+// 262143 of 768 bf16, 57 us, most of 403 MB, 16 rows of a wave under way at a time (8 were slower, at twice the occupancy too).
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void chunk_sum_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ pos, int n,
                                                         unsigned rows, const T* __restrict__ dy, int width, float* __restrict__ part) {
@@ -303,7 +315,8 @@ __global__ __launch_bounds__(64) void super_sum_kernel(const unsigned* __restric
 }
 
 // Every row of the table, written once: a wave takes the sorted positions of its id (found by binary search) in order, whole
-// aligned chunks and runs of chunks from their sums; an id without positions gets zeros.
+// aligned chunks and runs of chunks from their sums; an id without positions gets zeros.  Bound by the chain of search, positions,
+// rows and store: 16384 x 768 fp32 (50 MB) of 1601 ids 15.5 us, of 262143 ids 63 us with the rows that no chunk holds.
 constexpr int ROWS_PER_WG = 7;       // eight boundaries: two rounds of the workgroup's four waves
 template <typename T, typename TO, int VEC>
 __global__ __launch_bounds__(256) void table_grad_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ pos, int n,
@@ -472,7 +485,7 @@ int mi355_embedding_bwd(const void* ids, int ids64, long long n, const void* dy,
     unsigned *keys = (unsigned*)(w + g.keys), *pos = (unsigned*)(w + g.pos);
     const unsigned R = (unsigned)rows;
     if (n > 0 && n <= RANKED) {
-        hipLaunchKernelGGL(rank_sort_kernel, dim3((unsigned)((n + 256 / SHARES - 1) / (256 / SHARES))), dim3(256), (size_t)n * 4, st, ids, ids64, (int)n, R, keys, pos);
+        hipLaunchKernelGGL(rank_sort_kernel, dim3((unsigned)((n + 256 / SHARES - 1) / (256 / SHARES))), dim3(256), ((size_t)n + 4 * SHARES - 1) / (4 * SHARES) * (16 * SHARES), st, ids, ids64, (int)n, R, keys, pos);
     } else if (n > 0) {
         unsigned* counts = (unsigned*)(w + g.counts);
         unsigned *k2 = (unsigned*)(w + g.keys2), *p2 = (unsigned*)(w + g.pos2);
