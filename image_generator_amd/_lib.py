@@ -77,6 +77,22 @@ def _load():
 
 
 lib = _load()
+_host = None
+
+
+def host():
+    """The Python extension of the host's side (csrc/host.cpp), bound to the entries of `lib`."""
+    global _host
+    if _host is None:
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise ImportError(f"{os.path.join(_HERE, '_host.so')} is missing or does not load: build it with "
+                              f"`make -C {os.path.join(_HERE, 'csrc')}` (there is no fallback path)") from e
+        names = [n for n in parse_header() if n.startswith(("mi355_doc_attention_", "mi355_embedding_"))]
+        module.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, check)
+        _host = module
+    return _host
 
 
 def check(rc: int, what: str = ""):

@@ -11,7 +11,7 @@ import math
 
 import torch
 
-from ._lib import lib, check
+from ._lib import lib, check, host
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -611,65 +611,12 @@ def attention_bwd(q, k, v, o, do, lse, heads, dq, dk, dv):
                                   _stream()), "attention_bwd")
 
 
-def _here(*tensors):
-    """Operands of one launch: all on the current device (a launch goes to its stream).  Returns that device's index."""
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise RuntimeError(f"tensors on {tensors[0].device} and {t.device}; HIP device tensors required (no CPU path)")
-    if dev < 0:
-        raise RuntimeError("HIP device tensors required (no CPU path)")
-    if torch._C._cuda_getDevice() != dev:
-        raise RuntimeError(f"tensors on {tensors[0].device}, the current device is {torch._C._cuda_getDevice()}")
-    return dev
-
-
-def _doc_offsets(name, t, n, dtype):
-    if t is not None and (t.numel() != n or t.dtype != dtype or not t.is_contiguous()):
-        raise ValueError(f"doc_attention: {name} must be {n} contiguous {dtype} values, got {t.numel()} {t.dtype}")
-
-
-def _doc_matrix(name, t, heads, width):
-    if t.dtype != BF16 or t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1:
-        raise RuntimeError(f"doc_attention: {name} must be a bf16 matrix [tokens, heads * width] with adjacent columns")
-    if t.shape[1] != heads * width:
-        raise ValueError(f"doc_attention: {name} {tuple(t.shape)} for {heads} heads of width {width}")
-
-
-def _ld(t):
-    # the stride between the rows of one row is whatever made the tensor (a transposed column, say) and is not looked at
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed):
-    """Checks shared by the two directions of the document attention; (leading arguments, trailing arguments, sizes, device)."""
-    if kv_heads is None:
-        kv_heads = heads
-    if k_offsets is None:
-        k_offsets = q_offsets
-    dev = _here(q, k, v, q_offsets, k_offsets, prefix, slopes)
-    if heads < 1 or kv_heads < 1 or heads % kv_heads:
-        raise ValueError(f"doc_attention: {heads} query heads on {kv_heads} key heads")
-    width = q.shape[-1] // heads
-    _doc_matrix("q", q, heads, width)
-    _doc_matrix("k", k, kv_heads, width)
-    _doc_matrix("v", v, kv_heads, width)
-    if k.shape[0] != v.shape[0]:
-        raise ValueError(f"doc_attention: {k.shape[0]} keys, {v.shape[0]} values")
-    docs = q_offsets.numel() - 1
-    if docs < 1:
-        raise ValueError("doc_attention: offsets hold at least two entries")
-    _doc_offsets("q_offsets", q_offsets, docs + 1, torch.int32)
-    if k_offsets is not q_offsets:
-        _doc_offsets("k_offsets", k_offsets, docs + 1, torch.int32)
-    _doc_offsets("prefix", prefix, docs, torch.int32)
-    _doc_offsets("slopes", slopes, heads, F32)
-    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("doc_attention: no gradient reaches the slopes (detach them)")
-    if align not in ("end", "start"):
-        raise ValueError(f"doc_attention: align {align!r} is neither 'end' nor 'start'")
-    head = (q_offsets.data_ptr(), k_offsets.data_ptr(), docs, _ptr(prefix), _ptr(slopes), cap or 0.0, causal, align == "start")
-    return head, (width ** -0.5 if scale is None else scale, drop_p, seed), (q.shape[0], k.shape[0], heads, kv_heads, width), dev
+def _where(t):
+    """(current device, its stream) for operands that live on a HIP device; the call itself refuses others."""
+    if not t.is_cuda:
+        return -1, 0
+    dev = torch._C._cuda_getDevice()
+    return dev, torch._C._cuda_getCurrentRawStream(dev)
 
 
 def doc_attention_fwd(q, k, v, heads, q_offsets, k_offsets=None, kv_heads=None, causal=False, prefix=None, slopes=None, cap=0.0,
@@ -680,77 +627,34 @@ def doc_attention_fwd(q, k, v, heads, q_offsets, k_offsets=None, kv_heads=None, 
     their starts, and sees its document's keys; with `causal` those up to c and the document's first `prefix[n]`.  `cap`:
     scores become cap tanh(s / cap); `slopes` [heads]: minus slope times |c - j|.  Returns (out [Tq, heads * d],
     lse [heads, Tq]); a query that sees nothing gets zeros and -inf."""
-    head, tail, sizes, dev = _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed)
-    out = torch.empty(q.shape, dtype=BF16, device=q.device)
-    lse = torch.empty((heads, q.shape[0]), dtype=F32, device=q.device)
-    need = lib.mi355_doc_attention_fwd_workspace_bytes(*sizes)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    check(lib.mi355_doc_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *head, *sizes,
-                                      _ld(q), _ld(k), _ld(v), out.stride(0), *tail, _ptr(ws), need,
-                                      torch._C._cuda_getCurrentRawStream(dev)), "doc_attention_fwd")
-    return out, lse
+    return host().doc_attention_fwd(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed, *_where(q))
 
 
 def doc_attention_bwd(do, q, k, v, o, lse, heads, q_offsets, k_offsets=None, kv_heads=None, causal=False, prefix=None, slopes=None,
                       cap=0.0, scale=None, align="end", drop_p=0.0, seed=0, dq=None, dk=None, dv=None):
     """(dq, dk, dv) of `doc_attention_fwd` for the gradient `do` of its output; `o`, `lse` are what it returned.  dq / dk / dv:
     bf16 matrices to write (slices of one buffer, say, that share no element with each other or an operand); new ones by default."""
-    head, tail, sizes, _ = _doc_args(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed)
-    _here(q, do, o, lse, dq, dk, dv)
-    dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=q.device) if d is None else d for t, d in ((q, dq), (k, dk), (v, dv)))
-    for name, t, like in (("do", do, q), ("o", o, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        if t.shape != like.shape or t.dtype != BF16 or t.stride(1) != 1 and t.shape[1] > 1:
-            raise RuntimeError(f"doc_attention_bwd: {name} must be a bf16 matrix {tuple(like.shape)} with adjacent columns")
-    to = [t.data_ptr() for t in (dq, dk, dv) if t.numel()]
-    if len(set(to)) < len(to) or not {t.data_ptr() for t in (q, k, v, o, do)}.isdisjoint(to):
-        raise ValueError("doc_attention_bwd: a gradient in the place of an operand or of another gradient")
-    if lse.shape != (heads, q.shape[0]) or lse.dtype != F32 or not lse.is_contiguous():
-        raise RuntimeError("doc_attention_bwd: lse is not the forward pass's")
-    ws = torch.empty(int(lib.mi355_doc_attention_bwd_workspace_bytes(*sizes, q_offsets.numel() - 1, causal)), dtype=torch.uint8, device=q.device)
-    check(lib.mi355_doc_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), dq.data_ptr(),
-                                      dk.data_ptr(), dv.data_ptr(), *head, *sizes, _ld(q), _ld(k), _ld(v), _ld(o), _ld(do), _ld(dq), _ld(dk),
-                                      _ld(dv), *tail, ws.data_ptr(), ws.numel(), _stream()),
-          "doc_attention_bwd")
-    return dq, dk, dv
+    return host().doc_attention_bwd(q, k, v, heads, q_offsets, k_offsets, kv_heads, causal, prefix, slopes, cap, scale, align, drop_p, seed, do, o, lse,
+                                    dq, dk, dv, *_where(q))
 
 
-def _ids(ids):
-    if ids.dtype not in (torch.int32, torch.int64):
-        raise RuntimeError(f"embedding: ids must be int32 or int64, got {ids.dtype}")
-    return ids.contiguous()
+_OUT = {BF16: True, F32: False}
 
 
 def embedding_fwd(ids, table, scale=1.0, out_dtype=BF16):
     """scale * table[ids]: ids int32 / int64 of any shape, table [rows, width] fp32 or bf16; out bf16 or fp32.  An id outside
     the table reads as a NaN row (ids are on the device, nothing waits for them)."""
-    _here(table, ids)
-    if table.dim() != 2 or table.dtype not in (F32, BF16) or not table.is_contiguous():
-        raise RuntimeError("embedding: the table must be a contiguous fp32 or bf16 matrix")
-    if out_dtype not in (F32, BF16):
+    if out_dtype not in _OUT:
         raise RuntimeError(f"embedding: outputs are fp32 or bf16, not {out_dtype}")
-    ids = _ids(ids)
-    out = torch.empty((*ids.shape, table.shape[1]), dtype=out_dtype, device=table.device)
-    check(lib.mi355_embedding_fwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(), table.data_ptr(), table.dtype == BF16,
-                                  table.shape[0], table.shape[1], scale, out.data_ptr(), out_dtype == BF16, _stream()),
-          "embedding_fwd")
-    return out
+    return host().embedding_fwd(ids, table, scale, _OUT[out_dtype], *_where(table))
 
 
 def embedding_bwd(ids, dy, rows, scale=1.0, out_dtype=F32):
     """Gradient [rows, width] of the table of `embedding_fwd`: scale times the sum of the dy rows of each id, in an order
     that the ids alone decide (same call, same bits)."""
-    _here(dy, ids)
-    if dy.dtype not in (F32, BF16) or out_dtype not in (F32, BF16):
+    if out_dtype not in _OUT:
         raise RuntimeError("embedding_bwd: gradients are fp32 or bf16")
-    if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape:
-        raise RuntimeError(f"embedding_bwd: gradient {tuple(dy.shape)} of ids {tuple(ids.shape)}")
-    ids, dy = _ids(ids), dy.contiguous()
-    width = dy.shape[-1]
-    ws = torch.empty(int(lib.mi355_embedding_bwd_workspace_bytes(ids.numel(), rows, width)), dtype=torch.uint8, device=dy.device)
-    out = torch.empty((rows, width), dtype=out_dtype, device=dy.device)
-    check(lib.mi355_embedding_bwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(), dy.data_ptr(), dy.dtype == BF16, rows, width,
-                                  scale, out.data_ptr(), out_dtype == BF16, ws.data_ptr(), ws.numel(), _stream()), "embedding_bwd")
-    return out
+    return host().embedding_bwd(ids, dy, rows, scale, _OUT[out_dtype], *_where(dy))
 
 
 def gelu_bf16(x):

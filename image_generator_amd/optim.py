@@ -7,17 +7,15 @@ for every 256 elements of a tensor: 2.03 instead of 8 bytes of state for a param
 from __future__ import annotations
 
 import math
-import operator
 
 import numpy as np
 import torch
 
-from ._lib import lib, check
+from ._lib import lib, check, host
 from .ops import BF16, F32, PinnedRing, _stream
 
 BLOCK = 256            # elements that share a scale
 _WG_BLOCKS = 8         # blocks per workgroup of the update
-_SHAPE, _DTYPE = operator.attrgetter("shape"), operator.attrgetter("dtype")
 _HYPER = 16            # doubles in front of the gradient addresses in the step's upload
 
 
@@ -95,7 +93,9 @@ class TensorAdamW:
         _disjoint([c for c in copies if c is not None], "copies")
         self.copies = copies
         self._written = [t for t in self.params + copies if t is not None]
-        self._places = list(map(torch.Tensor.data_ptr, self._written))
+        self._places = np.empty(len(self._written), dtype=np.int64)
+        host().places(self._written, self._places.ctypes.data, True)
+        self._places_at = self._places.ctypes.data
         rows = [[p.data_ptr(), 0 if c is None else c.data_ptr(), p.numel(), s] for p, c, s in zip(self.params, copies, self.starts)]
         rows += [[0, 0, n, 0] for n in self.watched]
         self._recs = torch.tensor(rows, dtype=torch.int64).to(self.device)
@@ -106,20 +106,22 @@ class TensorAdamW:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("TensorAdamW: bind() before the capture (and before every replay); only apply() can be captured")
         self._on_device()
-        owned = grads is None
-        grads = [p.grad for p in self.params] if owned else list(grads)
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"TensorAdamW: {len(grads)} gradients of {len(self.params)} parameters")
-        if list(map(torch.Tensor.data_ptr, self._written)) != self._places:
+        if host().places(self._written, self._places_at, False):
             raise RuntimeError("TensorAdamW: a parameter or copy has moved to other memory (set_copies() takes the new places)")
-        words, kept = self._addresses(grads, owned)
         watched = [None] * len(self.watched) if watched is None else list(watched)
         if len(watched) != len(self.watched):
             raise ValueError(f"TensorAdamW: {len(watched)} watched gradients, {len(self.watched)} announced")
         for n, g in zip(self.watched, watched):
             if g is not None and (g.numel() != n or g.device != self.device or g.dtype not in (F32, BF16) or not g.is_contiguous()):
                 raise ValueError("TensorAdamW: a watched gradient must be a contiguous fp32 or bf16 tensor of the announced size")
-            words.append(0 if g is None else g.data_ptr() | (g.dtype == BF16))
+        slot, kept = self._ring.acquire(), []
+        words = (self.params, self.device.index, slot.data_ptr() + 8 * _HYPER)
+        if host().gradient_words(grads, *words) >= 0:
+            grads, kept = self._contiguous(grads)
+            host().gradient_words(grads, *words)
         if lr is not None:
             self.lr = lr
         self.t += 1
@@ -127,42 +129,29 @@ class TensorAdamW:
         c1, c2 = 1 - b1 ** self.t, 1 - b2 ** self.t
         hyper = (self.lr, b1, b2, self.eps, self.wd, c1, c2, self.max_norm or 0.0, 1 - self.lr * self.wd, self.lr / c1, 1 / math.sqrt(c2),
                  *(1 - float(np.float32(b)) if self.fp32_betas else 1 - b for b in self.betas))
-        h = self._ring.acquire().numpy()
-        h[:_HYPER].view("float64")[:len(hyper)] = hyper
-        h[_HYPER:] = words
-        self._upload.copy_(self._ring.acquire(), non_blocking=True)
+        h = slot.numpy()
+        h[:len(hyper)].view("float64")[:] = hyper
+        for i, g in enumerate(watched, _HYPER + len(grads)):
+            h[i] = 0 if g is None else g.data_ptr() | (g.dtype == BF16)
+        self._upload.copy_(slot, non_blocking=True)
         self._ring.copied()
         self._ring.release()
         self._kept, self._bound = kept, True
 
-    def _addresses(self, grads, owned):
-        """(what the device table holds for each gradient, copies made here)."""
-        # the common case in a few sweeps: every gradient there, of its parameter's shape, contiguous, one type, this device
-        # (a parameter's own `.grad` has its shape and device already)
-        if type(None) not in set(map(type, grads)) and all(map(torch.Tensor.is_contiguous, grads)):
-            if owned or (list(map(_SHAPE, grads)) == self._shapes and set(map(torch.Tensor.get_device, grads)) == {self.device.index}):
-                kinds = set(map(_DTYPE, grads))
-                if kinds == {F32}:
-                    return list(map(torch.Tensor.data_ptr, grads)), []
-                if kinds == {BF16}:
-                    return [a | 1 for a in map(torch.Tensor.data_ptr, grads)], []
-        words, kept = [], []
+    def _contiguous(self, grads):
+        """(gradients with contiguous copies of those that are not, the copies); refuses what is no gradient of its parameter."""
+        out, kept = [], []
         for i, (p, g) in enumerate(zip(self.params, grads)):
-            if g is None:
-                words.append(0)
-                continue
-            if g.shape != p.shape or g.device != self.device:
-                raise ValueError(f"TensorAdamW: gradient {i} is {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)} on {self.device}")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                kept.append(g)
-            if g.dtype == F32:
-                words.append(g.data_ptr())
-            elif g.dtype == BF16:
-                words.append(g.data_ptr() | 1)
-            else:
-                raise ValueError(f"TensorAdamW: gradient {i} is {g.dtype}, neither fp32 nor bf16")
-        return words, kept
+            if g is not None:
+                if g.shape != p.shape or g.device != self.device:
+                    raise ValueError(f"TensorAdamW: gradient {i} is {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)} on {self.device}")
+                if g.dtype not in (F32, BF16):
+                    raise ValueError(f"TensorAdamW: gradient {i} is {g.dtype}, neither fp32 nor bf16")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    kept.append(g)
+            out.append(g)
+        return out, kept
 
     def apply(self):
         """The launches of the step that `bind` began (capturable)."""
@@ -177,15 +166,16 @@ class TensorAdamW:
                                          self._map.shape[0], self.bits, m.data_ptr(), ptr(ms), v.data_ptr(), ptr(us),
                                          self._partial.data_ptr(), self._upload.data_ptr(), self.state.data_ptr(), self._elements,
                                          _stream()), "multi_adamw")
-        torch.autograd.graph.increment_version(self._written)
+        host().bump(self._written)
 
     def step(self, grads=None, lr=None, watched=None):
         self.bind(grads, lr, watched)
         self.apply()
 
     def _on_device(self):
-        if torch.cuda.current_device() != self.device.index:
-            raise RuntimeError(f"TensorAdamW: parameters on {self.device}, the current device is {torch.cuda.current_device()}")
+        current = torch._C._cuda_getDevice()
+        if current != self.device.index:
+            raise RuntimeError(f"TensorAdamW: parameters on {self.device}, the current device is {current}")
 
     def moments(self):
         """(first, second) moments as flat fp32 tensors, each parameter padded to a multiple of 256 elements: the states

@@ -71,3 +71,47 @@ def test_doc_attention_refusals():
                     (dict(ws_bytes=8), "workspace"), (dict(prefix=16), "prefix")):
         assert bwd(**kw) == -1 and why in err(), (kw, err())
     assert lib.mi355_doc_attention_bwd_workspace_bytes(-1, 4, 2, 2, 32, 1, 0) == 0 and lib.mi355_doc_attention_fwd_workspace_bytes(4, 4, 3, 2, 32) == 0
+
+
+def test_host_extension_refusals():
+    """The native checks turn every bad call into a Python error."""
+    import numpy as np
+    from image_generator_amd._lib import host
+    h = host()
+    for fn in (h.doc_attention_fwd, h.doc_attention_bwd, h.embedding_fwd, h.embedding_bwd, h.gradient_words, h.places, h.bump, h.bind):
+        with pytest.raises(TypeError):
+            fn()
+    with pytest.raises(TypeError, match="tensor"):
+        h.embedding_fwd(3, 4, 1.0, True, -1, 0)
+    with pytest.raises(KeyError):
+        h.bind({}, print)
+    with pytest.raises(TypeError, match="list"):
+        h.places((), 0, True)
+    ts = [torch.zeros(3), torch.zeros(0), torch.ones(2)]
+    at = np.empty(3, dtype=np.int64)
+    assert h.places(ts, at.ctypes.data, True) is False and at.tolist() == [t.data_ptr() for t in ts]
+    assert h.places(ts, at.ctypes.data, False) is False
+    ts[2].data = torch.ones(2)
+    assert h.places(ts, at.ctypes.data, False) is True
+    assert h.gradient_words([None, None], ts[:2], 0, at.ctypes.data) == -1 and at.tolist()[:2] == [0, 0]
+    assert h.gradient_words([None, ts[1]], ts[:2], 0, at.ctypes.data) == 1          # on no device
+    with pytest.raises(ValueError, match="gradients"):
+        h.gradient_words([None], ts, 0, at.ctypes.data)
+    with pytest.raises(TypeError, match="tensor"):
+        h.gradient_words([3], ts[:1], 0, at.ctypes.data)
+    before = ts[0]._version
+    h.bump(ts)
+    assert ts[0]._version == before + 1
+    with torch.inference_mode():
+        h.bump([torch.zeros(2)])
+
+
+def test_host_extension_argument_errors():
+    from image_generator_amd import ops
+    q, off = torch.zeros(4, 64, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(TypeError):
+        ops.doc_attention_fwd(q, q, q, heads="2", q_offsets=off)
+    with pytest.raises(TypeError):
+        ops.doc_attention_fwd(q, None, q, heads=2, q_offsets=off)
+    with pytest.raises(RuntimeError, match="not"):
+        ops.embedding_fwd(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), out_dtype=torch.float16)
