@@ -84,6 +84,7 @@ def host():
     """The Python extension of the host's side (csrc/host.cpp), bound to the entries of `lib`."""
     global _host
     if _host is None:
+        import torch  # noqa: F401  (its libraries are what the extension is linked against)
         try:
             from . import _host as module
         except ImportError as e:
