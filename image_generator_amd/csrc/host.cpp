@@ -4,6 +4,7 @@
 //
 // A Python extension (`image_generator_amd/_host.so`); the entries it calls are handed over by bind(), from the library that the
 // process has loaded.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
@@ -45,10 +46,8 @@ PyObject* guarded(F f) {
     } catch (const Failed&) {
     } catch (const Raise& e) {
         PyErr_SetString(e.type, e.text.c_str());
-    } catch (const c10::Error& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {                  // torch's own, out of memory among them
+        torch::translate_exception_to_python(std::current_exception());
     }
     return nullptr;
 }
