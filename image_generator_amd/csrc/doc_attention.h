@@ -27,8 +27,10 @@ struct DocArgs {
     float scale, cap, rcap;         // rcap = 1 / cap
     unsigned drop_thresh, seed;     // an entry is dropped when its hash < drop_thresh
     float drop_scale;
-    float* part;                    // split forward: partial results
+    float* part;                    // partial results of `splits` runs (of keys: forward; of rows: dK and dV); 1: none
     int splits;
+    float* part_q;                  // the dQ pass's, over `splits_q` runs of keys
+    int splits_q;
 };
 
 #define LOG2E 1.4426950408889634f

@@ -11,6 +11,10 @@ static const char* bad_sizes(int docs, int Tq, int Tk, int Hq, int Hkv, int D) {
     return nullptr;
 }
 static size_t bwd_rows_bytes(int Tq, int Hq) { return ((size_t)Tq * 16 + (size_t)Tq * Hq * 4 + 255) / 256 * 256; }
+static size_t part_q_bytes(int Tq, int Tk, int Hq, int Hkv, int D, int docs) {
+    const int s = key_runs(Tq, Tk, Hq, Hkv, docs);
+    return s > 1 ? ((size_t)s * Tq * Hq * D * 4 + 255) / 256 * 256 : 0;
+}
 static bool off16(const void* a) { return ((uintptr_t)a & 15) != 0; }
 static bool bad_ld(long long ld) { return ld < 0 || ld % 8 != 0 || ld > (1 << 23); }
 
@@ -36,9 +40,9 @@ static int fill(DocArgs& a, const char* who, int docs, int Tq, int Tk, int Hq, i
 
 extern "C" {
 
-size_t mi355_doc_attention_fwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D) {
-    if (bad_sizes(1, Tq, Tk, Hq, Hkv, D)) return 0;
-    return doc_fwd_workspace(Tq, Tk, Hq, Hkv, D);
+size_t mi355_doc_attention_fwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D, int docs) {
+    if (bad_sizes(docs, Tq, Tk, Hq, Hkv, D)) return 0;
+    return doc_fwd_workspace(Tq, Tk, Hq, Hkv, D, docs);
 }
 
 int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int* q_off, const int* k_off, int docs,
@@ -52,7 +56,7 @@ int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* o
     if (off16(q) || off16(k) || off16(v) || off16(out)) return mi355_fail(MI355_ERR_ARG, "doc_attention: operands not 16-byte aligned");
     if (bad_ld(ldq) || bad_ld(ldk) || bad_ld(ldv) || bad_ld(ldo) || ldo < (long long)Hq * D)
         return mi355_fail(MI355_ERR_ARG, "doc_attention: row strides must be multiples of 8, at most 2^23");
-    const size_t need = mi355_doc_attention_fwd_workspace_bytes(Tq, Tk, Hq, Hkv, D);
+    const size_t need = mi355_doc_attention_fwd_workspace_bytes(Tq, Tk, Hq, Hkv, D, docs);
     if (need && (!ws || ws_bytes < need || off16(ws))) return mi355_fail(MI355_ERR_ARG, "doc_attention: workspace of %zu bytes, %zu needed, 16-byte aligned", ws ? ws_bytes : 0, need);
     a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.out = (bf16_t*)out; a.lse = lse;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
@@ -65,7 +69,7 @@ int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* o
 size_t mi355_doc_attention_bwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D, int docs, int causal) {
     if (bad_sizes(docs, Tq, Tk, Hq, Hkv, D)) return 0;
     const int splits = doc_bwd_kv_splits(Tq, Tk, Hq, Hkv, docs, causal != 0);
-    return bwd_rows_bytes(Tq, Hq) + (splits > 1 ? (size_t)splits * Tk * Hkv * 2 * D * 4 : 0) + 16;
+    return bwd_rows_bytes(Tq, Hq) + part_q_bytes(Tq, Tk, Hq, Hkv, D, docs) + (splits > 1 ? (size_t)splits * Tk * Hkv * 2 * D * 4 : 0) + 16;
 }
 
 int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq, void* dk,
@@ -91,7 +95,9 @@ int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const v
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.lddo = lddo; a.lddq = lddq; a.lddk = lddk; a.lddv = lddv;
     a.rows = (int4*)ws;
     a.delta = (float*)((char*)ws + (size_t)Tq * 16);
-    a.part = (float*)((char*)ws + bwd_rows_bytes(Tq, Hq));
+    a.part_q = (float*)((char*)ws + bwd_rows_bytes(Tq, Hq));
+    a.splits_q = key_runs(Tq, Tk, Hq, Hkv, docs);
+    a.part = (float*)((char*)ws + bwd_rows_bytes(Tq, Hq) + part_q_bytes(Tq, Tk, Hq, Hkv, D, docs));
     a.splits = doc_bwd_kv_splits(Tq, Tk, Hq, Hkv, docs, a.causal);
     const hipStream_t st = (hipStream_t)stream;
     ProfScope prof(FAM_ATTN, st, 10.0 * Tq * (double)Tk / docs * Hq * D);

@@ -21,8 +21,10 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     __shared__ __attribute__((aligned(16))) char ring0[2 * TILE_BYTES<NO>], ring1[2 * TILE_BYTES<NO>], ring2[BUFS == 3 ? 2 * TILE_BYTES<NO> : 16];
     __shared__ __attribute__((aligned(16))) int range[4][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
-    int tile, hk;
-    if (!unit_of(tiles, p.Hkv, tile, hk)) return;
+    int unit, hk;
+    if (!unit_of(tiles * p.splits_q, p.Hkv, unit, hk)) return;
+    const int split = unit / tiles;
+    int tile = unit - split * tiles;
     if (p.causal) tile = tiles - 1 - tile;       // the last rows of a document see most: the longest work first
     const unsigned rows = (unsigned)p.Tq * (unsigned)p.G, R = tile * 128u + wave * 32 + l31;
     const bool live = R < rows;
@@ -38,7 +40,7 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     load_row(ov, p.o + (size_t)token * p.ldo + (size_t)head * p.D, p.D);
     load_row(qf, q_row(p, token, head), p.D);
     RowSpan span = row_span_in(p, token, doc_of_wave(p.q_off, p.docs, window, first, __builtin_amdgcn_readlane(token, 31), token));
-    if (live && hh == 0 && head == 0) p.rows[token] = make_int4(span.lo, span.hi, span.c, 0);
+    if (live && hh == 0 && head == 0 && split == 0) p.rows[token] = make_int4(span.lo, span.hi, span.c, 0);
     if (!live) span.lo = span.hi = 0;
     const bool sees = span.hi > span.lo;
     const int lo = wave_min_i(sees ? span.lo : 0x7fffffff);
@@ -62,14 +64,16 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
         vf.dma(to + TILE_BYTES<NO>, vbase, p.ldv, p.D, k0, khi - k0);
     };
     // up to BUFS tiles stay where they are; of more, all but one buffer are filled ahead
-    const bool resident = klo >= khi || khi - klo <= BUFS * 64;
+    int k_from, k_to;
+    run_of(klo, khi, p.splits_q, split, k_from, k_to);
+    const bool resident = p.splits_q == 1 && (klo >= khi || khi - klo <= BUFS * 64);
     auto start = [&](int from, int to) __attribute__((always_inline)) {
         if (from >= to) return;                  // (rows that see nothing leave `from` at the largest int)
         request(ring0, from);
         if ((BUFS == 3 || resident) && from + 64 < to) request(ring1, from + 64);
         if (BUFS == 3 && resident && from + 128 < to) request(ring2, from + 128);
     };
-    start(klo, khi);
+    start(k_from, k_to);
     keep_row(gf, sees, p.D);
     keep_row(ov, sees, p.D);
     float delta = 0.f;
@@ -139,16 +143,16 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
         if (few) delta = sum;
         if (!resident) {
             __syncthreads();
-            start(klo, khi);
+            start(k_from, k_to);
         }
     }
-    if (live && hh == 0) p.delta[at] = delta;
+    if (live && hh == 0 && split == 0) p.delta[at] = delta;
     f32x16 dqT[NO];
 #pragma unroll
     for (int i = 0; i < NO; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dqT[i][r] = 0.f;
-    each_tile(klo, khi, lo, hi, [&](const char* Ks, int k0) __attribute__((always_inline)) {
+    each_tile(k_from, k_to, lo, hi, [&](const char* Ks, int k0) __attribute__((always_inline)) {
         const char* Vs = Ks + TILE_BYTES<NO>;
         const bool masked = k0 < in_lo || k0 + 64 > in_hi;
 #pragma unroll
@@ -201,6 +205,18 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
                 for (int db = 0; db < NO; ++db) dqT[db] = mfma(rd.frag_t(Ks, db, kb * 2 + st), dsf[st], dqT[db]);
         }
     });
+    if (p.splits_q > 1) {
+        if (!live) return;
+        float* part = p.part_q + (((size_t)split * p.Tq + token) * p.Hq + head) * p.D;
+#pragma unroll
+        for (int db = 0; db < NO; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = db * 32 + 8 * g + 4 * hh;
+                if (d < p.D) *(f32x4*)(part + d) = f32x4{dqT[db][4 * g], dqT[db][4 * g + 1], dqT[db][4 * g + 2], dqT[db][4 * g + 3]};
+            }
+        return;
+    }
     __syncthreads();
     put_rows<NO>(ring0 + wave * 32 * TILE_LD<NO>, dqT, p.scale, !sees, live ? p.dq + (size_t)token * p.lddq + (size_t)head * p.D : nullptr, p.D);
     for (unsigned bad = bad_rows(sees && !(not_finite(dqT) == 0.f)); bad; bad &= bad - 1) {
@@ -210,13 +226,53 @@ __global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocA
     }
 }
 
+// the runs of a row, added in order: half a wave for a row
+__global__ __launch_bounds__(256) void doc_dq_join_kernel(const DocArgs p) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const size_t rows = (size_t)p.Tq * p.Hq, R0 = ((size_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 2;
+    if (R0 >= rows) return;
+    const size_t R = min(R0 + half, rows - 1);
+    const int token = (int)(R / p.Hq), head = (int)(R - (size_t)token * p.Hq);
+    const int4 span = p.rows[token];
+    const bool sees = span.y > span.x;
+    const int d = min((lane & 31) * 4, p.D - 4);
+    const float* part = p.part_q + R * p.D + d;
+    const size_t step = rows * p.D;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int z = 0; z < p.splits_q; z += 4) {
+        f32x4 v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = *(const f32x4*)(part + min(z + e, p.splits_q - 1) * step);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (z + e < p.splits_q) acc += v[e];
+    }
+    bool bad = false;
+    bf16x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bad |= !(acc[e] * 0.f == 0.f);
+        y[e] = sees ? (bf16_t)(acc[e] * p.scale) : (bf16_t)0.f;
+    }
+    if (R0 + half < rows && (lane & 31) * 4 < p.D) *(bf16x4*)(p.dq + (size_t)token * p.lddq + (size_t)head * p.D + d) = y;
+    const unsigned long long bads = __ballot(sees && bad && R0 + half < rows);
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h)
+        if ((unsigned)(bads >> (32 * h))) {
+            const int t = __shfl(token, 32 * h, 64), q = __shfl(head, 32 * h, 64);
+            const RowSpan s = {__shfl(span.x, 32 * h, 64), __shfl(span.y, 32 * h, 64), __shfl(span.z, 32 * h, 64)};
+            const size_t at = (size_t)q * p.Tq + t;
+            plain_dq_row(p, t, q, s, p.lse[at], p.delta[at]);
+        }
+}
+
 template <int ND, int NO>
 int launch(const DocArgs& a, hipStream_t st) {
     const int tiles = (int)(((long long)a.Tq * a.G + 127) / 128);
-    const dim3 grid(unit_grid(tiles, a.Hkv));
+    const dim3 grid(unit_grid((long long)tiles * a.splits_q, a.Hkv));
     if (a.drop_thresh) hipLaunchKernelGGL((doc_dq_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a, tiles);
     else if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) hipLaunchKernelGGL((doc_dq_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a, tiles);
     else hipLaunchKernelGGL((doc_dq_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a, tiles);
+    if (a.splits_q > 1) hipLaunchKernelGGL(doc_dq_join_kernel, dim3((unsigned)(((size_t)a.Tq * a.Hq + 7) / 8)), dim3(256), 0, st, a);
     return mi355_check_launch("doc_attention_dq");
 }
 

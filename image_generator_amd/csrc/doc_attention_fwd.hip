@@ -141,11 +141,39 @@ struct Rows {                        // a wave's 32 rows
     }
     // the two lanes of a row hold the sums of the keys whose scores they hold
     __device__ __forceinline__ void join() { l += __shfl_xor(l, 32, 64); }
-    __device__ __forceinline__ bool fits() const { return span.hi <= span.lo || (l > 0x1p-60f && l < 0x1p100f); }
+    // the row sees keys of the run [from, to)
+    __device__ __forceinline__ bool some(int from, int to) const { return max(span.lo, from) < min(span.hi, to); }
+    __device__ __forceinline__ bool fits(int from, int to) const { return !some(from, to) || (l > 0x1p-60f && l < 0x1p100f); }
     // rows whose result is not finite
     __device__ __forceinline__ unsigned bad() const {
         const float z = not_finite(o) + l * 0.f;
         return bad_rows(span.hi > span.lo && !(z == 0.f));
+    }
+    // The unnormalised result of the run [from, to), for the join; R0: the wave's first row of `rows`.  m = -inf: no key of the run is
+    // seen, the values stay unwritten and unread.
+    __device__ __forceinline__ void leave(const DocArgs& p, unsigned rows, unsigned R0, int hk, int split, int from, int to) const {
+        const int lane = threadIdx.x & 63, hh = lane >> 5;
+        const size_t row = ((size_t)hk * rows + R0 + (lane & 31)) * p.splits + split;
+        float2* ml = (float2*)p.part;
+        float* parts = p.part + (size_t)p.Hkv * rows * p.splits * 2;
+        const bool any = some(from, to) && !(l == 0.f);
+        if (hh == 0) ml[row] = make_float2(any ? m : -INFINITY, any ? l : 0.f);
+#pragma unroll
+        for (int db = 0; db < NO; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = db * 32 + 8 * g + 4 * hh;
+                if (any && d < p.D) *(f32x4*)(parts + row * p.D + d) = f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+            }
+        for (unsigned bads = from < to ? bad() : 0u; bads; bads &= bads - 1) {
+            const int t = __builtin_ctz(bads);
+            float pm, pl, po[2];
+            plain_row(p, __shfl(token, t, 64), __shfl(head, t, 64), max(__shfl(span.lo, t, 64), from), min(__shfl(span.hi, t, 64), to), __shfl(span.c, t, 64), pm, pl, po);
+            const size_t at = ((size_t)hk * rows + R0 + t) * p.splits + split;
+            if (lane == 0) ml[at] = make_float2(pm, pl);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) if (lane + 64 * u < p.D) parts[at * p.D + lane + 64 * u] = po[u];
+        }
     }
 };
 
@@ -154,8 +182,10 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
     __shared__ __attribute__((aligned(16))) char even[2 * TILE_BYTES<NO>], odd[2 * TILE_BYTES<NO>];      // K and V, twice
     __shared__ int range[4][2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
-    int tile, hk;
-    if (!unit_of(tiles, p.Hkv, tile, hk)) return;
+    int unit, hk;
+    if (!unit_of(tiles * p.splits, p.Hkv, unit, hk)) return;
+    const int split = unit / tiles;
+    int tile = unit - split * tiles;
     if (p.causal) tile = tiles - 1 - tile;       // the last rows of a document see most: the longest work first
     Rows<ND, NO> w;
     w.init(p, tile * 128u + wave * 32, hk);
@@ -163,6 +193,8 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
     __syncthreads();
     const int klo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
     const int khi = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
+    int from, to;
+    run_of(klo, khi, p.splits, split, from, to);
     const Bend bend(p);
     const bf16_t *kbase = p.k + (size_t)hk * p.D, *vbase = p.v + (size_t)hk * p.D;
     const Reads<ND, NO> at;
@@ -178,23 +210,32 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
             if (k0 < w.hi && k0 + 64 > w.lo) w.template tile<KIND, decltype(fast)::value>(p, bend, at, Ks, Ks + TILE_BYTES<NO>, k0);
         };
         w.reset(decltype(fast)::value ? 0.f : -INFINITY);
-        if (klo < khi) request(even, klo);
-        if constexpr (decltype(fast)::value) w.settle(p);
-        for (int k0 = klo; k0 < khi; k0 += 128) {
+        if (from < to) request(even, from);
+        w.settle(p);
+        for (int k0 = from; k0 < to; k0 += 128) {
             tiles_landed();                        // ... and every wave has left the tile before
-            if (k0 + 64 < khi) request(odd, k0 + 64);
+            if (k0 + 64 < to) request(odd, k0 + 64);
             visit(even, k0);
-            if (k0 + 64 >= khi) break;
+            if (k0 + 64 >= to) break;
             tiles_landed();
-            if (k0 + 128 < khi) request(even, k0 + 128);
+            if (k0 + 128 < to) request(even, k0 + 128);
             visit(odd, k0 + 64);
         }
         w.join();
     };
-    pass(std::true_type{});
-    if (__syncthreads_or(!w.fits())) {           // (the loop has barriers: the workgroup decides as one)
+    // far runs under a distance bias have nothing but tiny sums
+    bool shifted = p.splits > 1 && bend.biased;
+    if (!shifted) {
+        pass(std::true_type{});
+        shifted = __syncthreads_or(!w.fits(from, to));             // (the loop has barriers: the workgroup decides as one)
+    }
+    if (shifted) {
         pass(std::false_type{});
         __syncthreads();
+    }
+    if (p.splits > 1) {
+        w.leave(p, tiles * 128u, tile * 128u + wave * 32, hk, split, from, to);
+        return;
     }
     const bool none = w.span.hi <= w.span.lo;
     put_rows<NO>(even + wave * 32 * TILE_LD<NO>, w.o, w.l > 0.f ? 1.f / w.l : 0.f, none,
@@ -256,31 +297,7 @@ __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) 
         }
         w.join();
     }
-    const bool some = max(w.span.lo, from) < min(w.span.hi, to);     // the row sees keys of this run
-    const size_t rows = (size_t)gridDim.x * 32, row = ((size_t)hk * rows + R) * p.splits + split;
-    float2* ml = (float2*)p.part;
-    float* part = p.part + (size_t)p.Hkv * rows * p.splits * 2 + row * p.D;
-    // (m = -inf: no key of the run is seen, the values stay unwritten and unread)
-    const bool any = some && !(w.l == 0.f);
-    if (hh == 0) ml[row] = make_float2(any ? w.m : -INFINITY, any ? w.l : 0.f);
-#pragma unroll
-    for (int db = 0; db < NO; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int d = db * 32 + 8 * g + 4 * hh;
-            if (any && d < p.D) *(f32x4*)(part + d) = f32x4{w.o[db][4 * g], w.o[db][4 * g + 1], w.o[db][4 * g + 2], w.o[db][4 * g + 3]};
-        }
-    for (unsigned bad = from < to ? w.bad() : 0u; bad; bad &= bad - 1) {
-        const int t = __builtin_ctz(bad);
-        const int lo = max(__shfl(w.span.lo, t, 64), from), hi = min(__shfl(w.span.hi, t, 64), to);
-        float m, l, o[2];
-        plain_row(p, __shfl(w.token, t, 64), __shfl(w.head, t, 64), lo, hi, __shfl(w.span.c, t, 64), m, l, o);
-        const size_t at = ((size_t)hk * rows + blockIdx.x * 32u + t) * p.splits + split;
-        if (lane == 0) ml[at] = make_float2(m, l);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-            if (lane + 64 * u < p.D) p.part[(size_t)p.Hkv * rows * p.splits * 2 + at * p.D + lane + 64 * u] = o[u];
-    }
+    w.leave(p, gridDim.x * 32u, blockIdx.x * 32u, hk, split, from, to);
 }
 
 // out = sum o_s 2^(m_s - M) / sum l_s 2^(m_s - M) over the runs of a row: a wave per row, at most 64 runs
@@ -329,18 +346,23 @@ __global__ __launch_bounds__(256) void doc_fwd_join_kernel(const DocArgs p, unsi
     if (lane == 0) p.lse[(size_t)head * p.Tq + token] = nan ? NAN : l == 0.f ? -INFINITY : M + log2f(l);
 }
 
-// Runs per row where the unsplit grid (a workgroup for 128 rows of a key head) leaves most of the chip idle and there are keys to
-// deal out: about 2048 waves, runs of four tiles at least, at most 64 of them.  0: no split.
-static int fwd_splits(int Tq, int Tk, int Hq, int Hkv) {
-    const long long rows = (long long)Tq * (Hq / Hkv);
-    const long long wgs = (rows + 127) / 128 * Hkv;
-    if (wgs >= 256 || Tk < 1024) return 0;
+// Rows of a document that are few (single queries) share no tile worth its staging: waves take runs by themselves, about 2048 of them,
+// of four tiles at least, at most 64 for a row.  Longer documents: key_runs().
+struct Plan {
+    bool waves;
+    int splits;
+    size_t rows;                     // of a key head, padded to whole tiles
+};
+static Plan plan(int Tq, int Tk, int Hq, int Hkv, int docs) {
+    const long long rows = (long long)Tq * (Hq / Hkv), wgs = (rows + 127) / 128 * Hkv;
+    if (rows >= 64ll * docs || wgs >= 256 || Tk < 1024) return {false, key_runs(Tq, Tk, Hq, Hkv, docs), (size_t)(rows + 127) / 128 * 128};
     long long s = 2048 / ((rows + 31) / 32 * Hkv);
     const long long most = (Tk + 255) / 256;
     if (s > most) s = most;
     if (s > 64) s = 64;
     s = s / 4 * 4;
-    return s < 4 ? 0 : (int)s;
+    if (s < 4) return {false, 1, (size_t)(rows + 127) / 128 * 128};
+    return {true, (int)s, (size_t)(rows + 31) / 32 * 32};
 }
 
 template <int ND, int NO, int KIND>
@@ -357,26 +379,28 @@ int launch_split(const DocArgs& a, hipStream_t st) {
 }
 
 template <int ND, int NO>
-int launch(const DocArgs& a, hipStream_t st) {
+int launch(const DocArgs& a, const Plan& how, hipStream_t st) {
     const bool bent = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
-    if (a.splits)
+    if (how.waves)
         return a.drop_thresh ? launch_split<ND, NO, DROPPED>(a, st) : bent ? launch_split<ND, NO, BENT>(a, st) : launch_split<ND, NO, PLAIN>(a, st);
-    const int tiles = (int)(((long long)a.Tq * a.G + 127) / 128);
-    const dim3 grid(unit_grid(tiles, a.Hkv));
+    const int tiles = (int)(how.rows / 128);
+    const dim3 grid(unit_grid((long long)tiles * a.splits, a.Hkv));
     if (a.drop_thresh) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, DROPPED>), grid, dim3(256), 0, st, a, tiles);
     else if (bent) hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, BENT>), grid, dim3(256), 0, st, a, tiles);
     else hipLaunchKernelGGL((doc_fwd_kernel<ND, NO, PLAIN>), grid, dim3(256), 0, st, a, tiles);
+    if (a.splits > 1) hipLaunchKernelGGL(doc_fwd_join_kernel, dim3((unsigned)(((long long)a.Tq * a.G + 3) / 4), a.Hkv), dim3(256), 0, st, a, (unsigned)how.rows);
     return mi355_check_launch("doc_attention_fwd");
 }
 
 }  // namespace
 
 int doc_fwd_tiles(const DocArgs& a, hipStream_t st) {
+    const Plan how = plan(a.Tq, a.Tk, a.Hq, a.Hkv, a.docs);
     DocArgs b = a;
-    b.splits = fwd_splits(a.Tq, a.Tk, a.Hq, a.Hkv);
-    return BY_WIDTH(a.D, launch, b, st);
+    b.splits = how.splits;
+    return BY_WIDTH(a.D, launch, b, how, st);
 }
-size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D) {
-    const size_t s = fwd_splits(Tq, Tk, Hq, Hkv), rows = ((size_t)Tq * (Hq / Hkv) + 31) / 32 * 32 * Hkv;
-    return rows * s * (D + 2) * 4;
+size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D, int docs) {
+    const Plan how = plan(Tq, Tk, Hq, Hkv, docs);
+    return how.splits > 1 ? how.rows * Hkv * how.splits * (D + 2) * 4 : 0;
 }

@@ -295,7 +295,28 @@ int doc_fwd_tiles(const DocArgs& a, hipStream_t st);
 int doc_bwd_q_tiles(const DocArgs& a, hipStream_t st);
 int doc_bwd_kv_tiles(const DocArgs& a, hipStream_t st);
 int doc_bwd_kv_splits(int Tq, int Tk, int Hq, int Hkv, int docs, int causal);
-size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D);
+size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D, int docs);
+
+// Runs of keys for each tile of 128 rows, where the tiles alone leave much of the chip idle (few heads, few long documents): as many as
+// make 768 workgroups, three to a CU, each run of at least RUN_TILES tiles; 1: none.  A second launch adds the runs up.
+constexpr int RUN_TILES = 6;
+inline int key_runs(int Tq, int Tk, int Hq, int Hkv, int docs) {
+    const long long wgs = ((long long)Tq * (Hq / Hkv) + 127) / 128 * Hkv;
+    long long s = wgs >= 384 || wgs == 0 ? 1 : 768 / wgs;
+    const long long most = (long long)Tk / docs / (64 * RUN_TILES);
+    if (s > most) s = most;
+    return s < 2 ? 1 : s > 32 ? 32 : (int)s;
+}
+// the run `split` of [lo, hi), cut at whole tiles
+__device__ __forceinline__ void run_of(int lo, int hi, int splits, int split, int& from, int& to) {
+    from = lo;
+    to = hi;
+    if (splits > 1 && lo < hi) {
+        const int n = (hi - lo + 63) / 64, each = (n + splits - 1) / splits;
+        from = lo + min(n, each * split) * 64;
+        to = min(hi, lo + min(n, each * (split + 1)) * 64);
+    }
+}
 
 // FN<ND, NO>(args...) for the head width: ND 16-wide steps of a contraction over it, NO 32-wide blocks of it
 #define BY_WIDTH(D, FN, ...)                              \

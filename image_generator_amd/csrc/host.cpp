@@ -190,7 +190,7 @@ PyObject* doc_attention_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Docs d = docs_of(a, whole32(a[DOC_ARGS], "device"));
         void* stream = (void*)whole(a[DOC_ARGS + 1]);
         at::Tensor out = at::empty(d.q->sizes(), d.q->options()), lse = at::empty({d.heads, d.Tq}, d.q->options().dtype(at::kFloat)), ws;
-        const size_t need = lib.mi355_doc_attention_fwd_workspace_bytes(d.Tq, d.Tk, d.heads, d.kv_heads, d.width);
+        const size_t need = lib.mi355_doc_attention_fwd_workspace_bytes(d.Tq, d.Tk, d.heads, d.kv_heads, d.width, d.docs);
         if (need) ws = at::empty({(int64_t)need}, d.q->options().dtype(at::kByte));
         checked(without_gil([&] {
             return lib.mi355_doc_attention_fwd(d.q->data_ptr(), d.k->data_ptr(), d.v->data_ptr(), out.data_ptr(), (float*)lse.data_ptr(),

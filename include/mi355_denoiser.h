@@ -434,7 +434,7 @@ int mi355_copy2d_f32_batched(const long long* table, int n, void* stream);
  * drop_p, seed: dropout on the probabilities, the same in both directions for the same seed.
  * Everything is summed in an order that depends on the sizes alone: equal calls return equal bits.  ws: a device buffer of the
  * queried size (which may be 0), 16-byte aligned, for this call alone. */
-size_t mi355_doc_attention_fwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D);
+size_t mi355_doc_attention_fwd_workspace_bytes(int Tq, int Tk, int Hq, int Hkv, int D, int docs);
 int mi355_doc_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int* q_off, const int* k_off,
                             int docs, const int* prefix, const float* slopes, float cap, int causal, int align_start, int Tq,
                             int Tk, int Hq, int Hkv, int D, long long ldq, long long ldk, long long ldv, long long ldo,

@@ -496,3 +496,56 @@ def test_gradients_of_few_keys_do_not_carry_the_rounding_of_the_result(lens, d, 
         for name, want, bound in (("dq", scale * dS @ K, scale * tol @ K.abs()), ("dk", scale * dS.T @ Q, scale * tol.T @ Q.abs())):
             x = got[name][rows].cpu().double()
             assert ((x - want).abs() <= 1.05 * (bound + 2.0 ** -8 * want.abs()) + 1e-30).all(), (name, n, float((x - want).abs().max()), float(want.abs().max()))
+
+
+@pytest.mark.parametrize("lens", [[2500, 40], [1, 2600], [1900]])
+@pytest.mark.parametrize("how", [dict(), dict(causal=True), dict(causal=True, cap=5.0, bias=True), dict(bias=True), dict(causal=True, drop_p=0.3, seed=7), dict(cap=3.0, prefix=True, causal=True)],
+                         ids=["plain", "causal", "bent", "bias", "dropped", "prefix"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 1, 64), (1, 1, 96), (2, 2, 128)])
+def test_few_tiles_over_many_keys(lens, how, heads, kv_heads, d):
+    """Few heads, few long documents: the keys of a tile of rows are dealt out in runs, in both directions."""
+    from image_generator_amd._lib import lib
+    off = offsets(lens)
+    T = int(off[-1])
+    assert lib.mi355_doc_attention_fwd_workspace_bytes(T, T, heads, kv_heads, d, len(lens)) > 0            # in runs
+    how = dict(how)
+    if how.pop("bias", False):
+        how["slopes"] = torch.tensor([0.5, 0.01][:heads])            # far runs that weigh nothing, and some that do
+    if how.pop("prefix", False):
+        how["prefix"] = torch.tensor([n // 3 for n in lens], dtype=torch.int32)
+    x = inputs(T, T, heads, kv_heads, d, 35)
+    got = run(*x, heads=heads, kv_heads=kv_heads, q_offsets=off, **how)
+    p, seed = how.pop("drop_p", 0.0), how.pop("seed", 0)
+    ref = reference(*x, heads, kv_heads, off, off, keep=keep_mask(heads, T, T, p, seed) if p else None, drop=p, **how)
+    check(got, ref)
+    assert (got["lse"].cpu().double() - ref[1]).abs().max() < 2.0 ** -8
+    again = run(*x, heads=heads, kv_heads=kv_heads, q_offsets=off, **how, drop_p=p, seed=seed)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_what_is_not_finite_in_one_run(value):
+    """A key that only the last rows see, and one of the other document: nobody else is touched by either."""
+    off = offsets([2000, 500])
+    q, k, v, do = inputs(2500, 2500, 1, 1, 64, 36)
+    clean = [t.clone() for t in (q, k, v, do)]
+    for at in (1950, 2300):
+        k[at, 3] = value
+        v[at, 5] = value
+    got = run(q, k, v, do, heads=1, q_offsets=off, causal=True)
+    ref = reference(*clean, 1, 1, off, off, causal=True)
+    fine = torch.cat((torch.arange(0, 1950), torch.arange(2000, 2300)))
+    for n in ("out", "dq"):
+        val, tol = ref[0][n]
+        assert ((got[n].cpu().double() - val).abs() <= tol)[fine].all(), n
+    assert not torch.isfinite(got["out"][1950:2000]).all() and not torch.isfinite(got["dq"][2300:]).all()
+
+
+def test_queries_behind_many_keys_in_runs():
+    """Appended queries over a long past, fewer keys than queries in one document, and tokens of none."""
+    qo, ko = offsets([300, 200, 0], 5), offsets([3000, 100, 900], 2)
+    x = inputs(520, 4010, 2, 1, 48, 37)
+    how = dict(causal=True, slopes=torch.tensor([0.02, 0.0]))
+    got = run(*x, heads=2, kv_heads=1, q_offsets=qo, k_offsets=ko, **how)
+    check(got, reference(*x, 2, 1, qo, ko, **how))
+    assert (got["out"][:5] == 0).all() and (got["dq"][505:] == 0).all() and (got["dk"][-8:] == 0).all()

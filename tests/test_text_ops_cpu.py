@@ -70,7 +70,7 @@ def test_doc_attention_refusals():
     for kw, why in ((dict(ld=4), "strides"), (dict(ldd=32), "overlap"), (dict(ptr=24), "aligned"), (dict(ptr=None), "null"),
                     (dict(ws_bytes=8), "workspace"), (dict(prefix=16), "prefix")):
         assert bwd(**kw) == -1 and why in err(), (kw, err())
-    assert lib.mi355_doc_attention_bwd_workspace_bytes(-1, 4, 2, 2, 32, 1, 0) == 0 and lib.mi355_doc_attention_fwd_workspace_bytes(4, 4, 3, 2, 32) == 0
+    assert lib.mi355_doc_attention_bwd_workspace_bytes(-1, 4, 2, 2, 32, 1, 0) == 0 and lib.mi355_doc_attention_fwd_workspace_bytes(4, 4, 3, 2, 32, 1) == 0
 
 
 def test_host_extension_refusals():
