@@ -29,6 +29,7 @@ struct DocArgs {
     float drop_scale;
     float* part;                    // partial results of `splits` runs (of keys: forward; of rows: dK and dV); 1: none
     int splits;
+    int wave_rows;                  // rows of a wave that takes runs of keys by itself
     float* part_q;                  // the dQ pass's, over `splits_q` runs of keys
     int splits_q;
 };

@@ -331,7 +331,7 @@ int launch(const DocArgs& a, hipStream_t st) {
 }  // namespace
 
 // Workgroups without a split: one per 128 keys and key head, each passing about G * (the rows of one document, and of the others
-// that its keys belong to).  Runs of at least 8 tiles; without a causal mask as many as are resident at once (two workgroups
+// that its keys belong to).  Runs of at least three tiles; without a causal mask as many as are resident at once (two workgroups
 // per CU: 8 x 4096 rows over 210 keys took 48 us with three times as many, 36 us with these), with one four times as many, which
 // evens out that the first keys of a document are passed by all its rows and the last by few (twice as many were slower).
 int doc_bwd_kv_splits(int Tq, int Tk, int Hq, int Hkv, int docs, int causal) {
@@ -339,7 +339,7 @@ int doc_bwd_kv_splits(int Tq, int Tk, int Hq, int Hkv, int docs, int causal) {
     const double wgs = (double)((Tk + 127) / 128) * Hkv, keys_per_doc = (double)Tk / docs;
     const double tiles = (double)Tq * (Hq / Hkv) / docs * (1.0 + 127.0 / (keys_per_doc < 1.0 ? 1.0 : keys_per_doc)) / 64.0;
     const double cap = (double)Tq * (Hq / Hkv) / 64.0;
-    double s = (causal ? 2048.0 : 512.0) / wgs, most = (tiles < cap ? tiles : cap) / 8.0;
+    double s = (causal ? 2048.0 : 512.0) / wgs, most = (tiles < cap ? tiles : cap) / 3.0;
     if (s > most) s = most;
     return s < 2.0 ? 1 : s > 64.0 ? 64 : (int)s;
 }

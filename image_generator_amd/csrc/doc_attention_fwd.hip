@@ -32,9 +32,9 @@ struct Rows {                        // a wave's 32 rows
     int in_lo, in_hi;                // their intersection
     int c_min;                       // first key position of a row
 
-    // R0: the wave's first row
-    __device__ __forceinline__ void init(const DocArgs& p, unsigned R0, int hk) {
-        const unsigned rows = (unsigned)p.Tq * (unsigned)p.G, R = R0 + (threadIdx.x & 31);
+    // R0: the wave's first row, `rows` the end of its rows (32 at most)
+    __device__ __forceinline__ void init(const DocArgs& p, unsigned R0, unsigned rows, int hk) {
+        const unsigned R = R0 + (threadIdx.x & 31);
         live = R < rows;
         row_of(p, live ? R : rows - 1, hk, token, head);
         const int first = __builtin_amdgcn_readfirstlane(token);
@@ -156,8 +156,8 @@ struct Rows {                        // a wave's 32 rows
         const size_t row = ((size_t)hk * rows + R0 + (lane & 31)) * p.splits + split;
         float2* ml = (float2*)p.part;
         float* parts = p.part + (size_t)p.Hkv * rows * p.splits * 2;
-        const bool any = some(from, to) && !(l == 0.f);
-        if (hh == 0) ml[row] = make_float2(any ? m : -INFINITY, any ? l : 0.f);
+        const bool any = live && some(from, to) && !(l == 0.f);
+        if (live && hh == 0) ml[row] = make_float2(any ? m : -INFINITY, any ? l : 0.f);
 #pragma unroll
         for (int db = 0; db < NO; ++db)
 #pragma unroll
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
     int tile = unit - split * tiles;
     if (p.causal) tile = tiles - 1 - tile;       // the last rows of a document see most: the longest work first
     Rows<ND, NO> w;
-    w.init(p, tile * 128u + wave * 32, hk);
+    w.init(p, tile * 128u + wave * 32, (unsigned)p.Tq * (unsigned)p.G, hk);
     if (lane == 0) { range[wave][0] = w.hi > w.lo ? w.lo : 0x7fffffff; range[wave][1] = w.hi; }
     __syncthreads();
     const int klo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
@@ -256,12 +256,12 @@ __global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_fwd
 template <int ND, int NO, int KIND>
 __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem_all[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, hh = lane >> 5;
+    const int wave = threadIdx.x >> 6;
     char *Ks = smem_all + wave * 2 * TILE_BYTES<NO>, *Vs = Ks + TILE_BYTES<NO>;
     const int hk = blockIdx.y, split = blockIdx.z * 4 + wave;
-    const unsigned R = blockIdx.x * 32u + l31;
+    const unsigned R0 = blockIdx.x * (unsigned)p.wave_rows;
     Rows<ND, NO> w;
-    w.init(p, blockIdx.x * 32u, hk);
+    w.init(p, R0, min((unsigned)p.Tq * (unsigned)p.G, R0 + p.wave_rows), hk);
     int from, to;
     {
         const int tiles = (w.hi - w.lo + 63) / 64, each = (tiles + p.splits - 1) / p.splits;
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256, 1) void doc_fwd_split_kernel(const DocArgs p) 
         }
         w.join();
     }
-    w.leave(p, gridDim.x * 32u, blockIdx.x * 32u, hk, split, from, to);
+    w.leave(p, gridDim.x * (unsigned)p.wave_rows, R0, hk, split, from, to);
 }
 
 // out = sum o_s 2^(m_s - M) / sum l_s 2^(m_s - M) over the runs of a row: a wave per row, at most 64 runs
@@ -347,22 +347,28 @@ __global__ __launch_bounds__(256) void doc_fwd_join_kernel(const DocArgs p, unsi
 }
 
 // Rows of a document that are few (single queries) share no tile worth its staging: waves take runs by themselves, about 2048 of them,
-// of four tiles at least, at most 64 for a row.  Longer documents: key_runs().
+// one tile at least, at most 64 for a row.  Where 64 runs of 32 rows make less than 768, a wave takes fewer rows, down to a
+// group's: a tile of keys is of use to its own document's rows alone, so nothing is read twice (30 queries of one head over 5000
+// keys each: 112 -> 17 us; but the fewer documents a wave has, the less even the runs: 48 queries of two groups over 339 602
+// keys, 82 us with 32 rows, 86 with 8).  Longer documents, and few keys (a tile or six, where a second launch costs more): key_runs().
 struct Plan {
     bool waves;
-    int splits;
+    int splits, wave_rows;
     size_t rows;                     // of a key head, padded to whole tiles
 };
-static Plan plan(int Tq, int Tk, int Hq, int Hkv, int docs) {
-    const long long rows = (long long)Tq * (Hq / Hkv), wgs = (rows + 127) / 128 * Hkv;
-    if (rows >= 64ll * docs || wgs >= 256 || Tk < 1024) return {false, key_runs(Tq, Tk, Hq, Hkv, docs), (size_t)(rows + 127) / 128 * 128};
-    long long s = 2048 / ((rows + 31) / 32 * Hkv);
-    const long long most = (Tk + 255) / 256;
+static Plan plan(int Tq, long long Tk, int Hq, int Hkv, int docs) {
+    const long long G = Hq / Hkv, rows = (long long)Tq * G, wgs = (rows + 127) / 128 * Hkv;
+    const Plan tiled = {false, key_runs(Tq, (int)Tk, Hq, Hkv, docs), 0, (size_t)(rows + 127) / 128 * 128};
+    if (rows >= 64ll * docs || wgs >= 256 || Tk < 384) return tiled;
+    int R = 32;
+    while (R > 1 && R / 2 >= G && (rows + R - 1) / R * Hkv * 64 < 768 && Tk * R / rows > 64 * 64) R /= 2;
+    const long long tiles = (rows + R - 1) / R;
+    long long s = 2048 / (tiles * Hkv);
+    const long long most = (Tk / tiles + 63) / 64;
     if (s > most) s = most;
     if (s > 64) s = 64;
-    s = s / 4 * 4;
-    if (s < 4) return {false, 1, (size_t)(rows + 127) / 128 * 128};
-    return {true, (int)s, (size_t)(rows + 31) / 32 * 32};
+    s = s < 4 ? 4 : s / 4 * 4;
+    return {true, (int)s, R, (size_t)(tiles * R)};
 }
 
 template <int ND, int NO, int KIND>
@@ -372,9 +378,9 @@ int launch_split(const DocArgs& a, hipStream_t st) {
     static hipError_t set;
     std::call_once(once, [] { set = hipFuncSetAttribute((const void*)doc_fwd_split_kernel<ND, NO, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
     if (set != hipSuccess) return mi355_fail(MI355_ERR_LAUNCH, "doc_attention: %s", hipGetErrorString(set));
-    const unsigned tiles = (unsigned)(((long long)a.Tq * a.G + 31) / 32);
+    const unsigned tiles = (unsigned)(((long long)a.Tq * a.G + a.wave_rows - 1) / a.wave_rows);
     hipLaunchKernelGGL((doc_fwd_split_kernel<ND, NO, KIND>), dim3(tiles, a.Hkv, a.splits / 4), dim3(256), LDS, st, a);
-    hipLaunchKernelGGL(doc_fwd_join_kernel, dim3((unsigned)(((long long)a.Tq * a.G + 3) / 4), a.Hkv), dim3(256), 0, st, a, tiles * 32);
+    hipLaunchKernelGGL(doc_fwd_join_kernel, dim3((unsigned)(((long long)a.Tq * a.G + 3) / 4), a.Hkv), dim3(256), 0, st, a, tiles * a.wave_rows);
     return mi355_check_launch("doc_attention_fwd(split)");
 }
 
@@ -398,6 +404,7 @@ int doc_fwd_tiles(const DocArgs& a, hipStream_t st) {
     const Plan how = plan(a.Tq, a.Tk, a.Hq, a.Hkv, a.docs);
     DocArgs b = a;
     b.splits = how.splits;
+    b.wave_rows = how.wave_rows;
     return BY_WIDTH(a.D, launch, b, how, st);
 }
 size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D, int docs) {

@@ -299,7 +299,7 @@ size_t doc_fwd_workspace(int Tq, int Tk, int Hq, int Hkv, int D, int docs);
 
 // Runs of keys for each tile of 128 rows, where the tiles alone leave much of the chip idle (few heads, few long documents): as many as
 // make 768 workgroups, three to a CU, each run of at least RUN_TILES tiles; 1: none.  A second launch adds the runs up.
-constexpr int RUN_TILES = 6;
+constexpr int RUN_TILES = 3;
 inline int key_runs(int Tq, int Tk, int Hq, int Hkv, int docs) {
     const long long wgs = ((long long)Tq * (Hq / Hkv) + 127) / 128 * Hkv;
     long long s = wgs >= 384 || wgs == 0 ? 1 : 768 / wgs;

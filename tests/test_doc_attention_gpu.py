@@ -549,3 +549,13 @@ def test_queries_behind_many_keys_in_runs():
     got = run(*x, heads=2, kv_heads=1, q_offsets=qo, k_offsets=ko, **how)
     check(got, reference(*x, 2, 1, qo, ko, **how))
     assert (got["out"][:5] == 0).all() and (got["dq"][505:] == 0).all() and (got["dk"][-8:] == 0).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(1, 1, 40), (3, 1, 64), (4, 2, 96), (8, 1, 128)])
+@pytest.mark.parametrize("ql", [[1] * 6, [3, 1, 0, 2, 1, 5]])
+def test_single_queries_over_long_pasts(heads, kv_heads, d, ql):
+    """Waves that take runs of keys by themselves, with as few rows each as it takes to fill the chip."""
+    qo, ko = offsets(ql), offsets([9000, 5000, 0, 1, 7000, 300])
+    x = inputs(int(qo[-1]), int(ko[-1]), heads, kv_heads, d, 38)
+    how = dict(causal=True, slopes=torch.tensor([0.5, 0.01, 0.0, 0.001, 0.1, 0.2, 0.003, 0.02][:heads]))
+    check(run(*x, heads=heads, kv_heads=kv_heads, q_offsets=qo, k_offsets=ko, **how), reference(*x, heads, kv_heads, qo, ko, **how))
