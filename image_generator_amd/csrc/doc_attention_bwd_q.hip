@@ -15,7 +15,7 @@ namespace {
 constexpr int FEW = 32;              // keys of a row whose delta is summed over them
 
 template <int ND, int NO, int KIND>
-__global__ __launch_bounds__(256, NO <= 2 ? 3 : 2) void doc_dq_kernel(const DocArgs p, int tiles) {
+__global__ __launch_bounds__(256, NO <= 2 && KIND == PLAIN ? 3 : 2) void doc_dq_kernel(const DocArgs p, int tiles) {
     // three: captions' tiles stay in place for both walks; of the widest heads they would leave one workgroup to a CU
     constexpr int BUFS = NO <= 3 && KIND == PLAIN ? 3 : 2;
     __shared__ __attribute__((aligned(16))) char ring0[2 * TILE_BYTES<NO>], ring1[2 * TILE_BYTES<NO>], ring2[BUFS == 3 ? 2 * TILE_BYTES<NO> : 16];
