@@ -4,10 +4,10 @@
 // dS is rounded to bf16 (the matrix units' type): 2^-9 of each entry at most beside the result's own rounding, 0.24 % instead of
 // 0.17 % in the 2-norm; -lse and -delta start the accumulators, in fp32.
 //
-// Measured, with what bounds it: 58 255 caption tokens, 8 heads of 96 (537 MB): 149 us, 3.6 TB/s, bound by the chain of a short
+// Measured, with what bounds it: 58 255 caption tokens, 8 heads of 96 (537 MB): 147 us, 3.7 TB/s, bound by the chain of a short
 // workgroup (offsets, rows, keys, three tiles, store) at two workgroups per CU.  Four documents of 4001 .. 8191 tokens, 8 heads on 2
-// of 64, causal with prefix, cap and bias (223 GFLOP): 409 us, 545 TFLOP/s, bound by vector issue (80 % of the cycles: tanh, bias,
-// exp2 and the conversions of a score against three products).  32768 image rows over 210 keys, 8 heads of 40: 34 us, 2.5 TB/s.
+// of 64, causal with prefix, cap and bias (223 GFLOP): 424 us, 526 TFLOP/s, bound by vector issue (80 % of the cycles: tanh, bias,
+// exp2 and the conversions of a score against three products); at three waves per SIMD its registers spill, 430 us.  32768 image rows over 210 keys, 8 heads of 40: 34 us, 2.5 TB/s.
 #include "doc_tiles.h"
 
 namespace {

@@ -183,7 +183,7 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(const void* __restri
         const bool in = i < n;
         key[u] = in ? pass_key<FIRST>(ids, ids64, keys, i, rows) : 0u;
         const unsigned d = (key[u] >> shift) & mask;
-        unsigned long long same = __ballot(in);              // lanes of this round that hold the same digit
+        unsigned long long same = __ballot(in);              // lanes of this step that hold the same digit
         for (int b = 0; b < bits; ++b) {
             const unsigned long long has = __ballot((d >> b) & 1);
             same &= (d >> b) & 1 ? has : ~has;
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(64) void super_sum_kernel(const unsigned* __restric
 // Every row of the table, written once: a wave takes the sorted positions of its id (found by binary search) in order, whole
 // aligned chunks and runs of chunks from their sums; an id without positions gets zeros.  Bound by the chain of search, positions,
 // rows and store: 16384 x 768 fp32 (50 MB) of 1601 ids 15.5 us, of 262143 ids 63 us with the rows that no chunk holds.
-constexpr int ROWS_PER_WG = 7;       // eight boundaries: two rounds of the workgroup's four waves
+constexpr int ROWS_PER_WG = 7;       // eight boundaries: two for each of four waves
 template <typename T, typename TO, int VEC>
 __global__ __launch_bounds__(256) void table_grad_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ pos, int n,
                                                          unsigned rows, const T* __restrict__ dy, int width, float scale,
