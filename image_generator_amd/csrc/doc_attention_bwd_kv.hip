@@ -282,14 +282,13 @@ __global__ __launch_bounds__(256, NO <= 2 || (NO == 3 && KIND == PLAIN) ? 2 : 1)
         plain_dkdv_key(p, key0 + __builtin_ctz(bad), hk);
 }
 
-// the partial gradients of a key, added in order: a wave per (key, key head)
+// The partial gradients of a key, added in order: a wave per (key, key head).  A key that no row sees has sums of zeros, or, beside rows
+// that are not finite, what plain_dkdv_key replaces by zeros.
 __global__ __launch_bounds__(256) void doc_dkdv_join_kernel(const DocArgs p) {
     const int lane = threadIdx.x & 63;
     const size_t u = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (u >= (size_t)p.Tk * p.Hkv) return;
     const int key = (int)(u / p.Hkv), hk = (int)(u % p.Hkv);
-    const int2 span = key_span(p, key);
-    const bool seen = span.y > span.x;
     const int n = 2 * p.D, at = min(lane * 4, n - 4);      // dK then dV: at most 256 values, four a lane
     const float* part = p.part + u * n + at;
     const size_t step = (size_t)p.Tk * p.Hkv * n;
@@ -311,10 +310,10 @@ __global__ __launch_bounds__(256) void doc_dkdv_join_kernel(const DocArgs p) {
         bf16_t* to = v ? p.dv + (size_t)key * p.lddv + (size_t)hk * p.D + at - p.D : p.dk + (size_t)key * p.lddk + (size_t)hk * p.D + at;
         bf16x4 y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = seen ? (bf16_t)(v ? acc[e] : acc[e] * p.scale) : (bf16_t)0.f;
+        for (int e = 0; e < 4; ++e) y[e] = (bf16_t)(v ? acc[e] : acc[e] * p.scale);
         *(bf16x4*)to = y;
     }
-    if (seen && __ballot(bad) != 0) plain_dkdv_key(p, key, hk);
+    if (__ballot(bad) != 0) plain_dkdv_key(p, key, hk);
 }
 
 template <int ND, int NO>
