@@ -559,3 +559,34 @@ def test_single_queries_over_long_pasts(heads, kv_heads, d, ql):
     x = inputs(int(qo[-1]), int(ko[-1]), heads, kv_heads, d, 38)
     how = dict(causal=True, slopes=torch.tensor([0.5, 0.01, 0.0, 0.001, 0.1, 0.2, 0.003, 0.02][:heads]))
     check(run(*x, heads=heads, kv_heads=kv_heads, q_offsets=qo, k_offsets=ko, **how), reference(*x, heads, kv_heads, qo, ko, **how))
+
+
+@pytest.mark.parametrize("ql,kl,train", [([2500, 40], None, True), ([1] * 4, [3000, 100, 4000, 50], False)], ids=["tiles", "waves"])
+def test_runs_captured_and_replayed_in_two_graphs(ql, kl, train):
+    """Partial results live in workspaces of the capture: two graphs, replayed in turn with eager calls between, do not meet in them."""
+    from image_generator_amd import ops
+    qo = offsets(ql).cuda()
+    ko = qo if kl is None else offsets(kl).cuda()
+    xs = [[t.cuda() for t in inputs(int(qo[-1]), int(ko[-1]), 2, 1, 64, 40 + i)] for i in range(2)]
+    how = dict(heads=2, kv_heads=1, q_offsets=qo, k_offsets=ko, causal=True)
+
+    def call(x):
+        out, lse = ops.doc_attention_fwd(*x[:3], **how)
+        return (out, lse, *(ops.doc_attention_bwd(x[3], *x[:3], out, lse, **how) if train else ()))
+
+    call(xs[0])
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for x in xs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(call(x))
+    for _ in range(3):
+        for x in xs:
+            for t in x:
+                t.normal_()
+        for g in graphs:
+            g.replay()
+        want = [call(x) for x in xs]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
