@@ -139,14 +139,21 @@ __device__ __forceinline__ double lane63(double x) {
     const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)b, 63), hi = (unsigned)__builtin_amdgcn_readlane((int)(b >> 32), 63);
     return __longlong_as_double(((long long)hi << 32) | lo);
 }
-__device__ __forceinline__ double wave_max_pos(double x) {
-    x = fmax(x, dpp_d<0x111, 0xf>(x));
-    x = fmax(x, dpp_d<0x112, 0xf>(x));
-    x = fmax(x, dpp_d<0x114, 0xf>(x));
-    x = fmax(x, dpp_d<0x118, 0xf>(x));
-    x = fmax(x, dpp_d<0x142, 0xa>(x));
-    x = fmax(x, dpp_d<0x143, 0xc>(x));
-    return lane63(x);
+__device__ __forceinline__ unsigned wave_max_u(unsigned x) {
+    int v = (int)x;
+    auto top = [](int a, int b) { return (int)max((unsigned)a, (unsigned)b); };
+    v = top(v, dpp<0x111, 0xf>(v, v));
+    v = top(v, dpp<0x112, 0xf>(v, v));
+    v = top(v, dpp<0x114, 0xf>(v, v));
+    v = top(v, dpp<0x118, 0xf>(v, v));
+    v = top(v, dpp<0x142, 0xa>(v, v));
+    v = top(v, dpp<0x143, 0xc>(v, v));
+    return (unsigned)__builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ double wave_max_pos(double x) {        // the same of doubles: the upper halves, then the lower ones of their lanes
+    const unsigned long long b = (unsigned long long)__double_as_longlong(x);
+    const unsigned hi = (unsigned)(b >> 32), top = wave_max_u(hi), low = wave_max_u(hi == top ? (unsigned)b : 0u);
+    return __longlong_as_double((long long)((unsigned long long)top << 32 | low));
 }
 __device__ __forceinline__ double wave_sum_d(double x) {
     x += dpp_d<0x111, 0xf>(x);
@@ -293,12 +300,18 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
             uss[u] = u_scales[blk];
         }
     }
-    double norm;
-    if (!norm_of(partial, state, norm) || g == 0) return;
-    const double b1 = hyper[H_B1], b2 = hyper[H_B2], omb1 = hyper[H_OMB1], omb2 = hyper[H_OMB2];
+    // what the norm says, by one wave for the four (the sum, a root and a division in fp64 were an eighth of the instructions)
+    __shared__ double said[2];
+    if (wave == 0) {
+        double norm, clip = 1.0;
+        const bool fine = norm_of(partial, state, norm);
+        if (hyper[H_MAX] > 0.0) { clip = hyper[H_MAX] / (norm + 1e-6); if (clip > 1.0) clip = 1.0; }
+        if (lane == 0) { said[0] = clip; said[1] = fine ? 1.0 : 0.0; }
+    }
+    __syncthreads();
+    if (said[1] == 0.0 || g == 0) return;
+    const double c = said[0], b1 = hyper[H_B1], b2 = hyper[H_B2], omb1 = hyper[H_OMB1], omb2 = hyper[H_OMB2];
     const float eps = (float)hyper[H_EPS], decay = (float)hyper[H_DECAY], step = (float)hyper[H_STEP], rbc2 = (float)hyper[H_RBC2];
-    double c = 1.0;
-    if (hyper[H_MAX] > 0.0) { c = hyper[H_MAX] / (norm + 1e-6); if (c > 1.0) c = 1.0; }
     const double omb1c = omb1 * c, omb2c = omb2 * c * c;
 #pragma unroll
     for (int u = 0; u < MINE; ++u) {
@@ -335,8 +348,7 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
         // Codes from fp32 roots, whose positions are good to 6.3e-5 (two roots of 1 ulp each on a ratio rounded once, times 255);
         // a lane with a position within twice that of the border of two codes takes the fp64 roots: one wave and block in ten.
         constexpr float SURE = 0.5f - 1.25e-4f;
-        int qm[4], qu[4];
-        f32x4 uf;
+        f32x4 qm, qu, uf;                                            // codes as whole floats
         bool near = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -344,8 +356,8 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
             const float ratio = __builtin_amdgcn_sqrtf((float)(ve[e] * ru2)), tu = 255.f * __builtin_amdgcn_sqrtf(ratio);
             const float fm = floorf(tm + 0.5f), fu = floorf(tu + 0.5f);
             near |= fabsf(tm - fm) > SURE || fabsf(tu - fu) > SURE;
-            qm[e] = (int)fm;
-            qu[e] = (int)fu;
+            qm[e] = fm;
+            qu[e] = fu;
             uf[e] = ratio * umax;
         }
         if (umax == 0.f) {                                           // (uniform) roots too small to be held still divide
@@ -357,20 +369,18 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
         if (near) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                qm[e] = (int)fma(127.0, root(fabs(me[e]) * rm), HALF);
-                qu[e] = (int)fma(255.0, root(root(ve[e] * ru2)), HALF);
+                qm[e] = (float)(int)fma(127.0, root(fabs(me[e]) * rm), HALF);
+                qu[e] = (float)(int)fma(255.0, root(root(ve[e] * ru2)), HALF);
             }
         }
         if (in) store_param(t, i, pv);
         unsigned mo = 0, uo = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            int q = min(qm[e], 127);
-            if (mf[e] < 0.f) q = -q;
-            mo |= (unsigned)(q & 255) << (8 * e);
-            q = min(qu[e], 255);
-            if (ve[e] > 0.0 && umax > 0.f) q = max(q, 1);
-            uo |= (unsigned)q << (8 * e);
+            // (no ratio is above 1 + 2^-24, no code above 127 and 255)
+            const float sq = mf[e] < 0.f ? -qm[e] : qm[e];
+            mo = __builtin_amdgcn_cvt_pk_u8_f32(sq < 0.f ? sq + 256.f : sq, e, mo);
+            uo = __builtin_amdgcn_cvt_pk_u8_f32(ve[e] > 0.0 && umax > 0.f ? fmaxf(qu[e], 1.f) : qu[e], e, uo);
         }
         m_codes[w] = mo;
         u_codes[w] = uo;
