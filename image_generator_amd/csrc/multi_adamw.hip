@@ -118,16 +118,18 @@ __global__ __launch_bounds__(512) void multi_sumsq_kernel(const Rec* __restrict_
 // Reductions over a wave by DPP: within rows of 16 lanes, then across them; lane 63 holds the result.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int dpp(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false); }
-__device__ __forceinline__ float wave_max_pos(float x) {          // of values >= 0, whose bits order like whole numbers
-    int v = __float_as_int(x);
-    v = max(v, dpp<0x111, 0xf>(v, v));
-    v = max(v, dpp<0x112, 0xf>(v, v));
-    v = max(v, dpp<0x114, 0xf>(v, v));
-    v = max(v, dpp<0x118, 0xf>(v, v));
-    v = max(v, dpp<0x142, 0xa>(v, v));
-    v = max(v, dpp<0x143, 0xc>(v, v));
-    return __int_as_float(__builtin_amdgcn_readlane(v, 63));
+// the largest of whole numbers: 0, what lanes without a source get, changes none, which lets the move join the comparison
+__device__ __forceinline__ unsigned wave_max_u(unsigned v) {
+    v = max(v, (unsigned)dpp<0x111, 0xf>(0, (int)v));
+    v = max(v, (unsigned)dpp<0x112, 0xf>(0, (int)v));
+    v = max(v, (unsigned)dpp<0x114, 0xf>(0, (int)v));
+    v = max(v, (unsigned)dpp<0x118, 0xf>(0, (int)v));
+    v = max(v, (unsigned)dpp<0x142, 0xa>(0, (int)v));
+    v = max(v, (unsigned)dpp<0x143, 0xc>(0, (int)v));
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
+// of values >= 0, whose bits order like whole numbers
+__device__ __forceinline__ float wave_max_pos(float x) { return __uint_as_float(wave_max_u(__float_as_uint(x))); }
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_d(double x) {               // lanes without a source get 0
     const long long b = __double_as_longlong(x);
@@ -138,17 +140,6 @@ __device__ __forceinline__ double lane63(double x) {
     const long long b = __double_as_longlong(x);
     const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)b, 63), hi = (unsigned)__builtin_amdgcn_readlane((int)(b >> 32), 63);
     return __longlong_as_double(((long long)hi << 32) | lo);
-}
-__device__ __forceinline__ unsigned wave_max_u(unsigned x) {
-    int v = (int)x;
-    auto top = [](int a, int b) { return (int)max((unsigned)a, (unsigned)b); };
-    v = top(v, dpp<0x111, 0xf>(v, v));
-    v = top(v, dpp<0x112, 0xf>(v, v));
-    v = top(v, dpp<0x114, 0xf>(v, v));
-    v = top(v, dpp<0x118, 0xf>(v, v));
-    v = top(v, dpp<0x142, 0xa>(v, v));
-    v = top(v, dpp<0x143, 0xc>(v, v));
-    return (unsigned)__builtin_amdgcn_readlane(v, 63);
 }
 __device__ __forceinline__ double wave_max_pos(double x) {        // the same of doubles: the upper halves, then the lower ones of their lanes
     const unsigned long long b = (unsigned long long)__double_as_longlong(x);
