@@ -140,15 +140,17 @@ __device__ __forceinline__ void tile_landed(bool more) {
 // Reductions over a wave by DPP: within rows of 16 lanes, then across them; lane 63 holds the result.  (By way of the LDS, as
 // __shfl_xor goes, the five of a tile were a chain of 3000 cycles.)
 template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int dpp(int none, int v) { return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false); }   // `none`: lanes without a source
 __device__ __forceinline__ int wave_min_i(int v) {
-    v = min(v, dpp<0x111, 0xf>(v)); v = min(v, dpp<0x112, 0xf>(v)); v = min(v, dpp<0x114, 0xf>(v)); v = min(v, dpp<0x118, 0xf>(v));
-    v = min(v, dpp<0x142, 0xa>(v)); v = min(v, dpp<0x143, 0xc>(v));
+    constexpr int N = 0x7fffffff;
+    v = min(v, dpp<0x111, 0xf>(N, v)); v = min(v, dpp<0x112, 0xf>(N, v)); v = min(v, dpp<0x114, 0xf>(N, v)); v = min(v, dpp<0x118, 0xf>(N, v));
+    v = min(v, dpp<0x142, 0xa>(N, v)); v = min(v, dpp<0x143, 0xc>(N, v));
     return __builtin_amdgcn_readlane(v, 63);
 }
 __device__ __forceinline__ int wave_max_i(int v) {
-    v = max(v, dpp<0x111, 0xf>(v)); v = max(v, dpp<0x112, 0xf>(v)); v = max(v, dpp<0x114, 0xf>(v)); v = max(v, dpp<0x118, 0xf>(v));
-    v = max(v, dpp<0x142, 0xa>(v)); v = max(v, dpp<0x143, 0xc>(v));
+    constexpr int N = (int)0x80000000;
+    v = max(v, dpp<0x111, 0xf>(N, v)); v = max(v, dpp<0x112, 0xf>(N, v)); v = max(v, dpp<0x114, 0xf>(N, v)); v = max(v, dpp<0x118, 0xf>(N, v));
+    v = max(v, dpp<0x142, 0xa>(N, v)); v = max(v, dpp<0x143, 0xc>(N, v));
     return __builtin_amdgcn_readlane(v, 63);
 }
 

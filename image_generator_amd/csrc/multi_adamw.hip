@@ -263,8 +263,9 @@ __device__ __forceinline__ int sbyte(unsigned w, int e) { return (int)(w << (24 
 __device__ __forceinline__ int ubyte(unsigned w, int e) { return (int)((w >> (8 * e)) & 255u); }
 
 // States of 8 bits, 18 bytes a parameter.  A wave takes two blocks, every load of both ahead of the norm's sum; a scale needs the
-// largest value of its block, hence one wave a block and DPP reductions.  69.9 million parameters (1.26 GB) 272 us, 4.6 TB/s; 243 million
-// with bf16 gradients (3.9 GB) 948 us, 4.1 TB/s: between the copy's 5.2 TB/s and the fp64 steps, conversions and roots of an element.
+// largest value of its block, hence one wave a block and DPP reductions.  69.9 million parameters (1.26 GB) 227 us, 5.6 TB/s; 243 million
+// with bf16 gradients (3.9 GB) 855 us, 4.6 TB/s, at 87 % of the vector units' cycles: fp64 steps, conversions and roots, 80 instructions
+// an element.
 __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict__ recs, const long long* __restrict__ grads,
                                                            const int2* __restrict__ map, unsigned* __restrict__ m_codes,
                                                            float* __restrict__ m_scales, unsigned* __restrict__ u_codes,
@@ -278,7 +279,23 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
     f32x4 pvs[MINE], gvs[MINE];
     unsigned mcs[MINE], ucs[MINE];
     float mss[MINE], uss[MINE];
-    if (g != 0) {
+    // a run that lies inside the tensor, at aligned addresses: nothing to look at lane by lane
+    const bool whole = (long long)(at.y + WG_BLOCKS) * BLK <= t.n && ((t.p | t.p16 * 2) & 15) == 0 && ((g & 1 ? (g & ~1ll) * 2 : g) & 15) == 0;
+    if (whole && g != 0) {
+#pragma unroll
+        for (int u = 0; u < MINE; ++u) {
+            const size_t tb = (size_t)(at.y + u * 4 + wave), i = tb * BLK + lane * 4, blk = (size_t)t.block0 + tb;
+            pvs[u] = *(const f32x4*)((const float*)t.p + i);
+            if (g & 1) {
+                const bf16x4 v = __builtin_nontemporal_load((const bf16x4*)((const bf16_t*)(g & ~1ll) + i));
+                gvs[u] = f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+            } else gvs[u] = *(const f32x4*)((const float*)g + i);
+            mcs[u] = m_codes[blk * (BLK / 4) + lane];
+            ucs[u] = u_codes[blk * (BLK / 4) + lane];
+            mss[u] = m_scales[blk];
+            uss[u] = u_scales[blk];
+        }
+    } else if (g != 0) {
 #pragma unroll
         for (int u = 0; u < MINE; ++u) {
             const size_t tb = (size_t)(at.y + u * 4 + wave), i = tb * BLK + lane * 4;
@@ -336,9 +353,10 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
         mmax = mmax >= 0x1p-126f ? mmax : 0.f;
         umax = umax >= 0x1p-126f ? umax : 0.f;
         const double rm = inverse(mmax), ru = inverse(umax), ru2 = ru * ru;
-        // Codes from fp32 roots, whose positions are good to 6.3e-5 (two roots of 1 ulp each on a ratio rounded once, times 255);
-        // a lane with a position within twice that of the border of two codes takes the fp64 roots: one wave and block in ten.
-        constexpr float SURE = 0.5f - 1.25e-4f;
+        // Codes from fp32 roots, whose positions are good to 6.5e-5: a ratio rounded once, two roots of 1 ulp, a product, times 255 -
+        // 255 ((2^-24 / 2 + 2^-23) / 2 + 2^-23 + 2^-24).  A lane with a position within 8e-5 of the border of two codes takes the
+        // fp64 roots: one wave and block in twelve.
+        constexpr float SURE = 0.5f - 8e-5f;
         f32x4 qm, qu, uf;                                            // codes as whole floats
         bool near = false;
 #pragma unroll
@@ -364,7 +382,10 @@ __global__ __launch_bounds__(256) void multi_adamw8_kernel(const Rec* __restrict
                 qu[e] = (float)(int)fma(255.0, root(root(ve[e] * ru2)), HALF);
             }
         }
-        if (in) store_param(t, i, pv);
+        if (whole) {
+            *(f32x4*)((float*)t.p + i) = pv;
+            if (t.p16) *(bf16x4*)((bf16_t*)t.p16 + i) = bf16x4{(bf16_t)pv[0], (bf16_t)pv[1], (bf16_t)pv[2], (bf16_t)pv[3]};
+        } else if (in) store_param(t, i, pv);
         unsigned mo = 0, uo = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
