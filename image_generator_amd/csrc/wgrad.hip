@@ -9,8 +9,9 @@
 //
 // Tile: 160(co) x 160(ci) x 64 pixels per 256-thread workgroup (2x2 waves, 5x5 MFMA 16x16x32 each).
 // LDS row stride 352 B = 11 x 32 B keeps the 8 rows touched by one half-wave transposed read on
-// distinct banks.  The pixel range is split across workgroups (split-K); partial sums are combined
-// with fp32 atomics into a zero-initialised (or accumulating) fp32 gradient buffer.
+// distinct banks.  The pixel range is split across workgroups (split-K).  Partial sums are combined
+// with fp32 atomics into a zero-initialised (or accumulating) fp32 gradient buffer, whose last bits then depend on the
+// order in which the workgroups end; or (ORDERED) they are stored in a workspace that a second launch adds up in order.
 #include "common.h"
 #include <algorithm>
 #include <stdlib.h>
@@ -43,6 +44,8 @@ constexpr int WG_BK = 64;           // pixels per k tile
 constexpr int WG_LD = 352;          // LDS row stride in bytes
 constexpr int WG_CH = 5;            // 16-byte chunks per thread per operand
 
+// ORDERED: dw is [splits][Cout][taps][Cin] and dbias [splits][Cout]; every split stores its own partial sums.
+template <bool ORDERED>
 __device__ __forceinline__ void wgrad_body(const WgradArgs& p, const int block_id, const int grid_blocks, char* smem) {
     char* As = smem;                       // dy tile  [64][160]
     char* Bs = smem + WG_BK * WG_LD;       // x tile   [64][160]
@@ -173,11 +176,13 @@ __device__ __forceinline__ void wgrad_body(const WgradArgs& p, const int block_i
         if (tid < WG_BT && co0 + tid < p.Cout) {
             float v = 0.f;
             for (int r = 0; r < WG_BK; ++r) v += red[r * WG_BT + tid];
-            atomicAdd(p.dbias + co0 + tid, v);
+            if (ORDERED) p.dbias[(size_t)split * p.Cout + co0 + tid] = v;
+            else atomicAdd(p.dbias + co0 + tid, v);
         }
     }
 
     const int ktot = p.taps * p.Cin;
+    float* const dw = ORDERED ? p.dw + (size_t)split * p.Cout * ktot : p.dw;
 #pragma unroll
     for (int i = 0; i < 5; ++i)
 #pragma unroll
@@ -187,16 +192,17 @@ __device__ __forceinline__ void wgrad_body(const WgradArgs& p, const int block_i
                 const int co = co0 + wm0 + i * 16 + g * 4 + r;
                 const int ci = ci0 + wn0 + j * 16 + li;
                 if (co < p.Cout && ci < p.Cin) {
-                    float* dst = p.dw + (size_t)co * ktot + (size_t)tap * p.Cin + ci;
-                    if (p.use_atomic) unsafeAtomicAdd(dst, acc[i][j][r]);
+                    float* dst = dw + (size_t)co * ktot + (size_t)tap * p.Cin + ci;
+                    if (!ORDERED && p.use_atomic) unsafeAtomicAdd(dst, acc[i][j][r]);
                     else *dst = acc[i][j][r];
                 }
             }
 }
 
+template <bool ORDERED>
 __global__ __launch_bounds__(256, 2) void wgrad_kernel(const WgradArgs p) {
     __shared__ __attribute__((aligned(16))) char smem[2 * WG_BK * WG_LD];
-    wgrad_body(p, blockIdx.x, gridDim.x, smem);
+    wgrad_body<ORDERED>(p, blockIdx.x, gridDim.x, smem);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -243,7 +249,7 @@ __device__ __forceinline__ int fast_div(int n, int d, float rd) {
 }
 
 // MODE 0: dense (linear layer / 1x1 conv), 1: stride-1 taps on power-of-two Ho x Wo, 2: generic gather
-template <int MODE, bool BIAS>
+template <int MODE, bool BIAS, bool ORDERED>
 __device__ __forceinline__ void wgrad_dma_body(const WgradArgs& p, const int block_id, const int grid_blocks, char* smem) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const int tid = threadIdx.x, lane = tid & 63;
@@ -478,11 +484,15 @@ __device__ __forceinline__ void wgrad_dma_body(const WgradArgs& p, const int blo
             t += __shfl_xor(t, 16);
             t += __shfl_xor(t, 32);
             const int co = co0 + wm0 + i * 16 + li;
-            if (g == 0 && co < p.Cout) atomicAdd(p.dbias + co, t);
+            if (g == 0 && co < p.Cout) {
+                if (ORDERED) p.dbias[(size_t)split * p.Cout + co] = t;
+                else atomicAdd(p.dbias + co, t);
+            }
         }
     }
 
     const int ktot = p.taps * p.Cin;
+    float* const dw = ORDERED ? p.dw + (size_t)split * p.Cout * ktot : p.dw;
     float sq = 0.f;
 #pragma unroll
     for (int i = 0; i < 5; ++i)
@@ -494,21 +504,23 @@ __device__ __forceinline__ void wgrad_dma_body(const WgradArgs& p, const int blo
                 const int ci = ci0 + wn0 + j * 16 + li;
                 if (co < p.Cout && ci < p.Cin) {
                     const size_t idx = (size_t)co * ktot + (size_t)tap * p.Cin + ci;
-                    if (p.use_atomic) unsafeAtomicAdd(p.dw + idx, acc[i][j][r]);
+                    if (ORDERED) dw[idx] = acc[i][j][r];
+                    else if (p.use_atomic) unsafeAtomicAdd(dw + idx, acc[i][j][r]);
                     else {
                         if (p.dw16 != nullptr) p.dw16[idx] = f2bf(acc[i][j][r]);
-                        else p.dw[idx] = acc[i][j][r];
+                        else dw[idx] = acc[i][j][r];
                         sq += acc[i][j][r] * acc[i][j][r];
                     }
                 }
             }
-    if (p.sumsq != nullptr && !p.use_atomic) {
+    if (!ORDERED && p.sumsq != nullptr && !p.use_atomic) {
         sq = wave_sum(sq);
         if (lane == 0) atomicAdd(p.sumsq + ((block_id * 4 + wave) & (WG_SQ_SLOTS - 1)), sq);
     }
 #endif
 }
 
+template <bool ORDERED>
 __device__ __forceinline__ void wgrad_dma_dispatch(const WgradArgs& p, const int block_id, const int grid_blocks, char* smem) {
     const bool linear = p.stride == 1 && !p.ups;
     const int mode = (p.ksize == 1 && linear) ? 0 : (linear && p.lw >= 0) ? 1 : 2;
@@ -523,19 +535,20 @@ __device__ __forceinline__ void wgrad_dma_dispatch(const WgradArgs& p, const int
         bias = lid % p.taps == 0 && cg == 0 && r % gw == 0;
     }
     if (bias) {
-        if (mode == 0) wgrad_dma_body<0, true>(p, block_id, grid_blocks, smem);
-        else if (mode == 1) wgrad_dma_body<1, true>(p, block_id, grid_blocks, smem);
-        else wgrad_dma_body<2, true>(p, block_id, grid_blocks, smem);
+        if (mode == 0) wgrad_dma_body<0, true, ORDERED>(p, block_id, grid_blocks, smem);
+        else if (mode == 1) wgrad_dma_body<1, true, ORDERED>(p, block_id, grid_blocks, smem);
+        else wgrad_dma_body<2, true, ORDERED>(p, block_id, grid_blocks, smem);
     } else {
-        if (mode == 0) wgrad_dma_body<0, false>(p, block_id, grid_blocks, smem);
-        else if (mode == 1) wgrad_dma_body<1, false>(p, block_id, grid_blocks, smem);
-        else wgrad_dma_body<2, false>(p, block_id, grid_blocks, smem);
+        if (mode == 0) wgrad_dma_body<0, false, ORDERED>(p, block_id, grid_blocks, smem);
+        else if (mode == 1) wgrad_dma_body<1, false, ORDERED>(p, block_id, grid_blocks, smem);
+        else wgrad_dma_body<2, false, ORDERED>(p, block_id, grid_blocks, smem);
     }
 }
 
+template <bool ORDERED>
 __global__ __launch_bounds__(256, 2) void wgrad_dma_kernel(const WgradArgs p) {
     __shared__ __attribute__((aligned(16))) char smem[6 * WD_TILE];     // [stage][A | B]
-    wgrad_dma_dispatch(p, blockIdx.x, gridDim.x, smem);
+    wgrad_dma_dispatch<ORDERED>(p, blockIdx.x, gridDim.x, smem);
 }
 
 // Many independent weight-gradient problems in ONE launch (deferred from the backward pass): job j owns
@@ -558,7 +571,35 @@ __global__ __launch_bounds__(256, 2) void wgrad_grouped_kernel(const WgradJob* _
     }
     const WgradJob& j = jobs[lo];
     WgradArgs p = j.a;
-    wgrad_dma_dispatch(p, bid - j.first_block, j.nblocks, smem);
+    wgrad_dma_dispatch<false>(p, bid - j.first_block, j.nblocks, smem);
+}
+
+// out[i] = sum of part[s][i] over the splits, in their order, and behind it dbias[i] (+)= the sum of its partial rows.  VEC 4: out
+// is 16-byte aligned (n is a multiple of 8).
+template <int VEC>
+__global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict__ part, float* __restrict__ out, size_t n, int splits,
+                                                         const float* __restrict__ bpart, float* __restrict__ dbias, int cout, int add_bias) {
+    typedef float vec __attribute__((ext_vector_type(VEC)));
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+    if (i < n) {
+        const float* v = part + i;
+        vec acc = *(const vec*)v;
+        int s = 1;
+        for (; s + 4 <= splits; s += 4) {
+            const vec a = *(const vec*)(v + s * n), b = *(const vec*)(v + (s + 1) * n);
+            const vec c = *(const vec*)(v + (s + 2) * n), d = *(const vec*)(v + (s + 3) * n);
+            acc = (((acc + a) + b) + c) + d;
+        }
+        for (; s < splits; ++s) acc += *(const vec*)(v + s * n);
+        *(vec*)(out + i) = acc;
+    } else if (dbias != nullptr) {
+        const size_t c0 = i - n;
+        for (size_t c = c0; c < c0 + VEC && c < (size_t)cout; ++c) {
+            float acc = bpart[c];
+            for (int s = 1; s < splits; ++s) acc += bpart[(size_t)s * cout + c];
+            dbias[c] = add_bias ? dbias[c] + acc : acc;
+        }
+    }
 }
 
 // Column sums of a bf16 matrix in segments of `seg` rows: out[s][n] = sum_{m in segment s} y[m][n].
@@ -729,19 +770,18 @@ int mi355_wgrad_grouped(const void* jobs, int njobs, int total_blocks, double fl
     return mi355_check_launch("wgrad_grouped_kernel");
 }
 
-int mi355_wgrad_bf16(const void* dy, const void* x, float* dw, float* dbias, int B, int H, int W, int Cin, int Cout,
-                     int ksize, int stride, int ups, int Ho, int Wo, int accumulate, void* stream) {
-    if (!dy || !x || !dw) return mi355_fail(MI355_ERR_ARG, "wgrad: null pointer");
+}  // extern "C"
+
+// Geometry, loader and pixel split of a launch of its own.
+static int wgrad_single(WgradArgs& a, bool& dma, int B, int H, int W, int Cin, int Cout, int ksize, int stride, int ups, int Ho, int Wo) {
     if (ksize != 1 && ksize != 3) return mi355_fail(MI355_ERR_UNSUPPORTED, "wgrad: ksize %d", ksize);
     if ((Cin & 7) || (Cout & 7)) return mi355_fail(MI355_ERR_ARG, "wgrad: channels must be multiples of 8");
-    WgradArgs a = {};
-    a.dy = (const bf16_t*)dy; a.x = (const bf16_t*)x; a.dw = dw; a.dbias = dbias;
     wgrad_geometry(a, B, H, W, Cin, Cout, ksize, stride, ups, Ho, Wo);
     const int tiles = a.tiles_co * a.tiles_ci * a.taps;
     // The LDS-DMA kernel is the default; operands of 2 GB or more (beyond a buffer descriptor's reach) and
     // MI355_WGRAD_V1=1 take the register-staged kernel.
     static const bool force_v1 = getenv("MI355_WGRAD_V1") != nullptr;
-    const bool dma = wgrad_dma_extents(a) && !force_v1;
+    dma = wgrad_dma_extents(a) && !force_v1;
     const int bk = dma ? WD_BK : WG_BK;
     const int nkt = (a.M + bk - 1) / bk;
     // split choice: waves of 512 co-resident workgroups, ~1 us per 64-pixel k-tile, fp32 atomics at ~1.3 TB/s
@@ -761,6 +801,29 @@ int mi355_wgrad_bf16(const void* dy, const void* x, float* dw, float* dbias, int
     }
     a.kt_per_split = (nkt + s - 1) / s;
     a.splits = (nkt + a.kt_per_split - 1) / a.kt_per_split;
+    return MI355_OK;
+}
+
+template <bool ORDERED>
+static int wgrad_launch(WgradArgs& a, bool dma, hipStream_t st) {
+    if (dma) {
+        const int blocks = wgrad_dma_blocks(a);      // also completes `a` (block count, block order)
+        hipLaunchKernelGGL(wgrad_dma_kernel<ORDERED>, dim3(blocks), dim3(256), 0, st, a);
+    }
+    else
+        hipLaunchKernelGGL(wgrad_kernel<ORDERED>, dim3(a.tiles_co * a.tiles_ci * a.taps * a.splits), dim3(256), 0, st, a);
+    return mi355_check_launch("wgrad_kernel");
+}
+
+extern "C" {
+
+int mi355_wgrad_bf16(const void* dy, const void* x, float* dw, float* dbias, int B, int H, int W, int Cin, int Cout,
+                     int ksize, int stride, int ups, int Ho, int Wo, int accumulate, void* stream) {
+    if (!dy || !x || !dw) return mi355_fail(MI355_ERR_ARG, "wgrad: null pointer");
+    WgradArgs a = {};
+    a.dy = (const bf16_t*)dy; a.x = (const bf16_t*)x; a.dw = dw; a.dbias = dbias;
+    bool dma;
+    if (const int rc = wgrad_single(a, dma, B, H, W, Cin, Cout, ksize, stride, ups, Ho, Wo)) return rc;
     // accumulate: 0 = overwrite (zero first when split), 1 = add to existing values,
     //             2 = dw and dbias were zeroed by the caller (plain stores when unsplit, no memsets here)
     a.use_atomic = (a.splits > 1 || accumulate == 1) ? 1 : 0;
@@ -768,13 +831,45 @@ int mi355_wgrad_bf16(const void* dy, const void* x, float* dw, float* dbias, int
     if (a.splits > 1 && accumulate == 0) mi355_zero_async(dw, (size_t)Cout * a.taps * Cin * sizeof(float), st);
     if (dbias && accumulate == 0) mi355_zero_async(dbias, (size_t)Cout * sizeof(float), st);
     ProfScope prof(FAM_WGRAD, st, 2.0 * a.M * Cout * (double)a.taps * Cin);
-    if (dma) {
-        const int blocks = wgrad_dma_blocks(a);      // also completes `a` (block count, block order)
-        hipLaunchKernelGGL(wgrad_dma_kernel, dim3(blocks), dim3(256), 0, st, a);
+    return wgrad_launch<false>(a, dma, st);
+}
+
+static size_t wgrad_part_bytes(const WgradArgs& a) {
+    return a.splits > 1 ? (size_t)a.splits * ((size_t)a.Cout * a.taps * a.Cin + a.Cout) * sizeof(float) : 0;
+}
+long long mi355_wgrad_ordered_bytes(int B, int H, int W, int Cin, int Cout, int ksize, int stride, int ups, int Ho, int Wo) {
+    WgradArgs a = {};
+    bool dma;
+    return wgrad_single(a, dma, B, H, W, Cin, Cout, ksize, stride, ups, Ho, Wo) ? -1 : (long long)wgrad_part_bytes(a);
+}
+
+int mi355_wgrad_bf16_ordered(const void* dy, const void* x, float* dw, float* dbias, int B, int H, int W, int Cin, int Cout, int ksize,
+                             int stride, int ups, int Ho, int Wo, int add_bias, void* ws, size_t ws_bytes, void* stream) {
+    if (!dy || !x || !dw) return mi355_fail(MI355_ERR_ARG, "wgrad_ordered: null pointer");
+    WgradArgs a = {};
+    a.dy = (const bf16_t*)dy; a.x = (const bf16_t*)x; a.dw = dw; a.dbias = dbias;
+    bool dma;
+    if (const int rc = wgrad_single(a, dma, B, H, W, Cin, Cout, ksize, stride, ups, Ho, Wo)) return rc;
+    const size_t need = wgrad_part_bytes(a);
+    if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
+        return mi355_fail(MI355_ERR_ARG, "wgrad_ordered: workspace of %zu bytes, %zu needed, 16-byte aligned", ws ? ws_bytes : (size_t)0, need);
+    hipStream_t st = (hipStream_t)stream;
+    ProfScope prof(FAM_WGRAD, st, 2.0 * a.M * Cout * (double)a.taps * Cin);
+    if (!need) {
+        if (dbias && !add_bias) mi355_zero_async(dbias, (size_t)Cout * sizeof(float), st);
+        return wgrad_launch<false>(a, dma, st);          // one addition for each bias, whatever the order of the workgroups
     }
-    else
-        hipLaunchKernelGGL(wgrad_kernel, dim3(tiles * a.splits), dim3(256), 0, st, a);
-    return mi355_check_launch("wgrad_kernel");
+    const size_t n = (size_t)Cout * a.taps * Cin;
+    float *part = (float*)ws, *bpart = part + a.splits * n;
+    a.dw = part;
+    a.dbias = dbias ? bpart : nullptr;
+    if (const int rc = wgrad_launch<true>(a, dma, st)) return rc;
+    const bool vec = ((uintptr_t)dw & 15) == 0;
+    const size_t threads = (n + (dbias ? Cout : 0)) / (vec ? 4 : 1);         // (n and Cout are multiples of 8)
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    if (vec) hipLaunchKernelGGL(wgrad_join_kernel<4>, grid, dim3(256), 0, st, part, dw, n, a.splits, bpart, dbias, Cout, add_bias);
+    else hipLaunchKernelGGL(wgrad_join_kernel<1>, grid, dim3(256), 0, st, part, dw, n, a.splits, bpart, dbias, Cout, add_bias);
+    return mi355_check_launch("wgrad_join_kernel");
 }
 
 long long mi355_colsum_scratch_floats(int M, int N, int seg) {

@@ -296,15 +296,22 @@ def conv2d(x, w, cout, ksize, stride=1, ups=False, dil=False, out_hw=None, bias=
 
 def wgrad(dy, x, cin, cout, ksize=1, stride=1, ups=False, geom=None, out=None, accumulate=False, dbias=None):
     """fp32 [Cout][k*k][Cin].  Linear: dy [M,Cout], x [M,Cin].  Conv: geom=(B,H,W,Ho,Wo).
-    dbias (optional fp32 [Cout]) receives the bias gradient from the same pass."""
+    dbias (optional fp32 [Cout]) receives the bias gradient from the same pass.  Partial sums of a split over pixels are
+    added in their order (same call, same bits); with accumulate=1, onto what `out` holds, in any order."""
     if geom is None:
         B, H, W, Ho, Wo = dy.shape[0], 1, 1, 1, 1
     else:
         B, H, W, Ho, Wo = geom
     if out is None:
         out = torch.empty((cout, ksize * ksize, cin), dtype=F32, device=dy.device)
-    check(lib.mi355_wgrad_bf16(dy.data_ptr(), x.data_ptr(), out.data_ptr(), _ptr(dbias), B, H, W, cin, cout, ksize, stride,
-                               int(ups), Ho, Wo, int(accumulate), _stream()), "wgrad")
+    shape = (B, H, W, cin, cout, ksize, stride, int(ups), Ho, Wo)
+    if int(accumulate) == 1:
+        check(lib.mi355_wgrad_bf16(dy.data_ptr(), x.data_ptr(), out.data_ptr(), _ptr(dbias), *shape, 1, _stream()), "wgrad")
+        return out
+    need = int(lib.mi355_wgrad_ordered_bytes(*shape))
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need > 0 else None
+    check(lib.mi355_wgrad_bf16_ordered(dy.data_ptr(), x.data_ptr(), out.data_ptr(), _ptr(dbias), *shape, int(accumulate) == 2,
+                                       _ptr(ws), max(need, 0), _stream()), "wgrad")
     return out
 
 

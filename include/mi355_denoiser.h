@@ -193,6 +193,12 @@ int mi355_conv2d_bf16(const void* x, int B, int H, int W, int C, const void* w, 
  * dbias (optional, [Cout] fp32) receives the column sums of dy (bias gradient) from the same pass. */
 int mi355_wgrad_bf16(const void* dy, const void* x, float* dw, float* dbias, int B, int H, int W, int Cin, int Cout,
                      int ksize, int stride, int ups, int Ho, int Wo, int accumulate, void* stream);
+/* The same with the partial sums of a split over pixels added in their order, not with atomics: equal calls return equal bits.
+ * dw is overwritten, dbias overwritten or (add_bias) added to.  ws: a device buffer of mi355_wgrad_ordered_bytes (0 where nothing
+ * is split, -1 for bad sizes), 16-byte aligned, for this call alone. */
+long long mi355_wgrad_ordered_bytes(int B, int H, int W, int Cin, int Cout, int ksize, int stride, int ups, int Ho, int Wo);
+int mi355_wgrad_bf16_ordered(const void* dy, const void* x, float* dw, float* dbias, int B, int H, int W, int Cin, int Cout,
+                             int ksize, int stride, int ups, int Ho, int Wo, int add_bias, void* ws, size_t ws_bytes, void* stream);
 
 /* Deferred, batched weight gradients: fill job records on the host, copy them to the device, launch once.
  * mi355_wgrad_job_fill returns the job's block count (multiple of 8); first_block = running sum of them.
