@@ -359,7 +359,7 @@ struct Plan {
 static Plan plan(int Tq, long long Tk, int Hq, int Hkv, int docs) {
     const long long G = Hq / Hkv, rows = (long long)Tq * G, wgs = (rows + 127) / 128 * Hkv;
     const Plan tiled = {false, key_runs(Tq, (int)Tk, Hq, Hkv, docs), 0, (size_t)(rows + 127) / 128 * 128};
-    if (rows >= 64ll * docs || wgs >= 256 || Tk < 384) return tiled;
+    if (rows == 0 || rows >= 64ll * docs || wgs >= 256 || Tk < 384) return tiled;
     int R = 32;
     while (R > 1 && R / 2 >= G && (rows + R - 1) / R * Hkv * 64 < 768 && Tk * R / rows > 64 * 64) R /= 2;
     const long long tiles = (rows + R - 1) / R;

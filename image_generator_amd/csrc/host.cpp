@@ -109,7 +109,7 @@ void here(std::initializer_list<const at::Tensor*> all, int current) {
     if (first.get_device() != current) raise(PyExc_RuntimeError, "tensors on %s, the current device is %d", first.device().str().c_str(), current);
 }
 
-bool adjacent(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 && t.dim() == 2 && (t.stride(1) == 1 || t.size(1) <= 1); }
+bool adjacent(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 && t.dim() == 2 && (t.stride(1) == 1 || t.size(1) <= 1 || t.size(0) == 0); }
 // the stride between the rows of one row is whatever made the tensor (a transposed column, say) and is not looked at
 long long row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
