@@ -68,13 +68,13 @@ class ContrastiveTrainer:
         loss.backward()
         packs = self.enc._train_packs()
         copies = [packs[n].w16 if n in packs else None for n in self.names]
-        if [c is not None and c.data_ptr() for c in copies] != [c is not None and c.data_ptr() for c in self.opt.copies]:
+        if self.opt.moved() or [c is not None and c.data_ptr() for c in copies] != [c is not None and c.data_ptr() for c in self.opt.copies]:
             self.opt.set_copies(copies)
         tgrads = [None if p.grad is None else p.grad.to(F32).contiguous() for p in self.temp]
         o = self.opt
         o.betas, o.eps, o.wd, o.t = self.betas, self.eps, self.wd, self.t
-        self.t += 1
         o.step([None if p.grad is None else p.grad.to(F32) for p in self.params], lr=self.lr, watched=tgrads)
+        self.t = o.t
         s = _stream()
         for pk in packs.values():        # the data-gradient operands of the next step
             check(lib.mi355_transpose_bf16(pk.w16.data_ptr(), pk.w16_t.data_ptr(), 1, pk.n, pk.k, s), "transpose")

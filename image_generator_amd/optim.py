@@ -100,6 +100,10 @@ class TensorAdamW:
         rows += [[0, 0, n, 0] for n in self.watched]
         self._recs = torch.tensor(rows, dtype=torch.int64).to(self.device)
 
+    def moved(self):
+        """Whether a parameter or copy lies elsewhere than `set_copies` found it."""
+        return host().places(self._written, self._places_at, False)
+
     def bind(self, grads=None, lr=None, watched=None):
         """Begin a step: gradients (default: the parameters' own `.grad`; None leaves a parameter alone) and learning rate.
         Addresses and scalars go to the device in one asynchronous copy on the current stream."""
@@ -109,8 +113,8 @@ class TensorAdamW:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"TensorAdamW: {len(grads)} gradients of {len(self.params)} parameters")
-        if host().places(self._written, self._places_at, False):
-            raise RuntimeError("TensorAdamW: a parameter or copy has moved to other memory (set_copies() takes the new places)")
+        if self.moved():
+            raise RuntimeError("TensorAdamW: a parameter or copy has moved to other memory (set_copies(copies) takes the new places)")
         watched = [None] * len(self.watched) if watched is None else list(watched)
         if len(watched) != len(self.watched):
             raise ValueError(f"TensorAdamW: {len(watched)} watched gradients, {len(self.watched)} announced")

@@ -1,0 +1,53 @@
+"""What `ContrastiveTrainer` takes: parameters whose storage is replaced between steps, and the calls around it."""
+import pytest
+import torch
+
+from test_packed_encoder_gpu import D, fixture
+
+pytestmark = pytest.mark.gpu
+
+
+def trainer(dropout=0.0, **kw):
+    from image_generator_amd.encoder_trainer import ContrastiveTrainer
+    from image_generator_amd.loss import ContrastiveLoss
+    z, enc, ids, off, padded, mask = fixture(dropout)
+    tr = ContrastiveTrainer(enc, ContrastiveLoss(0.07).to(D), lr=1e-3, **kw)
+    return tr, enc, (padded, mask, torch.from_numpy(z["img"]).to(D)), (ids, off, torch.from_numpy(z["img"]).to(D))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_parameter_may_move_between_steps(bits):
+    """`p.data = x` for every parameter (the embedding and the norms have no bf16 copy): the same steps as without."""
+    a, enc_a, _, step = trainer(state_bits=bits)
+    b, enc_b, _, _ = trainer(state_bits=bits)
+    a.train_step_packed(*step)
+    b.train_step_packed(*step)
+    old = [p.data for p in enc_b.parameters()]
+    kept = [x.clone() for x in old]
+    for p in enc_b.parameters():
+        p.data = p.data.clone()
+    for _ in range(2):
+        a.train_step_packed(*step)
+        b.train_step_packed(*step)
+    assert a.t == b.t == 3
+    for (n, p), q in zip(enc_a.named_parameters(), enc_b.parameters()):
+        assert torch.equal(p, q), n
+    assert all(torch.equal(x, y) for x, y in zip(old, kept))              # nothing was written to the old places
+    named = dict(enc_b.named_parameters())
+    for n, pk in enc_b._train_packs().items():
+        assert torch.equal(pk.w16, named[n].detach().to(torch.bfloat16)), n
+
+
+def test_a_step_that_raises_is_not_counted(monkeypatch):
+    tr, enc, _, step = trainer()
+    tr.train_step_packed(*step)
+
+    def refuse(*a, **kw):
+        raise ValueError("no")
+    monkeypatch.setattr(tr.opt, "bind", refuse)
+    with pytest.raises(ValueError, match="no"):
+        tr.train_step_packed(*step)
+    assert tr.t == 1 and tr.step_count == 1
+    monkeypatch.undo()
+    tr.train_step_packed(*step)
+    assert tr.t == tr.opt.t == 2 and tr.step_count == 2
