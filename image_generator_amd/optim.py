@@ -28,7 +28,8 @@ class TensorAdamW:
     follow as `bind(..., watched=[...])`.
 
     fp32_betas: a new gradient's weights are 1 - beta of betas rounded to fp32, as `trainer.FusedAdamW` forms them (1 - 0.999 is
-    7e-6 off then), instead of 1 - beta rounded itself; an option of 32-bit states.
+    7e-6 off then), instead of 1 - beta rounded itself, and any eps >= 0 is taken, as there (with eps = 0, an element that never had a
+    gradient becomes NaN); an option of 32-bit states.
 
     `step(grads)` uploads what changes (addresses, bias corrections) and launches.  For a captured graph: `bind(grads)` before
     the capture and before every replay, `apply()` inside it; the gradients stay the caller's to keep."""
@@ -38,7 +39,8 @@ class TensorAdamW:
         self.params = list(params)
         if not self.params:
             raise ValueError("TensorAdamW: no parameters")
-        if not all(0 <= b < 1 for b in betas) or not eps >= 2.0 ** -126:      # (0 / 0 behind a smaller one: untouched rows have m = v = 0)
+        # (0 / 0 behind a smaller eps: untouched rows have m = v = 0)
+        if not all(0 <= b < 1 for b in betas) or not eps >= (0.0 if fp32_betas and state_bits == 32 else 2.0 ** -126):
             raise ValueError(f"TensorAdamW: betas {tuple(betas)} not below 1, or eps {eps} not a normal fp32 number above 0")
         if state_bits not in (8, 32):
             raise ValueError(f"TensorAdamW: states of 8 or 32 bits, not {state_bits}")

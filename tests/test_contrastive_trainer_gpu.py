@@ -51,3 +51,23 @@ def test_a_step_that_raises_is_not_counted(monkeypatch):
     monkeypatch.undo()
     tr.train_step_packed(*step)
     assert tr.t == tr.opt.t == 2 and tr.step_count == 2
+
+
+def test_eps_zero():
+    """eps = 0, as before the optimizer over many tensors: a first step of every element with a gradient is lr, by its sign.
+
+    The first step moves by lr sqrt(1 - b2) (1 - b1') / ((1 - b1) sqrt(1 - b2')), betas rounded to fp32 on one side: 2^-25 / 0.001 / 2 =
+    1.5e-5 and 2^-25 / 0.1 = 3e-7 of it, and some ten roundings of 2^-24; the parameter's product with 1 - lr wd and the difference
+    another 2^-23 of it."""
+    tr, enc, _, step = trainer(eps=0.0)
+    before = [p.detach().double() for p in enc.parameters()]
+    tr.train_step_packed(*step)
+    for (n, p), old in zip(enc.named_parameters(), before):
+        seen = p.grad.abs() > 1e-12                      # (its square is a normal fp32 number)
+        want = old * (1 - tr.lr * tr.wd) - tr.lr * p.grad.double().sign()
+        off = (p.detach().double() - want).abs()
+        assert bool((off <= tr.lr * 2.0 ** -15 + 2.0 ** -23 * old.abs())[seen].all()), n
+    with pytest.raises(ValueError, match="eps"):
+        trainer(eps=-1e-8)
+    with pytest.raises(ValueError, match="eps"):
+        trainer(eps=0.0, state_bits=8)                   # roots that are held as 0 divide by eps alone
