@@ -36,14 +36,15 @@ class ContrastiveTrainer:
         dev = next(text_encoder.parameters()).device
         if dev.type != "cuda":
             raise RuntimeError("ContrastiveTrainer: parameters must live on the HIP device (no CPU path)")
-        self.names, self.params = zip(*((n, p) for n, p in text_encoder.named_parameters() if p.requires_grad))
+        named = [(n, p) for n, p in text_encoder.named_parameters() if p.requires_grad]
+        self.names, self.params = [n for n, _ in named], [p for _, p in named]
         # the loss's single scalar: AdamW in a few one-element tensor ops, lr 0.1 x the encoder's (train_encoder.py:42-49),
         # gated by the optimizer's norm, in which its gradient counts
         self.temp = [p for p in criterion.parameters() if p.requires_grad]
         self.temp_m = [torch.zeros_like(p) for p in self.temp]
         self.temp_v = [torch.zeros_like(p) for p in self.temp]
         self.opt = TensorAdamW(self.params, lr, betas, eps, weight_decay, state_bits=state_bits, watched=[p.numel() for p in self.temp],
-                               fp32_betas=state_bits == 32)
+                               fp32_betas=state_bits == 32, device=dev)
         self.state = self.opt.state            # [0] = norm of the step's gradients (no clipping: only its finiteness is used)
         if state_bits == 32:
             self.m, self.v = self.opt.split(self.opt.m), self.opt.split(self.opt.v)

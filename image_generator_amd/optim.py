@@ -25,7 +25,7 @@ class TensorAdamW:
     (`skipped_steps`), as in `trainer.FusedAdamW`; like there, its number still advances the bias correction.
 
     watched: sizes of further gradients, stepped by someone else, that count in the norm (and in the test for finite values); they
-    follow as `bind(..., watched=[...])`.
+    follow as `bind(..., watched=[...])`.  device: where they are, if there is no parameter.
 
     fp32_betas: a new gradient's weights are 1 - beta of betas rounded to fp32, as `trainer.FusedAdamW` forms them (1 - 0.999 is
     7e-6 off then), instead of 1 - beta rounded itself, and any eps >= 0 is taken, as there (with eps = 0, an element that never had a
@@ -35,19 +35,19 @@ class TensorAdamW:
     the capture and before every replay, `apply()` inside it; the gradients stay the caller's to keep."""
 
     def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=0.0, state_bits=32, copies=None,
-                 watched=(), fp32_betas=False):
+                 watched=(), fp32_betas=False, device=None):
         self.params = list(params)
-        if not self.params:
+        if not self.params and device is None:
             raise ValueError("TensorAdamW: no parameters")
         # (0 / 0 behind a smaller eps: untouched rows have m = v = 0)
         if not all(0 <= b < 1 for b in betas) or not eps >= (0.0 if fp32_betas and state_bits == 32 else 2.0 ** -126):
             raise ValueError(f"TensorAdamW: betas {tuple(betas)} not below 1, or eps {eps} not a normal fp32 number above 0")
         if state_bits not in (8, 32):
             raise ValueError(f"TensorAdamW: states of 8 or 32 bits, not {state_bits}")
-        dev = self.params[0].device
+        dev = self.params[0].device if self.params else torch.device(device)
+        if dev.type != "cuda" or dev.index is None:
+            raise RuntimeError("TensorAdamW: parameters must live on the HIP device (no CPU path)")
         for p in self.params:
-            if not p.is_cuda:
-                raise RuntimeError("TensorAdamW: parameters must live on the HIP device (no CPU path)")
             if p.device != dev:
                 raise ValueError(f"TensorAdamW: parameters on {dev} and {p.device}")
             if p.dtype != F32 or not p.is_contiguous():
@@ -63,12 +63,13 @@ class TensorAdamW:
         for b in blocks:
             self.starts.append(self.starts[-1] + b)
         total = self.starts[-1]
+        room = max(total, 1)                          # (an address for the launch, also where only watched gradients count)
         if state_bits == 32:
-            self.m, self.v = (torch.zeros(total * BLOCK, dtype=F32, device=dev) for _ in range(2))
+            self.m, self.v = (torch.zeros(room * BLOCK, dtype=F32, device=dev) for _ in range(2))
         else:
-            self.m_codes = torch.zeros(total * BLOCK, dtype=torch.int8, device=dev)
-            self.u_codes = torch.zeros(total * BLOCK, dtype=torch.uint8, device=dev)
-            self.m_scales, self.u_scales = (torch.zeros(total, dtype=F32, device=dev) for _ in range(2))
+            self.m_codes = torch.zeros(room * BLOCK, dtype=torch.int8, device=dev)
+            self.u_codes = torch.zeros(room * BLOCK, dtype=torch.uint8, device=dev)
+            self.m_scales, self.u_scales = (torch.zeros(room, dtype=F32, device=dev) for _ in range(2))
         parts = [torch.stack((torch.full((-(-b // _WG_BLOCKS),), i, dtype=torch.int32),
                               torch.arange(0, b, _WG_BLOCKS, dtype=torch.int32)), 1) for i, b in enumerate(blocks + [-(-n // BLOCK) for n in self.watched]) if b]
         self._map = torch.cat(parts).to(dev) if parts else torch.zeros((0, 2), dtype=torch.int32, device=dev)

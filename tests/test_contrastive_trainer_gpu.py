@@ -71,3 +71,31 @@ def test_eps_zero():
         trainer(eps=-1e-8)
     with pytest.raises(ValueError, match="eps"):
         trainer(eps=0.0, state_bits=8)                   # roots that are held as 0 divide by eps alone
+
+
+def test_frozen_encoder():
+    """Nothing of the encoder trains (the image tower's turn): the temperature moves, the image gradients come back."""
+    from image_generator_amd.encoder_trainer import ContrastiveTrainer
+    from image_generator_amd.loss import ContrastiveLoss
+    for bits in (32, 8):
+        z, enc, ids, off, padded, mask = fixture()
+        enc.requires_grad_(False)
+        img = torch.from_numpy(z["img"]).to(D)
+        before = [p.detach().clone() for p in enc.parameters()]
+        crit = ContrastiveLoss(0.07).to(D)
+        temp = crit.log_temp.detach().clone()
+        tr = ContrastiveTrainer(enc, crit, lr=1e-3, state_bits=bits)
+        for step in (lambda x: tr.train_step(padded, mask, x), lambda x: tr.train_step_packed(ids, off, x)):
+            loss, d_img = step(img)
+            assert torch.isfinite(loss) and float(d_img.norm()) > 0
+        assert not torch.equal(crit.log_temp.detach(), temp) and tr.skipped_steps() == 0
+        assert tr.opt.grad_norm() == pytest.approx(abs(float(crit.log_temp.grad)), rel=1e-6)
+        temp = crit.log_temp.detach().clone()
+        bad = img.clone()
+        bad[0, 0] = float("nan")
+        tr.train_step(padded, mask, bad)
+        assert tr.skipped_steps() == 1 and torch.equal(crit.log_temp.detach(), temp)
+        assert all(torch.equal(x, p) for x, p in zip(before, enc.parameters()))
+        crit.requires_grad_(False)
+        loss, d_img = ContrastiveTrainer(enc, crit, lr=1e-3, state_bits=bits).train_step(padded, mask, img)
+        assert torch.isfinite(loss) and float(d_img.norm()) > 0
