@@ -47,7 +47,8 @@ class ContrastiveTrainer:
                                fp32_betas=state_bits == 32, device=dev)
         self.state = self.opt.state            # [0] = norm of the step's gradients (no clipping: only its finiteness is used)
         if state_bits == 32:
-            self.m, self.v = self.opt.split(self.opt.m), self.opt.split(self.opt.v)
+            self._moments = self.opt.split(self.opt.m), self.opt.split(self.opt.v)
+            self.m, self.v = (list(views) for views in self._moments)
         self.step_count = 0
 
     def train_step(self, input_ids, attention_mask, image_embeds):
@@ -73,6 +74,8 @@ class ContrastiveTrainer:
             self.opt.set_copies(copies)
         tgrads = [None if p.grad is None else p.grad.to(F32).contiguous() for p in self.temp]
         o = self.opt
+        if o.bits == 32:
+            self._take_moments()
         o.betas, o.eps, o.wd, o.t = self.betas, self.eps, self.wd, self.t
         o.step([None if p.grad is None else p.grad.to(F32) for p in self.params], lr=self.lr, watched=tgrads)
         self.t = o.t
@@ -83,6 +86,18 @@ class ContrastiveTrainer:
         self._temperature_step(tgrads)
         self.step_count += 1
         return loss.detach(), img.grad
+
+    def _take_moments(self):
+        """Moments that a program put into `m` and `v` (a checkpoint's, say) go where the optimizer holds them."""
+        for name, views in zip("mv", self._moments):
+            held = getattr(self, name)
+            if len(held) != len(views):
+                raise ValueError(f"ContrastiveTrainer: {len(held)} moments of {len(views)} parameters")
+            if any(x is not y for x, y in zip(held, views)):
+                for x, y in zip(held, views):
+                    if x is not y:
+                        y.copy_(x.reshape(y.shape))
+                setattr(self, name, list(views))
 
     def _temperature_step(self, tgrads):
         b1, b2 = self.betas

@@ -99,3 +99,32 @@ def test_frozen_encoder():
         crit.requires_grad_(False)
         loss, d_img = ContrastiveTrainer(enc, crit, lr=1e-3, state_bits=bits).train_step(padded, mask, img)
         assert torch.isfinite(loss) and float(d_img.norm()) > 0
+
+
+def test_moments_put_back_by_hand():
+    """`trainer.m` / `.v` are lists of the parameters' moments: entries or lists that a program puts in their place are stepped on."""
+    a, enc_a, _, step = trainer()
+    for _ in range(2):
+        a.train_step_packed(*step)
+    saved = [p.detach().clone() for p in enc_a.parameters()], [m.clone() for m in a.m], [v.cpu() for v in a.v], a.temp_m[0].clone(), a.temp_v[0].clone()
+    temp = a.crit.log_temp.detach().clone()
+    a.train_step_packed(*step)
+    for whole in (True, False):
+        b, enc_b, _, _ = trainer()
+        with torch.no_grad():
+            for p, x in zip(enc_b.parameters(), saved[0]):
+                p.copy_(x)
+            b.crit.log_temp.copy_(temp)
+        if whole:
+            b.m, b.v = tuple(saved[1]), list(saved[2])
+        else:
+            for i, (m, v) in enumerate(zip(saved[1], saved[2])):
+                b.m[i], b.v[i] = m, v
+        b.temp_m[0], b.temp_v[0] = saved[3].clone(), saved[4].clone()
+        b.t = 2
+        b.train_step_packed(*step)
+        for (n, p), q, m, k in zip(enc_a.named_parameters(), enc_b.parameters(), a.m, b.m):
+            assert torch.equal(p, q) and torch.equal(m, k), n
+    b.m = b.m[:-1]
+    with pytest.raises(ValueError, match="moments"):
+        b.train_step_packed(*step)
