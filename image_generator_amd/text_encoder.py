@@ -213,6 +213,49 @@ class TextEncoder(nn.Module):
         self.transformer = _Encoder(embed_dim, n_head, embed_dim * 4, dropout, num_layers)
         self.norm = nn.LayerNorm(embed_dim)
         self.projection = nn.Linear(embed_dim, projection_dim)
+        # (moves with the module; in the state dict only where it is set, see _save_to_state_dict)
+        self.register_buffer("distance_slopes", None, persistent=False)
+
+    # ---- options that the reference does not have ------------------------------------------------
+    # Its encoder attends without positions or caps.  `score_cap`: scores s become cap tanh(s / cap).  `distance_slopes` [heads]
+    # (fp32): a score falls by slope times the distance of the two tokens, which gives the encoder the order of the words without a
+    # parameter.  0 / None leave the reference's arithmetic.  Every path computes them - padded, packed, training, inference - and a
+    # state dict holds those that are set: a checkpoint without them (the reference's) has the reference's keys, and loading it leaves
+    # what the module has.
+    score_cap = 0.0
+    _OPTIONS = ("score_cap", "distance_slopes")
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        if self.score_cap:
+            destination[prefix + "score_cap"] = torch.tensor(float(self.score_cap), dtype=torch.float64)
+        if self.distance_slopes is not None:
+            destination[prefix + "distance_slopes"] = self.distance_slopes if keep_vars else self.distance_slopes.detach()
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        mine = {n: state_dict[prefix + n] for n in self._OPTIONS if prefix + n in state_dict}
+        super()._load_from_state_dict({k: v for k, v in state_dict.items() if k not in {prefix + n for n in mine}}, prefix, *args)
+        if "score_cap" in mine:
+            self.score_cap = float(mine["score_cap"])
+        if "distance_slopes" in mine:
+            self.distance_slopes = mine["distance_slopes"].detach().to(self.embedding.weight.device, torch.float32, copy=True)
+
+    def _score_options(self):
+        """The keyword arguments of the document attention for the options that are set, None if there are none."""
+        if not self.score_cap and self.distance_slopes is None:
+            return None
+        return dict(cap=self.score_cap, slopes=self.distance_slopes)
+
+    @staticmethod
+    def _padded_documents(B, T, kv_len, device):
+        """A padded batch as documents of `ops.doc_attention`: caption b has the queries bT .. (b + 1)T and the keys bT .. bT + kv_len[b];
+        the padding behind them is a document without queries."""
+        starts = torch.arange(0, (B + 1) * T, T, dtype=torch.int32, device=device) if T else torch.zeros(B + 1, dtype=torch.int32, device=device)
+        if kv_len is None:
+            return dict(q_offsets=starts, k_offsets=None, align="start")
+        a, b = starts[:-1], starts[1:]
+        return dict(q_offsets=torch.cat((torch.stack((a, b), 1).view(-1), starts[-1:])),
+                    k_offsets=torch.cat((torch.stack((a, a + kv_len), 1).view(-1), starts[-1:])), align="start")
 
     # ---- inference on the HIP kernels -----------------------------------------------------------
     def _forward_hip(self, input_ids, attention_mask):
@@ -223,11 +266,17 @@ class TextEncoder(nn.Module):
         H = self.transformer.layers[0].self_attn.num_heads
         x = ops.cast_bf16(self.embedding(input_ids).contiguous()).view(B * T, D)      # gather, then fp32 -> bf16
         kv_len, bad = self._key_counts(attention_mask)
+        options = self._score_options()
+        docs = None if options is None else self._padded_documents(B, T, kv_len, x.device)
         for i, layer in enumerate(self.transformer.layers):
             pre = f"transformer.layers.{i}."
             sa = layer.self_attn
             qkv = ops.gemm(x, w16[pre + "self_attn.in_proj_weight"], bias=sa.in_proj_bias).view(B, T, 3 * D)
-            a, _ = ops.attention_fwd(qkv[:, :, :D], qkv[:, :, D:2 * D], qkv[:, :, 2 * D:], H, kv_len=kv_len)
+            if options is None:
+                a, _ = ops.attention_fwd(qkv[:, :, :D], qkv[:, :, D:2 * D], qkv[:, :, 2 * D:], H, kv_len=kv_len)
+            else:
+                flat = qkv.view(B * T, 3 * D)
+                a, _ = ops.doc_attention_fwd(flat[:, :D], flat[:, D:2 * D], flat[:, 2 * D:], H, **docs, **options)
             x = ops.gemm(a.view(B * T, D), w16[pre + "self_attn.out_proj.weight"], bias=sa.out_proj.bias, residual=x)
             x = ops.layernorm_bf16(x, layer.norm1.weight, layer.norm1.bias, layer.norm1.eps)
             f = ops.gelu_bf16(ops.gemm(x, w16[pre + "linear1.weight"], bias=layer.linear1.bias))
@@ -299,6 +348,7 @@ class TextEncoder(nn.Module):
     def _forward_train_hip(self, input_ids, attention_mask, return_pooled):
         """Every row computed, dropout active when `self.training`: the reference's training arithmetic
         (encoder/text_encoder.py:29-43 under train_encoder.py:103-105) on the library's kernels, differentiable."""
+        from . import ops
         from .ops import LinearFn, LayerNormFn
         packs = self._train_packs()
         B, T = input_ids.shape
@@ -307,13 +357,18 @@ class TextEncoder(nn.Module):
         p = float(self.transformer.layers[0].p) if self.training else 0.0
         seed = int(torch.randint(0, 2 ** 31 - 1, (1,))) if p > 0 else 0     # CPU generator: no device synchronisation
         kv_len, bad = self._key_counts(attention_mask)
+        options = self._score_options()
+        docs = None if options is None else self._padded_documents(B, T, kv_len, input_ids.device)
         x = _ToBf16Fn.apply(self.embedding(input_ids)).view(B * T, D)
         for i, layer in enumerate(self.transformer.layers):
             pre = f"transformer.layers.{i}."
             sa = layer.self_attn
             s0 = (seed + 7919 * (4 * i + 1)) & 0x7FFFFFFF
             qkv = LinearFn.apply(x, packs[pre + "self_attn.in_proj_weight"], sa.in_proj_bias, None, False, sa.in_proj_weight)
-            a = _AttnTrainFn.apply(qkv.view(B, T, 3 * D), kv_len, H, p, s0).view(B * T, D)
+            if options is None:
+                a = _AttnTrainFn.apply(qkv.view(B, T, 3 * D), kv_len, H, p, s0).view(B * T, D)
+            else:
+                a = ops.doc_attention(qkv.view(B * T, 3 * D), heads=H, drop_p=p, seed=s0, **docs, **options)
             if p > 0:
                 a = LinearFn.apply(a, packs[pre + "self_attn.out_proj.weight"], sa.out_proj.bias, None, False, sa.out_proj.weight)
                 h = _DropoutAddFn.apply(a, x, p, s0 + 1)
@@ -338,12 +393,6 @@ class TextEncoder(nn.Module):
         return self._poison(y.view(B, T, -1), bad)
 
     # ---- captions without padding ---------------------------------------------------------------
-    # Options of the packed path that the reference does not have (its encoder attends without positions or caps): scores
-    # capped by a tanh, and a bias that falls with the distance of two tokens (slope per head), which gives the encoder the
-    # order of the words without a parameter.  None / 0 leave the reference's arithmetic.
-    score_cap = 0.0
-    distance_slopes = None
-
     def forward_packed(self, input_ids, offsets, return_pooled=True):
         """The encoder on captions that lie one behind another: input_ids [tokens] (int32 / int64), caption n the tokens
         offsets[n] .. offsets[n + 1] (int32 on the device, any layout that `ops.doc_attention_fwd` takes).  Returns the
@@ -362,7 +411,7 @@ class TextEncoder(nn.Module):
         D = self.embedding.embedding_dim
         p = float(layers[0].p) if self.training else 0.0
         seed = int(torch.randint(0, 2 ** 31 - 1, (1,))) if p > 0 else 0     # CPU generator: no device synchronisation
-        how = dict(heads=H, cap=self.score_cap, slopes=self.distance_slopes, drop_p=p)
+        how = dict(heads=H, drop_p=p, **(self._score_options() or {}))
         x = ops.embedding(input_ids, self.embedding.weight)
         if return_pooled:        # one query for each caption, its first token: position 0 (no row for an empty caption)
             first = torch.where(offsets[1:] > offsets[:-1], offsets[:-1], -1)
