@@ -61,6 +61,7 @@ __device__ __forceinline__ Doc doc_at(const int* __restrict__ off, int docs, int
 // chain of loads, a third of a caption tile's time; here the 64 offsets around the place where documents of equal length would
 // have this one are loaded at once and usually hold it - if not, a search that probes 64 places a step says where they are -
 // and the lanes take their documents from those registers.
+// (At most 2^30 documents: the estimate in fp32 is then some hundred places past the last offset at most, and no index passes 32 bits.)
 // Loads return in order: the window is asked for before the rows' own operands, behind which it would wait (OffWindow).
 struct OffWindow { int w, val; };        // first offset; the lane's
 __device__ __forceinline__ OffWindow off_window(const int* __restrict__ off, int docs, int total, int i0) {

@@ -4,7 +4,7 @@
 namespace {
 
 static const char* bad_sizes(int docs, int Tq, int Tk, int Hq, int Hkv, int D) {
-    if (docs < 1 || docs == 0x7fffffff || Tq < 0 || Tk < 0) return "no document, or a negative number of tokens";
+    if (docs < 1 || docs > (1 << 30) || Tq < 0 || Tk < 0) return "no document, more than 2^30 documents, or a negative number of tokens";
     if (Hq < 1 || Hkv < 1 || Hq % Hkv) return "query heads must be a multiple of key heads";
     if (D < 8 || D > 128 || D % 8) return "heads must be a multiple of 8 wide, at most 128";
     if ((long long)Tq * Hq >= (1ll << 30) || (long long)Tk * Hkv >= (1ll << 30)) return "2^30 rows or more";
