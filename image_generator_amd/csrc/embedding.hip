@@ -414,7 +414,8 @@ static GradPlan grad_plan(long long n, long long rows, int width) {
 static const char* bad_shape(long long n, long long rows, long long width) {
     if (n < 0 || rows < 1 || width < 1) return "negative count or empty table";
     if (n > (1ll << 30) || rows > (1ll << 30) || width > (1 << 20)) return "more than 2^30 ids or rows, or 2^20 columns";
-    if (n * width >= (1ll << 32)) return "more than 2^32 elements";
+    // a launch has fewer than 2^32 threads in whole workgroups of 256, and rows of an odd width take a thread for each element
+    if (n * width > (1ll << 32) - 256) return "more than 2^32 - 256 elements";
     return nullptr;
 }
 

@@ -460,7 +460,7 @@ int mi355_doc_attention_bwd(const void* q, const void* k, const void* v, const v
  * where no id names it.  The order depends on the ids alone: equal calls return equal bits.
  * ids: int32, or int64 (ids64 != 0).  An id outside [0, rows) reads as a NaN row and adds to no gradient.  ws: a device
  * buffer of mi355_embedding_bwd_workspace_bytes(n, rows, width), 16-byte aligned, for this call alone.
- * Limits: n, rows <= 2^30 (bwd: rows <= 2^26), width <= 2^20, n * width < 2^32. */
+ * Limits: n, rows <= 2^30 (bwd: rows <= 2^26), width <= 2^20, n * width <= 2^32 - 256. */
 int mi355_embedding_fwd(const void* ids, int ids64, long long n, const void* table, int table_bf16, long long rows, int width,
                         float scale, void* out, int out_bf16, void* stream);
 size_t mi355_embedding_bwd_workspace_bytes(long long n, long long rows, int width);

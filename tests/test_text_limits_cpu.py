@@ -20,3 +20,16 @@ def test_documents_up_to_2_30():
         assert bwd(docs) == -1 and "document" in err()
         assert lib.mi355_doc_attention_bwd_workspace_bytes(4, 4, 2, 2, 32, docs, 0) == 0
     assert lib.mi355_doc_attention_bwd_workspace_bytes(4, 4, 2, 2, 32, 1 << 30, 0) > 0
+
+
+def test_embedding_rows_element_by_element():
+    """Odd widths take a thread for each element, and a launch has fewer than 2^32 threads in whole workgroups of 256."""
+    from image_generator_amd._lib import lib
+    rows = lambda n, width, out=16: lib.mi355_embedding_fwd(16, 1, n, 16, 0, 4, width, 1.0, out, 1, None)  # noqa: E731
+    grad = lambda n, width: lib.mi355_embedding_bwd(16, 1, n, 16, 1, 4, width, 1.0, 16, 0, 16, 0, None)  # noqa: E731
+    n, width = 65537, 65535                                  # 2^32 - 1 elements
+    assert n * width == 2 ** 32 - 1
+    assert rows(n, width) == -1 and "2^32" in err()
+    assert lib.mi355_embedding_bwd_workspace_bytes(n, 4, width) == 0
+    assert grad(n, width) == -1 and "2^32" in err()
+    assert grad(n - 1, width) == -1 and "workspace" in err()      # the largest below
