@@ -24,7 +24,8 @@ static int fill(DocArgs& a, const char* who, int docs, int Tq, int Tk, int Hq, i
     if (!q_off || !k_off) return mi355_fail(MI355_ERR_ARG, "%s: null pointer", who);
     if (prefix && !causal) return mi355_fail(MI355_ERR_ARG, "%s: a prefix without the causal mask it lifts", who);
     // the tanh is 1 - 2 / (1 + 2^x), good to 2^-22 of the cap: 2^-12 of a nat at the limit
-    if (!(cap >= 0.f) || !(cap <= 1024.f)) return mi355_fail(MI355_ERR_ARG, "%s: cap %g, not between 0 (none) and 1024", who, (double)cap);
+    // and below the normal range 1 / cap is infinite
+    if (!(cap == 0.f || (cap >= 0x1p-126f && cap <= 1024.f))) return mi355_fail(MI355_ERR_ARG, "%s: cap %g, neither 0 (none) nor between 2^-126 and 1024", who, (double)cap);
     if (!(drop_p >= 0.f && drop_p < 1.f)) return mi355_fail(MI355_ERR_ARG, "%s: dropout %g", who, (double)drop_p);
     a.docs = docs; a.Tq = Tq; a.Tk = Tk; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.D = D;
     a.q_off = q_off; a.k_off = k_off; a.prefix = prefix; a.slopes = slopes;

@@ -33,3 +33,14 @@ def test_embedding_rows_element_by_element():
     assert lib.mi355_embedding_bwd_workspace_bytes(n, 4, width) == 0
     assert grad(n, width) == -1 and "2^32" in err()
     assert grad(n - 1, width) == -1 and "workspace" in err()      # the largest below
+
+
+def test_caps_whose_reciprocal_is_no_number():
+    """Below 2^-126, 1 / cap is infinite and a score of 0 would be 0 times it."""
+    from image_generator_amd._lib import lib
+    for cap in (1e-45, 2.0 ** -127, 1e-39):
+        assert lib.mi355_doc_attention_fwd(16, 16, 16, 16, 16, 16, 16, 1, None, None, cap, 0, 0, 4, 4, 2, 2, 32, 64, 64, 64, 64, 1.0, 0.0, 0, None, 0,
+                                           None) == -1 and "cap" in err()
+        assert lib.mi355_doc_attention_bwd(*[16] * 9, 16, 16, 1, None, None, cap, 0, 0, 4, 4, 2, 2, 32, *[64] * 8, 1.0, 0.0, 0, None, 0, None) == -1 and "cap" in err()
+    assert lib.mi355_doc_attention_fwd(None, 16, 16, None, None, 16, 16, 1, None, None, 2.0 ** -126, 0, 0, 0, 4, 2, 2, 32, 64, 64, 64, 64, 1.0, 0.0, 0, None, 0,
+                                       None) == 0
