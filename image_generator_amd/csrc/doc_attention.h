@@ -115,7 +115,6 @@ __device__ __forceinline__ RowSpan row_span_in(const DocArgs& p, int i, const Do
     }
     return s;
 }
-__device__ __forceinline__ RowSpan row_span(const DocArgs& p, int i) { return row_span_in(p, i, doc_at(p.q_off, p.docs, i)); }
 
 // tokens whose rows may see key j of document k: [first, last)
 __device__ __forceinline__ int2 key_span_in(const DocArgs& p, int j, const Doc& k) {
