@@ -59,13 +59,18 @@ def parse():
     return ap.parse_args()
 
 
-def source_fingerprint():
-    """sha256 over the kernel sources and the modules that choose the launches: a committed counter profile applies to a
+# sources whose kernels (and host code) the benchmarked step does not launch: the data-file reader and the packed text operators
+NOT_IN_STEP = {"lmdb_reader.cpp", "host.cpp", "doc_attention.h", "doc_tiles.h", "doc_attention.hip", "doc_attention_fwd.hip",
+               "doc_attention_bwd_q.hip", "doc_attention_bwd_kv.hip", "embedding.hip", "multi_adamw.hip"}
+
+
+def source_fingerprint(root=ROOT):
+    """sha256 over the kernel sources of the step and the modules that choose its launches: a committed counter profile applies to a
     run only if it was collected from the same code."""
     h = hashlib.sha256()
-    pkg = os.path.join(ROOT, "image_generator_amd")
+    pkg = os.path.join(root, "image_generator_amd")
     files = sorted(os.path.join(pkg, "csrc", f) for f in os.listdir(os.path.join(pkg, "csrc"))
-                   if f.endswith((".hip", ".h", ".cpp")) and f != "lmdb_reader.cpp")      # the data-file reader launches nothing
+                   if f.endswith((".hip", ".h", ".cpp")) and f not in NOT_IN_STEP)
     files += [os.path.join(pkg, f) for f in ("ops.py", "unet.py", "trainer.py")]
     for f in files:
         h.update(open(f, "rb").read())
