@@ -322,21 +322,25 @@ PyObject** items(PyObject* list, Py_ssize_t& n) {
     return ((PyListObject*)list)->ob_item;
 }
 
-// gradient_words(gradients, parameters, device, address of int64[n]): what the device table holds for each gradient - its address,
-// the lowest bit set for bf16, 0 for None - and -1, or the index of the first that is no contiguous fp32 or bf16 tensor of
-// its parameter's shape on the device
+// gradient_words(gradients, parameters, device, address of int64[n], address of int64[n] or nothing): what the device table holds for
+// each gradient - its address, the lowest bit set for bf16, 0 for None - and -1, or the index of the first that is no contiguous
+// fp32 or bf16 tensor of its parameter's shape on the device.  The second array: the parameters' sizes as the device knows them; one
+// that has another by now raises.
 PyObject* gradient_words(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        if (n != 4) raise(PyExc_TypeError, "gradient_words: %zd arguments", n);
+        if (n != 4 && n != 5) raise(PyExc_TypeError, "gradient_words: %zd arguments", n);
         Py_ssize_t count, others;
         PyObject** g = items(a[0], count);
         PyObject** p = items(a[1], others);
         if (count != others) raise(PyExc_ValueError, "gradient_words: %zd gradients of %zd parameters", count, others);
         const int device = whole32(a[2], "device");
         long long* to = (long long*)whole(a[3]);
+        const long long* sizes = n == 5 ? (const long long*)whole(a[4]) : nullptr;
         for (Py_ssize_t i = 0; i < count; ++i) {
             if (g[i] == Py_None) { to[i] = 0; continue; }
             const at::Tensor &t = tensor(g[i], "a gradient"), &like = tensor(p[i], "a parameter");
+            if (sizes && like.numel() != sizes[i])
+                raise(PyExc_ValueError, "TensorAdamW: parameter %zd has become %lld elements, its states are of %lld", i, (long long)like.numel(), sizes[i]);
             if (!t.is_cuda() || t.get_device() != device || !is_float(t) || t.sizes() != like.sizes() || !t.is_contiguous()) return PyLong_FromSsize_t(i);
             to[i] = (long long)t.data_ptr() | (t.scalar_type() == at::kBFloat16);
         }

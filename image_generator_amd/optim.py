@@ -54,6 +54,7 @@ class TensorAdamW:
                 raise ValueError("TensorAdamW: parameters must be contiguous fp32 tensors")
         _disjoint(self.params, "parameters")
         self._shapes = [p.shape for p in self.params]
+        self._sizes = np.array([p.numel() for p in self.params], dtype=np.int64)
         self.lr, self.betas, self.eps, self.wd, self.max_norm = lr, tuple(betas), eps, weight_decay, max_grad_norm
         self.bits, self.device, self.t = state_bits, dev, 0
         self.fp32_betas = fp32_betas
@@ -125,7 +126,7 @@ class TensorAdamW:
             if g is not None and (g.numel() != n or g.device != self.device or g.dtype not in (F32, BF16) or not g.is_contiguous()):
                 raise ValueError("TensorAdamW: a watched gradient must be a contiguous fp32 or bf16 tensor of the announced size")
         slot, kept = self._ring.acquire(), []
-        words = (self.params, self.device.index, slot.data_ptr() + 8 * _HYPER)
+        words = (self.params, self.device.index, slot.data_ptr() + 8 * _HYPER, self._sizes.ctypes.data)
         if host().gradient_words(grads, *words) >= 0:
             grads, kept = self._contiguous(grads)
             host().gradient_words(grads, *words)

@@ -128,3 +128,18 @@ def test_moments_put_back_by_hand():
     b.m = b.m[:-1]
     with pytest.raises(ValueError, match="moments"):
         b.train_step_packed(*step)
+
+
+def test_optimizer_refuses_a_parameter_cut_short_where_it_lies():
+    from image_generator_amd.optim import TensorAdamW
+    p = torch.ones(4096, device=D)
+    opt = TensorAdamW([p], lr=0.5, weight_decay=0.0)
+    whole, p.data = p.data, p.data[:100]
+    with pytest.raises(ValueError, match="has become 100 elements"):
+        opt.step([torch.ones(100, device=D)])
+    assert opt.t == 0 and bool((whole == 1).all())
+    opt.step([None])
+    p.data = whole
+    opt.step([torch.ones(4096, device=D)])
+    # the second step (one without a gradient counts), the first gradient: m = 0.1, v = 0.001
+    assert torch.allclose(p, torch.full_like(p, 1 - 0.5 * (0.1 / (1 - 0.9 ** 2)) / (0.001 / (1 - 0.999 ** 2)) ** 0.5))

@@ -44,3 +44,19 @@ def test_caps_whose_reciprocal_is_no_number():
         assert lib.mi355_doc_attention_bwd(*[16] * 9, 16, 16, 1, None, None, cap, 0, 0, 4, 4, 2, 2, 32, *[64] * 8, 1.0, 0.0, 0, None, 0, None) == -1 and "cap" in err()
     assert lib.mi355_doc_attention_fwd(None, 16, 16, None, None, 16, 16, 1, None, None, 2.0 ** -126, 0, 0, 0, 4, 2, 2, 32, 64, 64, 64, 64, 1.0, 0.0, 0, None, 0,
                                        None) == 0
+
+
+def test_a_parameter_of_another_size_is_refused():
+    """A gradient has its parameter's shape; a parameter cut short where it lies would have the step read past that gradient."""
+    import numpy as np
+    import pytest
+    import torch
+    from image_generator_amd._lib import host
+    p, other = torch.zeros(8), torch.zeros(3)
+    to, sizes = np.empty(2, dtype=np.int64), np.array([3, 8], dtype=np.int64)
+    words = lambda g: host().gradient_words([None, g], [other, p], 0, to.ctypes.data, sizes.ctypes.data)  # noqa: E731
+    assert words(torch.zeros(8)) == 1                        # (on no device)
+    p.data = p.data[:5]
+    with pytest.raises(ValueError, match="parameter 1 has become 5 elements"):
+        words(torch.zeros(5))
+    assert words(None) == -1
