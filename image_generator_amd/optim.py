@@ -71,9 +71,11 @@ class TensorAdamW:
             self.m_codes = torch.zeros(room * BLOCK, dtype=torch.int8, device=dev)
             self.u_codes = torch.zeros(room * BLOCK, dtype=torch.uint8, device=dev)
             self.m_scales, self.u_scales = (torch.zeros(room, dtype=F32, device=dev) for _ in range(2))
-        parts = [torch.stack((torch.full((-(-b // _WG_BLOCKS),), i, dtype=torch.int32),
-                              torch.arange(0, b, _WG_BLOCKS, dtype=torch.int32)), 1) for i, b in enumerate(blocks + [-(-n // BLOCK) for n in self.watched]) if b]
-        self._map = torch.cat(parts).to(dev) if parts else torch.zeros((0, 2), dtype=torch.int32, device=dev)
+        wgs = np.array([-(-b // _WG_BLOCKS) for b in blocks + [-(-n // BLOCK) for n in self.watched]], dtype=np.int64)
+        places = np.empty((int(wgs.sum()), 2), dtype=np.int32)           # (tensor, first block within it) of each workgroup
+        places[:, 0] = np.repeat(np.arange(len(wgs)), wgs)
+        places[:, 1] = (np.arange(len(places)) - np.repeat(np.cumsum(wgs) - wgs, wgs)) * _WG_BLOCKS
+        self._map = torch.from_numpy(places).to(dev)
         self._elements = float(sum(p.numel() for p in self.params))
         self._partial = torch.zeros(int(lib.mi355_multi_adamw_parts()), dtype=torch.float64, device=dev)
         self.state = torch.zeros(2, dtype=F32, device=dev)          # norm of the last step, skipped steps
@@ -100,9 +102,13 @@ class TensorAdamW:
         self._places = np.empty(len(self._written), dtype=np.int64)
         host().places(self._written, self._places.ctypes.data, True)
         self._places_at = self._places.ctypes.data
-        rows = [[p.data_ptr(), 0 if c is None else c.data_ptr(), p.numel(), s] for p, c, s in zip(self.params, copies, self.starts)]
-        rows += [[0, 0, n, 0] for n in self.watched]
-        self._recs = torch.tensor(rows, dtype=torch.int64).to(self.device)
+        rows = np.zeros((len(self.params) + len(self.watched), 4), dtype=np.int64)
+        rows[:len(copies), 0] = self._places[:len(copies)]               # (the parameters come first in `_written`)
+        rows[:len(copies), 1] = [0 if c is None else c.data_ptr() for c in copies]
+        rows[:len(copies), 2] = self._sizes
+        rows[:len(copies), 3] = self.starts[:-1]
+        rows[len(copies):, 2] = self.watched
+        self._recs = torch.from_numpy(rows).to(self.device)
 
     def moved(self):
         """Whether a parameter or copy lies elsewhere than `set_copies` found it."""
