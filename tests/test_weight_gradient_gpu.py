@@ -120,3 +120,37 @@ def test_equal_training_steps_leave_equal_weights():
             first = grads
         for a, b in zip(first, grads):
             assert torch.equal(a, b)
+
+
+def test_the_register_staged_kernel_too():
+    """The kernel for operands of 2 GB and more, taken by an environment switch that a process reads once: a process of its own."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import sys, torch
+sys.path[:0] = [%r, %r]
+import test_weight_gradient_gpu as t
+from image_generator_amd import ops
+from image_generator_amd._lib import lib
+for case in t.CASES:
+    M, cin, cout, ksize, B, H, W, stride = case
+    x, dy, geom = t._operands(M, cin, cout, ksize, B, H, W, stride, seed=9)
+    col = t._columns(x, ksize, geom, stride)
+    want, size = torch.einsum("mo,mtc->otc", dy.double(), col), torch.einsum("mo,mtc->otc", dy.double().abs(), col.abs())
+    xd, dyd = x.to(t.D), dy.to(t.D)
+    runs = []
+    for _ in range(8):
+        db = torch.empty(cout, device=t.D)
+        runs.append((ops.wgrad(dyd, xd, cin, cout, ksize, stride, geom=geom, dbias=db), db))
+    assert all(torch.equal(a, runs[0][0]) and torch.equal(b, runs[0][1]) for a, b in runs), case
+    out, db = (v.cpu().double() for v in runs[0])
+    terms = dy.shape[0] + 64
+    assert bool(((out - want).abs() <= terms * 2.0 ** -24 * size).all()), case
+    assert bool(((db - dy.double().sum(0)).abs() <= terms * 2.0 ** -24 * dy.double().abs().sum(0)).all()), case
+assert lib.mi355_wgrad_ordered_bytes(4096, 1, 1, 128, 128, 1, 1, 0, 1, 1) > 0
+print("done")
+""" % (root, os.path.join(root, "tests"))
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "MI355_WGRAD_V1": "1"}, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip().endswith("done"), (r.returncode, r.stdout[-500:], r.stderr[-2000:])
