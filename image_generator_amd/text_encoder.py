@@ -399,12 +399,14 @@ class TextEncoder(nn.Module):
         pooled, normalised rows [captions, projection_dim], or every token's projected state [tokens, projection_dim].
         The arithmetic of `forward` on the same captions, right-padded (encoder/text_encoder.py:25-43), without the
         padding rows: dropout included when `self.training`, with masks of its own.  An empty caption comes back as NaN,
-        and so does an id outside the vocabulary; tokens of no caption attend to nothing."""
+        and so does an id outside the vocabulary; tokens of no caption attend to nothing.  There is at least one token."""
         from . import ops
         from .ops import LinearFn, LayerNormFn
         self._require_kernels(input_ids)
         if input_ids.dim() != 1 or offsets.dim() != 1:
             raise ValueError("TextEncoder.forward_packed: input_ids and offsets are vectors")
+        if input_ids.numel() == 0:
+            raise ValueError("TextEncoder.forward_packed: no tokens")
         packs = self._train_packs()
         layers = self.transformer.layers
         H = layers[0].self_attn.num_heads

@@ -87,3 +87,9 @@ def test_state_dict_keeps_them():
     assert holder["text"].score_cap == 0.5 and torch.equal(holder["text"].distance_slopes.cpu(), enc.distance_slopes.cpu())
     with pytest.raises(RuntimeError, match="nonsense"):
         make().load_state_dict({**plain, "nonsense": torch.zeros(1)})
+
+
+def test_a_batch_without_tokens_is_refused():
+    _, enc, ids, off, _, _ = fixture()
+    with pytest.raises(ValueError, match="no tokens"):
+        enc.forward_packed(ids[:0], torch.zeros_like(off))
