@@ -433,8 +433,8 @@ int mi355_copy2d_f32_batched(const long long* table, int n, void* stream);
  * Query i sits at key position c = i - q_end + k_end (align_start: i - q_begin + k_begin) and sees the keys j of its document,
  * with `causal` those with j <= c or j < k_begin + prefix[n] (prefix: int32 [docs] or NULL):
  *   t = scale q.k;  t = cap tanh(t / cap) if cap > 0;  score = t - slopes[head] |c - j|;  out = softmax(score) v
- * cap: 0 (none), or 2^-126 .. 1024.  slopes: fp32 [Hq] or NULL.  Hq is a multiple of Hkv; query head h reads key head h / (Hq / Hkv).  D: a multiple
- * of 8, <= 128.  Limits: Tq * Hq, Tk * Hkv < 2^30, docs <= 2^30, row strides <= 2^23.
+ * cap: 0 (none), or 2^-126 .. 1024.  slopes: fp32 [Hq] or NULL.  Hq is a multiple of Hkv; query head h reads key head
+ * h / (Hq / Hkv).  D: a multiple of 8, <= 128.  Limits: Tq * Hq, Tk * Hkv < 2^30, docs <= 2^30, row strides <= 2^23.
  * A query that sees no key, or belongs to no document, gets a row of zeros and lse = -infinity; keys of no document get zero
  * gradients.  What a query does not see never reaches its result, infinities and NaN included.  lse [Hq][Tq] in log2 units.
  * drop_p, seed: dropout on the probabilities, the same in both directions for the same seed.
