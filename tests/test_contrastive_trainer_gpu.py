@@ -7,19 +7,22 @@ from test_packed_encoder_gpu import D, fixture
 pytestmark = pytest.mark.gpu
 
 
-def trainer(dropout=0.0, **kw):
+def trainer(dropout=0.0, temperature=True, **kw):
+    """temperature=False: held fixed, for steps that are compared bit by bit (its gradient is a sum in any order)."""
     from image_generator_amd.encoder_trainer import ContrastiveTrainer
     from image_generator_amd.loss import ContrastiveLoss
     z, enc, ids, off, padded, mask = fixture(dropout)
-    tr = ContrastiveTrainer(enc, ContrastiveLoss(0.07).to(D), lr=1e-3, **kw)
+    crit = ContrastiveLoss(0.07).to(D)
+    crit.requires_grad_(temperature)
+    tr = ContrastiveTrainer(enc, crit, lr=1e-3, **kw)
     return tr, enc, (padded, mask, torch.from_numpy(z["img"]).to(D)), (ids, off, torch.from_numpy(z["img"]).to(D))
 
 
 @pytest.mark.parametrize("bits", [32, 8])
 def test_a_parameter_may_move_between_steps(bits):
     """`p.data = x` for every parameter (the embedding and the norms have no bf16 copy): the same steps as without."""
-    a, enc_a, _, step = trainer(state_bits=bits)
-    b, enc_b, _, _ = trainer(state_bits=bits)
+    a, enc_a, _, step = trainer(state_bits=bits, temperature=False)
+    b, enc_b, _, _ = trainer(state_bits=bits, temperature=False)
     a.train_step_packed(*step)
     b.train_step_packed(*step)
     old = [p.data for p in enc_b.parameters()]
@@ -103,24 +106,21 @@ def test_frozen_encoder():
 
 def test_moments_put_back_by_hand():
     """`trainer.m` / `.v` are lists of the parameters' moments: entries or lists that a program puts in their place are stepped on."""
-    a, enc_a, _, step = trainer()
+    a, enc_a, _, step = trainer(temperature=False)
     for _ in range(2):
         a.train_step_packed(*step)
-    saved = [p.detach().clone() for p in enc_a.parameters()], [m.clone() for m in a.m], [v.cpu() for v in a.v], a.temp_m[0].clone(), a.temp_v[0].clone()
-    temp = a.crit.log_temp.detach().clone()
+    saved = [p.detach().clone() for p in enc_a.parameters()], [m.clone() for m in a.m], [v.cpu() for v in a.v]
     a.train_step_packed(*step)
     for whole in (True, False):
-        b, enc_b, _, _ = trainer()
+        b, enc_b, _, _ = trainer(temperature=False)
         with torch.no_grad():
             for p, x in zip(enc_b.parameters(), saved[0]):
                 p.copy_(x)
-            b.crit.log_temp.copy_(temp)
         if whole:
             b.m, b.v = tuple(saved[1]), list(saved[2])
         else:
             for i, (m, v) in enumerate(zip(saved[1], saved[2])):
                 b.m[i], b.v[i] = m, v
-        b.temp_m[0], b.temp_v[0] = saved[3].clone(), saved[4].clone()
         b.t = 2
         b.train_step_packed(*step)
         for (n, p), q, m, k in zip(enc_a.named_parameters(), enc_b.parameters(), a.m, b.m):
